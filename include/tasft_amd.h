@@ -480,6 +480,130 @@ int tasft_mask_from_indices(const int32_t* indices, int64_t rows, int64_t k,
                             int64_t index_row_stride, int64_t num_k_blocks, uint8_t* block_mask,
                             int* error_flag, void* stream);
 
+/*
+ * Rotary position embedding of queries and keys, and its inverse (its gradient). The reference
+ * takes Q and K after its model's own rotation (tasft/modules/tasft_attention.py:426).
+ *
+ * The first rotary_dim (even) dims of every row are pairs, (i, i + rotary_dim/2) or, interleaved,
+ * (2i, 2i + 1); pair j of a row at position p turns by the angle p * inv_freq[j] (formed in 64
+ * bits) and is multiplied by `scale`; the other dims are copied. Computed in fp32, rounded once.
+ * inverse != 0 turns the other way (with the same scale): the gradient of the first.
+ * q, q_out [B, Hq, S, D], k, k_out [B, Hkv, S, D] with element strides (b, h, s, d), any of them,
+ * d 1; an output may not overlap an input other than exactly itself. num_kv_heads 0: q alone.
+ * positions: device int32 (positions_64 0) or int64, strides pos_strides (b, s). inv_freq: device
+ * [rotary_dim / 2] doubles. head_dim at most 256.
+ */
+int tasft_rotary(const void* q, const void* k, void* q_out, void* k_out, const void* positions,
+                 int positions_64, const double* inv_freq, int64_t batch, int64_t num_q_heads,
+                 int64_t num_kv_heads, int64_t seq_len, int64_t head_dim, int64_t rotary_dim,
+                 const int64_t* q_strides, const int64_t* k_strides, const int64_t* qo_strides,
+                 const int64_t* ko_strides, const int64_t* pos_strides, int interleaved, int inverse,
+                 float scale, int dtype, void* stream);
+
+/*
+ * New tokens into a paged cache: rotates q and k as tasft_rotary does and writes k and v to the
+ * pages. No reference counterpart (vLLM writes its cache itself,
+ * tasft/inference/vllm_patch.py:172-176).
+ *
+ * q, q_out [T, Hq, D], k and v [T, Hkv, D] (strides token, head, dim): sequence n is tokens
+ * cu_seqlens[n] .. cu_seqlens[n+1]-1 (device int32 [N + 1], non-decreasing, from 0), the last of
+ * its kv_lens[n] (device int32 [N]): token i of len goes to slot kv_lens[n] - len + i, row
+ * slot % page_size of page block_table[n * block_table_stride + slot / page_size] of the pools
+ * [num_pages, page_size, Hkv, D] (strides page, token, head, dim). A slot outside
+ * [0, max_pages * page_size) and a page outside the pool are not written. positions: the tokens'
+ * positions (int32 or int64, stride pos_stride), or NULL for their slots. slot_positions
+ * [N, Hkv, max_pages * page_size] int32 contiguous (or NULL) receives them at the slots. q_out
+ * rows of tokens at or after cu_seqlens[N] are 0, and such tokens are not written to the pages.
+ * page_size a power of two. Two tokens that share a slot race.
+ */
+int tasft_rotary_append_paged(
+    const void* q, const void* k, const void* v, void* q_out, void* k_pages, void* v_pages,
+    const int32_t* block_table, const int32_t* kv_lens, const int32_t* cu_seqlens, const void* positions,
+    int positions_64, const double* inv_freq, int32_t* slot_positions, int64_t num_seqs, int64_t tokens,
+    int64_t num_q_heads, int64_t num_kv_heads, int64_t head_dim, int64_t rotary_dim, int64_t page_size,
+    int64_t num_pages, int64_t max_pages, const int64_t* q_strides, const int64_t* k_strides,
+    const int64_t* v_strides, const int64_t* qo_strides, const int64_t* kp_strides,
+    const int64_t* vp_strides, int64_t block_table_stride, int64_t pos_stride, int interleaved,
+    float scale, int dtype, void* stream);
+
+/* Bytes of workspace tasft_chunk_paged_fwd needs (0 at one split). */
+size_t tasft_chunk_workspace_bytes(int64_t tokens, int64_t num_q_heads, int64_t head_dim,
+                                   int64_t num_splits);
+
+/*
+ * Attention of a chunk of new tokens over a paged cache that holds them already. No reference
+ * counterpart (its vLLM backend attends within the flat tokens of a call,
+ * tasft/inference/vllm_patch.py:172-176, or to one new token).
+ *
+ * q, out [T, Hq, D] (strides token, head, dim); sequences, pools, block_table and kv_lens as in
+ * tasft_rotary_append_paged (kv_lens clamped to [0, max_pages * page_size], table entries into
+ * the pool). Token i of sequence n is at position p = kv_lens[n] - len + i and sees the keys
+ * j < kv_lens[n], j <= p when causal, of the blocks that block_mask selects:
+ * [N, Hq, mask_rows, ceil(max_pages * page_size / block_size)] bytes (byte strides; NULL: all),
+ * row r for the query block floor((kv_lens[n] - len) / block_size) + r (rows past mask_rows use
+ * its last). out = softmax(q.k * scale) v over them, rows without keys 0; lse [T, Hq] fp32
+ * contiguous (or NULL) the natural logarithm of the sum of exponentials, -inf without keys. Rows
+ * of tokens at or after cu_seqlens[N] get 0 and -inf. What a row does not see does not reach it,
+ * infinities and NaN included. Sequences are at most max_seqlen tokens of a call.
+ * head_dim 64 or 128; block_size 32, 64 or 128; page_size a power of two >= 8; strides multiples
+ * of 8 on 16-byte aligned bases. num_splits (1 to 1024) shares the keys of a row among
+ * workgroups, joined by a second launch; workspace: tasft_chunk_workspace_bytes(...) bytes.
+ */
+int tasft_chunk_paged_fwd(
+    const void* q, const void* k_pages, const void* v_pages, void* out, float* lse,
+    const uint8_t* block_mask, const int32_t* block_table, const int32_t* kv_lens,
+    const int32_t* cu_seqlens, void* workspace, size_t workspace_bytes, int64_t num_seqs,
+    int64_t tokens, int64_t num_q_heads, int64_t num_kv_heads, int64_t max_seqlen, int64_t head_dim,
+    int64_t block_size, int64_t mask_rows, int64_t page_size, int64_t num_pages, int64_t max_pages,
+    int64_t num_splits, const int64_t* q_strides, const int64_t* kp_strides,
+    const int64_t* vp_strides, const int64_t* o_strides, const int64_t* mask_strides,
+    int64_t block_table_stride, float scale, int causal, int dtype, void* stream);
+
+/*
+ * The attention weight that each cached key received from a chunk: scores_out[n, g, j] =
+ * scores[n, g, j] (0 if NULL) + sum over the chunk's tokens and the query heads of KV head g
+ * that see key j of exp(q.k_j * scale - lse), in a fixed order. No reference counterpart.
+ *
+ * lse: what tasft_chunk_paged_fwd returned (strides token, head); rows of -inf add nothing.
+ * scores (strides sequence, head, slot) and scores_out (contiguous; may be scores itself when
+ * that is contiguous) are [N, Hkv, max_pages * page_size] fp32; slots at or past kv_lens[n] keep
+ * their score. The other arguments as in tasft_chunk_paged_fwd.
+ */
+int tasft_key_weights(
+    const void* q, const void* k_pages, const uint8_t* block_mask, const int32_t* block_table,
+    const int32_t* kv_lens, const int32_t* cu_seqlens, const float* lse, const float* scores,
+    float* scores_out, int64_t num_seqs, int64_t tokens, int64_t num_q_heads, int64_t num_kv_heads,
+    int64_t max_seqlen, int64_t head_dim, int64_t block_size, int64_t mask_rows, int64_t page_size,
+    int64_t num_pages, int64_t max_pages, const int64_t* q_strides, const int64_t* kp_strides,
+    const int64_t* lse_strides, const int64_t* score_strides, const int64_t* mask_strides,
+    int64_t block_table_stride, float scale, int causal, int dtype, void* stream);
+
+/* Bytes of workspace tasft_evict_paged needs (budget at most max_pages * page_size). */
+size_t tasft_evict_workspace_bytes(int64_t num_seqs, int64_t num_kv_heads, int64_t budget);
+
+/*
+ * Eviction from a paged cache by accumulated weight. No reference counterpart.
+ *
+ * Per (sequence n, KV head) the first n' = min(kv_lens[n], budget) of these slots stay: those
+ * whose position is below `sinks` or above newest - recent (newest: the head's largest position),
+ * then by falling weight (NaN first), ties to the lowest slot. The kept slots at n' and behind
+ * move, in slot order, to the slots below n' that are not kept, in slot order; the pools change in
+ * place, nothing else of them is written. kv_lens_out[n] = n'; scores_out and positions_out
+ * [N, Hkv, max_pages * page_size] contiguous hold the kept slots' values where they are now, and
+ * 0 and -1 from n' on. scores fp32 and positions int32 have element strides (sequence, head,
+ * slot); outputs must not overlap them. Sequences must not share pages that they evict from; a
+ * row whose page lies outside the pool is not moved. recent + sinks <= budget. head_dim a
+ * multiple of 8 up to 256, page_size a power of two, 16-bit pools (any type) with strides of
+ * multiples of 8. At most 65535 (sequence, KV head) pairs.
+ */
+int tasft_evict_paged(void* k_pages, void* v_pages, const int32_t* block_table, const int32_t* kv_lens,
+                      const float* scores, const int32_t* positions, int32_t* kv_lens_out,
+                      float* scores_out, int32_t* positions_out, void* workspace, size_t workspace_bytes,
+                      int64_t num_seqs, int64_t num_kv_heads, int64_t head_dim, int64_t page_size,
+                      int64_t num_pages, int64_t max_pages, int64_t budget, int64_t recent, int64_t sinks,
+                      const int64_t* kp_strides, const int64_t* vp_strides, const int64_t* score_strides,
+                      const int64_t* position_strides, int64_t block_table_stride, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -6,6 +6,7 @@ to load, every kernel entry point raises ``KernelError``.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import functools
 import threading
@@ -48,6 +49,13 @@ EXPORTED_SYMBOLS = (
     "tasft_mask_compact_workspace_bytes",
     "tasft_mask_compact",
     "tasft_mask_from_indices",
+    "tasft_rotary",
+    "tasft_rotary_append_paged",
+    "tasft_chunk_workspace_bytes",
+    "tasft_chunk_paged_fwd",
+    "tasft_key_weights",
+    "tasft_evict_workspace_bytes",
+    "tasft_evict_paged",
 )
 
 _lock = threading.Lock()
@@ -137,6 +145,33 @@ _SIGNATURES: dict[str, tuple[object, list[object]]] = {
         [_P, _I64, _I64, _I64, _I64, _I64P, _I, _P, _P, _I64, _P, _SZ, _P],
     ),
     "tasft_mask_from_indices": (_I, [_P, _I64, _I64, _I64, _I64, _P, _P, _P]),
+    "tasft_rotary": (
+        _I,
+        [_P, _P, _P, _P, _P, _I, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I64P, _I64P, _I64P, _I64P,
+         _I64P, _I, _I, _F, _I, _P],
+    ),
+    "tasft_rotary_append_paged": (
+        _I,
+        [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64,
+         _I64, _I64, _I64, _I64P, _I64P, _I64P, _I64P, _I64P, _I64P, _I64, _I64, _I, _F, _I, _P],
+    ),
+    "tasft_chunk_workspace_bytes": (_SZ, [_I64, _I64, _I64, _I64]),
+    "tasft_chunk_paged_fwd": (
+        _I,
+        [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _SZ, _I64, _I64, _I64, _I64, _I64, _I64, _I64,
+         _I64, _I64, _I64, _I64, _I64, _I64P, _I64P, _I64P, _I64P, _I64P, _I64, _F, _I, _I, _P],
+    ),
+    "tasft_key_weights": (
+        _I,
+        [_P, _P, _P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64,
+         _I64, _I64, _I64P, _I64P, _I64P, _I64P, _I64P, _I64, _F, _I, _I, _P],
+    ),
+    "tasft_evict_workspace_bytes": (_SZ, [_I64, _I64, _I64]),
+    "tasft_evict_paged": (
+        _I,
+        [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _SZ, _I64, _I64, _I64, _I64, _I64, _I64, _I64,
+         _I64, _I64, _I64P, _I64P, _I64P, _I64P, _I64, _P],
+    ),
 }
 
 
@@ -225,6 +260,14 @@ def stream_handle(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
+def on_device(device: torch.device):
+    """A context in which ``device`` is the current one (nothing where it is already): a kernel is
+    launched on a stream of the current device."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)
+
+
 def kernel_layout(t: torch.Tensor, align: bool = True) -> bool:
     """True if the kernels read ``t`` in place: unit stride on the last dim, the others
     multiples of 8 elements and (with ``align``) a 16-byte aligned base."""
@@ -245,5 +288,5 @@ def check(status: int, what: str, context: dict[str, object] | None = None) -> N
 
 
 __all__ = ["DTYPE_BF16", "DTYPE_F16", "EXPORTED_SYMBOLS", "KERNEL_DTYPES", "LIB_PATH", "check",
-           "dtype_code", "is_available", "kept_strides", "kernel_layout", "load_library", "ptr",
-           "stream_handle", "strides", "strides_array"]
+           "dtype_code", "is_available", "kept_strides", "kernel_layout", "load_library", "on_device",
+           "ptr", "stream_handle", "strides", "strides_array"]

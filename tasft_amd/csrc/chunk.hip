@@ -1,0 +1,874 @@
+// Attention of a chunk of new tokens over a paged cache.
+//
+// Sequence n of a packed batch has kv_len tokens in its pages, the last len of them new:
+// token i of the chunk is at position p = kv_len - len + i and sees keys j <= p (causal), of
+// key blocks its block mask selects if there is one:
+//   o_i = softmax_j(q_i . k_j scale) v_j,   lse_i = log sum_j exp(q_i . k_j scale).
+// A row that sees no key gives 0 and -inf.
+//
+// The rows of one KV head are its chunk's tokens times the query heads of its group: they share
+// K and V, so a workgroup takes a tile of 128 of them, in token order (dense), or 128 positions
+// of one head aligned to the mask's blocks (masked). Four waves own 32 rows each and share
+// 64-key tiles of K and V in LDS, brought by DMA through the page table a tile ahead: two
+// stages, one barrier a tile. S^T = K Q^T with v_mfma_f32_32x32x16, so a lane owns one row: its
+// running maximum and sum stay in the lane (and the one 32 away), and the accumulator of S^T is
+// the B operand of O^T = V^T P^T. P is rounded to the input type for that product (as the MFMA
+// takes it); maxima, sums, O and the log-sum are fp32.
+//
+// Masked scores are -inf before the exponential, and a key past kv_len is never read (its row
+// arrives as zeros). A tile in which only some rows see a key could still carry an infinity or
+// NaN of V into the others as 0 * inf: there V is looked over, and such a tile takes a slow
+// path that adds each key to the rows that see it.
+#include "common.h"
+
+#include "../../include/tasft_amd.h"
+
+namespace tasft {
+
+constexpr int kTile = 64;                // keys per tile
+constexpr float kChunkMove = 8.f;        // a new maximum moves the exp2 reference only if this far above it
+constexpr float kLn2 = 0.69314718055994531f;
+
+struct ChunkParams {
+  const uint16_t* q;
+  const uint16_t* k;
+  const uint16_t* v;
+  uint16_t* o;
+  float* lse;  // [T, Hq] or null
+  const uint8_t* mask;
+  const int32_t* table;
+  const int32_t* kv_lens;
+  const int32_t* cu;
+  float* ws_o;   // [T * Hq][P][D]
+  float* ws_ml;  // [T * Hq][P][2]
+  int64_t sq[2], so[2];  // (token, head)
+  int64_t sk[3], sv[3];  // (page, token, head)
+  int64_t sm[4];         // mask bytes (sequence, head, query block, key block)
+  int64_t bt_stride;
+  int N, T, Hq, Hkv, G, L;
+  int ps_shift, num_pages, cap;  // cap: slots of the table
+  int bs_shift, mask_rows;       // mask blocks of 1 << bs_shift tokens
+  int QT, P;                     // row tiles per sequence and KV head (or head), key splits
+  float scale_log2;
+  int causal;
+};
+
+// A sequence's chunk: its first token, length, cache length and first position.
+struct ChunkSeq {
+  int t0, len, kv, p0;
+};
+
+__device__ __forceinline__ ChunkSeq chunk_seq(const ChunkParams& p, int n) {
+  ChunkSeq s;
+  s.t0 = min(max(p.cu[n], 0), p.T);
+  const int t1 = min(max(p.cu[n + 1], s.t0), p.T);
+  s.len = min(t1 - s.t0, p.L);
+  s.kv = min(max(p.kv_lens[n], 0), p.cap);
+  s.p0 = s.kv - s.len;
+  return s;
+}
+
+// Rows of tokens behind the last sequence: 0 and -inf, shared out over the launch.
+template <int D>
+__device__ __forceinline__ void chunk_zero_tail(const ChunkParams& p, int64_t wg, int64_t wgs, int tid, int threads) {
+  const int end = min(max(p.cu[p.N], 0), p.T);
+  for (int64_t t = end + wg; t < p.T; t += wgs)
+    for (int i = tid; i < p.Hq * (D / 8); i += threads) {
+      const int h = i / (D / 8), c = i % (D / 8);
+      *(u32x4_t*)(p.o + t * p.so[0] + h * p.so[1] + c * 8) = (u32x4_t){0u, 0u, 0u, 0u};
+      if (c == 0 && p.lse) p.lse[t * p.Hq + h] = -INFINITY;
+    }
+}
+
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_rsrc(const uint16_t* base, int rows, int64_t stride, int d) {
+  const int n = rows > 0 ? (int)(((rows - 1) * stride + d) * 2) : 0;
+  return __builtin_amdgcn_make_buffer_rsrc((void*)base, (short)0, n, 0x00020000);
+}
+
+__device__ __forceinline__ void chunk_dma(__amdgpu_buffer_rsrc_t r, uint8_t* dst, int voff) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (TASFT_LDS void*)dst, 16, voff, 0, 0, 0);
+}
+
+__device__ __forceinline__ void chunk_barrier() { asm volatile("s_barrier" ::: "memory"); }
+
+// LDS position of 16-byte chunk cc of row r: K rows are read 32 at a time, V rows transposed.
+template <int D>
+__device__ __forceinline__ int chunk_swz_k(int r, int cc) {
+  return cc ^ (D == 128 ? (r & 15) : ((r >> 1) & 7));
+}
+template <int D>
+__device__ __forceinline__ int chunk_swz_v(int r, int cc) {
+  return cc ^ (D == 128 ? ((r & 3) << 2) : (((r >> 1) & 1) << 2));
+}
+
+// A pair of 16-bit values with infinities and NaN replaced by 0.
+template <int DT>
+__device__ __forceinline__ uint32_t finite2(uint32_t w) {
+  constexpr uint32_t E = DT == kF16 ? 0x7c00u : 0x7f80u;
+  if ((w & E) == E) w &= 0xffff0000u;
+  if ((w & (E << 16)) == (E << 16)) w &= 0xffffu;
+  return w;
+}
+
+// A uniform 32-bit load from read-only memory through the scalar cache.
+typedef const __attribute__((address_space(4))) int32_t* const_i32;
+__device__ __forceinline__ int scalar_load(const int32_t* p) { return *(const_i32)(uintptr_t)p; }
+
+constexpr int kRowWaves = 4;
+constexpr int kRowTile = 32 * kRowWaves;
+constexpr int kRowTileShift = 7;
+static_assert(kRowTile == 1 << kRowTileShift, "row tile");
+
+template <int D, int DT, bool MASKED>
+__global__ void __launch_bounds__(kRowWaves * kWave) __attribute__((amdgpu_waves_per_eu(2, 2)))
+chunk_rows_kernel(const ChunkParams p) {
+  constexpr int KSTEPS = D / 16;
+  constexpr int DTILES = D / 32;
+  constexpr int ROWB = D * 2;
+  constexpr int TILE = kTile * ROWB;
+  constexpr int RPU = 1024 / ROWB;         // rows of a 1 KB DMA unit
+  constexpr int UPW = 16 / RPU;            // units of a wave's 16 rows
+  __shared__ __attribute__((aligned(1024))) uint8_t k0_lds[TILE];
+  __shared__ __attribute__((aligned(1024))) uint8_t v0_lds[TILE];
+  __shared__ __attribute__((aligned(1024))) uint8_t k1_lds[TILE];
+  __shared__ __attribute__((aligned(1024))) uint8_t v1_lds[TILE];
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int col = lane & 31, half = lane >> 5;
+  const int grp16 = lane >> 4, t16 = lane & 15, tr_row = t16 >> 2, tr_cb = t16 & 3;
+
+  chunk_zero_tail<D>(p, blockIdx.x, gridDim.x, tid, kRowWaves * kWave);
+
+  // The (sequence, KV head) whose K and V the workgroup reads, and its place among those that do:
+  // one XCD's L2 serves them all.
+  const int members = p.QT * (MASKED ? p.G : 1) * p.P;
+  int64_t group;
+  int member;
+  xcd_group_map(blockIdx.x, (int64_t)p.N * p.Hkv, members, &group, &member);
+  const int n = (int)(group / p.Hkv), kvh = (int)(group % p.Hkv);
+  const int split = member % p.P;
+  member /= p.P;
+  const int qt = member % p.QT, gm = member / p.QT;
+  const ChunkSeq sq = chunk_seq(p, n);
+  if (sq.len == 0) return;
+
+  // This lane's row (token i of the chunk, head h), the wave's range of tokens and the workgroup's
+  // last token.
+  int i, h, i_first, i_last, i_end;
+  bool row_ok;
+  if constexpr (MASKED) {
+    // Positions aligned to the row tile: a wave's 32 rows lie in one mask block.
+    const int base = ((sq.p0 >> kRowTileShift) << kRowTileShift) + qt * kRowTile - sq.p0;
+    if (base >= sq.len) return;
+    i_first = max(base + wave * 32, 0);
+    i_last = min(base + wave * 32 + 31, sq.len - 1);
+    i_end = min(base + kRowTile, sq.len) - 1;
+    i = base + wave * 32 + col;
+    h = kvh * p.G + gm;
+    row_ok = i >= 0 && i < sq.len;
+  } else {
+    const int rows = sq.len * p.G, r0 = qt * kRowTile;
+    if (r0 >= rows) return;
+    const int rw = r0 + wave * 32, r = rw + col;
+    i = r / p.G;
+    h = kvh * p.G + (r - i * p.G);
+    row_ok = r < rows;
+    i_first = rw / p.G;
+    i_last = rw < rows ? min(rw + 31, rows - 1) / p.G : -1;
+    i_end = (min(r0 + kRowTile, rows) - 1) / p.G;
+  }
+  const bool wave_on = i_first <= i_last;
+  if (!row_ok) {  // reads a row of the chunk, is not stored
+    i = min(max(i, 0), sq.len - 1);
+    h = kvh * p.G;
+  }
+  // Keys a row sees: 0 .. lim. All rows of the wave see the keys to all_see, none one past any_see.
+  const int lim = p.causal ? min(sq.p0 + i, sq.kv - 1) : sq.kv - 1;
+  const int all_see = p.causal ? min(sq.p0 + i_first, sq.kv - 1) : sq.kv - 1;
+  const int any_see = !wave_on ? -1 : (p.causal ? min(sq.p0 + i_last, sq.kv - 1) : sq.kv - 1);
+  const int wg_see = p.causal ? min(sq.p0 + i_end, sq.kv - 1) : sq.kv - 1;
+  const int tiles = wg_see < 0 ? 0 : wg_see / kTile + 1;
+  const int tile_a = (int)((int64_t)split * tiles / p.P), tile_b = (int)((int64_t)(split + 1) * tiles / p.P);
+
+  // Q as the B operand, lane (col, half): dims 16 ks + 8 half .. + 7 of its row.
+  u32x4_t qf[KSTEPS];
+  {
+    const uint16_t* qr = p.q + (int64_t)(sq.t0 + i) * p.sq[0] + h * p.sq[1] + half * 8;
+#pragma unroll
+    for (int ks = 0; ks < KSTEPS; ++ks) qf[ks] = *(const u32x4_t*)(qr + ks * 16);
+  }
+
+  // The tiles of the split in order; masked: those that any row's block mask selects, with this
+  // wave's own two bits (the 32-key halves, which differ at mask blocks of 32 only).
+  int cursor = tile_a, chunk = tile_a - kWave, own_next = 0;
+  uint64_t ubits = 0, own0 = 0, own1 = 0;
+  const uint8_t* mseq = nullptr;
+  int row_lo = 0, row_hi = 0, row_own = 0;
+  if constexpr (MASKED) {
+    mseq = p.mask + n * p.sm[0] + (int64_t)(kvh * p.G + gm) * p.sm[1];
+    const int block0 = sq.p0 >> p.bs_shift;
+    auto row_of = [&](int j) { return min(max(((sq.p0 + j) >> p.bs_shift) - block0, 0), p.mask_rows - 1); };
+    row_lo = row_of(max(((sq.p0 >> kRowTileShift) << kRowTileShift) + qt * kRowTile - sq.p0, 0));
+    row_hi = row_of(i_end);
+    row_own = wave_on ? row_of(i_first) : -1;
+  }
+  auto next_tile = [&]() -> int {
+    if constexpr (!MASKED) {
+      return cursor < tile_b ? cursor++ : -1;
+    } else {
+      while (ubits == 0) {
+        chunk += kWave;
+        if (chunk >= tile_b) return -1;
+        const int kt = min(chunk + lane, tile_b - 1);
+        const int b0 = p.bs_shift == 5 ? 2 * kt : kt >> (p.bs_shift - 6);
+        const int b1 = p.bs_shift == 5 ? min(2 * kt + 1, (p.cap - 1) >> 5) : b0;
+        uint32_t any = 0, mine0 = 0, mine1 = 0;
+        for (int r = row_lo; r <= row_hi; ++r) {
+          const uint32_t x = mseq[r * p.sm[2] + b0 * p.sm[3]], y = mseq[r * p.sm[2] + b1 * p.sm[3]];
+          any |= x | y;
+          if (r == row_own) mine0 = x, mine1 = y;
+        }
+        ubits = __ballot(any != 0 && chunk + lane < tile_b);
+        own0 = __ballot(mine0 != 0);
+        own1 = __ballot(mine1 != 0);
+      }
+      const int b = __builtin_ctzll(ubits);
+      ubits &= ubits - 1;
+      own_next = (int)((own0 >> b) & 1) | (int)((own1 >> b) & 1) << 1;
+      return chunk + b;
+    }
+  };
+
+  // A wave brings rows 16 wave .. +15 of a tile, eight rows (one page at least) per buffer
+  // resource, which ends with the last row below kv_len: rows past it arrive as zeros. Per-lane
+  // source offsets: the lane loads the chunk that the self-inverse swizzle maps to its 16 bytes.
+  const uint16_t* kbase = p.k + kvh * p.sk[2];
+  const uint16_t* vbase = p.v + kvh * p.sv[2];
+  const int32_t* table = p.table + n * p.bt_stride;
+  int koff[UPW], voff[UPW];
+#pragma unroll
+  for (int u = 0; u < UPW; ++u) {
+    const int r8 = (u * RPU + lane / (ROWB / 16)) & 7, pos = lane % (ROWB / 16);
+    const int row = wave * 16 + u * RPU + lane / (ROWB / 16);
+    koff[u] = (r8 * (int)p.sk[1] + chunk_swz_k<D>(row, pos) * 8) * 2;
+    voff[u] = (r8 * (int)p.sv[1] + chunk_swz_v<D>(row, pos) * 8) * 2;
+  }
+  struct Pages {
+    int a, b;
+  };
+  auto load_pages = [&](int kt) -> Pages {
+    const int r = kt * kTile + wave * 16, last = (sq.kv - 1) >> p.ps_shift;
+    return {scalar_load(table + min(r >> p.ps_shift, last)), scalar_load(table + min((r + 8) >> p.ps_shift, last))};
+  };
+  auto dma_tile = [&](uint8_t* kt_lds, uint8_t* vt_lds, int kt, Pages pg) {
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int r = kt * kTile + wave * 16 + 8 * e;
+      const int64_t page = min(max(e ? pg.b : pg.a, 0), p.num_pages - 1);
+      const int in_page = r & ((1 << p.ps_shift) - 1), rows = min(sq.kv - r, 8);
+      const __amdgpu_buffer_rsrc_t kr = rows_rsrc(kbase + page * p.sk[0] + in_page * p.sk[1], rows, p.sk[1], D);
+      const __amdgpu_buffer_rsrc_t vr = rows_rsrc(vbase + page * p.sv[0] + in_page * p.sv[1], rows, p.sv[1], D);
+#pragma unroll
+      for (int u = e * (UPW / 2); u < (e + 1) * (UPW / 2); ++u) {
+        chunk_dma(kr, kt_lds + (wave * UPW + u) * 1024, koff[u]);
+        chunk_dma(vr, vt_lds + (wave * UPW + u) * 1024, voff[u]);
+      }
+    }
+  };
+
+  f32x16_t oacc[DTILES];
+#pragma unroll
+  for (int dt = 0; dt < DTILES; ++dt) oacc[dt] = (f32x16_t){};
+  float m_ref = -INFINITY;  // exp2 reference of this lane's row (log2 domain)
+  float l_run = 0.f;
+  int fix_from = 0x7fffffff;  // first tile whose infinities or NaN of V were left out
+
+  auto compute = [&](const uint8_t* kS, const uint8_t* vS, int kt, int own) {
+    const int key0 = kt * kTile;
+    if (key0 > any_see || (MASKED && own == 0)) return;
+    u32x4_t kf[2][KSTEPS];
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int ks = 0; ks < KSTEPS; ++ks) {
+        const int r = t * 32 + col;
+        kf[t][ks] = *(const u32x4_t*)(kS + r * ROWB + chunk_swz_k<D>(r, ks * 2 + half) * 16);
+      }
+    f32x16_t s0 = (f32x16_t){}, s1 = (f32x16_t){};
+#pragma unroll
+    for (int ks = 0; ks < KSTEPS; ++ks) {
+      s0 = mfma16<DT>(kf[0][ks], qf[ks], s0);
+      s1 = mfma16<DT>(kf[1][ks], qf[ks], s1);
+    }
+    // Register rr of s0 / s1 is key 4 half + off(rr) (+ 32), off = 8 (rr / 4) + rr % 4.
+    const bool mixed = key0 + kTile - 1 > all_see || (MASKED && own != 3);
+    const int lim0 = MASKED && !(own & 1) ? -1 : lim - key0 - 4 * half;
+    const int lim1 = MASKED && !(own & 2) ? -1 : lim - key0 - 4 * half - 32;
+    if (mixed) {
+#pragma unroll
+      for (int rr = 0; rr < 16; ++rr) {
+        const int off = 8 * (rr >> 2) + (rr & 3);
+        s0[rr] = off > lim0 ? -INFINITY : s0[rr];
+        s1[rr] = off > lim1 ? -INFINITY : s1[rr];
+      }
+    }
+    float ma = fmaxf(fmaxf(s0[0], s0[1]), s0[2]), mb = fmaxf(fmaxf(s1[0], s1[1]), s1[2]);
+#pragma unroll
+    for (int rr = 3; rr < 15; rr += 2) {
+      ma = fmaxf(fmaxf(ma, s0[rr]), s0[rr + 1]);
+      mb = fmaxf(fmaxf(mb, s1[rr]), s1[rr + 1]);
+    }
+    const float mloc = pair_max32(fmaxf(fmaxf(ma, s0[15]), fmaxf(mb, s1[15]))) * p.scale_log2;
+    const bool move = mloc > m_ref + kChunkMove;
+    if (__ballot(move)) {
+      const float alpha = move ? __builtin_amdgcn_exp2f(m_ref - mloc) : 1.f;
+      l_run *= alpha;
+#pragma unroll
+      for (int dt = 0; dt < DTILES; ++dt) oacc[dt] *= alpha;
+      m_ref = move ? mloc : m_ref;
+    }
+    const float m_use = (m_ref == -INFINITY) ? 0.f : m_ref;
+    float lsum0 = 0.f, lsum1 = 0.f;
+#pragma unroll
+    for (int rr = 0; rr < 16; ++rr) {
+      const float e0 = __builtin_amdgcn_exp2f(fmaf(s0[rr], p.scale_log2, -m_use));
+      const float e1 = __builtin_amdgcn_exp2f(fmaf(s1[rr], p.scale_log2, -m_use));
+      s0[rr] = e0;
+      s1[rr] = e1;
+      lsum0 += e0;
+      lsum1 += e1;
+    }
+    l_run += lsum0 + lsum1;
+    u32x4_t pb[4];
+#pragma unroll
+    for (int pp = 0; pp < 4; ++pp) {
+      const f32x16_t& sv = (pp < 2) ? s0 : s1;
+      const int o = 8 * (pp & 1);
+      pb[pp] = (u32x4_t){pack16x2<DT>(sv[o + 0], sv[o + 1]), pack16x2<DT>(sv[o + 2], sv[o + 3]),
+                         pack16x2<DT>(sv[o + 4], sv[o + 5]), pack16x2<DT>(sv[o + 6], sv[o + 7])};
+    }
+    u32x2_t vlo[4][DTILES], vhi[4][DTILES];
+#pragma unroll
+    for (int pp = 0; pp < 4; ++pp) {
+      const int kk = 16 * pp + 4 * (grp16 >> 1);
+#pragma unroll
+      for (int dt = 0; dt < DTILES; ++dt) {
+        const int d0 = dt * 32 + 16 * (grp16 & 1) + 4 * tr_cb;
+        const int cc = d0 >> 3, sub = (d0 & 7) * 2;
+        const int r1 = kk + tr_row, r2 = r1 + 8;
+        vlo[pp][dt] = ds_read_tr16_b64((const void*)(vS + r1 * ROWB + chunk_swz_v<D>(r1, cc) * 16 + sub));
+        vhi[pp][dt] = ds_read_tr16_b64((const void*)(vS + r2 * ROWB + chunk_swz_v<D>(r2, cc) * 16 + sub));
+      }
+    }
+    if (mixed) {
+      bool bad = false;
+#pragma unroll
+      for (int pp = 0; pp < 4; ++pp)
+#pragma unroll
+        for (int dt = 0; dt < DTILES; ++dt)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const uint32_t a = vlo[pp][dt][j], b = vhi[pp][dt][j];
+            vlo[pp][dt][j] = finite2<DT>(a);
+            vhi[pp][dt][j] = finite2<DT>(b);
+            bad = bad || ((vlo[pp][dt][j] ^ a) | (vhi[pp][dt][j] ^ b)) != 0u;
+          }
+      if (__ballot(bad)) fix_from = min(fix_from, kt);
+    }
+#pragma unroll
+    for (int pp = 0; pp < 4; ++pp)
+#pragma unroll
+      for (int dt = 0; dt < DTILES; ++dt) {
+        const u32x4_t a = {vlo[pp][dt][0], vlo[pp][dt][1], vhi[pp][dt][0], vhi[pp][dt][1]};
+        oacc[dt] = mfma16<DT>(a, pb[pp], oacc[dt]);
+      }
+  };
+
+  int cur = next_tile(), own_cur = own_next;
+  int nxt = -1, own_nxt = 0;
+  Pages pg = {0, 0};
+  if (cur >= 0) {
+    dma_tile(k0_lds, v0_lds, cur, load_pages(cur));
+    nxt = next_tile();
+    own_nxt = own_next;
+    if (nxt >= 0) pg = load_pages(nxt);
+  }
+  // One tile from a stage while the next one's DMA fills the other: by the barrier every wave's
+  // share of this tile has landed and every wave is done with the tile before it.
+  auto step = [&](uint8_t* ka, uint8_t* va, uint8_t* kb, uint8_t* vb) {
+    __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0)
+    chunk_barrier();
+    int nn = -1;
+    Pages pn = pg;
+    if (nxt >= 0) {
+      dma_tile(kb, vb, nxt, pg);
+      nn = next_tile();
+      if (nn >= 0) pn = load_pages(nn);
+    }
+    compute(ka, va, cur, own_cur);
+    cur = nxt;
+    own_cur = own_nxt;
+    nxt = nn;
+    own_nxt = own_next;
+    pg = pn;
+  };
+  while (cur >= 0) {
+    step(k0_lds, v0_lds, k1_lds, v1_lds);
+    if (cur < 0) break;
+    step(k1_lds, v1_lds, k0_lds, v0_lds);
+  }
+
+  if (fix_from != 0x7fffffff) {
+    // Infinities and NaN of V in tiles that only some of the wave's rows see: key by key, from
+    // memory, to the rows that see the key. (Where a later tile had them in its product, once
+    // more changes nothing.)
+    const float m_use = (m_ref == -INFINITY) ? 0.f : m_ref;
+    const int last = min(any_see, tile_b * kTile - 1);
+#pragma nounroll
+    for (int key = fix_from * kTile; key <= last; ++key) {
+      const int64_t page = min(max(table[key >> p.ps_shift], 0), p.num_pages - 1);
+      const int in_page = key & ((1 << p.ps_shift) - 1);
+      const uint16_t* vr = vbase + page * p.sv[0] + in_page * p.sv[1];
+      const uint32_t w = *(const uint32_t*)(vr + (lane * 2) % D);
+      if (!__ballot(finite2<DT>(w) != w)) continue;
+      bool sees = row_ok && key <= lim;
+      if constexpr (MASKED) {
+        const uint8_t* m = mseq + row_own * p.sm[2];
+        sees = sees && m[(key >> p.bs_shift) * p.sm[3]] != 0;
+      }
+      const uint16_t* kr = kbase + page * p.sk[0] + in_page * p.sk[1] + half * 8;
+      float dot = 0.f;
+#pragma unroll
+      for (int ks = 0; ks < KSTEPS; ++ks) {
+        float x[8], y[8];
+        unpack16x8<DT>(*(const u32x4_t*)(kr + ks * 16), x);
+        unpack16x8<DT>(qf[ks], y);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) dot = fmaf(x[j], y[j], dot);
+      }
+      const float pk = __builtin_amdgcn_exp2f(fmaf(pair_sum32(dot), p.scale_log2, -m_use));
+#pragma unroll
+      for (int dt = 0; dt < DTILES; ++dt)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const uint32_t x = vr[dt * 32 + 8 * (e >> 2) + 4 * half + (e & 3)];
+          oacc[dt][e] += sees && finite2<DT>(x) != x ? pk * bits16_to_f32<DT>(x) : 0.f;
+        }
+    }
+  }
+
+  const float l_tot = pair_sum32(l_run);
+  const int64_t tok = sq.t0 + i;
+  if (p.P > 1) {
+    const int64_t row = (tok * p.Hq + h) * p.P + split;
+    if (row_ok) {
+      if (half == 0) {
+        p.ws_ml[row * 2] = m_ref;
+        p.ws_ml[row * 2 + 1] = l_tot;
+      }
+      float* wo = p.ws_o + row * D;
+#pragma unroll
+      for (int dt = 0; dt < DTILES; ++dt)
+#pragma unroll
+        for (int gq = 0; gq < 4; ++gq)
+          *(f32x4_t*)(wo + dt * 32 + 8 * gq + 4 * half) =
+              (f32x4_t){oacc[dt][4 * gq], oacc[dt][4 * gq + 1], oacc[dt][4 * gq + 2], oacc[dt][4 * gq + 3]};
+    }
+    return;
+  }
+  if (p.lse && row_ok && half == 0) p.lse[tok * p.Hq + h] = (m_ref + __builtin_amdgcn_logf(l_tot)) * kLn2;
+  const float inv = 1.f / (l_tot > 0.f ? l_tot : 1.f);  // empty rows: 0; NaN rows stay NaN
+  // Whole rows through LDS: 16-byte chunk c of row r at position c ^ (r % chunks).
+  __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
+  chunk_barrier();                     // every wave is done with the tiles
+  uint8_t* ost = ((wave & 2) ? v0_lds : k0_lds) + (wave & 1) * (32 * ROWB);
+  constexpr int CPR = ROWB / 16;
+#pragma unroll
+  for (int dt = 0; dt < DTILES; ++dt)
+#pragma unroll
+    for (int gq = 0; gq < 4; ++gq) {
+      const int d0 = dt * 32 + 8 * gq + 4 * half;
+      const u32x2_t w = {pack16x2<DT>(oacc[dt][4 * gq + 0] * inv, oacc[dt][4 * gq + 1] * inv),
+                         pack16x2<DT>(oacc[dt][4 * gq + 2] * inv, oacc[dt][4 * gq + 3] * inv)};
+      *(u32x2_t*)(ost + col * ROWB + (((d0 >> 3) ^ (col & (CPR - 1))) << 4) + (d0 & 7) * 2) = w;
+    }
+  const int64_t at = row_ok ? tok * p.so[0] + h * p.so[1] : -1;
+#pragma unroll
+  for (int j = 0; j < 32 * CPR / kWave; ++j) {
+    const int r = j * (kWave / CPR) + lane / CPR, c = lane % CPR;
+    const u32x4_t x = *(const u32x4_t*)(ost + r * ROWB + ((c ^ (r & (CPR - 1))) << 4));
+    const int64_t to = __shfl(at, r, kWave);
+    if (to >= 0) *(u32x4_t*)(p.o + to + c * 8) = x;
+  }
+}
+
+// Joins the P splits of every row: D / 4 lanes a row, the partial sums of splits that saw no key
+// are not read (they may be unwritten).
+template <int D, int DT>
+__global__ void __launch_bounds__(256) chunk_combine_kernel(const ChunkParams p) {
+  constexpr int LPR = D / 4;
+  const int64_t row = (int64_t)blockIdx.x * (256 / LPR) + threadIdx.x / LPR;
+  const int c = threadIdx.x % LPR;
+  const int64_t t = row / p.Hq;
+  const int h = (int)(row - t * p.Hq);
+  if (t >= min(max(p.cu[p.N], 0), p.T)) return;
+  const float* ml = p.ws_ml + row * p.P * 2;
+  const float* os = p.ws_o + row * p.P * D + c * 4;
+  float M = -INFINITY;
+  for (int s = 0; s < p.P; ++s) M = fmaxf(M, ml[2 * s]);
+  const float Mu = (M == -INFINITY) ? 0.f : M;
+  float L = 0.f;
+  f32x4_t O = {0.f, 0.f, 0.f, 0.f};
+  for (int s = 0; s < p.P; ++s) {
+    const float l = ml[2 * s + 1];
+    if (__float_as_uint(l) == 0u) continue;
+    const float f = __builtin_amdgcn_exp2f(ml[2 * s] - Mu);
+    const f32x4_t x = *(const f32x4_t*)(os + (int64_t)s * D);
+    L += l * f;
+    O += x * f;
+  }
+  const float inv = 1.f / (L > 0.f ? L : 1.f);
+  const u32x2_t w = {pack16x2<DT>(O[0] * inv, O[1] * inv), pack16x2<DT>(O[2] * inv, O[3] * inv)};
+  *(u32x2_t*)(p.o + t * p.so[0] + h * p.so[1] + c * 4) = w;
+  if (p.lse && c == 0) p.lse[row] = (M + __builtin_amdgcn_logf(L)) * kLn2;
+}
+
+// ---------------------------------------------------------------------------------------
+// Accumulated key weights: out[n, g, j] = in[n, g, j] + sum over the chunk's rows that see key j
+// of exp(q . k_j scale - lse). The transpose of the attention's reduction: a wave keeps 64 keys
+// (their K in registers as the A operand) and walks the rows 32 at a time (Q as the B operand,
+// from L2), adding exp2 of the scores to one register per key; lanes are summed once at the end.
+// KW of the four waves hold different keys, 4 / KW share out the rows of the same: many keys want
+// few readings of Q (KW = 4), few keys want many workgroups (KW = 1). Fixed order, no atomics.
+// ---------------------------------------------------------------------------------------
+struct WeightParams {
+  ChunkParams c;
+  const float* scores;  // [N, Hkv, cap] (element strides ss) or null
+  int64_t ss[3];
+  float* out;           // [N, Hkv, cap] contiguous
+  const float* lse;     // [T, Hq], strides (token, head)
+  int64_t sl[2];
+};
+
+template <int D, int DT, int KW, bool MASKED>
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2)))
+chunk_weights_kernel(const WeightParams wp) {
+  constexpr int KSTEPS = D / 16;
+  constexpr int ROWB = D * 2;
+  constexpr int RPU = 1024 / ROWB;
+  constexpr int RW = 4 / KW;               // waves that share one set of keys
+  constexpr int ROWS = kTile / RW;         // K rows a wave brings
+  constexpr int TILE = kTile * ROWB;
+  const ChunkParams& p = wp.c;
+  constexpr int RED = 4 * 32 * kWave * 4;  // the sums of every wave, once K is in registers
+  __shared__ __attribute__((aligned(1024))) uint8_t k_lds[KW * TILE > RED ? KW * TILE : RED];
+  float(*red)[32][kWave] = (float(*)[32][kWave])k_lds;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int kg = wave % KW, rg = wave / KW;
+  const int col = lane & 31, half = lane >> 5;
+  const int per = (p.cap + KW * kTile - 1) / (KW * kTile);  // workgroups per (sequence, KV head)
+  int64_t group;
+  int member;
+  xcd_group_map(blockIdx.x, (int64_t)p.N * p.Hkv, per, &group, &member);
+  const int n = (int)(group / p.Hkv), kvh = (int)(group % p.Hkv);
+  const ChunkSeq sq = chunk_seq(p, n);
+  const int key0 = (member * KW + kg) * kTile;
+  const int wg0 = member * KW * kTile;
+
+  float total = 0.f;  // of key key0 + lane, in the first wave of its keys
+  if (wg0 < sq.kv && sq.len > 0) {
+    uint8_t* kS = k_lds + kg * TILE;
+    {
+      const uint16_t* kbase = p.k + kvh * p.sk[2];
+      const int32_t* table = p.table + n * p.bt_stride;
+      const int last = (sq.kv - 1) >> p.ps_shift;
+#pragma unroll
+      for (int e = 0; e < ROWS / 8; ++e) {
+        const int r0 = rg * ROWS + 8 * e, r = key0 + r0;
+        const int64_t page = min(max(scalar_load(table + min(r >> p.ps_shift, last)), 0), p.num_pages - 1);
+        const int in_page = r & ((1 << p.ps_shift) - 1);
+        const __amdgpu_buffer_rsrc_t kr =
+            rows_rsrc(kbase + page * p.sk[0] + in_page * p.sk[1], min(sq.kv - r, 8), p.sk[1], D);
+#pragma unroll
+        for (int u = 0; u < 8 / RPU; ++u) {
+          const int r8 = u * RPU + lane / (ROWB / 16), row = r0 + r8;
+          chunk_dma(kr, kS + r0 * ROWB + u * 1024,
+                    (r8 * (int)p.sk[1] + chunk_swz_k<D>(row, lane % (ROWB / 16)) * 8) * 2);
+        }
+      }
+    }
+    __builtin_amdgcn_s_waitcnt(0x0070);
+    chunk_barrier();
+    u32x4_t kf[2][KSTEPS];
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int ks = 0; ks < KSTEPS; ++ks) {
+        const int r = t * 32 + col;
+        kf[t][ks] = *(const u32x4_t*)(kS + r * ROWB + chunk_swz_k<D>(r, ks * 2 + half) * 16);
+      }
+    f32x16_t a0 = (f32x16_t){}, a1 = (f32x16_t){};
+    const int rows = sq.len * p.G;
+    // The first row that sees this wave's first key.
+    const int first = p.causal ? max(key0 - sq.p0, 0) : 0;
+    const int block0 = sq.p0 >> (MASKED ? p.bs_shift : 0);
+    const int r_first = key0 >= sq.kv ? rows : (int)min((int64_t)first * p.G, (int64_t)rows);
+    for (int r0 = (r_first / 32 + rg) * 32; r0 < rows; r0 += 32 * RW) {
+      const int r = min(r0 + col, rows - 1), i = r / p.G, h = kvh * p.G + (r - i * p.G);
+      const int64_t tok = sq.t0 + i;
+      const uint16_t* qr = p.q + tok * p.sq[0] + h * p.sq[1] + half * 8;
+      u32x4_t qf[KSTEPS];
+#pragma unroll
+      for (int ks = 0; ks < KSTEPS; ++ks) qf[ks] = *(const u32x4_t*)(qr + ks * 16);
+      const float lse = wp.lse[tok * wp.sl[0] + h * wp.sl[1]];
+      const int lim = p.causal ? min(sq.p0 + i, sq.kv - 1) : sq.kv - 1;
+      // A row without keys (lse -inf) or behind the last one adds nothing.
+      const bool on = r0 + col < rows && lse != -INFINITY;
+      int lim0 = on ? lim - key0 - 4 * half : -1, lim1 = lim0 < 0 ? -1 : lim0 - 32;
+      if constexpr (MASKED) {
+        const int mr = min(max(((sq.p0 + i) >> p.bs_shift) - block0, 0), p.mask_rows - 1);
+        const uint8_t* m = p.mask + n * p.sm[0] + h * p.sm[1] + mr * p.sm[2];
+        const int last_block = (p.cap - 1) >> p.bs_shift;
+        const bool m0 = m[min(key0 >> p.bs_shift, last_block) * p.sm[3]] != 0;
+        const bool m1 = m[min((key0 + 32) >> p.bs_shift, last_block) * p.sm[3]] != 0;
+        if (!m0) lim0 = -1;
+        if (!m1) lim1 = -1;
+      }
+      f32x16_t s0 = (f32x16_t){}, s1 = (f32x16_t){};
+#pragma unroll
+      for (int ks = 0; ks < KSTEPS; ++ks) {
+        s0 = mfma16<DT>(kf[0][ks], qf[ks], s0);
+        s1 = mfma16<DT>(kf[1][ks], qf[ks], s1);
+      }
+      const float l2 = lse * kLog2e;
+#pragma unroll
+      for (int rr = 0; rr < 16; ++rr) {
+        const int off = 8 * (rr >> 2) + (rr & 3);
+        const float e0 = __builtin_amdgcn_exp2f(fmaf(s0[rr], p.scale_log2, -l2));
+        const float e1 = __builtin_amdgcn_exp2f(fmaf(s1[rr], p.scale_log2, -l2));
+        a0[rr] += off > lim0 ? 0.f : e0;
+        a1[rr] += off > lim1 ? 0.f : e1;
+      }
+    }
+    __syncthreads();  // every wave has its K
+#pragma unroll
+    for (int rr = 0; rr < 16; ++rr) {
+      red[wave][rr][lane] = a0[rr];
+      red[wave][16 + rr][lane] = a1[rr];
+    }
+    __syncthreads();
+    if (rg == 0) {
+      // Key lane: tile lane / 32, half (lane / 4) % 2, register of the rest. The columns start
+      // at the lane's own, so that lanes read different banks.
+      const int k32 = lane & 31, hh = (k32 >> 2) & 1, reg = (lane >> 5) * 16 + (k32 >> 3) * 4 + (k32 & 3);
+#pragma unroll
+      for (int w = 0; w < RW; ++w)
+        for (int j = 0; j < 32; ++j) total += red[w * KW + kg][reg][hh * 32 + ((j + lane) & 31)];
+    }
+  }
+  const int key = key0 + lane;
+  if (rg == 0 && key < p.cap) {
+    const float before = wp.scores ? wp.scores[n * wp.ss[0] + kvh * wp.ss[1] + key * wp.ss[2]] : 0.f;
+    wp.out[((int64_t)n * p.Hkv + kvh) * p.cap + key] = key < sq.kv ? before + total : before;
+  }
+}
+
+}  // namespace tasft
+
+using namespace tasft;
+
+// Checks shared by both entry points; fills the parameters that they share.
+static int chunk_params(ChunkParams& p, const char* what, const void* q, const void* k_pages, const uint8_t* mask,
+                        const int32_t* table, const int32_t* kv_lens, const int32_t* cu, int64_t num_seqs,
+                        int64_t tokens, int64_t num_q_heads, int64_t num_kv_heads, int64_t max_seqlen,
+                        int64_t head_dim, int64_t block_size, int64_t mask_rows, int64_t page_size,
+                        int64_t num_pages, int64_t max_pages, const int64_t* q_strides, const int64_t* kp_strides,
+                        const int64_t* mask_strides, int64_t bt_stride, float scale, int causal, int dtype) {
+  if (!q || !k_pages || !table || !kv_lens || !cu || !q_strides || !kp_strides || (mask && !mask_strides))
+    return set_error(kErrInvalidArgument, "%s: null pointer argument", what);
+  if (dtype != kBf16 && dtype != kF16)
+    return set_error(kErrUnsupported, "%s: dtype must be bf16 (0) or fp16 (1), got %d", what, dtype);
+  if (num_seqs <= 0 || tokens <= 0 || num_q_heads <= 0 || num_kv_heads <= 0 || max_seqlen <= 0 || num_pages <= 0 ||
+      max_pages <= 0 || (mask && mask_rows <= 0))
+    return set_error(kErrInvalidArgument, "%s: sizes must be positive", what);
+  if (num_q_heads % num_kv_heads != 0)
+    return set_error(kErrInvalidArgument, "%s: num_q_heads must be a multiple of num_kv_heads", what);
+  if (head_dim != 64 && head_dim != 128)
+    return set_error(kErrUnsupported, "%s: head_dim must be 64 or 128, got %lld", what, (long long)head_dim);
+  if (mask && block_size != 32 && block_size != 64 && block_size != 128)
+    return set_error(kErrUnsupported, "%s: block_size must be 32, 64 or 128, got %lld", what, (long long)block_size);
+  if (page_size < 8 || (page_size & (page_size - 1)))
+    return set_error(kErrUnsupported, "%s: page_size must be a power of two >= 8, got %lld", what,
+                     (long long)page_size);
+  if (!(scale > 0.f)) return set_error(kErrInvalidArgument, "%s: scale must be positive", what);
+  const int64_t lim = 0x7fffffff;
+  if (num_seqs > lim - 1 || tokens > lim || num_pages > lim || page_size > lim || max_pages > lim ||
+      max_pages * page_size > lim - 255 || tokens * (num_q_heads / num_kv_heads) > lim - 255 || mask_rows > lim ||
+      num_q_heads > 65535)
+    return set_error(kErrUnsupported, "%s: sizes exceed 32 bits", what);
+  if (!strides_nonneg(q_strides, 3) || !strides_nonneg(kp_strides, 4) || bt_stride < 0 ||
+      (mask && !strides_nonneg(mask_strides, 4)))
+    return set_error(kErrInvalidArgument, "%s: strides must be non-negative", what);
+  if (q_strides[2] != 1 || kp_strides[3] != 1)
+    return set_error(kErrInvalidArgument, "%s: head dims must be contiguous", what);
+  if ((q_strides[0] & 7) || (q_strides[1] & 7) || (kp_strides[0] & 7) || (kp_strides[1] & 7) ||
+      (kp_strides[2] & 7) || ((uintptr_t)q & 15) || ((uintptr_t)k_pages & 15))
+    return set_error(kErrInvalidArgument, "%s: strides must be multiples of 8 on 16-byte aligned bases", what);
+  if (kp_strides[1] >= (int64_t)1 << 26)
+    return set_error(kErrUnsupported, "%s: token stride of the pools too large", what);
+  p.q = (const uint16_t*)q;
+  p.k = (const uint16_t*)k_pages;
+  p.mask = mask;
+  p.table = table;
+  p.kv_lens = kv_lens;
+  p.cu = cu;
+  p.sq[0] = q_strides[0];
+  p.sq[1] = q_strides[1];
+  for (int i = 0; i < 3; ++i) p.sk[i] = kp_strides[i];
+  if (mask)
+    for (int i = 0; i < 4; ++i) p.sm[i] = mask_strides[i];
+  p.bt_stride = bt_stride;
+  p.N = (int)num_seqs;
+  p.T = (int)tokens;
+  p.Hq = (int)num_q_heads;
+  p.Hkv = (int)num_kv_heads;
+  p.G = (int)(num_q_heads / num_kv_heads);
+  p.L = (int)(max_seqlen < tokens ? max_seqlen : tokens);
+  p.ps_shift = __builtin_ctzll((unsigned long long)page_size);
+  p.num_pages = (int)num_pages;
+  p.cap = (int)(max_pages * page_size);
+  p.bs_shift = mask ? __builtin_ctzll((unsigned long long)block_size) : 6;
+  p.mask_rows = (int)mask_rows;
+  p.scale_log2 = scale * kLog2e;
+  p.causal = causal;
+  p.P = 1;
+  return kOk;
+}
+
+extern "C" size_t tasft_chunk_workspace_bytes(int64_t tokens, int64_t num_q_heads, int64_t head_dim,
+                                              int64_t num_splits) {
+  if (tokens <= 0 || num_q_heads <= 0 || head_dim <= 0 || num_splits <= 1) return 0;
+  return (size_t)(tokens * num_q_heads * num_splits) * (size_t)(head_dim + 2) * sizeof(float);
+}
+
+template <int D, int DT>
+static int launch_chunk(const ChunkParams& p, int64_t grid, hipStream_t stream) {
+  const dim3 g((unsigned)grid), b(kRowWaves * kWave);
+  if (p.mask)
+    hipLaunchKernelGGL((chunk_rows_kernel<D, DT, true>), g, b, 0, stream, p);
+  else
+    hipLaunchKernelGGL((chunk_rows_kernel<D, DT, false>), g, b, 0, stream, p);
+  if (const int rc = check_launch("chunk attention")) return rc;
+  if (p.P == 1) return kOk;
+  constexpr int RPW = 256 / (D / 4);
+  const int64_t rows = (int64_t)p.T * p.Hq;
+  hipLaunchKernelGGL((chunk_combine_kernel<D, DT>), dim3((unsigned)((rows + RPW - 1) / RPW)), dim3(256), 0, stream, p);
+  return check_launch("chunk combine");
+}
+
+extern "C" int tasft_chunk_paged_fwd(
+    const void* q, const void* k_pages, const void* v_pages, void* out, float* lse, const uint8_t* block_mask,
+    const int32_t* block_table, const int32_t* kv_lens, const int32_t* cu_seqlens, void* workspace,
+    size_t workspace_bytes, int64_t num_seqs, int64_t tokens, int64_t num_q_heads, int64_t num_kv_heads,
+    int64_t max_seqlen, int64_t head_dim, int64_t block_size, int64_t mask_rows, int64_t page_size,
+    int64_t num_pages, int64_t max_pages, int64_t num_splits, const int64_t* q_strides, const int64_t* kp_strides,
+    const int64_t* vp_strides, const int64_t* o_strides, const int64_t* mask_strides, int64_t block_table_stride,
+    float scale, int causal, int dtype, void* stream) {
+  const char* what = "chunk attention";
+  ChunkParams p = {};
+  if (!v_pages || !out || !vp_strides || !o_strides)
+    return set_error(kErrInvalidArgument, "chunk attention: null pointer argument");
+  if (const int rc = chunk_params(p, what, q, k_pages, block_mask, block_table, kv_lens, cu_seqlens, num_seqs, tokens,
+                                  num_q_heads, num_kv_heads, max_seqlen, head_dim, block_size, mask_rows, page_size,
+                                  num_pages, max_pages, q_strides, kp_strides, mask_strides, block_table_stride,
+                                  scale, causal, dtype))
+    return rc;
+  if (!strides_nonneg(vp_strides, 4) || !strides_nonneg(o_strides, 3))
+    return set_error(kErrInvalidArgument, "chunk attention: strides must be non-negative");
+  if (vp_strides[3] != 1 || o_strides[2] != 1)
+    return set_error(kErrInvalidArgument, "chunk attention: head dims must be contiguous");
+  if ((vp_strides[0] & 7) || (vp_strides[1] & 7) || (vp_strides[2] & 7) || (o_strides[0] & 7) || (o_strides[1] & 7) ||
+      ((uintptr_t)v_pages & 15) || ((uintptr_t)out & 15))
+    return set_error(kErrInvalidArgument, "chunk attention: strides must be multiples of 8 on 16-byte aligned bases");
+  if (vp_strides[1] >= (int64_t)1 << 26)
+    return set_error(kErrUnsupported, "chunk attention: token stride of the pools too large");
+  if (num_splits < 1 || num_splits > 1024)
+    return set_error(kErrInvalidArgument, "chunk attention: num_splits must be in [1, 1024]");
+  if (num_splits > 1 &&
+      (!workspace || workspace_bytes < tasft_chunk_workspace_bytes(tokens, num_q_heads, head_dim, num_splits)))
+    return set_error(kErrWorkspace, "chunk attention: workspace too small");
+  if ((uintptr_t)workspace & 15)
+    return set_error(kErrInvalidArgument, "chunk attention: workspace must be 16-byte aligned");
+  p.v = (const uint16_t*)v_pages;
+  p.o = (uint16_t*)out;
+  p.lse = lse;
+  for (int i = 0; i < 3; ++i) p.sv[i] = vp_strides[i];
+  p.so[0] = o_strides[0];
+  p.so[1] = o_strides[1];
+  p.P = (int)num_splits;
+  p.ws_o = (float*)workspace;
+  p.ws_ml = (float*)workspace + tokens * num_q_heads * num_splits * head_dim;
+  // Row tiles: masked ones are aligned to positions, so a chunk can touch one more.
+  const int64_t rows = p.mask ? p.L + kRowTile - 1 : (int64_t)p.L * p.G;
+  p.QT = (int)((rows + kRowTile - 1) / kRowTile);
+  const int64_t grid = (int64_t)p.N * p.Hkv * p.QT * (p.mask ? p.G : 1) * p.P;
+  if (grid > 0x7fffffff) return set_error(kErrUnsupported, "chunk attention: launch too large");
+  const hipStream_t st = (hipStream_t)stream;
+  if (head_dim == 128)
+    return dtype == kF16 ? launch_chunk<128, kF16>(p, grid, st) : launch_chunk<128, kBf16>(p, grid, st);
+  return dtype == kF16 ? launch_chunk<64, kF16>(p, grid, st) : launch_chunk<64, kBf16>(p, grid, st);
+}
+
+template <int D, int DT>
+static void launch_weights(const WeightParams& w, hipStream_t stream) {
+  const ChunkParams& p = w.c;
+  const int64_t heads = (int64_t)p.N * p.Hkv;
+  auto grid = [&](int kw) { return heads * ((p.cap + kw * kTile - 1) / (kw * kTile)); };
+  if (grid(4) >= 512) {
+    const dim3 g((unsigned)grid(4));
+    if (p.mask) hipLaunchKernelGGL((chunk_weights_kernel<D, DT, 4, true>), g, dim3(256), 0, stream, w);
+    else hipLaunchKernelGGL((chunk_weights_kernel<D, DT, 4, false>), g, dim3(256), 0, stream, w);
+  } else {
+    const dim3 g((unsigned)grid(1));
+    if (p.mask) hipLaunchKernelGGL((chunk_weights_kernel<D, DT, 1, true>), g, dim3(256), 0, stream, w);
+    else hipLaunchKernelGGL((chunk_weights_kernel<D, DT, 1, false>), g, dim3(256), 0, stream, w);
+  }
+}
+
+extern "C" int tasft_key_weights(
+    const void* q, const void* k_pages, const uint8_t* block_mask, const int32_t* block_table,
+    const int32_t* kv_lens, const int32_t* cu_seqlens, const float* lse, const float* scores, float* scores_out,
+    int64_t num_seqs, int64_t tokens, int64_t num_q_heads, int64_t num_kv_heads, int64_t max_seqlen,
+    int64_t head_dim, int64_t block_size, int64_t mask_rows, int64_t page_size, int64_t num_pages,
+    int64_t max_pages, const int64_t* q_strides, const int64_t* kp_strides, const int64_t* lse_strides,
+    const int64_t* score_strides, const int64_t* mask_strides, int64_t block_table_stride, float scale, int causal,
+    int dtype, void* stream) {
+  const char* what = "key weights";
+  WeightParams w = {};
+  if (!lse || !scores_out || !lse_strides || (scores && !score_strides))
+    return set_error(kErrInvalidArgument, "key weights: null pointer argument");
+  if (const int rc = chunk_params(w.c, what, q, k_pages, block_mask, block_table, kv_lens, cu_seqlens, num_seqs,
+                                  tokens, num_q_heads, num_kv_heads, max_seqlen, head_dim, block_size, mask_rows,
+                                  page_size, num_pages, max_pages, q_strides, kp_strides, mask_strides,
+                                  block_table_stride, scale, causal, dtype))
+    return rc;
+  if (!strides_nonneg(lse_strides, 2) || (scores && !strides_nonneg(score_strides, 3)))
+    return set_error(kErrInvalidArgument, "key weights: strides must be non-negative");
+  if (num_seqs * num_kv_heads * ((int64_t)w.c.cap / kTile + 1) > 0x7fffffff)
+    return set_error(kErrUnsupported, "key weights: launch too large");
+  w.scores = scores;
+  if (scores)
+    for (int i = 0; i < 3; ++i) w.ss[i] = score_strides[i];
+  w.out = scores_out;
+  w.lse = lse;
+  w.sl[0] = lse_strides[0];
+  w.sl[1] = lse_strides[1];
+  const hipStream_t st = (hipStream_t)stream;
+  if (head_dim == 128)
+    dtype == kF16 ? launch_weights<128, kF16>(w, st) : launch_weights<128, kBf16>(w, st);
+  else
+    dtype == kF16 ? launch_weights<64, kF16>(w, st) : launch_weights<64, kBf16>(w, st);
+  return check_launch(what);
+}

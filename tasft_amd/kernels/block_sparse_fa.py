@@ -14,6 +14,7 @@ Additive, keyword-compatible extensions:
     mapping of ``tasft/modules/tasft_attention.py:725-729``), so callers no longer
     expand K/V.
   * ``forward_decode``: split-K block-sparse decode for one new token per sequence.
+  * ``forward_chunk_paged``: a chunk of new tokens per sequence over a paged cache.
 """
 from __future__ import annotations
 
@@ -27,6 +28,7 @@ from torch.nn import functional
 
 from tasft_amd import _native
 from tasft_amd.exceptions import KernelError
+from tasft_amd.kernels.paged_cache import check_batch, check_pools, chunk_mask, readable
 from tasft_amd.types import VALID_BLOCK_SIZES
 
 _VALID_HEAD_DIMS = frozenset({64, 128})
@@ -500,7 +502,6 @@ class BlockSparseFlashAttention:
         _native.check(status, "tasft_bsfa_decode_fwd", {"shape": [B, H, S_kv, D]})
         return out
 
-    # ------------------------------------------------------------------ stats
     def forward_decode_paged(
         self,
         q: torch.Tensor,
@@ -618,6 +619,87 @@ class BlockSparseFlashAttention:
                                                               "page_size": page_size})
         return out
 
+    # ------------------------------------------------------------------ chunk over a paged cache
+    def forward_chunk_paged(
+        self,
+        q: torch.Tensor,
+        k_pages: torch.Tensor,
+        v_pages: torch.Tensor,
+        block_table: torch.Tensor,
+        kv_lens: torch.Tensor,
+        cu_seqlens: torch.Tensor,
+        block_mask: torch.Tensor | None = None,
+        *,
+        max_seqlen: int | None = None,
+        causal: bool = True,
+        return_lse: bool = False,
+        num_splits: int | None = None,
+    ) -> torch.Tensor | tuple[torch.Tensor, torch.Tensor]:
+        """Attention of a chunk of new tokens of each sequence over its paged cache: a piece of a
+        long prompt, drafted tokens to be checked, or one token each. The cache already holds the
+        new tokens (``append_paged``). The reference has no such call (its vLLM backend attends
+        within the tokens of a call, ``tasft/inference/vllm_patch.py:172-176``).
+
+        Args:
+            q: ``[T, Hq, D]`` packed queries (bf16 or fp16), sequence n's at
+                ``cu_seqlens[n] .. cu_seqlens[n + 1] - 1``.
+            k_pages, v_pages, block_table: the pools and table of ``forward_decode_paged``.
+            kv_lens: ``[N]`` cached lengths, the chunk's tokens included (they are the last ones).
+                On the device it is trusted to be at most ``max_pages * page_size`` (the kernel
+                clamps it); on the CPU it is checked.
+            cu_seqlens: ``[N + 1]`` offsets; on the CPU they are checked, on the device trusted,
+                and ``max_seqlen`` must be given (a sequence's tokens behind its first
+                ``max_seqlen`` are not computed).
+            block_mask: ``[N, Hq, R, NB]`` with ``NB = ceil(max_pages * page_size / block_size)``
+                and ``R = (max_seqlen + block_size - 2) // block_size + 1``: row r of sequence n is
+                query block ``(kv_lens[n] - len_n) // block_size + r``, the rows of
+                ``AttnGate.forward(query_offset=kv_lens[n] - len_n)``. None: every key.
+            causal: a token sees no key behind its own position.
+            return_lse: also return the log-sum-exp of every row.
+            num_splits: workgroups that share the keys of a row (default: enough to fill the GPU).
+
+        Returns:
+            ``[T, Hq, D]``: rows that see no key, and rows of tokens behind ``cu_seqlens[N]``, are
+            0. With ``return_lse`` also ``[T, Hq]`` fp32, -inf for those rows.
+        """
+        check_pools(k_pages, v_pages)
+        b = check_batch(q, k_pages, block_table, kv_lens, cu_seqlens, max_seqlen)
+        T, H, D = q.shape
+        Hkv = k_pages.shape[2]
+        dev = q.device
+        if v_pages.device != dev:
+            raise KernelError("Tensors must be on one CUDA device", context={"v_pages": str(v_pages.device)})
+        if D not in _VALID_HEAD_DIMS:
+            raise KernelError(f"HIP kernel supports head_dim in {sorted(_VALID_HEAD_DIMS)}, got {D}",
+                              context={"head_dim": D, "supported": sorted(_VALID_HEAD_DIMS)})
+        mask = None if block_mask is None else chunk_mask(block_mask, b, H, self.block_size, dev)
+        if num_splits is None:
+            num_splits = default_chunk_splits(b.num_seqs, Hkv, H // Hkv, min(b.max_seqlen, T), b.slots,
+                                              mask is not None)
+        elif not 1 <= num_splits <= 1024:
+            raise KernelError(f"num_splits must be in [1, 1024], got {num_splits}",
+                              context={"num_splits": num_splits})
+        q, k_pages, v_pages = readable(q), readable(k_pages), readable(v_pages)
+        out = torch.empty((T, H, D), dtype=q.dtype, device=dev)
+        lse = torch.empty((T, H), dtype=torch.float32, device=dev) if return_lse else None
+        if T > 0:
+            lib = _native.load_library()
+            ws_bytes = lib.tasft_chunk_workspace_bytes(T, H, D, num_splits)
+            workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
+            with _native.on_device(dev):
+                status = lib.tasft_chunk_paged_fwd(
+                    q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr(), _native.ptr(lse),
+                    _native.ptr(mask), b.table.data_ptr(), b.kv_lens.data_ptr(), b.cu.data_ptr(),
+                    _native.ptr(workspace), ws_bytes, b.num_seqs, T, H, Hkv, b.max_seqlen, D, self.block_size,
+                    0 if mask is None else mask.shape[2], b.page_size, k_pages.shape[0], b.max_pages, num_splits,
+                    _native.strides(q), _native.strides(k_pages), _native.strides(v_pages), _native.strides(out),
+                    None if mask is None else _native.strides(mask), b.table.stride(0), 1.0 / math.sqrt(D),
+                    1 if causal else 0, _native.dtype_code(q.dtype, "chunk attention"),
+                    _native.stream_handle(dev))
+            _native.check(status, "tasft_chunk_paged_fwd", {"tokens": T, "sequences": b.num_seqs})
+        return (out, lse) if return_lse else out
+
+    # ------------------------------------------------------------------ stats
     def compute_sparsity_stats(self, block_mask: torch.Tensor) -> SparsityStats:
         """Full-grid statistics (reference ``block_sparse_fa.py:574-595``; syncs the device)."""
         total_blocks = block_mask.numel()
@@ -714,6 +796,20 @@ def default_decode_splits(batch: int, num_kv_heads: int, num_blocks: int,
     return int(max(1, want, math.ceil(num_blocks / 1024)))
 
 
+def default_chunk_splits(num_seqs: int, num_kv_heads: int, q_per_kv: int, chunk: int, slots: int,
+                         masked: bool = False) -> int:
+    """Key splits of ``forward_chunk_paged``: one where its row tiles (128 rows of a KV head's
+    tokens and query heads, or with a mask 128 positions of a head) give two workgroups per CU
+    (256 on MI355X), else enough for that, at least four 64-key tiles each."""
+    if masked:
+        tiles = num_seqs * num_kv_heads * q_per_kv * math.ceil(chunk / 128)
+    else:
+        tiles = num_seqs * num_kv_heads * math.ceil(chunk * q_per_kv / 128)
+    if tiles >= 384:
+        return 1
+    return max(1, min(math.ceil(512 / tiles), math.ceil(slots / 256), 64))
+
+
 def executed_blocks(block_mask: torch.Tensor, causal: bool = True) -> torch.Tensor:
     """Number of (query block, key block) tiles the prefill kernel computes (device tensor)."""
     m = block_mask != 0
@@ -727,6 +823,7 @@ __all__ = [
     "BlockSparseFlashAttention",
     "KernelBackend",
     "SparsityStats",
+    "default_chunk_splits",
     "default_decode_splits",
     "detect_kernels",
     "executed_blocks",

@@ -1,0 +1,234 @@
+"""Rotary position embedding of queries and keys, for training and for the attention calls.
+
+The attention, gate and cache entry points of this package take Q and K after the rotation, as
+the reference does (``tasft/modules/tasft_attention.py:426``, which gets them from its model's own
+rotary module). ``rotary_frequencies`` gives the inverse frequencies of a model's configuration,
+``apply_rotary`` rotates a batch (with gradients), and ``append_paged`` (in
+``tasft_amd.kernels.paged_cache``) rotates new tokens on their way into a paged cache.
+"""
+from __future__ import annotations
+
+import math
+
+import torch
+
+from tasft_amd import _native
+from tasft_amd.exceptions import KernelError
+
+_MAX_HEAD_DIM = 256
+
+
+def rotary_frequencies(
+    rotary_dim: int,
+    base: float = 10000.0,
+    scaling: dict | None = None,
+    device: torch.device | str | None = None,
+) -> tuple[torch.Tensor, float]:
+    """Inverse frequencies ``[rotary_dim / 2]`` in 64 bits, and the factor on cosine and sine.
+
+    Args:
+        rotary_dim: rotated dims of a head (even).
+        base: the frequencies are ``base ** (-2 j / rotary_dim)``.
+        scaling: a model configuration's ``rope_scaling``: ``None`` or ``{"rope_type": "default"}``;
+            ``"linear"`` (``factor``): positions divided by the factor; ``"llama3"`` (``factor``,
+            ``low_freq_factor``, ``high_freq_factor``, ``original_max_position_embeddings``):
+            frequencies of fewer than ``low_freq_factor`` turns over the original length divided by
+            the factor, of more than ``high_freq_factor`` kept, those between blended; ``"yarn"``
+            (``factor``, ``original_max_position_embeddings``, optional ``beta_fast`` 32,
+            ``beta_slow`` 1, ``attention_factor``): blended by dimension between the dims that make
+            ``beta_fast`` and ``beta_slow`` turns, with the factor ``0.1 ln(factor) + 1`` on the
+            result. Types whose frequencies follow the running length are refused.
+        device: of the returned tensor.
+    """
+    if rotary_dim <= 0 or rotary_dim % 2 != 0:
+        raise ValueError(f"rotary_dim must be even and positive, got {rotary_dim}")
+    if not base > 0.0 or not math.isfinite(base):
+        raise ValueError(f"base must be positive and finite, got {base}")
+    inv = torch.tensor([base ** (-2.0 * j / rotary_dim) for j in range(rotary_dim // 2)], dtype=torch.float64)
+    kind = "default" if scaling is None else scaling.get("rope_type", scaling.get("type", "default"))
+    attention = 1.0
+    if kind != "default":
+        if kind not in ("linear", "llama3", "yarn"):
+            raise ValueError(f"rope_type must be default, linear, llama3 or yarn, got {kind!r}")
+        factor = _entry(scaling, "factor", kind)
+        if not factor > 0.0:
+            raise ValueError(f"factor must be positive, got {factor}")
+        if kind == "linear":
+            inv = inv / factor
+        else:
+            original = _entry(scaling, "original_max_position_embeddings", kind)
+            if kind == "llama3":
+                low, high = _entry(scaling, "low_freq_factor", kind), _entry(scaling, "high_freq_factor", kind)
+                if not 0.0 < low < high:
+                    raise ValueError(f"need 0 < low_freq_factor < high_freq_factor, got {low} and {high}")
+                keep = ((original * inv / (2.0 * math.pi) - low) / (high - low)).clamp(0.0, 1.0)
+            else:
+                keep = 1.0 - _yarn_ramp(rotary_dim, base, original, scaling)
+                given = scaling.get("attention_factor")
+                attention = float(given) if given is not None else (0.1 * math.log(factor) + 1.0 if factor > 1.0 else 1.0)
+            inv = inv / factor * (1.0 - keep) + inv * keep
+    return inv.to(device) if device is not None else inv, attention
+
+
+def _entry(scaling: dict, name: str, kind: str) -> float:
+    if scaling.get(name) is None:
+        raise ValueError(f"rope_type {kind!r} needs {name!r}")
+    return float(scaling[name])
+
+
+def _yarn_ramp(dim: int, base: float, original: float, scaling: dict) -> torch.Tensor:
+    """0 for the pairs that keep their frequency, 1 for those divided by the factor."""
+    fast, slow = float(scaling.get("beta_fast") or 32.0), float(scaling.get("beta_slow") or 1.0)
+
+    def pair_with_turns(turns: float) -> float:
+        return dim * math.log(original / (turns * 2.0 * math.pi)) / (2.0 * math.log(base))
+
+    low = max(math.floor(pair_with_turns(fast)), 0)
+    high = min(math.ceil(pair_with_turns(slow)), dim - 1)
+    at = torch.arange(dim // 2, dtype=torch.float64)
+    return ((at - low) / (high - low if high != low else 0.001)).clamp(0.0, 1.0)
+
+
+def check_frequencies(inv_freq: torch.Tensor, head_dim: int, device: torch.device) -> torch.Tensor:
+    """``inv_freq`` as the kernels read it (contiguous doubles on ``device``)."""
+    if head_dim > _MAX_HEAD_DIM:
+        raise KernelError(f"rotary kernels take head_dim up to {_MAX_HEAD_DIM}, got {head_dim}",
+                          context={"head_dim": head_dim})
+    if inv_freq.ndim != 1 or not 1 <= inv_freq.numel() <= head_dim // 2:
+        raise KernelError(f"inv_freq must be 1-D with 1 to head_dim / 2 = {head_dim // 2} entries, "
+                          f"got shape {tuple(inv_freq.shape)}", context={"inv_freq": list(inv_freq.shape)})
+    if not inv_freq.is_floating_point():
+        raise KernelError(f"inv_freq must be floating point, got {inv_freq.dtype}",
+                          context={"dtype": str(inv_freq.dtype)})
+    if inv_freq.requires_grad:
+        raise KernelError("inv_freq must not require grad: the rotation has no gradient for it", context={})
+    return inv_freq.to(device=device, dtype=torch.float64).contiguous()
+
+
+def check_positions(positions: torch.Tensor, device: torch.device) -> torch.Tensor:
+    if positions.dtype not in (torch.int32, torch.int64):
+        raise KernelError(f"positions must be int32 or int64, got {positions.dtype}",
+                          context={"dtype": str(positions.dtype)})
+    return positions if positions.device == device else positions.to(device)
+
+
+def _unit_last(t: torch.Tensor) -> torch.Tensor:
+    return t if t.stride(-1) == 1 else t.contiguous()
+
+
+def _strides4(t: torch.Tensor):
+    """(b, h, s, d) strides of ``[B, H, S, D]``, or of packed ``[T, H, D]`` as one batch entry."""
+    st = t.stride()
+    return _native.kept_strides(st if t.ndim == 4 else (0, st[1], st[0], st[2]))
+
+
+def _rotate(q, k, positions, inv_freq, interleaved, scale, inverse):
+    """``tasft_rotary`` on checked tensors; ``k`` may be None."""
+    q = _unit_last(q)
+    k = None if k is None else _unit_last(k)
+    q_out = torch.empty_like(q)
+    k_out = None if k is None else torch.empty_like(k)
+    if q.ndim == 4:
+        B, Hq, S, D = q.shape
+        ps = positions.stride()
+        pos_strides = (0 if positions.ndim == 1 or positions.shape[0] == 1 else ps[0], ps[-1])
+    else:
+        S, Hq, D = q.shape
+        B, pos_strides = 1, (0, positions.stride(0))
+    if q.numel() == 0:
+        return q_out, k_out
+    lib = _native.load_library()
+    with _native.on_device(q.device):
+        status = lib.tasft_rotary(
+            q.data_ptr(), _native.ptr(k), q_out.data_ptr(), _native.ptr(k_out), positions.data_ptr(),
+            1 if positions.dtype == torch.int64 else 0, inv_freq.data_ptr(), B, Hq,
+            0 if k is None else k.shape[1], S, D, 2 * inv_freq.numel(), _strides4(q),
+            None if k is None else _strides4(k), _strides4(q_out), None if k is None else _strides4(k_out),
+            _native.kept_strides(pos_strides), 1 if interleaved else 0, 1 if inverse else 0, scale,
+            _native.dtype_code(q.dtype, "rotary"), _native.stream_handle(q.device))
+    _native.check(status, "tasft_rotary", {"shape": list(q.shape)})
+    return q_out, k_out
+
+
+class _Rotary(torch.autograd.Function):
+    """The rotation is linear and its gradient is the inverse rotation of the outputs' gradients
+    (with the same factor), itself this function: derivatives of any order."""
+
+    @staticmethod
+    def forward(ctx, q, k, positions, inv_freq, interleaved, scale, inverse):
+        ctx.save_for_backward(positions, inv_freq)
+        ctx.cfg = (interleaved, scale, inverse)
+        ctx.set_materialize_grads(False)
+        return _rotate(q, k, positions, inv_freq, interleaved, scale, inverse)
+
+    @staticmethod
+    def backward(ctx, gq, gk):
+        positions, inv_freq = ctx.saved_tensors
+        interleaved, scale, inverse = ctx.cfg
+        want_q, want_k = ctx.needs_input_grad[:2]
+        given = [g for g, want in ((gq, want_q), (gk, want_k)) if want and g is not None]
+        if not given:
+            return (None,) * 7
+        out = list(_Rotary.apply(given[0], given[1] if len(given) > 1 else None, positions, inv_freq,
+                                 interleaved, scale, not inverse))
+        gq = out.pop(0) if want_q and gq is not None else None
+        gk = out.pop(0) if want_k and gk is not None else None
+        return gq, gk, None, None, None, None, None
+
+
+def apply_rotary(
+    q: torch.Tensor,
+    k: torch.Tensor | None,
+    positions: torch.Tensor,
+    inv_freq: torch.Tensor,
+    *,
+    interleaved: bool = False,
+    scale: float = 1.0,
+) -> tuple[torch.Tensor, torch.Tensor | None]:
+    """Queries and keys rotated by their positions, in one launch; differentiable in q and k.
+
+    Args:
+        q: ``[B, Hq, S, D]`` or packed ``[T, Hq, D]``, bf16 or fp16, any strides (a transposed view
+            of a projection is read in place).
+        k: ``[B, Hkv, S, D]`` / ``[T, Hkv, D]`` of q's dtype, or None.
+        positions: int32 or int64 ``[S]``, ``[B, S]`` (or ``[1, S]``), packed ``[T]``.
+        inv_freq: ``[R / 2]`` inverse frequencies (``rotary_frequencies``; float64 on the device is
+            read as it is, other types are converted at each call). ``R <= D``: the dims behind the
+            first R are copied.
+        interleaved: pairs ``(2j, 2j + 1)`` instead of ``(j, j + R / 2)``.
+        scale: factor on the rotated dims (the second value of ``rotary_frequencies``).
+
+    Returns:
+        The rotated q and k (None without k), new tensors of q's and k's layout.
+    """
+    if q.ndim not in (3, 4):
+        raise KernelError(f"Expected q of shape [B, H, S, D] or [T, H, D], got {tuple(q.shape)}",
+                          context={"q_shape": list(q.shape)})
+    _native.dtype_code(q.dtype, "rotary")
+    if k is not None:
+        # All but the head counts are the same.
+        if k.ndim != q.ndim or k.shape[1] == 0 or k.shape[:1] + k.shape[2:] != q.shape[:1] + q.shape[2:]:
+            raise KernelError("q and k shapes are incompatible",
+                              context={"q": list(q.shape), "k": list(k.shape)})
+        if k.dtype != q.dtype or k.device != q.device:
+            raise KernelError("q and k must have one dtype and device",
+                              context={"q": [str(q.dtype), str(q.device)], "k": [str(k.dtype), str(k.device)]})
+    if q.ndim == 4:
+        B, S = q.shape[0], q.shape[2]
+        fits = tuple(positions.shape) in ((S,), (1, S), (B, S))
+    else:
+        fits = tuple(positions.shape) == (q.shape[0],)
+    if not fits:
+        raise KernelError(f"positions of shape {tuple(positions.shape)} do not fit q {tuple(q.shape)}",
+                          context={"positions": list(positions.shape), "q": list(q.shape)})
+    positions = check_positions(positions, q.device)
+    inv_freq = check_frequencies(inv_freq, q.shape[-1], q.device)
+    if not q.is_cuda:
+        raise KernelError("Tensors must be on CUDA device", context={"device": str(q.device)})
+    args = (q, k, positions, inv_freq, bool(interleaved), float(scale), False)
+    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+        return _Rotary.apply(*args)
+    return _rotate(*args)
+
+
+__all__ = ["apply_rotary", "rotary_frequencies"]

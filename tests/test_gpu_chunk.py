@@ -1,0 +1,224 @@
+"""Chunk attention over a paged cache and the key weights, against the 64-bit form."""
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+import paged_ref as ref
+from helpers import require_gpu
+from tasft_amd.kernels import BlockSparseFlashAttention, accumulate_key_weights
+
+pytestmark = pytest.mark.gpu
+
+BF, HF = torch.bfloat16, torch.float16
+
+# lens, kv_lens, Hq, Hkv, D, page, dtype, causal
+CASES = [
+    ([1], [1], 1, 1, 128, 16, BF, True),
+    ([1], [1], 4, 4, 64, 8, HF, True),
+    ([1, 1, 1], [65, 700, 64], 8, 2, 128, 16, BF, True),
+    ([1, 1], [333, 20], 28, 4, 128, 32, HF, True),
+    ([1, 1], [130, 513], 16, 1, 64, 128, BF, True),
+    ([1], [300], 40, 1, 128, 16, BF, True),            # 40 query heads of one KV head
+    ([5, 3, 0, 8], [700, 64, 40, 8], 8, 2, 128, 16, BF, True),
+    ([5, 4], [129, 1000], 16, 16, 64, 32, HF, True),
+    ([2, 1, 7], [64, 65, 71], 6, 2, 128, 8, HF, True),
+    ([70, 1, 33], [70, 500, 300], 8, 2, 128, 16, BF, True),
+    ([130, 200], [130, 515], 4, 2, 64, 64, BF, True),
+    ([129], [1000], 7, 1, 128, 256, HF, True),
+    ([40, 64], [200, 64], 4, 1, 128, 16, BF, False),
+    ([3, 1], [77, 400], 8, 8, 64, 8, HF, False),
+    ([9, 70], [4, 50], 4, 2, 128, 16, BF, True),       # fewer cached keys than new tokens
+    ([300], [900], 2, 1, 64, 8, HF, True),
+]
+
+
+def _put(t, dev):
+    return [x.to(dev) for x in t]
+
+
+def _mask(case, seed, bs, density, rows=None):
+    lens, kv, hq = case[0], case[1], case[2]
+    page = case[5]
+    longest = max(lens)
+    r = rows or (longest + bs - 2) // bs + 1
+    cap = (max(max(1, -(-max(x, 1) // page)) for x in kv) + 1) * page
+    g = torch.Generator().manual_seed(seed)
+    return torch.rand((len(lens), hq, r, -(-cap // bs)), generator=g) < density
+
+
+def _check(out, lse, want, dtype, d, keys, what):
+    o, e = ref.attention_bounds(*want, dtype, d, keys)
+    err = (out.cpu().double() - want[0]).abs()
+    assert bool((err <= o).all()), f"{what}: output {float((err - o).max()):.3e} over the bound"
+    empty = want[1] == -math.inf
+    assert torch.equal(lse.cpu() == -math.inf, empty), f"{what}: empty rows"
+    le = (lse.cpu().double() - want[1])[~empty].abs()
+    assert bool((le <= e[~empty]).all()), f"{what}: log-sum {float((le - e[~empty]).max()):.3e} over the bound"
+
+
+@pytest.mark.parametrize("index", range(len(CASES)))
+def test_dense(index):
+    lens, kv, hq, hkv, d, page, dtype, causal = CASES[index]
+    dev = require_gpu()
+    t = ref.make(lens, kv, hq, hkv, d, page, dtype, seed=index, pad=3)
+    want = ref.attention(*t, causal=causal)
+    q, k, v, table, kvl, cu = _put(t, dev)
+    attn = BlockSparseFlashAttention(min_sparsity_for_speedup=0.0)
+    for splits in (None, 1, 3):
+        print(f"chunk {CASES[index]} splits={splits}", flush=True)
+        out, lse = attn.forward_chunk_paged(q, k, v, table, kvl, cu, max_seqlen=max(max(lens), 1), causal=causal,
+                                            return_lse=True, num_splits=splits)
+        torch.cuda.synchronize()
+        _check(out, lse, want, dtype, d, max(kv), f"splits {splits}")
+    assert torch.equal(out[-3:], torch.zeros_like(out[-3:]))
+    alone = attn.forward_chunk_paged(q, k, v, table, kvl, cu.cpu(), causal=causal, num_splits=3)
+    assert torch.equal(alone, out)
+
+
+@pytest.mark.parametrize("bs", [32, 64, 128])
+@pytest.mark.parametrize("index", range(2, len(CASES)))
+def test_block_mask(index, bs):
+    lens, kv, hq, hkv, d, page, dtype, causal = CASES[index]
+    dev = require_gpu()
+    t = ref.make(lens, kv, hq, hkv, d, page, dtype, seed=50 + index, pad=1)
+    attn = BlockSparseFlashAttention(block_size=bs, min_sparsity_for_speedup=0.0)
+    for density in (0.4, 0.05):  # at the second many rows see nothing
+        mask = _mask(CASES[index], index, bs, density)
+        want = ref.attention(*t, mask=mask, bs=bs, causal=causal)
+        q, k, v, table, kvl, cu = _put(t, dev)
+        for splits, m in ((None, mask.to(dev)), (2, mask.to(dev).transpose(1, 2).contiguous().transpose(1, 2)),
+                          (1, mask.to(torch.int32))):
+            print(f"chunk {CASES[index]} block {bs} density {density} splits={splits}", flush=True)
+            out, lse = attn.forward_chunk_paged(q, k, v, table, kvl, cu, m, max_seqlen=max(lens), causal=causal,
+                                                return_lse=True, num_splits=splits)
+            torch.cuda.synchronize()
+            _check(out, lse, want, dtype, d, max(kv), f"block {bs} splits {splits}")
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("masked", [False, True])
+@pytest.mark.parametrize(("lens", "kv"), [([100], [230]), ([6], [200]), ([1], [100])])
+def test_what_a_row_does_not_see_does_not_reach_it(lens, kv, masked, dtype):
+    """NaN and infinities in keys and values behind a token, in blocks its mask leaves out and
+    behind the cache's end change nothing; those it sees do."""
+    dev = require_gpu()
+    hq, hkv, d, page, bs = 4, 2, 128, 16, 32
+    t = ref.make(lens, kv, hq, hkv, d, page, dtype, seed=7)
+    q, k, v, table, kvl, cu = t
+    mask = _mask((lens, kv, hq, hkv, d, page), 5, bs, 0.5) if masked else None
+    if masked:
+        mask[..., 0] = True
+    attn = BlockSparseFlashAttention(block_size=bs, min_sparsity_for_speedup=0.0)
+
+    def run():
+        a = _put((q, k, v, table, kvl, cu), dev)
+        return attn.forward_chunk_paged(*a, None if mask is None else mask.to(dev), max_seqlen=max(lens),
+                                        return_lse=True)
+
+    print(f"chunk unseen values lens={lens} masked={masked} {dtype}", flush=True)
+    clean, clean_lse = run()
+    length, cached = lens[0], kv[0]
+    poison = [cached - 1, cached - length + length // 2, 40]
+    for slot in poison:
+        pg, row = int(table[0, slot // page]), slot % page
+        for g in range(hkv):
+            v[pg, row, g, 3] = float("inf")
+            v[pg, row, g, 70] = float("nan")
+            k[pg, row, g, 1] = float("nan") if slot != 40 else k[pg, row, g, 1]
+    out, lse = run()
+    for h in range(hq):
+        see = ref.visible(cached - length, length, cached, True, None if mask is None else mask[0], bs, h)
+        for i in range(length):
+            if not see[i, poison].any():
+                assert torch.equal(out[i, h], clean[i, h]) and torch.equal(lse[i, h], clean_lse[i, h])
+            elif see[i, 40] and not see[i, poison[:2]].any():
+                assert out[i, h, 3] == math.inf and bool(torch.isnan(out[i, h, 70]))
+                rest = torch.ones(d, dtype=torch.bool)
+                rest[[3, 70]] = False
+                assert torch.equal(out[i, h].cpu()[rest], clean[i, h].cpu()[rest])
+            else:
+                assert bool(torch.isnan(out[i, h]).all()) and bool(torch.isnan(lse[i, h]))
+
+
+@pytest.mark.parametrize("lens", [[1, 1], [6, 3], [90, 130]])
+def test_strides_and_large_scores(lens):
+    """Queries cut from a wider projection, head-major pools, a table with a row stride, and scores
+    whose running maximum moves far: equal to contiguous copies, and to the 64-bit form."""
+    dev = require_gpu()
+    hq, hkv, d, page = 8, 2, 64, 16
+    kv = [400, 333]
+    t = ref.make(lens, kv, hq, hkv, d, page, BF, seed=3, scale=4.0)
+    q, k, v, table, kvl, cu = t
+    for n in range(2):
+        for slot in range(kv[n]):  # growing keys
+            k[int(table[n, slot // page]), slot % page] *= 1.0 + slot / 100
+    want = ref.attention(*t)
+    q, k, v, table, kvl, cu = _put(t, dev)
+    attn = BlockSparseFlashAttention(min_sparsity_for_speedup=0.0)
+    print(f"chunk strides lens={lens}", flush=True)
+    out, lse = attn.forward_chunk_paged(q, k, v, table, kvl, cu, max_seqlen=max(lens), return_lse=True)
+    _check(out, lse, want, BF, d, max(kv), "large scores")
+    wide = torch.randn(q.shape[0], hq + 2 * hkv, d, device=dev).bfloat16()
+    wide[:, :hq] = q
+    hm = [x.permute(0, 2, 1, 3).contiguous().permute(0, 2, 1, 3) for x in (k, v)]
+    big = torch.zeros((2, table.shape[1] + 5), dtype=torch.int32, device=dev)
+    big[:, :table.shape[1]] = table
+    again = attn.forward_chunk_paged(wide[:, :hq], *hm, big[:, :table.shape[1]], kvl.long(), cu, max_seqlen=max(lens))
+    assert torch.equal(again, out)
+    odd = torch.empty(q.numel() + 1, dtype=BF, device=dev)[1:].view(q.shape).copy_(q)  # two bytes off
+    assert torch.equal(attn.forward_chunk_paged(odd, k, v, table, kvl, cu, max_seqlen=max(lens)), out)
+
+
+@pytest.mark.parametrize("lens", [[1], [4], [80]])
+def test_lengths_are_clamped(lens):
+    """A length past the table and table entries outside the pool read pages that exist; a negative
+    length reads nothing."""
+    dev = require_gpu()
+    t = ref.make(lens, [90], 4, 2, 128, 16, BF, seed=1)
+    q, k, v, table, kvl, cu = _put(t, dev)
+    k, v = k.nan_to_num(0.5), v.nan_to_num(0.5, posinf=0.5)
+    attn = BlockSparseFlashAttention(min_sparsity_for_speedup=0.0)
+    print(f"chunk clamped lens={lens}", flush=True)
+    over = attn.forward_chunk_paged(q, k, v, table, kvl + 100000, cu, max_seqlen=lens[0])
+    assert bool(torch.isfinite(over).all())
+    wild = table.clone()
+    wild[0, 0], wild[0, 1] = -7, 1 << 30
+    assert bool(torch.isfinite(attn.forward_chunk_paged(q, k, v, wild, kvl, cu, max_seqlen=lens[0])).all())
+    out, lse = attn.forward_chunk_paged(q, k, v, table, kvl - 1000, cu, max_seqlen=lens[0], return_lse=True)
+    assert not out.any() and bool((lse == -math.inf).all())
+
+
+@pytest.mark.parametrize("masked", [0, 32, 64, 128])
+@pytest.mark.parametrize("index", range(len(CASES)))
+def test_key_weights(index, masked):
+    case = CASES[index]
+    lens, kv, hq, hkv, d, page, dtype, causal = case
+    dev = require_gpu()
+    t = ref.make(lens, kv, hq, hkv, d, page, dtype, seed=100 + index, pad=2)
+    q, k, v, table, kvl, cu = t
+    mask = _mask(case, index, masked, 0.3) if masked else None
+    lse = ref.attention(*t, mask=mask, bs=masked or 64, causal=causal)[1].float()
+    cap = table.shape[1] * page
+    before = torch.rand((len(lens), hkv, cap), generator=torch.Generator().manual_seed(index))
+    total, dot = ref.key_weights(q, k, table, kvl, cu, lse, before, mask, masked or 64, causal)
+    weight = total - before.double()
+    print(f"key weights {case} mask {masked}", flush=True)
+    a = [x.to(dev) for x in (q, k, table, kvl, cu, lse)]
+    md = None if mask is None else mask.to(dev)
+    got = accumulate_key_weights(*a, before.to(dev), block_mask=md, block_size=masked or 64, causal=causal,
+                                 max_seqlen=max(lens))
+    torch.cuda.synchronize()
+    # Scores as in the attention's bound, twice for the exponent's own rounding; fp32 sums over rows.
+    rel = 2 * ((d + 3) * dot + 8 * (1 + dot)) * 2.0 ** -24 + (max(lens) * hq // hkv + 2) * 2.0 ** -24
+    err = (got.cpu().double() - total).abs()
+    assert bool((err <= rel * weight + 2.0 ** -23 * total).all()), float((err - rel * weight).max())
+    for n in range(len(lens)):
+        assert torch.equal(got[n, :, max(kv[n], 0):].cpu(), before[n, :, max(kv[n], 0):])
+    bare = accumulate_key_weights(*a, block_mask=md, block_size=masked or 64, causal=causal, max_seqlen=max(lens))
+    assert bool(((bare.cpu().double() - weight).abs() <= rel * weight + 2.0 ** -23 * weight).all())
+    # The weights of a row add up to one.
+    rows = int((lse[:int(cu[-1])] != -math.inf).sum())
+    assert abs(float(bare.double().sum()) - rows) <= (rel + 1e-5) * max(rows, 1)

@@ -1,0 +1,150 @@
+"""Rotary positions on the GPU against the 64-bit form: values, gradients, strides, refusals."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+import paged_ref as ref
+from helpers import require_gpu
+from tasft_amd.kernels import apply_rotary, rotary_frequencies
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = [torch.bfloat16, torch.float16]
+
+
+def _check(got, x, positions, inv, scale, inter, inverse=False, what=""):
+    want = ref.rotate(x.cpu(), positions.cpu(), inv.cpu(), scale, inter, inverse)
+    bound = ref.rotate_bound(x.cpu(), want, inv.cpu(), scale, inter, x.dtype)
+    err = (got.detach().cpu().double() - want).abs()
+    assert bool((err <= bound).all()), f"{what}: {float((err - bound).max()):.3e} over the bound"
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("inter", [False, True])
+@pytest.mark.parametrize(("D", "R"), [(128, 128), (64, 32), (128, 16), (80, 20), (96, 24), (64, 64), (256, 256),
+                                      (6, 2), (40, 8)])
+def test_values(D, R, inter, dtype):
+    dev = require_gpu()
+    print(f"rotary D={D} R={R} interleaved={inter} {dtype}", flush=True)
+    g = torch.Generator().manual_seed(D + R)
+    inv, scale = rotary_frequencies(R, 10000.0, device=dev)
+    for B, S, hq, hkv in ((2, 37, 6, 3), (1, 1, 1, 1), (3, 1500, 2, 2)):
+        q = torch.randn((B, hq, S, D), generator=g).to(dtype).to(dev)
+        k = torch.randn((B, hkv, S, D), generator=g).to(dtype).to(dev)
+        pos = torch.randint(0, 100000, (B, S), generator=g).to(dev)
+        a, b = apply_rotary(q, k, pos, inv, interleaved=inter, scale=1.25)
+        _check(a, q, pos[:, None], inv, 1.25, inter, what="q")
+        _check(b, k, pos[:, None], inv, 1.25, inter, what="k")
+        a2, none = apply_rotary(q, None, pos, inv, interleaved=inter, scale=1.25)
+        assert none is None and torch.equal(a, a2)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_positions_and_layouts(dtype):
+    """int32 and int64 positions of any size, shared by the batch or not; packed rows; transposed,
+    expanded, sliced and misaligned inputs give what contiguous ones give."""
+    dev = require_gpu()
+    g = torch.Generator().manual_seed(3)
+    B, S, H, D = 2, 33, 4, 64
+    inv, scale = rotary_frequencies(D, 500000.0, {"rope_type": "linear", "factor": 4.0}, device=dev)
+    base = torch.randn((B, S, H, D), generator=g).to(dtype).to(dev)
+    q = base.transpose(1, 2)
+    far = torch.arange(S, dtype=torch.int64, device=dev) + 2 ** 31 - 7
+    print("rotary layouts", flush=True)
+    out, _ = apply_rotary(q, None, far, inv)
+    _check(out, q, far, inv, scale, False)
+    near = torch.arange(S, device=dev)
+    want, _ = apply_rotary(q.contiguous(), None, near, inv)
+    for pos in (near.to(torch.int32), near.expand(B, S), near.view(1, S), near.to(torch.int32).expand(B, S)):
+        got, kk = apply_rotary(q, q, pos, inv)
+        assert torch.equal(got, want) and torch.equal(kk, want)
+        assert got.stride() == q.stride()
+    packed, _ = apply_rotary(base[0], None, near, inv)
+    assert torch.equal(packed, want[0].transpose(0, 1))
+    wide = torch.zeros((B, S, H, D + 3), dtype=dtype, device=dev)
+    wide[..., 1:D + 1] = base
+    odd = wide[..., 1:D + 1].transpose(1, 2)  # rows of 67 elements, two bytes off: no vectors
+    assert torch.equal(apply_rotary(odd, None, near, inv)[0], want)
+    every2 = torch.empty((B, H, S, 2 * D), dtype=dtype, device=dev)[..., ::2].copy_(q)
+    assert torch.equal(apply_rotary(every2, None, near, inv)[0], want)
+    one = q[:, :1, :1].expand(B, H, S, D)
+    assert torch.equal(apply_rotary(one, None, near, inv)[0], apply_rotary(one.contiguous(), None, near, inv)[0])
+    assert torch.equal(apply_rotary(q, None, near, inv.float())[0].float().isfinite().all().cpu(), torch.tensor(True))
+    empty, _ = apply_rotary(q[:, :, :0], None, near[:0], inv)
+    assert empty.shape == (B, H, 0, D)
+    # Infinities and NaN stay with their pair; position 0 keeps every value.
+    same, _ = apply_rotary(q, None, torch.zeros(S, dtype=torch.int64, device=dev), inv)
+    assert torch.equal(same, q)
+    bad = q.contiguous()
+    bad[0, 1, 5, 3] = float("nan")
+    got, _ = apply_rotary(bad, None, near, inv)
+    spoiled = torch.isnan(got)
+    assert spoiled.sum() == 2 and spoiled[0, 1, 5, 3] and spoiled[0, 1, 5, 3 + D // 2]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("inter", [False, True])
+def test_gradients(inter, dtype):
+    dev = require_gpu()
+    print(f"rotary gradients interleaved={inter} {dtype}", flush=True)
+    g = torch.Generator().manual_seed(11)
+    B, S, D, R = 2, 70, 128, 64
+    inv, scale = rotary_frequencies(R, 10000.0, {"rope_type": "yarn", "factor": 4.0,
+                                                 "original_max_position_embeddings": 4096}, device=dev)
+    q = torch.randn((B, 4, S, D), generator=g).to(dtype).to(dev).requires_grad_(True)
+    k = torch.randn((B, 2, S, D), generator=g).to(dtype).to(dev).requires_grad_(True)
+    gq, gk = torch.randn(q.shape, generator=g).to(dtype).to(dev), torch.randn(k.shape, generator=g).to(dtype).to(dev)
+    pos = torch.randint(0, 5000, (B, S), generator=g).to(dev)
+    a, b = apply_rotary(q, k, pos, inv, interleaved=inter, scale=scale)
+    dq, dk = torch.autograd.grad((a, b), (q, k), (gq, gk), retain_graph=True)
+    _check(dq, gq, pos[:, None], inv, scale, inter, inverse=True, what="dq")
+    _check(dk, gk, pos[:, None], inv, scale, inter, inverse=True, what="dk")
+    # One output alone, one input alone, a gradient of stride 0.
+    assert torch.equal(torch.autograd.grad(b, k, gk, retain_graph=True)[0], dk)
+    only, _ = apply_rotary(q, k.detach(), pos, inv, interleaved=inter, scale=scale)
+    assert torch.equal(torch.autograd.grad(only, q, gq)[0], dq)
+    ones = torch.ones((), dtype=dtype, device=dev).expand(a.shape)
+    assert torch.equal(torch.autograd.grad(a, q, ones, retain_graph=True)[0],
+                       torch.autograd.grad(a, q, ones.contiguous(), retain_graph=True)[0])
+    # Against differences: the operator is linear, <g, R(x + d) - R(x)> = <R^T g, d>, in 64 bits of
+    # the rounded values; every factor carries roundings of half a step.
+    d = torch.randn(q.shape, generator=g).to(dtype).to(dev)
+    moved, _ = apply_rotary(d, None, pos, inv, interleaved=inter, scale=scale)
+    left = (gq.double() * moved.double()).sum()
+    right = (dq.double() * d.double()).sum()
+    size = (gq.double().abs() * moved.double().abs()).sum() + (dq.double().abs() * d.double().abs()).sum()
+    assert abs(float(left - right)) <= 1.01 * ref.half_step(dtype) * float(size) + 1e-3
+    # A second derivative: the gradient of the gradient with respect to its own input.
+    gq2 = gq.clone().requires_grad_(True)
+    (dq2,) = torch.autograd.grad(a, q, gq2, create_graph=True)
+    (back,) = torch.autograd.grad(dq2, gq2, d)
+    assert torch.equal(back, moved)
+
+
+def test_graph_replay_and_streams():
+    dev = require_gpu()
+    inv, _ = rotary_frequencies(128, device=dev)
+    q = torch.randn(2, 8, 50, 128, device=dev).bfloat16()
+    k = torch.randn(2, 2, 50, 128, device=dev).bfloat16()
+    pos = torch.arange(50, device=dev)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    print("rotary graph", flush=True)
+    with torch.cuda.stream(side):
+        on_side = apply_rotary(q, k, pos, inv)
+        on_side = apply_rotary(q, k, pos, inv)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = apply_rotary(q, k, pos, inv)
+    for step in range(3):
+        q.normal_()
+        pos += 17
+        want = apply_rotary(q, k, pos, inv)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1])
+    assert on_side[0].shape == q.shape
