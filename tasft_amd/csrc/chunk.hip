@@ -19,11 +19,16 @@
 // arrives as zeros). A tile in which only some rows see a key could still carry an infinity or
 // NaN of V into the others as 0 * inf: there V is looked over, and such a tile takes a slow
 // path that adds each key to the rows that see it.
+#include <type_traits>
+
 #include "common.h"
 
 #include "../../include/tasft_amd.h"
 
 namespace tasft {
+
+// A lambda called at several places is otherwise made a function, its captures in scratch memory.
+#define TASFT_INLINE __attribute__((always_inline))
 
 constexpr int kTile = 64;                // keys per tile
 constexpr float kChunkMove = 8.f;        // a new maximum moves the exp2 reference only if this far above it
@@ -87,6 +92,11 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_rsrc(const uint16_t* base
 
 __device__ __forceinline__ void chunk_dma(__amdgpu_buffer_rsrc_t r, uint8_t* dst, int voff) {
   __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (TASFT_LDS void*)dst, 16, voff, 0, 0, 0);
+}
+
+// The same of 4 bytes a lane.
+__device__ __forceinline__ void chunk_dma4(__amdgpu_buffer_rsrc_t r, float* dst, int voff) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (TASFT_LDS void*)dst, 4, voff, 0, 0, 0);
 }
 
 __device__ __forceinline__ void chunk_barrier() { asm volatile("s_barrier" ::: "memory"); }
@@ -213,7 +223,7 @@ chunk_rows_kernel(const ChunkParams p) {
     row_hi = row_of(i_end);
     row_own = wave_on ? row_of(i_first) : -1;
   }
-  auto next_tile = [&]() -> int {
+  auto next_tile = [&]() TASFT_INLINE -> int {
     if constexpr (!MASKED) {
       return cursor < tile_b ? cursor++ : -1;
     } else {
@@ -257,22 +267,44 @@ chunk_rows_kernel(const ChunkParams p) {
   struct Pages {
     int a, b;
   };
-  auto load_pages = [&](int kt) -> Pages {
+  const bool pages16 = p.ps_shift >= 4;  // a wave's 16 rows lie in one page
+  auto load_pages = [&](int kt) TASFT_INLINE -> Pages {
     const int r = kt * kTile + wave * 16, last = (sq.kv - 1) >> p.ps_shift;
-    return {scalar_load(table + min(r >> p.ps_shift, last)), scalar_load(table + min((r + 8) >> p.ps_shift, last))};
+    Pages pg;
+    pg.a = pg.b = scalar_load(table + min(r >> p.ps_shift, last));
+    if (!pages16) pg.b = scalar_load(table + min((r + 8) >> p.ps_shift, last));
+    return pg;
   };
-  auto dma_tile = [&](uint8_t* kt_lds, uint8_t* vt_lds, int kt, Pages pg) {
+  const int64_t k8 = 8 * p.sk[1], v8 = 8 * p.sv[1];
+  const int krow = (int)p.sk[1] * 2, vrow = (int)p.sv[1] * 2;
+  auto dma_tile = [&](uint8_t* kt_lds, uint8_t* vt_lds, int kt, Pages pg) TASFT_INLINE {
+    const int r = kt * kTile + wave * 16;
+    const int page_a = min(max(pg.a, 0), p.num_pages - 1);
+    const int in_page = r & ((1 << p.ps_shift) - 1);
+    const uint16_t* kr = kbase + page_a * p.sk[0] + in_page * p.sk[1];
+    const uint16_t* vr = vbase + page_a * p.sv[0] + in_page * p.sv[1];
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      const int r = kt * kTile + wave * 16 + 8 * e;
-      const int64_t page = min(max(e ? pg.b : pg.a, 0), p.num_pages - 1);
-      const int in_page = r & ((1 << p.ps_shift) - 1), rows = min(sq.kv - r, 8);
-      const __amdgpu_buffer_rsrc_t kr = rows_rsrc(kbase + page * p.sk[0] + in_page * p.sk[1], rows, p.sk[1], D);
-      const __amdgpu_buffer_rsrc_t vr = rows_rsrc(vbase + page * p.sv[0] + in_page * p.sv[1], rows, p.sv[1], D);
+      if (e == 1) {
+        if (pages16) {
+          kr += k8;
+          vr += v8;
+        } else {
+          const int page_b = min(max(pg.b, 0), p.num_pages - 1);
+          const int in_b = (r + 8) & ((1 << p.ps_shift) - 1);
+          kr = kbase + page_b * p.sk[0] + in_b * p.sk[1];
+          vr = vbase + page_b * p.sv[0] + in_b * p.sv[1];
+        }
+      }
+      const int rows = min(sq.kv - r - 8 * e, 8);
+      const __amdgpu_buffer_rsrc_t krs = __builtin_amdgcn_make_buffer_rsrc(
+          (void*)kr, (short)0, rows > 0 ? (rows - 1) * krow + ROWB : 0, 0x00020000);
+      const __amdgpu_buffer_rsrc_t vrs = __builtin_amdgcn_make_buffer_rsrc(
+          (void*)vr, (short)0, rows > 0 ? (rows - 1) * vrow + ROWB : 0, 0x00020000);
 #pragma unroll
       for (int u = e * (UPW / 2); u < (e + 1) * (UPW / 2); ++u) {
-        chunk_dma(kr, kt_lds + (wave * UPW + u) * 1024, koff[u]);
-        chunk_dma(vr, vt_lds + (wave * UPW + u) * 1024, voff[u]);
+        chunk_dma(krs, kt_lds + (wave * UPW + u) * 1024, koff[u]);
+        chunk_dma(vrs, vt_lds + (wave * UPW + u) * 1024, voff[u]);
       }
     }
   };
@@ -284,7 +316,7 @@ chunk_rows_kernel(const ChunkParams p) {
   float l_run = 0.f;
   int fix_from = 0x7fffffff;  // first tile whose infinities or NaN of V were left out
 
-  auto compute = [&](const uint8_t* kS, const uint8_t* vS, int kt, int own) {
+  auto compute = [&](const uint8_t* kS, const uint8_t* vS, int kt, int own) TASFT_INLINE {
     const int key0 = kt * kTile;
     if (key0 > any_see || (MASKED && own == 0)) return;
     u32x4_t kf[2][KSTEPS];
@@ -396,7 +428,7 @@ chunk_rows_kernel(const ChunkParams p) {
   }
   // One tile from a stage while the next one's DMA fills the other: by the barrier every wave's
   // share of this tile has landed and every wave is done with the tile before it.
-  auto step = [&](uint8_t* ka, uint8_t* va, uint8_t* kb, uint8_t* vb) {
+  auto step = [&](uint8_t* ka, uint8_t* va, uint8_t* kb, uint8_t* vb) TASFT_INLINE {
     __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0)
     chunk_barrier();
     int nn = -1;
@@ -537,10 +569,15 @@ __global__ void __launch_bounds__(256) chunk_combine_kernel(const ChunkParams p)
 // ---------------------------------------------------------------------------------------
 // Accumulated key weights: out[n, g, j] = in[n, g, j] + sum over the chunk's rows that see key j
 // of exp(q . k_j scale - lse). The transpose of the attention's reduction: a wave keeps 64 keys
-// (their K in registers as the A operand) and walks the rows 32 at a time (Q as the B operand,
-// from L2), adding exp2 of the scores to one register per key; lanes are summed once at the end.
-// KW of the four waves hold different keys, 4 / KW share out the rows of the same: many keys want
-// few readings of Q (KW = 4), few keys want many workgroups (KW = 1). Fixed order, no atomics.
+// (their K in registers as the A operand) and walks the rows 32 at a time (Q as the B operand),
+// adding exp2 of the scores to one register per key; lanes are summed once at the end. Fixed
+// order, no atomics.
+//
+// KW of the four waves hold different keys, 4 / KW share out the rows of the same. Many keys
+// (KW = 4) read Q less often, few keys (KW = 1) want four times as many workgroups. RING: the
+// waves walk the same rows, 64 a step, that come by DMA into a ring of four LDS stages, three steps
+// ahead (a step is shorter than a trip to L2); otherwise each wave loads its rows into registers,
+// one tile ahead: few rows, or few keys.
 // ---------------------------------------------------------------------------------------
 struct WeightParams {
   ChunkParams c;
@@ -551,19 +588,36 @@ struct WeightParams {
   int64_t sl[2];
 };
 
-template <int D, int DT, int KW, bool MASKED>
-__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2)))
+// A lane's place among the rows of a KV head (token i of the chunk, query head g of the group),
+// moved a fixed number of rows at a time without a division.
+struct RowPlace {
+  int i, g;
+  __device__ __forceinline__ void move(int di, int dg, int G) {
+    i += di;
+    g += dg;
+    if (g >= G) {
+      g -= G;
+      ++i;
+    }
+  }
+};
+
+constexpr int vm_wait(int n) { return (n & 15) | ((n >> 4) << 14) | (7 << 4) | (15 << 8); }
+
+template <int D, int DT, int KW, bool RING, bool MASKED>
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(RING && D == 128 ? 2 : 3)))
 chunk_weights_kernel(const WeightParams wp) {
   constexpr int KSTEPS = D / 16;
   constexpr int ROWB = D * 2;
   constexpr int RPU = 1024 / ROWB;
-  constexpr int RW = 4 / KW;               // waves that share one set of keys
-  constexpr int ROWS = kTile / RW;         // K rows a wave brings
-  constexpr int TILE = kTile * ROWB;
+  constexpr int RW = 4 / KW;               // waves that share one of the KW sets of keys
+  constexpr int STAGE = RING ? kTile * ROWB : 16;
   const ChunkParams& p = wp.c;
-  constexpr int RED = 4 * 32 * kWave * 4;  // the sums of every wave, once K is in registers
-  __shared__ __attribute__((aligned(1024))) uint8_t k_lds[KW * TILE > RED ? KW * TILE : RED];
-  float(*red)[32][kWave] = (float(*)[32][kWave])k_lds;
+  __shared__ __attribute__((aligned(1024))) uint8_t s0_lds[STAGE];
+  __shared__ __attribute__((aligned(1024))) uint8_t s1_lds[STAGE];
+  __shared__ __attribute__((aligned(1024))) uint8_t s2_lds[STAGE];
+  __shared__ __attribute__((aligned(1024))) uint8_t s3_lds[STAGE];
+  __shared__ float lse_lds[4][4][kWave];   // stage, wave (its own copy), row; few keys: the sums
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int kg = wave % KW, rg = wave / KW;
@@ -577,65 +631,41 @@ chunk_weights_kernel(const WeightParams wp) {
   const int key0 = (member * KW + kg) * kTile;
   const int wg0 = member * KW * kTile;
 
-  float total = 0.f;  // of key key0 + lane, in the first wave of its keys
+  float total = 0.f;  // of this lane's key, in the first wave of its keys
   if (wg0 < sq.kv && sq.len > 0) {
-    uint8_t* kS = k_lds + kg * TILE;
-    {
-      const uint16_t* kbase = p.k + kvh * p.sk[2];
-      const int32_t* table = p.table + n * p.bt_stride;
-      const int last = (sq.kv - 1) >> p.ps_shift;
-#pragma unroll
-      for (int e = 0; e < ROWS / 8; ++e) {
-        const int r0 = rg * ROWS + 8 * e, r = key0 + r0;
-        const int64_t page = min(max(scalar_load(table + min(r >> p.ps_shift, last)), 0), p.num_pages - 1);
-        const int in_page = r & ((1 << p.ps_shift) - 1);
-        const __amdgpu_buffer_rsrc_t kr =
-            rows_rsrc(kbase + page * p.sk[0] + in_page * p.sk[1], min(sq.kv - r, 8), p.sk[1], D);
-#pragma unroll
-        for (int u = 0; u < 8 / RPU; ++u) {
-          const int r8 = u * RPU + lane / (ROWB / 16), row = r0 + r8;
-          chunk_dma(kr, kS + r0 * ROWB + u * 1024,
-                    (r8 * (int)p.sk[1] + chunk_swz_k<D>(row, lane % (ROWB / 16)) * 8) * 2);
-        }
-      }
-    }
-    __builtin_amdgcn_s_waitcnt(0x0070);
-    chunk_barrier();
+    // K as the A operand, from memory: keys 32 t + col, dims 16 ks + 8 half .. + 7. (Once per wave;
+    // through LDS it took the memory of another workgroup per CU.) Keys past the last one read it.
     u32x4_t kf[2][KSTEPS];
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
+    for (int t = 0; t < 2; ++t) {
+      const int r = min(key0 + t * 32 + col, sq.kv - 1);
+      const int64_t page = min(max(p.table[n * p.bt_stride + (r >> p.ps_shift)], 0), p.num_pages - 1);
+      const uint16_t* kr = p.k + page * p.sk[0] + (r & ((1 << p.ps_shift) - 1)) * p.sk[1] + kvh * p.sk[2] + half * 8;
 #pragma unroll
-      for (int ks = 0; ks < KSTEPS; ++ks) {
-        const int r = t * 32 + col;
-        kf[t][ks] = *(const u32x4_t*)(kS + r * ROWB + chunk_swz_k<D>(r, ks * 2 + half) * 16);
-      }
+      for (int ks = 0; ks < KSTEPS; ++ks) kf[t][ks] = *(const u32x4_t*)(kr + ks * 16);
+    }
     f32x16_t a0 = (f32x16_t){}, a1 = (f32x16_t){};
     const int rows = sq.len * p.G;
-    // The first row that sees this wave's first key.
-    const int first = p.causal ? max(key0 - sq.p0, 0) : 0;
+    // The first row that sees the workgroup's first key.
+    const int first = p.causal ? max(wg0 - sq.p0, 0) : 0;
     const int block0 = sq.p0 >> (MASKED ? p.bs_shift : 0);
-    const int r_first = key0 >= sq.kv ? rows : (int)min((int64_t)first * p.G, (int64_t)rows);
-    for (int r0 = (r_first / 32 + rg) * 32; r0 < rows; r0 += 32 * RW) {
-      const int r = min(r0 + col, rows - 1), i = r / p.G, h = kvh * p.G + (r - i * p.G);
-      const int64_t tok = sq.t0 + i;
-      const uint16_t* qr = p.q + tok * p.sq[0] + h * p.sq[1] + half * 8;
-      u32x4_t qf[KSTEPS];
-#pragma unroll
-      for (int ks = 0; ks < KSTEPS; ++ks) qf[ks] = *(const u32x4_t*)(qr + ks * 16);
-      const float lse = wp.lse[tok * wp.sl[0] + h * wp.sl[1]];
-      const int lim = p.causal ? min(sq.p0 + i, sq.kv - 1) : sq.kv - 1;
-      // A row without keys (lse -inf) or behind the last one adds nothing.
-      const bool on = r0 + col < rows && lse != -INFINITY;
-      int lim0 = on ? lim - key0 - 4 * half : -1, lim1 = lim0 < 0 ? -1 : lim0 - 32;
+    const int r_first = (int)min((int64_t)first * p.G, (int64_t)rows);
+
+    // Adds a tile of 32 rows: Q as the B operand; this lane's row is at `at`, its log-sum `lse`.
+    auto add_rows = [&](const u32x4_t* qf, RowPlace at, bool ok, float lse) TASFT_INLINE {
+      const int lim = p.causal ? min(sq.p0 + at.i, sq.kv - 1) : sq.kv - 1;
+      // How far the row sees into the two halves of the keys, in the lane's count. A row without
+      // keys (lse -inf) or behind the last one adds nothing.
+      int lim0 = ok && lse != -INFINITY ? lim - key0 - 4 * half : -1, lim1 = lim0 - 32;
       if constexpr (MASKED) {
-        const int mr = min(max(((sq.p0 + i) >> p.bs_shift) - block0, 0), p.mask_rows - 1);
-        const uint8_t* m = p.mask + n * p.sm[0] + h * p.sm[1] + mr * p.sm[2];
+        // (A row past the last one stays within the mask, by its row's and head's limits.)
+        const int mr = min(max(((sq.p0 + at.i) >> p.bs_shift) - block0, 0), p.mask_rows - 1);
+        const uint8_t* m = p.mask + n * p.sm[0] + (int64_t)(kvh * p.G + at.g) * p.sm[1] + mr * p.sm[2];
         const int last_block = (p.cap - 1) >> p.bs_shift;
-        const bool m0 = m[min(key0 >> p.bs_shift, last_block) * p.sm[3]] != 0;
-        const bool m1 = m[min((key0 + 32) >> p.bs_shift, last_block) * p.sm[3]] != 0;
-        if (!m0) lim0 = -1;
-        if (!m1) lim1 = -1;
+        if (m[min(key0 >> p.bs_shift, last_block) * p.sm[3]] == 0) lim0 = -1;
+        if (m[min((key0 + 32) >> p.bs_shift, last_block) * p.sm[3]] == 0) lim1 = -1;
       }
+      if (__ballot(max(lim0, lim1) >= 0) == 0) return;
       f32x16_t s0 = (f32x16_t){}, s1 = (f32x16_t){};
 #pragma unroll
       for (int ks = 0; ks < KSTEPS; ++ks) {
@@ -645,30 +675,175 @@ chunk_weights_kernel(const WeightParams wp) {
       const float l2 = lse * kLog2e;
 #pragma unroll
       for (int rr = 0; rr < 16; ++rr) {
-        const int off = 8 * (rr >> 2) + (rr & 3);
-        const float e0 = __builtin_amdgcn_exp2f(fmaf(s0[rr], p.scale_log2, -l2));
-        const float e1 = __builtin_amdgcn_exp2f(fmaf(s1[rr], p.scale_log2, -l2));
-        a0[rr] += off > lim0 ? 0.f : e0;
-        a1[rr] += off > lim1 ? 0.f : e1;
+        s0[rr] = __builtin_amdgcn_exp2f(fmaf(s0[rr], p.scale_log2, -l2));
+        s1[rr] = __builtin_amdgcn_exp2f(fmaf(s1[rr], p.scale_log2, -l2));
+      }
+      // The last key of a half has offset 27 in the lanes' own count.
+      if (__ballot(min(lim0, lim1) < 27) != 0) {
+        asm volatile("");  // a branch, not 64 selections in every tile
+#pragma unroll
+        for (int rr = 0; rr < 16; ++rr) {
+          const int off = 8 * (rr >> 2) + (rr & 3);
+          s0[rr] = off > lim0 ? 0.f : s0[rr];
+          s1[rr] = off > lim1 ? 0.f : s1[rr];
+        }
+      }
+      a0 += s0;
+      a1 += s1;
+    };
+    // The place of row r, of the last row if there is no such row.
+    auto place_of = [&](int r) TASFT_INLINE {
+      RowPlace at;
+      at.i = r / p.G;
+      at.g = r - at.i * p.G;
+      return at;
+    };
+    const int64_t head0 = (int64_t)kvh * p.G;
+
+    if constexpr (RING) {
+      constexpr int UNITS = 16 / RPU;  // of a wave's 16 rows of a step
+      constexpr int IN_FLIGHT = 2 * (UNITS + 1);
+      const int di = kTile / p.G, dg = kTile - di * p.G;
+      const int r_start = r_first / kTile * kTile;
+      const int steps = (rows - r_start + kTile - 1) / kTile;
+      // Byte offsets of the rows a lane brings, moved a step at a time (the host sees to it that 32
+      // bits hold them). The buffers end with the sequence's last row: rows past it are zeros.
+      const int tokb = (int)p.sq[0] * 2, headb = (int)p.sq[1] * 2;
+      const int tokl = (int)wp.sl[0] * 4, headl = (int)wp.sl[1] * 4;
+      const __amdgpu_buffer_rsrc_t qr = __builtin_amdgcn_make_buffer_rsrc(
+          (void*)(p.q + (int64_t)sq.t0 * p.sq[0] + head0 * p.sq[1]), (short)0,
+          (sq.len - 1) * tokb + (p.G - 1) * headb + ROWB, 0x00020000);
+      const __amdgpu_buffer_rsrc_t lr = __builtin_amdgcn_make_buffer_rsrc(
+          (void*)(wp.lse + (int64_t)sq.t0 * wp.sl[0] + head0 * wp.sl[1]), (short)0,
+          (sq.len - 1) * tokl + (p.G - 1) * headl + 4, 0x00020000);
+      struct Source {
+        int off, g;
+      };
+      auto move = [&](Source& x, int tb, int hb) TASFT_INLINE {
+        x.off += di * tb + dg * hb;
+        if (dg != 0) {
+          x.g += dg;
+          const bool wrap = x.g >= p.G;
+          x.off += wrap ? tb - p.G * hb : 0;
+          x.g -= wrap ? p.G : 0;
+        }
+      };
+      Source src[UNITS], lsrc;
+      RowPlace tile[2];
+#pragma unroll
+      for (int u = 0; u < UNITS; ++u) {
+        const int row = wave * 16 + u * RPU + lane / (ROWB / 16);
+        const RowPlace at = place_of(r_start + row);
+        src[u] = {at.i * tokb + at.g * headb + chunk_swz_k<D>(row, lane % (ROWB / 16)) * 16, at.g};
+      }
+      {
+        const RowPlace at = place_of(r_start + lane);
+        lsrc = {at.i * tokl + at.g * headl, at.g};
+      }
+#pragma unroll
+      for (int t = 0; t < 2; ++t) tile[t] = place_of(r_start + t * 32 + col);
+      auto dma_step = [&](uint8_t* stage, float* lstage) TASFT_INLINE {
+#pragma unroll
+        for (int u = 0; u < UNITS; ++u) {
+          chunk_dma(qr, stage + (wave * 16 + u * RPU) * ROWB, src[u].off);
+          move(src[u], tokb, headb);
+        }
+        chunk_dma4(lr, lstage, lsrc.off);
+        move(lsrc, tokl, headl);
+      };
+      dma_step(s0_lds, lse_lds[0][wave]);
+      dma_step(s1_lds, lse_lds[1][wave]);
+      dma_step(s2_lds, lse_lds[2][wave]);
+      // Every step issues the DMA of the one three steps on (past the end: zeros that no step
+      // reads), so that the wait is for a fixed count. By the barrier every wave's share has
+      // landed, and every wave is done with the stage that is filled next.
+      auto step = [&](const uint8_t* now, const float* lnow, uint8_t* then, float* lthen) TASFT_INLINE {
+        __builtin_amdgcn_s_waitcnt(vm_wait(IN_FLIGHT));
+        __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
+        chunk_barrier();
+        if constexpr (!MASKED) dma_step(then, lthen);
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          u32x4_t qf[KSTEPS];
+          const int r = t * 32 + col;
+#pragma unroll
+          for (int ks = 0; ks < KSTEPS; ++ks)
+            qf[ks] = *(const u32x4_t*)(now + r * ROWB + chunk_swz_k<D>(r, ks * 2 + half) * 16);
+          add_rows(qf, tile[t], tile[t].i < sq.len, lnow[r]);
+          tile[t].move(di, dg, p.G);
+        }
+        // Behind the mask bytes' loads: the wait for them would wait for it too.
+        if constexpr (MASKED) dma_step(then, lthen);
+      };
+      for (int s = 0; s < steps; s += 4) {
+        step(s0_lds, lse_lds[0][wave], s3_lds, lse_lds[3][wave]);
+        if (s + 1 >= steps) break;
+        step(s1_lds, lse_lds[1][wave], s0_lds, lse_lds[0][wave]);
+        if (s + 2 >= steps) break;
+        step(s2_lds, lse_lds[2][wave], s1_lds, lse_lds[1][wave]);
+        if (s + 3 >= steps) break;
+        step(s3_lds, lse_lds[3][wave], s2_lds, lse_lds[2][wave]);
+      }
+      __builtin_amdgcn_s_waitcnt(0x0f70);  // no DMA into this workgroup's LDS outlives it
+    } else {
+      constexpr int STEP = 32 * RW;
+      struct Rows {
+        u32x4_t q[KSTEPS];
+        RowPlace at;
+        float lse;
+        bool ok;
+      };
+      auto load_rows = [&](Rows& t, int r0) TASFT_INLINE {
+        t.ok = r0 + col < rows;
+        t.at = place_of(min(r0 + col, rows - 1));
+        const int64_t tok = sq.t0 + t.at.i, h = head0 + t.at.g;
+        const uint16_t* qr = p.q + tok * p.sq[0] + h * p.sq[1] + half * 8;
+#pragma unroll
+        for (int ks = 0; ks < KSTEPS; ++ks) t.q[ks] = *(const u32x4_t*)(qr + ks * 16);
+        t.lse = wp.lse[tok * wp.sl[0] + h * wp.sl[1]];
+      };
+      int r0 = (r_first / 32 + rg) * 32;
+      if (r0 < rows) {
+        Rows even, odd;
+        load_rows(even, r0);
+        for (; r0 < rows; r0 += 2 * STEP) {
+          load_rows(odd, r0 + STEP);  // past the end: the last row again, not used
+          add_rows(even.q, even.at, even.ok, even.lse);
+          if (r0 + STEP >= rows) break;
+          load_rows(even, r0 + 2 * STEP);
+          add_rows(odd.q, odd.at, odd.ok, odd.lse);
+        }
       }
     }
-    __syncthreads();  // every wave has its K
+    // Sums over the 32 rows of a half's lanes, halving the registers each time: lanes whose bit is
+    // set go on with the upper registers' sums. Lane col ends with the sum of register col.
+    float v[32];
 #pragma unroll
-    for (int rr = 0; rr < 16; ++rr) {
-      red[wave][rr][lane] = a0[rr];
-      red[wave][16 + rr][lane] = a1[rr];
+    for (int j = 0; j < 16; ++j) {
+      const auto sw = __builtin_amdgcn_permlane16_swap(__float_as_uint(a0[j]), __float_as_uint(a1[j]), false, false);
+      v[j] = __uint_as_float(sw[0]) + __uint_as_float(sw[1]);
     }
-    __syncthreads();
-    if (rg == 0) {
-      // Key lane: tile lane / 32, half (lane / 4) % 2, register of the rest. The columns start
-      // at the lane's own, so that lanes read different banks.
-      const int k32 = lane & 31, hh = (k32 >> 2) & 1, reg = (lane >> 5) * 16 + (k32 >> 3) * 4 + (k32 & 3);
+    auto halve = [&](auto ctrl, int n2, int bit) TASFT_INLINE {
 #pragma unroll
-      for (int w = 0; w < RW; ++w)
-        for (int j = 0; j < 32; ++j) total += red[w * KW + kg][reg][hh * 32 + ((j + lane) & 31)];
+      for (int j = 0; j < 8; ++j)
+        if (j < n2) {
+          const bool up = (lane & bit) != 0;
+          const float mine = up ? v[j + n2] : v[j], other = up ? v[j] : v[j + n2];
+          v[j] = mine + dpp_f32<decltype(ctrl)::value>(other);
+        }
+    };
+    halve(std::integral_constant<int, 0x140>{}, 8, 8);  // row_mirror
+    halve(std::integral_constant<int, 0x141>{}, 4, 4);  // row_half_mirror
+    halve(std::integral_constant<int, 0x1B>{}, 2, 2);   // quad_perm [3, 2, 1, 0]
+    halve(std::integral_constant<int, 0xB1>{}, 1, 1);   // quad_perm [1, 0, 3, 2]
+    total = v[0];
+    if constexpr (RW > 1) {
+      lse_lds[0][wave][lane] = total;
+      __syncthreads();
+      total = (lse_lds[0][0][lane] + lse_lds[0][1][lane]) + (lse_lds[0][2][lane] + lse_lds[0][3][lane]);
     }
   }
-  const int key = key0 + lane;
+  const int key = key0 + (col >> 4) * 32 + ((col & 15) >> 2) * 8 + (col & 3) + 4 * half;
   if (rg == 0 && key < p.cap) {
     const float before = wp.scores ? wp.scores[n * wp.ss[0] + kvh * wp.ss[1] + key * wp.ss[2]] : 0.f;
     wp.out[((int64_t)n * p.Hkv + kvh) * p.cap + key] = key < sq.kv ? before + total : before;
@@ -826,15 +1001,21 @@ static void launch_weights(const WeightParams& w, hipStream_t stream) {
   const ChunkParams& p = w.c;
   const int64_t heads = (int64_t)p.N * p.Hkv;
   auto grid = [&](int kw) { return heads * ((p.cap + kw * kTile - 1) / (kw * kTile)); };
-  if (grid(4) >= 512) {
-    const dim3 g((unsigned)grid(4));
-    if (p.mask) hipLaunchKernelGGL((chunk_weights_kernel<D, DT, 4, true>), g, dim3(256), 0, stream, w);
-    else hipLaunchKernelGGL((chunk_weights_kernel<D, DT, 4, false>), g, dim3(256), 0, stream, w);
-  } else {
-    const dim3 g((unsigned)grid(1));
-    if (p.mask) hipLaunchKernelGGL((chunk_weights_kernel<D, DT, 1, true>), g, dim3(256), 0, stream, w);
-    else hipLaunchKernelGGL((chunk_weights_kernel<D, DT, 1, false>), g, dim3(256), 0, stream, w);
-  }
+  // Byte offsets within a sequence's rows of Q and log-sums, a few steps past the end included.
+  const int64_t most = ((int64_t)1 << 31) - 1;
+  const bool small = ((int64_t)p.L + 5 * kTile) * p.sq[0] * 2 + p.G * p.sq[1] * 2 + D * 2 < most &&
+                     ((int64_t)p.L + 5 * kTile) * w.sl[0] * 4 + p.G * w.sl[1] * 4 + 4 < most;
+  auto run = [&](auto plain, auto masked, int64_t wgs) {
+    if (p.mask) hipLaunchKernelGGL(masked, dim3((unsigned)wgs), dim3(256), 0, stream, w);
+    else hipLaunchKernelGGL(plain, dim3((unsigned)wgs), dim3(256), 0, stream, w);
+  };
+  // Few keys (not two workgroups of 256 keys per CU): four times as many workgroups.
+  if (grid(4) < 512)
+    run(chunk_weights_kernel<D, DT, 1, false, false>, chunk_weights_kernel<D, DT, 1, false, true>, grid(1));
+  else if ((int64_t)p.L * p.G <= 128 || !small)
+    run(chunk_weights_kernel<D, DT, 4, false, false>, chunk_weights_kernel<D, DT, 4, false, true>, grid(4));
+  else
+    run(chunk_weights_kernel<D, DT, 4, true, false>, chunk_weights_kernel<D, DT, 4, true, true>, grid(4));
 }
 
 extern "C" int tasft_key_weights(

@@ -6,21 +6,19 @@
 // that reads them later, so nothing is shifted: the kept slots behind n' move into the holes
 // before it, both in ascending order. That moves each such key once and no other.
 //
-// Two launches. The first, one workgroup of 1024 threads per (sequence, head), finds the
-// weight of the n'-th key by a radix selection (three digits of 11, 11 and 10 bits over an
-// order-preserving image of the weight) and numbers holes and movers with ballots; a thread
-// keeps the images of its slots in registers (up to 32 of them, 32768 slots; beyond that they
-// are read again). The second copies rows, many workgroups per head. Sources lie behind n',
-// destinations before it: no row is read and written. Bound by the bytes of the moved rows and
-// of weights and positions, in small calls by the selection's chain of barriers.
+// Two launches. The first, one workgroup per (sequence, head), finds the weight of the n'-th key
+// by a radix selection (three digits of 11, 11 and 10 bits over an order-preserving image of the
+// weight, bins in LDS) and numbers holes and movers: ballots count them per round and wave, one
+// prefix over those counts places them. The second copies rows, many workgroups per head.
+// Sources lie behind n', destinations before it: no row is read and written. Bound by the bytes
+// of the moved rows and of weights and positions, in small calls by the selection's chain of
+// barriers.
 #include "common.h"
 
 #include "../../include/tasft_amd.h"
 
 namespace tasft {
 
-constexpr int kSelThreads = 1024;
-constexpr int kSelWaves = kSelThreads / kWave;
 constexpr int kBins = 2048;
 constexpr int kMoveThreads = 256;
 
@@ -51,30 +49,21 @@ __device__ __forceinline__ uint32_t weight_image(float w) {
   return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 
-// Exclusive prefix over the workgroup, in thread order, of a flag; `total` receives the sum.
-// `tmp` holds kSelWaves ints; a barrier separates two uses of one `tmp`.
-__device__ __forceinline__ int block_rank(bool f, int* tmp, int lane, int wave, int& total) {
-  const uint64_t bal = __ballot(f);
-  if (lane == 0) tmp[wave] = __popcll(bal);
-  __syncthreads();
-  int before = 0, all = 0;
-#pragma unroll
-  for (int w = 0; w < kSelWaves; ++w) {
-    const int c = tmp[w];
-    before += w < wave ? c : 0;
-    all += c;
-  }
-  total = all;
-  return before + __popcll(bal & ((1ull << lane) - 1ull));
-}
-
-// KPT: images a thread keeps (0: none, they are formed again from memory).
-template <int KPT>
-__global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const EvictParams p) {
-  __shared__ uint32_t hist[kBins];
-  __shared__ int wtmp[3][kSelWaves];
+// THREADS threads with KPT slots each, THREADS * KPT slots at a time: a thread's slots are
+// THREADS apart, so that a round of all threads is a run of slots in order. Where a head has more
+// slots (MANY), the runs of slots are taken one after the other, in each of the passes.
+template <int THREADS, int KPT, bool MANY>
+__global__ void __launch_bounds__(THREADS) evict_select_kernel(const EvictParams p) {
+  constexpr int WAVES = THREADS / kWave;
+  constexpr int RUN = THREADS * KPT;
+  constexpr int CELLS = WAVES * KPT;    // (round, wave) pairs of a run, in slot order
+  constexpr int BPT = kBins / THREADS;  // bins a thread sums up
+  static_assert(CELLS <= THREADS, "one thread a cell");
+  __shared__ uint32_t hist[3][kBins];
+  __shared__ int cells[3][CELLS], base[3][CELLS];
+  __shared__ int wtmp[WAVES];
   __shared__ int s_newest;
-  __shared__ uint32_t s_bin, s_left;
+  __shared__ uint32_t s_bin, s_left, s_count;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int nh = blockIdx.x, n = nh / p.Hkv, h = nh % p.Hkv;
   const int len = (int)min((int64_t)max(p.kv_lens[n], 0), p.cap);
@@ -88,130 +77,214 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const EvictPa
   if (h == 0 && tid == 0) p.kv_lens_out[n] = keep;
 
   // Slots behind the kept ones; with nothing to evict the rest is copied as it is.
-  for (int64_t i = keep + tid; i < p.cap; i += kSelThreads) {
-    so[i] = 0.f;
-    pout[i] = -1;
-  }
+  auto clear_rest = [&]() {
+    for (int64_t i = keep + tid; i < p.cap; i += THREADS) {
+      so[i] = 0.f;
+      pout[i] = -1;
+    }
+  };
   if (len <= p.budget) {
-    for (int i = tid; i < keep; i += kSelThreads) {
+    for (int i = tid; i < keep; i += THREADS) {
       so[i] = sc[i * ss];
       pout[i] = po[i * sp];
     }
+    clear_rest();
     if (tid == 0) moves[0] = 0;
     return;
   }
 
+  // Weights and positions of the first run, all loads in flight together. Up to 16 slots a thread
+  // they stay in registers, beyond that only the images do.
+  constexpr bool HOLD = KPT <= 16 && !MANY;
+  const int runs = MANY ? (len + RUN - 1) / RUN : 1;
+  float w[HOLD ? KPT : 1];
+  int32_t pos[HOLD ? KPT : 1];
+  uint32_t img[KPT];
+  int newest = -0x7fffffff - 1;
+#pragma unroll
+  for (int r = 0; r < KPT; ++r) {
+    const int i = min(r * THREADS + tid, len - 1);
+    const int32_t x = po[i * sp];
+    if constexpr (HOLD) {
+      w[r] = sc[i * ss];
+      pos[r] = x;
+    }
+    newest = max(newest, x);
+  }
+  for (int i = tid; i < 3 * kBins; i += THREADS) (&hist[0][0])[i] = 0;
   if (tid == 0) s_newest = -0x7fffffff - 1;
   __syncthreads();
-  int newest = -0x7fffffff - 1;
-  for (int i = tid; i < len; i += kSelThreads) newest = max(newest, po[i * sp]);
+  if constexpr (MANY)
+    for (int i = RUN + tid; i < len; i += THREADS) newest = max(newest, po[i * sp]);
 #pragma unroll
   for (int off = 32; off >= 1; off >>= 1) newest = max(newest, __shfl_xor(newest, off, kWave));
   if (lane == 0) atomicMax(&s_newest, newest);
   __syncthreads();
   const int64_t first_recent = (int64_t)s_newest - p.recent;  // positions above it are recent
-  auto image_at = [&](int i) -> uint32_t {
-    const int32_t pos = po[i * sp];
-    const float w = sc[i * ss];
-    return pos < p.sinks || pos > first_recent ? 0xffffffffu : weight_image(w);
+  auto image = [&](float weight, int32_t position) {
+    return position < p.sinks || position > first_recent ? 0xffffffffu : weight_image(weight);
   };
-  const int rounds = (len + kSelThreads - 1) / kSelThreads;
-  uint32_t img[KPT > 0 ? KPT : 1];
-  if constexpr (KPT > 0) {
+  // The thread's number again, opaque: addresses of one pass are not kept in registers for another.
+  auto again = [&]() {
+    int t = tid;
+    if constexpr (!HOLD) asm volatile("" : "+v"(t));
+    return t;
+  };
+  auto form_images = [&](int run) {  // 0 for slots past the last
 #pragma unroll
-    for (int r = 0; r < KPT; ++r) {
-      const int i = r * kSelThreads + tid;
-      img[r] = i < len ? image_at(i) : 0u;
-    }
-  }
-  // Calls f(slot, image, in range) for this thread's slots in ascending order; every thread of
-  // the workgroup makes the same number of calls.
-  auto each = [&](auto f) {
-    if constexpr (KPT > 0) {
+    for (int r0 = 0; r0 < KPT; r0 += 8) {
+      const int t = again();
 #pragma unroll
-      for (int r = 0; r < KPT; ++r)
-        if (r < rounds) f(r * kSelThreads + tid, img[r], r * kSelThreads + tid < len);
-    } else {
-      for (int r = 0; r < rounds; ++r) {
-        const int i = r * kSelThreads + tid;
-        f(i, i < len ? image_at(i) : 0u, i < len);
+      for (int r = r0; r < r0 + 8; ++r) {
+        const int i = run * RUN + r * THREADS + t, j = min(i, len - 1);
+        const uint32_t x = HOLD ? image(w[HOLD ? r : 0], pos[HOLD ? r : 0]) : image(sc[j * ss], po[j * sp]);
+        img[r] = i < len ? x : 0u;
       }
+      if constexpr (!HOLD) asm volatile("" ::: "memory");  // eight slots' loads at a time: registers
     }
+  };
+  form_images(0);
+  auto take_run = [&](int run) {
+    if constexpr (MANY) form_images(run);
   };
 
   // The keep-th largest image, digit by digit.
-  uint32_t prefix = 0, left = (uint32_t)keep;
+  uint32_t prefix = 0, left = (uint32_t)keep, equal = 0;
+#pragma unroll
   for (int d = 0; d < 3; ++d) {
     const int shift = d == 0 ? 21 : (d == 1 ? 10 : 0);
     const int bits = d == 2 ? 10 : 11;
     const uint32_t above = d == 0 ? 0u : (0xffffffffu << (shift + bits));
-    for (int i = tid; i < kBins; i += kSelThreads) hist[i] = 0;
-    __syncthreads();
-    each([&](int, uint32_t x, bool in) {
-      const bool on = in && (x & above) == prefix;
-      const uint32_t bin = (x >> shift) & ((1u << bits) - 1u);
-      // One bin for the whole wave (equal weights, protected runs): one addition.
-      const uint64_t live = __ballot(on);
-      if (live == 0) return;
-      const uint32_t first = (uint32_t)__builtin_amdgcn_readlane((int)bin, __builtin_ctzll(live));
-      if (__ballot(on && bin != first) == 0) {
-        if (lane == __builtin_ctzll(live)) atomicAdd(&hist[first], (uint32_t)__popcll(live));
-      } else if (on) {
-        atomicAdd(&hist[bin], 1u);
+    for (int run = 0; run < runs; ++run) {
+      take_run(run);
+#pragma unroll
+      for (int r = 0; r < KPT; ++r) {
+        const bool on = img[r] != 0u && (img[r] & above) == prefix;
+        const uint64_t live = __ballot(on);
+        if (live == 0) continue;
+        // One bin for the whole wave (equal weights, protected runs): one addition.
+        const uint32_t bin = (img[r] >> shift) & ((1u << bits) - 1u);
+        const int lead = __builtin_ctzll(live);
+        const uint32_t first = (uint32_t)__builtin_amdgcn_readlane((int)bin, lead);
+        if (__ballot(on && bin != first) == 0) {
+          if (lane == lead) atomicAdd(&hist[d][first], (uint32_t)__popcll(live));
+        } else if (on) {
+          atomicAdd(&hist[d][bin], 1u);
+        }
       }
-    });
+    }
     __syncthreads();
-    // Bins from the top: thread t holds bins 2047 - 2t and 2046 - 2t.
-    const uint32_t c0 = hist[kBins - 1 - 2 * tid], c1 = hist[kBins - 2 - 2 * tid];
-    uint32_t incl = c0 + c1;
+    // Bins from the top: thread t sums up the BPT bins from kBins - 1 - BPT t down.
+    const int top = kBins - 1 - BPT * tid;
+    uint32_t c[BPT], sum = 0;
+#pragma unroll
+    for (int j = 0; j < BPT; ++j) sum += c[j] = hist[d][top - j];
+    uint32_t incl = sum;
 #pragma unroll
     for (int off = 1; off < kWave; off <<= 1) {
       const uint32_t o = __shfl_up(incl, off, kWave);
       if (lane >= off) incl += o;
     }
-    if (lane == 63) wtmp[0][wave] = (int)incl;
+    if (lane == 63) wtmp[wave] = (int)incl;
     __syncthreads();
-    uint32_t before = incl - c0 - c1;
-    for (int w = 0; w < wave; ++w) before += (uint32_t)wtmp[0][w];
-    if (before < left && left <= before + c0) {
-      s_bin = kBins - 1 - 2 * tid;
-      s_left = left - before;
-    } else if (before + c0 < left && left <= before + c0 + c1) {
-      s_bin = kBins - 2 - 2 * tid;
-      s_left = left - before - c0;
+    uint32_t before = incl - sum;
+    for (int v = 0; v < wave; ++v) before += (uint32_t)wtmp[v];
+    if (before < left && left <= before + sum) {
+#pragma unroll
+      for (int j = 0; j < BPT; ++j) {
+        if (before < left && left <= before + c[j]) {
+          s_bin = top - j;
+          s_left = left - before;
+          s_count = c[j];
+        }
+        before += c[j];
+      }
     }
     __syncthreads();
     prefix |= s_bin << shift;
     left = s_left;
+    equal = s_count;
   }
-  const uint32_t limit = prefix;  // images above it stay, and the first `left` equal to it
+  // Images above `prefix` stay, and the first `left` of the `equal` ones equal to it.
+  const uint32_t limit = prefix;
+  const bool split_equal = left < equal;
 
-  int eq_base = 0, hole_base = 0, move_base = 0;
+  // Numbers of flagged slots before each (round, wave) of the run: its counts in `cells[which]`
+  // to `base[which]`; carry is the number before the run.
+  auto number_cells = [&](int which, int carry) {
+    int x = tid < CELLS ? cells[which][tid] : 0;
+    const int own = x;
+#pragma unroll
+    for (int off = 1; off < kWave; off <<= 1) {
+      const int o = __shfl_up(x, off, kWave);
+      if (lane >= off) x += o;
+    }
+    if (lane == 63) wtmp[wave] = x;
+    __syncthreads();
+    int before = carry + x - own;
+    for (int v = 0; v < wave; ++v) before += wtmp[v];
+    if (tid < CELLS) base[which][tid] = before;
+    int total = carry;
+#pragma unroll
+    for (int v = 0; v < WAVES; ++v) total += wtmp[v];
+    __syncthreads();
+    return total;
+  };
+  const uint64_t below = (1ull << lane) - 1ull;
   int* holes = moves + 1;
   int* sources = moves + 1 + p.budget;
-  each([&](int i, uint32_t x, bool in) {
-    int total;
-    const int eq = eq_base + block_rank(in && x == limit, wtmp[0], lane, wave, total);
-    eq_base += total;
-    const bool kept = in && (x > limit || (x == limit && eq < (int)left));
-    const bool front = in && i < keep;
-    const int hr = hole_base + block_rank(front && !kept, wtmp[1], lane, wave, total);
-    hole_base += total;
-    const int mr = move_base + block_rank(kept && !front, wtmp[2], lane, wave, total);
-    move_base += total;
-    if (front && kept) {
-      so[i] = sc[i * ss];
-      pout[i] = po[i * sp];
-    } else if (front) {
-      holes[hr] = i;
-    } else if (kept) {
-      sources[mr] = i;
+  int eq_seen = 0, hole_seen = 0, move_seen = 0;
+  for (int run = 0; run < runs; ++run) {
+    take_run(run);
+    if (split_equal) {
+#pragma unroll
+      for (int r = 0; r < KPT; ++r) {
+        const uint64_t bal = __ballot(img[r] == limit);
+        if (lane == 0) cells[0][r * WAVES + wave] = __popcll(bal);
+      }
+      __syncthreads();
+      eq_seen = number_cells(0, eq_seen);
     }
-  });
-  if (tid == 0) moves[0] = hole_base;  // as many movers as holes
+    // One bit a round: kept.
+    uint32_t kept = 0;
+#pragma unroll
+    for (int r = 0; r < KPT; ++r) {
+      const int i = run * RUN + r * THREADS + tid;
+      bool k = img[r] > limit || (img[r] == limit && !split_equal);
+      if (split_equal) {
+        const bool eq = img[r] == limit;
+        const uint64_t bal = __ballot(eq);
+        k = k || (eq && base[0][r * WAVES + wave] + __popcll(bal & below) < (int)left);
+      }
+      kept |= k ? 1u << r : 0u;
+      const uint64_t hb = __ballot(i < keep && !k), mb = __ballot(i >= keep && k);
+      if (lane == 0) {
+        cells[1][r * WAVES + wave] = __popcll(hb);
+        cells[2][r * WAVES + wave] = __popcll(mb);
+      }
+    }
+    __syncthreads();
+    hole_seen = number_cells(1, hole_seen);
+    move_seen = number_cells(2, move_seen);
+#pragma unroll
+    for (int r = 0; r < KPT; ++r) {
+      const int i = run * RUN + r * THREADS + again();
+      const bool k = (kept >> r) & 1u, hole = i < keep && !k, mover = i >= keep && k;
+      const uint64_t hb = __ballot(hole), mb = __ballot(mover);
+      if (hole) holes[base[1][r * WAVES + wave] + __popcll(hb & below)] = i;
+      if (mover) sources[base[2][r * WAVES + wave] + __popcll(mb & below)] = i;
+      if (i < keep && k) {
+        so[i] = HOLD ? w[HOLD ? r : 0] : sc[i * ss];
+        pout[i] = HOLD ? pos[HOLD ? r : 0] : po[i * sp];
+      }
+    }
+    if constexpr (MANY) __syncthreads();  // base is rewritten
+  }
+  if (tid == 0) moves[0] = hole_seen;  // as many movers as holes
+  clear_rest();
   __threadfence_block();
   __syncthreads();
-  for (int r = tid; r < hole_base; r += kSelThreads) {
+  for (int r = tid; r < hole_seen; r += THREADS) {
     const int to = holes[r], from = sources[r];
     so[to] = sc[from * ss];
     pout[to] = po[from * sp];
@@ -314,15 +387,17 @@ extern "C" int tasft_evict_paged(void* k_pages, void* v_pages, const int32_t* bl
   p.num_pages = (int)num_pages;
   const hipStream_t st = (hipStream_t)stream;
   const unsigned heads = (unsigned)(num_seqs * num_kv_heads);
-  const dim3 b(kSelThreads);
-  if (cap <= 2 * kSelThreads)
-    hipLaunchKernelGGL(evict_select_kernel<2>, dim3(heads), b, 0, st, p);
-  else if (cap <= 8 * kSelThreads)
-    hipLaunchKernelGGL(evict_select_kernel<8>, dim3(heads), b, 0, st, p);
-  else if (cap <= 32 * kSelThreads)
-    hipLaunchKernelGGL(evict_select_kernel<32>, dim3(heads), b, 0, st, p);
+  auto select = [&](auto kernel, int threads) { hipLaunchKernelGGL(kernel, dim3(heads), dim3(threads), 0, st, p); };
+  if (cap <= 2048)
+    select(evict_select_kernel<256, 8, false>, 256);
+  else if (cap <= 8192)
+    select(evict_select_kernel<1024, 8, false>, 1024);
+  else if (cap <= 16384)
+    select(evict_select_kernel<1024, 16, false>, 1024);
+  else if (cap <= 32768)
+    select(evict_select_kernel<1024, 32, false>, 1024);
   else
-    hipLaunchKernelGGL(evict_select_kernel<0>, dim3(heads), b, 0, st, p);
+    select(evict_select_kernel<1024, 32, true>, 1024);
   if (const int rc = check_launch("evict select")) return rc;
   // About 16 workgroups per CU over all heads, no more than a head's rows can use.
   const int64_t rows = kMoveThreads / (head_dim / 8);
