@@ -577,7 +577,7 @@ __global__ void __launch_bounds__(256) chunk_combine_kernel(const ChunkParams p)
 // (KW = 4) read Q less often, few keys (KW = 1) want four times as many workgroups. RING: the
 // waves walk the same rows, 64 a step, that come by DMA into a ring of four LDS stages, three steps
 // ahead (a step is shorter than a trip to L2); otherwise each wave loads its rows into registers,
-// one tile ahead: few rows, or few keys.
+// the next tile's under the exponentials of one: few rows, or few keys.
 // ---------------------------------------------------------------------------------------
 struct WeightParams {
   ChunkParams c;
@@ -652,7 +652,8 @@ chunk_weights_kernel(const WeightParams wp) {
     const int r_first = (int)min((int64_t)first * p.G, (int64_t)rows);
 
     // Adds a tile of 32 rows: Q as the B operand; this lane's row is at `at`, its log-sum `lse`.
-    auto add_rows = [&](const u32x4_t* qf, RowPlace at, bool ok, float lse) TASFT_INLINE {
+    // between() runs when Q has been used.
+    auto add_rows = [&](const u32x4_t* qf, RowPlace at, bool ok, float lse, auto between) TASFT_INLINE {
       const int lim = p.causal ? min(sq.p0 + at.i, sq.kv - 1) : sq.kv - 1;
       // How far the row sees into the two halves of the keys, in the lane's count. A row without
       // keys (lse -inf) or behind the last one adds nothing.
@@ -665,13 +666,15 @@ chunk_weights_kernel(const WeightParams wp) {
         if (m[min(key0 >> p.bs_shift, last_block) * p.sm[3]] == 0) lim0 = -1;
         if (m[min((key0 + 32) >> p.bs_shift, last_block) * p.sm[3]] == 0) lim1 = -1;
       }
-      if (__ballot(max(lim0, lim1) >= 0) == 0) return;
+      // Many tiles: those that no row sees are left out, and the selections of those that all see.
+      if (RING && __ballot(max(lim0, lim1) >= 0) == 0) return;
       f32x16_t s0 = (f32x16_t){}, s1 = (f32x16_t){};
 #pragma unroll
       for (int ks = 0; ks < KSTEPS; ++ks) {
         s0 = mfma16<DT>(kf[0][ks], qf[ks], s0);
         s1 = mfma16<DT>(kf[1][ks], qf[ks], s1);
       }
+      between();
       const float l2 = lse * kLog2e;
 #pragma unroll
       for (int rr = 0; rr < 16; ++rr) {
@@ -679,8 +682,8 @@ chunk_weights_kernel(const WeightParams wp) {
         s1[rr] = __builtin_amdgcn_exp2f(fmaf(s1[rr], p.scale_log2, -l2));
       }
       // The last key of a half has offset 27 in the lanes' own count.
-      if (__ballot(min(lim0, lim1) < 27) != 0) {
-        asm volatile("");  // a branch, not 64 selections in every tile
+      if (!RING || __ballot(min(lim0, lim1) < 27) != 0) {
+        if constexpr (RING) asm volatile("");  // a branch, not 64 selections in every tile
 #pragma unroll
         for (int rr = 0; rr < 16; ++rr) {
           const int off = 8 * (rr >> 2) + (rr & 3);
@@ -769,7 +772,7 @@ chunk_weights_kernel(const WeightParams wp) {
 #pragma unroll
           for (int ks = 0; ks < KSTEPS; ++ks)
             qf[ks] = *(const u32x4_t*)(now + r * ROWB + chunk_swz_k<D>(r, ks * 2 + half) * 16);
-          add_rows(qf, tile[t], tile[t].i < sq.len, lnow[r]);
+          add_rows(qf, tile[t], tile[t].i < sq.len, lnow[r], [] {});
           tile[t].move(di, dg, p.G);
         }
         // Behind the mask bytes' loads: the wait for them would wait for it too.
@@ -787,32 +790,22 @@ chunk_weights_kernel(const WeightParams wp) {
       __builtin_amdgcn_s_waitcnt(0x0f70);  // no DMA into this workgroup's LDS outlives it
     } else {
       constexpr int STEP = 32 * RW;
-      struct Rows {
-        u32x4_t q[KSTEPS];
-        RowPlace at;
-        float lse;
-        bool ok;
-      };
-      auto load_rows = [&](Rows& t, int r0) TASFT_INLINE {
-        t.ok = r0 + col < rows;
-        t.at = place_of(min(r0 + col, rows - 1));
-        const int64_t tok = sq.t0 + t.at.i, h = head0 + t.at.g;
+      u32x4_t qf[KSTEPS];
+      RowPlace at;
+      float lse;
+      auto load_rows = [&](int r0) TASFT_INLINE {  // past the end: the last row again, not used
+        at = place_of(min(r0 + col, rows - 1));
+        const int64_t tok = sq.t0 + at.i, h = head0 + at.g;
         const uint16_t* qr = p.q + tok * p.sq[0] + h * p.sq[1] + half * 8;
 #pragma unroll
-        for (int ks = 0; ks < KSTEPS; ++ks) t.q[ks] = *(const u32x4_t*)(qr + ks * 16);
-        t.lse = wp.lse[tok * wp.sl[0] + h * wp.sl[1]];
+        for (int ks = 0; ks < KSTEPS; ++ks) qf[ks] = *(const u32x4_t*)(qr + ks * 16);
+        lse = wp.lse[tok * wp.sl[0] + h * wp.sl[1]];
       };
       int r0 = (r_first / 32 + rg) * 32;
       if (r0 < rows) {
-        Rows even, odd;
-        load_rows(even, r0);
-        for (; r0 < rows; r0 += 2 * STEP) {
-          load_rows(odd, r0 + STEP);  // past the end: the last row again, not used
-          add_rows(even.q, even.at, even.ok, even.lse);
-          if (r0 + STEP >= rows) break;
-          load_rows(even, r0 + 2 * STEP);
-          add_rows(odd.q, odd.at, odd.ok, odd.lse);
-        }
+        load_rows(r0);
+        for (; r0 < rows; r0 += STEP)
+          add_rows(qf, at, r0 + col < rows, lse, [&]() TASFT_INLINE { load_rows(r0 + STEP); });
       }
     }
     // Sums over the 32 rows of a half's lanes, halving the registers each time: lanes whose bit is
