@@ -7,10 +7,11 @@
 // A row that sees no key gives 0 and -inf.
 //
 // The rows of one KV head are its chunk's tokens times the query heads of its group: they share
-// K and V, so a workgroup takes a tile of 128 of them, in token order (dense), or 128 positions
-// of one head aligned to the mask's blocks (masked). Four waves own 32 rows each and share
-// 64-key tiles of K and V in LDS, brought by DMA through the page table a tile ahead: two
-// stages, one barrier a tile. S^T = K Q^T with v_mfma_f32_32x32x16, so a lane owns one row: its
+// K and V. Dense: a workgroup takes a tile of 128 of them, in token order; four waves own 32 rows
+// each and share 64-key tiles of K and V in LDS, brought by DMA through the page table a tile
+// ahead: two stages, one barrier a tile. Masked: neighbouring heads and blocks see different keys,
+// so a workgroup takes 64 positions of one head aligned to the mask's blocks, two waves, with one
+// K and one V tile. S^T = K Q^T with v_mfma_f32_32x32x16, so a lane owns one row: its
 // running maximum and sum stay in the lane (and the one 32 away), and the accumulator of S^T is
 // the B operand of O^T = V^T P^T. P is rounded to the input type for that product (as the MFMA
 // takes it); maxima, sums, O and the log-sum are fp32.
@@ -99,6 +100,9 @@ __device__ __forceinline__ void chunk_dma4(__amdgpu_buffer_rsrc_t r, float* dst,
   __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (TASFT_LDS void*)dst, 4, voff, 0, 0, 0);
 }
 
+// s_waitcnt immediate: at most n vector memory operations outstanding.
+constexpr int vm_wait(int n) { return (n & 15) | ((n >> 4) << 14) | (7 << 4) | (15 << 8); }
+
 __device__ __forceinline__ void chunk_barrier() { asm volatile("s_barrier" ::: "memory"); }
 
 // LDS position of 16-byte chunk cc of row r: K rows are read 32 at a time, V rows transposed.
@@ -124,31 +128,36 @@ __device__ __forceinline__ uint32_t finite2(uint32_t w) {
 typedef const __attribute__((address_space(4))) int32_t* const_i32;
 __device__ __forceinline__ int scalar_load(const int32_t* p) { return *(const_i32)(uintptr_t)p; }
 
-constexpr int kRowWaves = 4;
-constexpr int kRowTile = 32 * kRowWaves;
-constexpr int kRowTileShift = 7;
-static_assert(kRowTile == 1 << kRowTileShift, "row tile");
+constexpr int kRowTile = 128;  // rows of a dense workgroup: four waves
+constexpr int kMaskTile = 64;  // positions of a masked one: two waves
 
 template <int D, int DT, bool MASKED>
-__global__ void __launch_bounds__(kRowWaves * kWave) __attribute__((amdgpu_waves_per_eu(2, 2)))
+__global__ void __launch_bounds__(MASKED ? 128 : 256) __attribute__((amdgpu_waves_per_eu(D == 64 && MASKED ? 3 : 2, D == 64 && MASKED ? 3 : 2)))
 chunk_rows_kernel(const ChunkParams p) {
+  constexpr int WAVES = MASKED ? 2 : 4;
+  constexpr int ROW_TILE = MASKED ? kMaskTile : kRowTile;
+  constexpr int ROW_SHIFT = MASKED ? 6 : 7;
+  static_assert(ROW_TILE == 1 << ROW_SHIFT && ROW_TILE == 32 * WAVES, "row tile");
   constexpr int KSTEPS = D / 16;
   constexpr int DTILES = D / 32;
   constexpr int ROWB = D * 2;
   constexpr int TILE = kTile * ROWB;
   constexpr int RPU = 1024 / ROWB;         // rows of a 1 KB DMA unit
-  constexpr int UPW = 16 / RPU;            // units of a wave's 16 rows
+  constexpr int WROWS = kTile / WAVES;     // rows of a tile that a wave brings
+  constexpr int UPW = WROWS / RPU;         // its units
+  constexpr int PIECES = WROWS / 8;        // its runs of eight rows, each within a page
+  constexpr int NKO = D == 128 ? 4 : 2, NVO = D == 128 ? 2 : 1;  // units with offsets of their own
   __shared__ __attribute__((aligned(1024))) uint8_t k0_lds[TILE];
   __shared__ __attribute__((aligned(1024))) uint8_t v0_lds[TILE];
-  __shared__ __attribute__((aligned(1024))) uint8_t k1_lds[TILE];
-  __shared__ __attribute__((aligned(1024))) uint8_t v1_lds[TILE];
+  __shared__ __attribute__((aligned(1024))) uint8_t k1_lds[MASKED ? 16 : TILE];
+  __shared__ __attribute__((aligned(1024))) uint8_t v1_lds[MASKED ? 16 : TILE];
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 31, half = lane >> 5;
   const int grp16 = lane >> 4, t16 = lane & 15, tr_row = t16 >> 2, tr_cb = t16 & 3;
 
-  chunk_zero_tail<D>(p, blockIdx.x, gridDim.x, tid, kRowWaves * kWave);
+  chunk_zero_tail<D>(p, blockIdx.x, gridDim.x, tid, WAVES * kWave);
 
   // The (sequence, KV head) whose K and V the workgroup reads, and its place among those that do:
   // one XCD's L2 serves them all.
@@ -169,16 +178,16 @@ chunk_rows_kernel(const ChunkParams p) {
   bool row_ok;
   if constexpr (MASKED) {
     // Positions aligned to the row tile: a wave's 32 rows lie in one mask block.
-    const int base = ((sq.p0 >> kRowTileShift) << kRowTileShift) + qt * kRowTile - sq.p0;
+    const int base = ((sq.p0 >> ROW_SHIFT) << ROW_SHIFT) + qt * ROW_TILE - sq.p0;
     if (base >= sq.len) return;
     i_first = max(base + wave * 32, 0);
     i_last = min(base + wave * 32 + 31, sq.len - 1);
-    i_end = min(base + kRowTile, sq.len) - 1;
+    i_end = min(base + ROW_TILE, sq.len) - 1;
     i = base + wave * 32 + col;
     h = kvh * p.G + gm;
     row_ok = i >= 0 && i < sq.len;
   } else {
-    const int rows = sq.len * p.G, r0 = qt * kRowTile;
+    const int rows = sq.len * p.G, r0 = qt * ROW_TILE;
     if (r0 >= rows) return;
     const int rw = r0 + wave * 32, r = rw + col;
     i = r / p.G;
@@ -186,7 +195,7 @@ chunk_rows_kernel(const ChunkParams p) {
     row_ok = r < rows;
     i_first = rw / p.G;
     i_last = rw < rows ? min(rw + 31, rows - 1) / p.G : -1;
-    i_end = (min(r0 + kRowTile, rows) - 1) / p.G;
+    i_end = (min(r0 + ROW_TILE, rows) - 1) / p.G;
   }
   const bool wave_on = i_first <= i_last;
   if (!row_ok) {  // reads a row of the chunk, is not stored
@@ -219,7 +228,7 @@ chunk_rows_kernel(const ChunkParams p) {
     mseq = p.mask + n * p.sm[0] + (int64_t)(kvh * p.G + gm) * p.sm[1];
     const int block0 = sq.p0 >> p.bs_shift;
     auto row_of = [&](int j) { return min(max(((sq.p0 + j) >> p.bs_shift) - block0, 0), p.mask_rows - 1); };
-    row_lo = row_of(max(((sq.p0 >> kRowTileShift) << kRowTileShift) + qt * kRowTile - sq.p0, 0));
+    row_lo = row_of(max(((sq.p0 >> ROW_SHIFT) << ROW_SHIFT) + qt * ROW_TILE - sq.p0, 0));
     row_hi = row_of(i_end);
     row_own = wave_on ? row_of(i_first) : -1;
   }
@@ -250,63 +259,57 @@ chunk_rows_kernel(const ChunkParams p) {
     }
   };
 
-  // A wave brings rows 16 wave .. +15 of a tile, eight rows (one page at least) per buffer
-  // resource, which ends with the last row below kv_len: rows past it arrive as zeros. Per-lane
-  // source offsets: the lane loads the chunk that the self-inverse swizzle maps to its 16 bytes.
+  // A wave brings rows WROWS wave .. of a tile, eight rows (within a page) per buffer resource,
+  // which ends with the last row below kv_len: rows past it arrive as zeros. Per-lane source
+  // offsets: the lane loads the chunk that the self-inverse swizzle maps to its 16 bytes.
   const uint16_t* kbase = p.k + kvh * p.sk[2];
   const uint16_t* vbase = p.v + kvh * p.sv[2];
   const int32_t* table = p.table + n * p.bt_stride;
-  int koff[UPW], voff[UPW];
+  int koff[NKO], voff[NVO];
 #pragma unroll
-  for (int u = 0; u < UPW; ++u) {
-    const int r8 = (u * RPU + lane / (ROWB / 16)) & 7, pos = lane % (ROWB / 16);
-    const int row = wave * 16 + u * RPU + lane / (ROWB / 16);
-    koff[u] = (r8 * (int)p.sk[1] + chunk_swz_k<D>(row, pos) * 8) * 2;
-    voff[u] = (r8 * (int)p.sv[1] + chunk_swz_v<D>(row, pos) * 8) * 2;
+  for (int u = 0; u < NKO; ++u) {
+    const int row = u * RPU + lane / (ROWB / 16), pos = lane % (ROWB / 16);
+    koff[u] = ((row & 7) * (int)p.sk[1] + chunk_swz_k<D>(row, pos) * 8) * 2;
+    if (u < NVO) voff[u] = ((row & 7) * (int)p.sv[1] + chunk_swz_v<D>(row, pos) * 8) * 2;
   }
   struct Pages {
-    int a, b;
+    int id[PIECES];
   };
-  const bool pages16 = p.ps_shift >= 4;  // a wave's 16 rows lie in one page
+  const bool one_page = (1 << p.ps_shift) >= WROWS;  // a wave's rows lie in one page
   auto load_pages = [&](int kt) TASFT_INLINE -> Pages {
-    const int r = kt * kTile + wave * 16, last = (sq.kv - 1) >> p.ps_shift;
+    const int r = kt * kTile + wave * WROWS, last = (sq.kv - 1) >> p.ps_shift;
     Pages pg;
-    pg.a = pg.b = scalar_load(table + min(r >> p.ps_shift, last));
-    if (!pages16) pg.b = scalar_load(table + min((r + 8) >> p.ps_shift, last));
+    pg.id[0] = scalar_load(table + min(r >> p.ps_shift, last));
+#pragma unroll
+    for (int e = 1; e < PIECES; ++e)
+      pg.id[e] = one_page ? pg.id[0] : scalar_load(table + min((r + 8 * e) >> p.ps_shift, last));
     return pg;
   };
-  const int64_t k8 = 8 * p.sk[1], v8 = 8 * p.sv[1];
-  const int krow = (int)p.sk[1] * 2, vrow = (int)p.sv[1] * 2;
-  auto dma_tile = [&](uint8_t* kt_lds, uint8_t* vt_lds, int kt, Pages pg) TASFT_INLINE {
-    const int r = kt * kTile + wave * 16;
-    const int page_a = min(max(pg.a, 0), p.num_pages - 1);
-    const int in_page = r & ((1 << p.ps_shift) - 1);
-    const uint16_t* kr = kbase + page_a * p.sk[0] + in_page * p.sk[1];
-    const uint16_t* vr = vbase + page_a * p.sv[0] + in_page * p.sv[1];
+  // The wave's share of a tile of K or V: base of the head's pool, its strides, row bytes.
+  auto dma_rows = [&](uint8_t* tile_lds, const uint16_t* base, const int64_t* st, const int* off, auto noff, int kt,
+                      const Pages& pg) TASFT_INLINE {
+    constexpr int NOFF = decltype(noff)::value;
+    const int rowb = (int)st[1] * 2, r = kt * kTile + wave * WROWS;
+    const uint16_t* from = nullptr;
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      if (e == 1) {
-        if (pages16) {
-          kr += k8;
-          vr += v8;
-        } else {
-          const int page_b = min(max(pg.b, 0), p.num_pages - 1);
-          const int in_b = (r + 8) & ((1 << p.ps_shift) - 1);
-          kr = kbase + page_b * p.sk[0] + in_b * p.sk[1];
-          vr = vbase + page_b * p.sv[0] + in_b * p.sv[1];
-        }
-      }
+    for (int e = 0; e < PIECES; ++e) {
+      if (e == 0 || !one_page)
+        from = base + min(max(pg.id[e], 0), p.num_pages - 1) * st[0] + ((r + 8 * e) & ((1 << p.ps_shift) - 1)) * st[1];
+      else
+        from += 8 * st[1];
       const int rows = min(sq.kv - r - 8 * e, 8);
-      const __amdgpu_buffer_rsrc_t krs = __builtin_amdgcn_make_buffer_rsrc(
-          (void*)kr, (short)0, rows > 0 ? (rows - 1) * krow + ROWB : 0, 0x00020000);
-      const __amdgpu_buffer_rsrc_t vrs = __builtin_amdgcn_make_buffer_rsrc(
-          (void*)vr, (short)0, rows > 0 ? (rows - 1) * vrow + ROWB : 0, 0x00020000);
+      const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
+          (void*)from, (short)0, rows > 0 ? (rows - 1) * rowb + ROWB : 0, 0x00020000);
 #pragma unroll
-      for (int u = e * (UPW / 2); u < (e + 1) * (UPW / 2); ++u) {
-        chunk_dma(krs, kt_lds + (wave * UPW + u) * 1024, koff[u]);
-        chunk_dma(vrs, vt_lds + (wave * UPW + u) * 1024, voff[u]);
-      }
+      for (int u = e * (8 / RPU); u < (e + 1) * (8 / RPU); ++u)
+        chunk_dma(rs, tile_lds + (wave * UPW + u) * 1024, off[u % NOFF]);
     }
+  };
+  auto dma_k = [&](uint8_t* tile_lds, int kt, const Pages& pg) TASFT_INLINE {
+    dma_rows(tile_lds, kbase, p.sk, koff, std::integral_constant<int, NKO>{}, kt, pg);
+  };
+  auto dma_v = [&](uint8_t* tile_lds, int kt, const Pages& pg) TASFT_INLINE {
+    dma_rows(tile_lds, vbase, p.sv, voff, std::integral_constant<int, NVO>{}, kt, pg);
   };
 
   f32x16_t oacc[DTILES];
@@ -316,9 +319,10 @@ chunk_rows_kernel(const ChunkParams p) {
   float l_run = 0.f;
   int fix_from = 0x7fffffff;  // first tile whose infinities or NaN of V were left out
 
-  auto compute = [&](const uint8_t* kS, const uint8_t* vS, int kt, int own) TASFT_INLINE {
-    const int key0 = kt * kTile;
-    if (key0 > any_see || (MASKED && own == 0)) return;
+  // Whether this wave has anything to do with a tile.
+  auto takes_part = [&](int kt, int own) { return kt * kTile <= any_see && (!MASKED || own != 0); };
+  // S^T of a tile. Register rr of s0 / s1 is key 4 half + off(rr) (+ 32), off = 8 (rr / 4) + rr % 4.
+  auto scores = [&](const uint8_t* kS, f32x16_t& s0, f32x16_t& s1) TASFT_INLINE {
     u32x4_t kf[2][KSTEPS];
 #pragma unroll
     for (int t = 0; t < 2; ++t)
@@ -327,14 +331,18 @@ chunk_rows_kernel(const ChunkParams p) {
         const int r = t * 32 + col;
         kf[t][ks] = *(const u32x4_t*)(kS + r * ROWB + chunk_swz_k<D>(r, ks * 2 + half) * 16);
       }
-    f32x16_t s0 = (f32x16_t){}, s1 = (f32x16_t){};
+    s0 = s1 = (f32x16_t){};
 #pragma unroll
     for (int ks = 0; ks < KSTEPS; ++ks) {
       s0 = mfma16<DT>(kf[0][ks], qf[ks], s0);
       s1 = mfma16<DT>(kf[1][ks], qf[ks], s1);
     }
-    // Register rr of s0 / s1 is key 4 half + off(rr) (+ 32), off = 8 (rr / 4) + rr % 4.
-    const bool mixed = key0 + kTile - 1 > all_see || (MASKED && own != 3);
+  };
+  // Whether some row of the wave does not see some key of the tile.
+  auto is_mixed = [&](int kt, int own) { return kt * kTile + kTile - 1 > all_see || (MASKED && own != 3); };
+  // The softmax step: P^T as the B operand of the second product.
+  auto softmax = [&](f32x16_t& s0, f32x16_t& s1, int kt, int own, bool mixed, u32x4_t (&pb)[4]) TASFT_INLINE {
+    const int key0 = kt * kTile;
     const int lim0 = MASKED && !(own & 1) ? -1 : lim - key0 - 4 * half;
     const int lim1 = MASKED && !(own & 2) ? -1 : lim - key0 - 4 * half - 32;
     if (mixed) {
@@ -372,7 +380,6 @@ chunk_rows_kernel(const ChunkParams p) {
       lsum1 += e1;
     }
     l_run += lsum0 + lsum1;
-    u32x4_t pb[4];
 #pragma unroll
     for (int pp = 0; pp < 4; ++pp) {
       const f32x16_t& sv = (pp < 2) ? s0 : s1;
@@ -380,6 +387,9 @@ chunk_rows_kernel(const ChunkParams p) {
       pb[pp] = (u32x4_t){pack16x2<DT>(sv[o + 0], sv[o + 1]), pack16x2<DT>(sv[o + 2], sv[o + 3]),
                          pack16x2<DT>(sv[o + 4], sv[o + 5]), pack16x2<DT>(sv[o + 6], sv[o + 7])};
     }
+  };
+  // O^T += V^T P^T.
+  auto add_values = [&](const uint8_t* vS, int kt, bool mixed, const u32x4_t (&pb)[4]) TASFT_INLINE {
     u32x2_t vlo[4][DTILES], vhi[4][DTILES];
 #pragma unroll
     for (int pp = 0; pp < 4; ++pp) {
@@ -418,37 +428,78 @@ chunk_rows_kernel(const ChunkParams p) {
   };
 
   int cur = next_tile(), own_cur = own_next;
-  int nxt = -1, own_nxt = 0;
-  Pages pg = {0, 0};
-  if (cur >= 0) {
-    dma_tile(k0_lds, v0_lds, cur, load_pages(cur));
-    nxt = next_tile();
-    own_nxt = own_next;
-    if (nxt >= 0) pg = load_pages(nxt);
-  }
-  // One tile from a stage while the next one's DMA fills the other: by the barrier every wave's
-  // share of this tile has landed and every wave is done with the tile before it.
-  auto step = [&](uint8_t* ka, uint8_t* va, uint8_t* kb, uint8_t* vb) TASFT_INLINE {
-    __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0)
-    chunk_barrier();
-    int nn = -1;
-    Pages pn = pg;
-    if (nxt >= 0) {
-      dma_tile(kb, vb, nxt, pg);
-      nn = next_tile();
-      if (nn >= 0) pn = load_pages(nn);
+  if constexpr (!MASKED) {
+    int nxt = -1;
+    Pages pg = {};
+    if (cur >= 0) {
+      const Pages first = load_pages(cur);
+      dma_k(k0_lds, cur, first);
+      dma_v(v0_lds, cur, first);
+      nxt = next_tile();
+      if (nxt >= 0) pg = load_pages(nxt);
     }
-    compute(ka, va, cur, own_cur);
-    cur = nxt;
-    own_cur = own_nxt;
-    nxt = nn;
-    own_nxt = own_next;
-    pg = pn;
-  };
-  while (cur >= 0) {
-    step(k0_lds, v0_lds, k1_lds, v1_lds);
-    if (cur < 0) break;
-    step(k1_lds, v1_lds, k0_lds, v0_lds);
+    // One tile from a stage while the next one's DMA fills the other: by the barrier every wave's
+    // share of this tile has landed and every wave is done with the tile before it.
+    auto step = [&](uint8_t* ka, uint8_t* va, uint8_t* kb, uint8_t* vb) TASFT_INLINE {
+      __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0)
+      chunk_barrier();
+      int nn = -1;
+      Pages pn = pg;
+      if (nxt >= 0) {
+        dma_k(kb, nxt, pg);
+        dma_v(vb, nxt, pg);
+        nn = next_tile();
+        if (nn >= 0) pn = load_pages(nn);
+      }
+      if (takes_part(cur, 3)) {
+        const bool mixed = is_mixed(cur, 3);
+        f32x16_t s0, s1;
+        u32x4_t pb[4];
+        scores(ka, s0, s1);
+        softmax(s0, s1, cur, 3, mixed, pb);
+        add_values(va, cur, mixed, pb);
+      }
+      cur = nxt;
+      nxt = nn;
+      pg = pn;
+    };
+    while (cur >= 0) {
+      step(k0_lds, v0_lds, k1_lds, v1_lds);
+      if (cur < 0) break;
+      step(k1_lds, v1_lds, k0_lds, v0_lds);
+    }
+  } else {
+    // One K and one V tile, four workgroups a CU (three waves per SIMD at D = 64): the V DMA starts
+    // once every wave is done with the V tile, the next K's once every wave has read this K.
+    constexpr int kWaitTile = vm_wait(UPW);  // all but the last tile's units have landed
+    Pages pg = {};
+    if (cur >= 0) {
+      pg = load_pages(cur);
+      dma_k(k0_lds, cur, pg);
+    }
+    while (cur >= 0) {
+      __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0): own share of K landed, V's reads returned
+      chunk_barrier();
+      dma_v(v0_lds, cur, pg);
+      const bool on = takes_part(cur, own_cur), mixed = is_mixed(cur, own_cur);
+      f32x16_t s0 = (f32x16_t){}, s1 = (f32x16_t){};
+      u32x4_t pb[4] = {};
+      if (on) scores(k0_lds, s0, s1);
+      __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): this wave's K reads returned
+      chunk_barrier();                     // every wave has read K
+      const int nxt = next_tile(), own_nxt = own_next;
+      // Always one K tile after V (the last one again at the end), so that V's wait is one count.
+      const Pages pn = load_pages(nxt >= 0 ? nxt : cur);
+      dma_k(k0_lds, nxt >= 0 ? nxt : cur, pn);
+      if (on) softmax(s0, s1, cur, own_cur, mixed, pb);
+      __builtin_amdgcn_s_waitcnt(kWaitTile);  // own share of V landed, the next K in flight
+      chunk_barrier();
+      if (on) add_values(v0_lds, cur, mixed, pb);
+      cur = nxt;
+      own_cur = own_nxt;
+      pg = pn;
+    }
+    __builtin_amdgcn_s_waitcnt(0x0f70);  // no DMA into this workgroup's LDS outlives it
   }
 
   if (fix_from != 0x7fffffff) {
@@ -601,8 +652,6 @@ struct RowPlace {
     }
   }
 };
-
-constexpr int vm_wait(int n) { return (n & 15) | ((n >> 4) << 14) | (7 << 4) | (15 << 8); }
 
 template <int D, int DT, int KW, bool RING, bool MASKED>
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(RING && D == 128 ? 2 : 3)))
@@ -923,7 +972,7 @@ extern "C" size_t tasft_chunk_workspace_bytes(int64_t tokens, int64_t num_q_head
 
 template <int D, int DT>
 static int launch_chunk(const ChunkParams& p, int64_t grid, hipStream_t stream) {
-  const dim3 g((unsigned)grid), b(kRowWaves * kWave);
+  const dim3 g((unsigned)grid), b(p.mask ? 128 : 256);
   if (p.mask)
     hipLaunchKernelGGL((chunk_rows_kernel<D, DT, true>), g, b, 0, stream, p);
   else
@@ -979,8 +1028,9 @@ extern "C" int tasft_chunk_paged_fwd(
   p.ws_o = (float*)workspace;
   p.ws_ml = (float*)workspace + tokens * num_q_heads * num_splits * head_dim;
   // Row tiles: masked ones are aligned to positions, so a chunk can touch one more.
-  const int64_t rows = p.mask ? p.L + kRowTile - 1 : (int64_t)p.L * p.G;
-  p.QT = (int)((rows + kRowTile - 1) / kRowTile);
+  const int64_t rows = p.mask ? (int64_t)p.L + kMaskTile - 1 : (int64_t)p.L * p.G;
+  const int tile = p.mask ? kMaskTile : kRowTile;
+  p.QT = (int)((rows + tile - 1) / tile);
   const int64_t grid = (int64_t)p.N * p.Hkv * p.QT * (p.mask ? p.G : 1) * p.P;
   if (grid > 0x7fffffff) return set_error(kErrUnsupported, "chunk attention: launch too large");
   const hipStream_t st = (hipStream_t)stream;

@@ -799,15 +799,16 @@ def default_decode_splits(batch: int, num_kv_heads: int, num_blocks: int,
 def default_chunk_splits(num_seqs: int, num_kv_heads: int, q_per_kv: int, chunk: int, slots: int,
                          masked: bool = False) -> int:
     """Key splits of ``forward_chunk_paged``: one where its row tiles (128 rows of a KV head's
-    tokens and query heads, or with a mask 128 positions of a head) give two workgroups per CU
-    (256 on MI355X), else enough for that, at least four 64-key tiles each."""
+    tokens and query heads, two workgroups per CU; with a mask 64 positions of a head, four per CU)
+    fill three quarters of the GPU's 256 CUs, else enough to fill it, at least four 64-key tiles
+    each."""
     if masked:
-        tiles = num_seqs * num_kv_heads * q_per_kv * math.ceil(chunk / 128)
+        tiles, full = num_seqs * num_kv_heads * q_per_kv * math.ceil(chunk / 64), 1024
     else:
-        tiles = num_seqs * num_kv_heads * math.ceil(chunk * q_per_kv / 128)
-    if tiles >= 384:
+        tiles, full = num_seqs * num_kv_heads * math.ceil(chunk * q_per_kv / 128), 512
+    if tiles >= 0.75 * full:
         return 1
-    return max(1, min(math.ceil(512 / tiles), math.ceil(slots / 256), 64))
+    return max(1, min(math.ceil(full / tiles), math.ceil(slots / 256), 64))
 
 
 def executed_blocks(block_mask: torch.Tensor, causal: bool = True) -> torch.Tensor:
