@@ -146,7 +146,6 @@ chunk_rows_kernel(const ChunkParams p) {
   constexpr int WROWS = kTile / WAVES;     // rows of a tile that a wave brings
   constexpr int UPW = WROWS / RPU;         // its units
   constexpr int PIECES = WROWS / 8;        // its runs of eight rows, each within a page
-  constexpr int NKO = D == 128 ? 4 : 2, NVO = D == 128 ? 2 : 1;  // units with offsets of their own
   __shared__ __attribute__((aligned(1024))) uint8_t k0_lds[TILE];
   __shared__ __attribute__((aligned(1024))) uint8_t v0_lds[TILE];
   __shared__ __attribute__((aligned(1024))) uint8_t k1_lds[MASKED ? 16 : TILE];
@@ -259,57 +258,64 @@ chunk_rows_kernel(const ChunkParams p) {
     }
   };
 
-  // A wave brings rows WROWS wave .. of a tile, eight rows (within a page) per buffer resource,
-  // which ends with the last row below kv_len: rows past it arrive as zeros. Per-lane source
-  // offsets: the lane loads the chunk that the self-inverse swizzle maps to its 16 bytes.
+  // A wave brings rows WROWS wave .. of a tile, from one page where pages hold that many, else eight
+  // rows from each. A buffer resource ends with the last row below kv_len: rows past it arrive as
+  // zeros. Per-lane source offsets, from the wave's first row: the lane loads the chunk that the
+  // self-inverse swizzle maps to its 16 bytes.
   const uint16_t* kbase = p.k + kvh * p.sk[2];
   const uint16_t* vbase = p.v + kvh * p.sv[2];
   const int32_t* table = p.table + n * p.bt_stride;
-  int koff[NKO], voff[NVO];
+  int koff[UPW], voff[UPW];
 #pragma unroll
-  for (int u = 0; u < NKO; ++u) {
+  for (int u = 0; u < UPW; ++u) {
     const int row = u * RPU + lane / (ROWB / 16), pos = lane % (ROWB / 16);
-    koff[u] = ((row & 7) * (int)p.sk[1] + chunk_swz_k<D>(row, pos) * 8) * 2;
-    if (u < NVO) voff[u] = ((row & 7) * (int)p.sv[1] + chunk_swz_v<D>(row, pos) * 8) * 2;
+    koff[u] = (row * (int)p.sk[1] + chunk_swz_k<D>(row, pos) * 8) * 2;
+    voff[u] = (row * (int)p.sv[1] + chunk_swz_v<D>(row, pos) * 8) * 2;
   }
   struct Pages {
     int id[PIECES];
   };
-  const bool one_page = (1 << p.ps_shift) >= WROWS;  // a wave's rows lie in one page
+  const bool one_page = (1 << p.ps_shift) >= WROWS;
   auto load_pages = [&](int kt) TASFT_INLINE -> Pages {
     const int r = kt * kTile + wave * WROWS, last = (sq.kv - 1) >> p.ps_shift;
-    Pages pg;
+    Pages pg = {};
     pg.id[0] = scalar_load(table + min(r >> p.ps_shift, last));
+    if (!one_page) {
 #pragma unroll
-    for (int e = 1; e < PIECES; ++e)
-      pg.id[e] = one_page ? pg.id[0] : scalar_load(table + min((r + 8 * e) >> p.ps_shift, last));
+      for (int e = 1; e < PIECES; ++e) pg.id[e] = scalar_load(table + min((r + 8 * e) >> p.ps_shift, last));
+    }
     return pg;
   };
-  // The wave's share of a tile of K or V: base of the head's pool, its strides, row bytes.
-  auto dma_rows = [&](uint8_t* tile_lds, const uint16_t* base, const int64_t* st, const int* off, auto noff, int kt,
+  // The wave's share of a tile of K or V: base of the head's pool, its strides.
+  auto dma_rows = [&](uint8_t* tile_lds, const uint16_t* base, const int64_t* st, const int* off, int kt,
                       const Pages& pg) TASFT_INLINE {
-    constexpr int NOFF = decltype(noff)::value;
-    const int rowb = (int)st[1] * 2, r = kt * kTile + wave * WROWS;
-    const uint16_t* from = nullptr;
-#pragma unroll
-    for (int e = 0; e < PIECES; ++e) {
-      if (e == 0 || !one_page)
-        from = base + min(max(pg.id[e], 0), p.num_pages - 1) * st[0] + ((r + 8 * e) & ((1 << p.ps_shift) - 1)) * st[1];
-      else
-        from += 8 * st[1];
-      const int rows = min(sq.kv - r - 8 * e, 8);
+    const int rowb = (int)st[1] * 2, r = kt * kTile + wave * WROWS, left = sq.kv - r;
+    const int in_page = (1 << p.ps_shift) - 1;
+    uint8_t* dst = tile_lds + wave * UPW * 1024;
+    if (one_page) {
+      const uint16_t* from = base + min(max(pg.id[0], 0), p.num_pages - 1) * st[0] + (r & in_page) * st[1];
       const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
-          (void*)from, (short)0, rows > 0 ? (rows - 1) * rowb + ROWB : 0, 0x00020000);
+          (void*)from, (short)0, left > 0 ? (min(left, WROWS) - 1) * rowb + ROWB : 0, 0x00020000);
 #pragma unroll
-      for (int u = e * (8 / RPU); u < (e + 1) * (8 / RPU); ++u)
-        chunk_dma(rs, tile_lds + (wave * UPW + u) * 1024, off[u % NOFF]);
+      for (int u = 0; u < UPW; ++u) chunk_dma(rs, dst + u * 1024, off[u]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < PIECES; ++e) {
+        // The resource of rows 8 e .. starts 8 e rows before them: offsets count from the wave's first.
+        const uint16_t* from = base + min(max(pg.id[e], 0), p.num_pages - 1) * st[0] +
+                               (((r + 8 * e) & in_page) - 8 * e) * st[1];
+        const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
+            (void*)from, (short)0, left > 8 * e ? (min(left, 8 * e + 8) - 1) * rowb + ROWB : 0, 0x00020000);
+#pragma unroll
+        for (int u = e * (8 / RPU); u < (e + 1) * (8 / RPU); ++u) chunk_dma(rs, dst + u * 1024, off[u]);
+      }
     }
   };
   auto dma_k = [&](uint8_t* tile_lds, int kt, const Pages& pg) TASFT_INLINE {
-    dma_rows(tile_lds, kbase, p.sk, koff, std::integral_constant<int, NKO>{}, kt, pg);
+    dma_rows(tile_lds, kbase, p.sk, koff, kt, pg);
   };
   auto dma_v = [&](uint8_t* tile_lds, int kt, const Pages& pg) TASFT_INLINE {
-    dma_rows(tile_lds, vbase, p.sv, voff, std::integral_constant<int, NVO>{}, kt, pg);
+    dma_rows(tile_lds, vbase, p.sv, voff, kt, pg);
   };
 
   f32x16_t oacc[DTILES];
@@ -933,7 +939,7 @@ static int chunk_params(ChunkParams& p, const char* what, const void* q, const v
   if ((q_strides[0] & 7) || (q_strides[1] & 7) || (kp_strides[0] & 7) || (kp_strides[1] & 7) ||
       (kp_strides[2] & 7) || ((uintptr_t)q & 15) || ((uintptr_t)k_pages & 15))
     return set_error(kErrInvalidArgument, "%s: strides must be multiples of 8 on 16-byte aligned bases", what);
-  if (kp_strides[1] >= (int64_t)1 << 26)
+  if (kp_strides[1] >= (int64_t)1 << 24)
     return set_error(kErrUnsupported, "%s: token stride of the pools too large", what);
   p.q = (const uint16_t*)q;
   p.k = (const uint16_t*)k_pages;
@@ -1009,7 +1015,7 @@ extern "C" int tasft_chunk_paged_fwd(
   if ((vp_strides[0] & 7) || (vp_strides[1] & 7) || (vp_strides[2] & 7) || (o_strides[0] & 7) || (o_strides[1] & 7) ||
       ((uintptr_t)v_pages & 15) || ((uintptr_t)out & 15))
     return set_error(kErrInvalidArgument, "chunk attention: strides must be multiples of 8 on 16-byte aligned bases");
-  if (vp_strides[1] >= (int64_t)1 << 26)
+  if (vp_strides[1] >= (int64_t)1 << 24)
     return set_error(kErrUnsupported, "chunk attention: token stride of the pools too large");
   if (num_splits < 1 || num_splits > 1024)
     return set_error(kErrInvalidArgument, "chunk attention: num_splits must be in [1, 1024]");
