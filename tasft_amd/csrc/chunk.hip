@@ -131,7 +131,9 @@ __device__ __forceinline__ int scalar_load(const int32_t* p) { return *(const_i3
 constexpr int kRowTile = 128;  // rows of a dense workgroup: four waves
 constexpr int kMaskTile = 64;  // positions of a masked one: two waves
 
-template <int D, int DT, bool MASKED>
+// PIECES: runs of a wave's share of a tile that lie in one page each (one where pages are at least as
+// long as the share). A template: the general form's scalar registers spilled, at a fifth of the time.
+template <int D, int DT, bool MASKED, int PIECES>
 __global__ void __launch_bounds__(MASKED ? 128 : 256) __attribute__((amdgpu_waves_per_eu(D == 64 && MASKED ? 3 : 2, D == 64 && MASKED ? 3 : 2)))
 chunk_rows_kernel(const ChunkParams p) {
   constexpr int WAVES = MASKED ? 2 : 4;
@@ -145,7 +147,8 @@ chunk_rows_kernel(const ChunkParams p) {
   constexpr int RPU = 1024 / ROWB;         // rows of a 1 KB DMA unit
   constexpr int WROWS = kTile / WAVES;     // rows of a tile that a wave brings
   constexpr int UPW = WROWS / RPU;         // its units
-  constexpr int PIECES = WROWS / 8;        // its runs of eight rows, each within a page
+  constexpr int PROWS = WROWS / PIECES;
+  static_assert(PROWS >= 8 && PROWS % RPU == 0, "a piece is whole units");
   __shared__ __attribute__((aligned(1024))) uint8_t k0_lds[TILE];
   __shared__ __attribute__((aligned(1024))) uint8_t v0_lds[TILE];
   __shared__ __attribute__((aligned(1024))) uint8_t k1_lds[MASKED ? 16 : TILE];
@@ -258,10 +261,9 @@ chunk_rows_kernel(const ChunkParams p) {
     }
   };
 
-  // A wave brings rows WROWS wave .. of a tile, from one page where pages hold that many, else eight
-  // rows from each. A buffer resource ends with the last row below kv_len: rows past it arrive as
-  // zeros. Per-lane source offsets, from the wave's first row: the lane loads the chunk that the
-  // self-inverse swizzle maps to its 16 bytes.
+  // A wave brings rows WROWS wave .. of a tile, PROWS from a page. A buffer resource ends with the
+  // last row below kv_len: rows past it arrive as zeros. Per-lane source offsets, from the wave's
+  // first row: the lane loads the chunk that the self-inverse swizzle maps to its 16 bytes.
   const uint16_t* kbase = p.k + kvh * p.sk[2];
   const uint16_t* vbase = p.v + kvh * p.sv[2];
   const int32_t* table = p.table + n * p.bt_stride;
@@ -275,47 +277,35 @@ chunk_rows_kernel(const ChunkParams p) {
   struct Pages {
     int id[PIECES];
   };
-  const bool one_page = (1 << p.ps_shift) >= WROWS;
   auto load_pages = [&](int kt) TASFT_INLINE -> Pages {
     const int r = kt * kTile + wave * WROWS, last = (sq.kv - 1) >> p.ps_shift;
-    Pages pg = {};
-    pg.id[0] = scalar_load(table + min(r >> p.ps_shift, last));
-    if (!one_page) {
+    Pages pg;
 #pragma unroll
-      for (int e = 1; e < PIECES; ++e) pg.id[e] = scalar_load(table + min((r + 8 * e) >> p.ps_shift, last));
-    }
+    for (int e = 0; e < PIECES; ++e) pg.id[e] = scalar_load(table + min((r + PROWS * e) >> p.ps_shift, last));
     return pg;
   };
-  // The wave's share of a tile of K or V: base of the head's pool, its strides.
-  auto dma_rows = [&](uint8_t* tile_lds, const uint16_t* base, const int64_t* st, const int* off, int kt,
+  // The wave's share of a tile of K or V: base of the head's pool, its page and token strides.
+  auto dma_rows = [&](uint8_t* tile_lds, const uint16_t* base, int64_t page_st, int tok_st, const int* off, int kt,
                       const Pages& pg) TASFT_INLINE {
-    const int rowb = (int)st[1] * 2, r = kt * kTile + wave * WROWS, left = sq.kv - r;
-    const int in_page = (1 << p.ps_shift) - 1;
-    uint8_t* dst = tile_lds + wave * UPW * 1024;
-    if (one_page) {
-      const uint16_t* from = base + min(max(pg.id[0], 0), p.num_pages - 1) * st[0] + (r & in_page) * st[1];
+    const int r = kt * kTile + wave * WROWS, left = sq.kv - r;
+#pragma unroll
+    for (int e = 0; e < PIECES; ++e) {
+      // A later piece's resource starts PROWS e rows before it: offsets count from the wave's first.
+      const int in_page = ((r + PROWS * e) & ((1 << p.ps_shift) - 1)) - PROWS * e;
+      const uint16_t* from = base + min(max(pg.id[e], 0), p.num_pages - 1) * page_st + (int64_t)in_page * tok_st;
+      const int rows = min(left, PROWS * (e + 1));
       const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
-          (void*)from, (short)0, left > 0 ? (min(left, WROWS) - 1) * rowb + ROWB : 0, 0x00020000);
+          (void*)from, (short)0, left > PROWS * e ? (rows - 1) * tok_st * 2 + ROWB : 0, 0x00020000);
 #pragma unroll
-      for (int u = 0; u < UPW; ++u) chunk_dma(rs, dst + u * 1024, off[u]);
-    } else {
-#pragma unroll
-      for (int e = 0; e < PIECES; ++e) {
-        // The resource of rows 8 e .. starts 8 e rows before them: offsets count from the wave's first.
-        const uint16_t* from = base + min(max(pg.id[e], 0), p.num_pages - 1) * st[0] +
-                               (((r + 8 * e) & in_page) - 8 * e) * st[1];
-        const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
-            (void*)from, (short)0, left > 8 * e ? (min(left, 8 * e + 8) - 1) * rowb + ROWB : 0, 0x00020000);
-#pragma unroll
-        for (int u = e * (8 / RPU); u < (e + 1) * (8 / RPU); ++u) chunk_dma(rs, dst + u * 1024, off[u]);
-      }
+      for (int u = e * (PROWS / RPU); u < (e + 1) * (PROWS / RPU); ++u)
+        chunk_dma(rs, tile_lds + (wave * UPW + u) * 1024, off[u]);
     }
   };
   auto dma_k = [&](uint8_t* tile_lds, int kt, const Pages& pg) TASFT_INLINE {
-    dma_rows(tile_lds, kbase, p.sk, koff, kt, pg);
+    dma_rows(tile_lds, kbase, p.sk[0], (int)p.sk[1], koff, kt, pg);
   };
   auto dma_v = [&](uint8_t* tile_lds, int kt, const Pages& pg) TASFT_INLINE {
-    dma_rows(tile_lds, vbase, p.sv, voff, kt, pg);
+    dma_rows(tile_lds, vbase, p.sv[0], (int)p.sv[1], voff, kt, pg);
   };
 
   f32x16_t oacc[DTILES];
@@ -978,11 +968,17 @@ extern "C" size_t tasft_chunk_workspace_bytes(int64_t tokens, int64_t num_q_head
 
 template <int D, int DT>
 static int launch_chunk(const ChunkParams& p, int64_t grid, hipStream_t stream) {
-  const dim3 g((unsigned)grid), b(p.mask ? 128 : 256);
-  if (p.mask)
-    hipLaunchKernelGGL((chunk_rows_kernel<D, DT, true>), g, b, 0, stream, p);
-  else
-    hipLaunchKernelGGL((chunk_rows_kernel<D, DT, false>), g, b, 0, stream, p);
+  auto run = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(p.mask ? 128 : 256), 0, stream, p);
+  };
+  if (p.mask) {
+    if (p.ps_shift >= 5) run(chunk_rows_kernel<D, DT, true, 1>);
+    else if (p.ps_shift == 4) run(chunk_rows_kernel<D, DT, true, 2>);
+    else run(chunk_rows_kernel<D, DT, true, 4>);
+  } else {
+    if (p.ps_shift >= 4) run(chunk_rows_kernel<D, DT, false, 1>);
+    else run(chunk_rows_kernel<D, DT, false, 2>);
+  }
   if (const int rc = check_launch("chunk attention")) return rc;
   if (p.P == 1) return kOk;
   constexpr int RPW = 256 / (D / 4);
