@@ -260,11 +260,16 @@ def stream_handle(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
+# The current device's index without torch.cuda's initialisation check (a tensor exists on it).
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+_HERE = contextlib.nullcontext()
+
+
 def on_device(device: torch.device):
     """A context in which ``device`` is the current one (nothing where it is already): a kernel is
     launched on a stream of the current device."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
+    if device.index is None or device.index == _current_device():
+        return _HERE
     return torch.cuda.device(device)
 
 

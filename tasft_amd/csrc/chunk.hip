@@ -128,6 +128,15 @@ __device__ __forceinline__ uint32_t finite2(uint32_t w) {
 typedef const __attribute__((address_space(4))) int32_t* const_i32;
 __device__ __forceinline__ int scalar_load(const int32_t* p) { return *(const_i32)(uintptr_t)p; }
 
+// The kernel's argument read again: what only the end of a kernel uses is not kept in scalar
+// registers over its main loop (they spilled).
+typedef const __attribute__((address_space(4))) ChunkParams* ParamsPtr;
+__device__ __forceinline__ ParamsPtr params_again() {
+  ParamsPtr p = (ParamsPtr)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  return p;
+}
+
 constexpr int kRowTile = 128;  // rows of a dense workgroup: four waves
 constexpr int kMaskTile = 64;  // positions of a masked one: two waves
 
@@ -498,6 +507,7 @@ chunk_rows_kernel(const ChunkParams p) {
     __builtin_amdgcn_s_waitcnt(0x0f70);  // no DMA into this workgroup's LDS outlives it
   }
 
+  const ParamsPtr pe = params_again();
   if (fix_from != 0x7fffffff) {
     // Infinities and NaN of V in tiles that only some of the wave's rows see: key by key, from
     // memory, to the rows that see the key. (Where a later tile had them in its product, once
@@ -506,17 +516,17 @@ chunk_rows_kernel(const ChunkParams p) {
     const int last = min(any_see, tile_b * kTile - 1);
 #pragma nounroll
     for (int key = fix_from * kTile; key <= last; ++key) {
-      const int64_t page = min(max(table[key >> p.ps_shift], 0), p.num_pages - 1);
-      const int in_page = key & ((1 << p.ps_shift) - 1);
-      const uint16_t* vr = vbase + page * p.sv[0] + in_page * p.sv[1];
+      const int64_t page = min(max(pe->table[n * pe->bt_stride + (key >> pe->ps_shift)], 0), pe->num_pages - 1);
+      const int in_page = key & ((1 << pe->ps_shift) - 1);
+      const uint16_t* vr = pe->v + kvh * pe->sv[2] + page * pe->sv[0] + in_page * pe->sv[1];
       const uint32_t w = *(const uint32_t*)(vr + (lane * 2) % D);
       if (!__ballot(finite2<DT>(w) != w)) continue;
       bool sees = row_ok && key <= lim;
       if constexpr (MASKED) {
-        const uint8_t* m = mseq + row_own * p.sm[2];
-        sees = sees && m[(key >> p.bs_shift) * p.sm[3]] != 0;
+        const uint8_t* m = pe->mask + n * pe->sm[0] + (int64_t)(kvh * pe->G + gm) * pe->sm[1] + row_own * pe->sm[2];
+        sees = sees && m[(key >> pe->bs_shift) * pe->sm[3]] != 0;
       }
-      const uint16_t* kr = kbase + page * p.sk[0] + in_page * p.sk[1] + half * 8;
+      const uint16_t* kr = pe->k + kvh * pe->sk[2] + page * pe->sk[0] + in_page * pe->sk[1] + half * 8;
       float dot = 0.f;
 #pragma unroll
       for (int ks = 0; ks < KSTEPS; ++ks) {
@@ -526,27 +536,28 @@ chunk_rows_kernel(const ChunkParams p) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) dot = fmaf(x[j], y[j], dot);
       }
-      const float pk = __builtin_amdgcn_exp2f(fmaf(pair_sum32(dot), p.scale_log2, -m_use));
+      const float pk = __builtin_amdgcn_exp2f(fmaf(pair_sum32(dot), pe->scale_log2, -m_use));
 #pragma unroll
       for (int dt = 0; dt < DTILES; ++dt)
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
           const uint32_t x = vr[dt * 32 + 8 * (e >> 2) + 4 * half + (e & 3)];
-          oacc[dt][e] += sees && finite2<DT>(x) != x ? pk * bits16_to_f32<DT>(x) : 0.f;
+          const bool add = sees & (finite2<DT>(x) != x);
+          oacc[dt][e] += add ? pk * bits16_to_f32<DT>(x) : 0.f;
         }
     }
   }
 
   const float l_tot = pair_sum32(l_run);
   const int64_t tok = sq.t0 + i;
-  if (p.P > 1) {
-    const int64_t row = (tok * p.Hq + h) * p.P + split;
+  if (pe->P > 1) {
+    const int64_t row = (tok * pe->Hq + h) * pe->P + split;
     if (row_ok) {
       if (half == 0) {
-        p.ws_ml[row * 2] = m_ref;
-        p.ws_ml[row * 2 + 1] = l_tot;
+        pe->ws_ml[row * 2] = m_ref;
+        pe->ws_ml[row * 2 + 1] = l_tot;
       }
-      float* wo = p.ws_o + row * D;
+      float* wo = pe->ws_o + row * D;
 #pragma unroll
       for (int dt = 0; dt < DTILES; ++dt)
 #pragma unroll
@@ -556,7 +567,7 @@ chunk_rows_kernel(const ChunkParams p) {
     }
     return;
   }
-  if (p.lse && row_ok && half == 0) p.lse[tok * p.Hq + h] = (m_ref + __builtin_amdgcn_logf(l_tot)) * kLn2;
+  if (pe->lse && row_ok && half == 0) pe->lse[tok * pe->Hq + h] = (m_ref + __builtin_amdgcn_logf(l_tot)) * kLn2;
   const float inv = 1.f / (l_tot > 0.f ? l_tot : 1.f);  // empty rows: 0; NaN rows stay NaN
   // Whole rows through LDS: 16-byte chunk c of row r at position c ^ (r % chunks).
   __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
@@ -572,45 +583,114 @@ chunk_rows_kernel(const ChunkParams p) {
                          pack16x2<DT>(oacc[dt][4 * gq + 2] * inv, oacc[dt][4 * gq + 3] * inv)};
       *(u32x2_t*)(ost + col * ROWB + (((d0 >> 3) ^ (col & (CPR - 1))) << 4) + (d0 & 7) * 2) = w;
     }
-  const int64_t at = row_ok ? tok * p.so[0] + h * p.so[1] : -1;
+  const int64_t at = row_ok ? tok * pe->so[0] + h * pe->so[1] : -1;
 #pragma unroll
   for (int j = 0; j < 32 * CPR / kWave; ++j) {
     const int r = j * (kWave / CPR) + lane / CPR, c = lane % CPR;
     const u32x4_t x = *(const u32x4_t*)(ost + r * ROWB + ((c ^ (r & (CPR - 1))) << 4));
     const int64_t to = __shfl(at, r, kWave);
-    if (to >= 0) *(u32x4_t*)(p.o + to + c * 8) = x;
+    if (to >= 0) *(u32x4_t*)(pe->o + to + c * 8) = x;
   }
 }
 
-// Joins the P splits of every row: D / 4 lanes a row, the partial sums of splits that saw no key
-// are not read (they may be unwritten).
+// Joins the P splits of every row; the partial sums of splits that saw no key are not used (they may
+// be unwritten). Up to kFewSplits: D / 4 lanes a row, every split's loads in flight together. More:
+// a workgroup a row, its factors computed once, the splits shared out over groups of D / 4 lanes,
+// four loads in flight each (one lane walking 64 splits took 34 us for 32 rows, this 6).
+constexpr int kFewSplits = 8;
+
 template <int D, int DT>
-__global__ void __launch_bounds__(256) chunk_combine_kernel(const ChunkParams p) {
-  constexpr int LPR = D / 4;
-  const int64_t row = (int64_t)blockIdx.x * (256 / LPR) + threadIdx.x / LPR;
-  const int c = threadIdx.x % LPR;
+__device__ __forceinline__ void chunk_store(const ChunkParams& p, int64_t row, int c, const f32x4_t& O, float L,
+                                            float M) {
   const int64_t t = row / p.Hq;
   const int h = (int)(row - t * p.Hq);
-  if (t >= min(max(p.cu[p.N], 0), p.T)) return;
-  const float* ml = p.ws_ml + row * p.P * 2;
-  const float* os = p.ws_o + row * p.P * D + c * 4;
-  float M = -INFINITY;
-  for (int s = 0; s < p.P; ++s) M = fmaxf(M, ml[2 * s]);
-  const float Mu = (M == -INFINITY) ? 0.f : M;
-  float L = 0.f;
-  f32x4_t O = {0.f, 0.f, 0.f, 0.f};
-  for (int s = 0; s < p.P; ++s) {
-    const float l = ml[2 * s + 1];
-    if (__float_as_uint(l) == 0u) continue;
-    const float f = __builtin_amdgcn_exp2f(ml[2 * s] - Mu);
-    const f32x4_t x = *(const f32x4_t*)(os + (int64_t)s * D);
-    L += l * f;
-    O += x * f;
-  }
   const float inv = 1.f / (L > 0.f ? L : 1.f);
   const u32x2_t w = {pack16x2<DT>(O[0] * inv, O[1] * inv), pack16x2<DT>(O[2] * inv, O[3] * inv)};
   *(u32x2_t*)(p.o + t * p.so[0] + h * p.so[1] + c * 4) = w;
   if (p.lse && c == 0) p.lse[row] = (M + __builtin_amdgcn_logf(L)) * kLn2;
+}
+
+template <int D, int DT>
+__global__ void __launch_bounds__(256) chunk_combine_few_kernel(const ChunkParams p) {
+  constexpr int LPR = D / 4;
+  const int64_t row = (int64_t)blockIdx.x * (256 / LPR) + threadIdx.x / LPR;
+  const int c = threadIdx.x % LPR;
+  if (row >= (int64_t)min(max(p.cu[p.N], 0), p.T) * p.Hq) return;
+  const float* ml = p.ws_ml + row * p.P * 2;
+  const float* os = p.ws_o + row * p.P * D + c * 4;
+  float m[kFewSplits], l[kFewSplits];
+  f32x4_t o[kFewSplits];
+#pragma unroll
+  for (int s = 0; s < kFewSplits; ++s) {  // past the last split: it again, not used
+    const int at = min(s, p.P - 1);
+    m[s] = ml[2 * at];
+    l[s] = ml[2 * at + 1];
+    o[s] = *(const f32x4_t*)(os + (int64_t)at * D);
+  }
+  float M = -INFINITY;
+#pragma unroll
+  for (int s = 0; s < kFewSplits; ++s) M = fmaxf(M, m[s]);
+  const float Mu = (M == -INFINITY) ? 0.f : M;
+  float L = 0.f;
+  f32x4_t O = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int s = 0; s < kFewSplits; ++s)
+    if (s < p.P && __float_as_uint(l[s]) != 0u) {
+      const float f = __builtin_amdgcn_exp2f(m[s] - Mu);
+      L += l[s] * f;
+      O += o[s] * f;
+    }
+  chunk_store<D, DT>(p, row, c, O, L, M);
+}
+
+template <int D, int DT>
+__global__ void __launch_bounds__(256) chunk_combine_kernel(const ChunkParams p) {
+  constexpr int LPR = D / 4, GROUPS = 256 / LPR;
+  __shared__ float fac[1024];
+  __shared__ float red[2][4];
+  __shared__ f32x4_t part[GROUPS][LPR];
+  const int64_t row = blockIdx.x;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = tid % LPR, grp = tid / LPR;
+  if (row >= (int64_t)min(max(p.cu[p.N], 0), p.T) * p.Hq) return;
+  const float* ml = p.ws_ml + row * p.P * 2;
+  const float* os = p.ws_o + row * p.P * D + c * 4;
+  float M = -INFINITY;
+  for (int s = tid; s < p.P; s += 256) M = fmaxf(M, ml[2 * s]);
+  M = wave_max(M);
+  if (lane == 0) red[0][wave] = M;
+  __syncthreads();
+  M = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
+  const float Mu = (M == -INFINITY) ? 0.f : M;
+  float L = 0.f;
+  for (int s = tid; s < p.P; s += 256) {
+    const float l = ml[2 * s + 1];
+    const bool none = __float_as_uint(l) == 0u;
+    const float f = none ? -1.f : __builtin_amdgcn_exp2f(ml[2 * s] - Mu);  // -1: not used
+    fac[s] = f;
+    L += none ? 0.f : l * f;
+  }
+  L = wave_sum(L);
+  if (lane == 0) red[1][wave] = L;
+  __syncthreads();
+  L = (red[1][0] + red[1][1]) + (red[1][2] + red[1][3]);
+  f32x4_t O = {0.f, 0.f, 0.f, 0.f};
+  for (int s0 = grp; s0 < p.P; s0 += 4 * GROUPS) {
+    f32x4_t x[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = *(const f32x4_t*)(os + (int64_t)min(s0 + i * GROUPS, p.P - 1) * D);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int s = s0 + i * GROUPS;
+      const float f = s < p.P ? fac[s] : -1.f;
+      if (__float_as_uint(f) != 0xbf800000u) O += x[i] * f;
+    }
+  }
+  part[grp][c] = O;
+  __syncthreads();
+  if (grp != 0) return;
+#pragma unroll
+  for (int g = 1; g < GROUPS; ++g) O += part[g][c];
+  chunk_store<D, DT>(p, row, c, O, L, M);
 }
 
 // ---------------------------------------------------------------------------------------
@@ -981,9 +1061,15 @@ static int launch_chunk(const ChunkParams& p, int64_t grid, hipStream_t stream) 
   }
   if (const int rc = check_launch("chunk attention")) return rc;
   if (p.P == 1) return kOk;
-  constexpr int RPW = 256 / (D / 4);
   const int64_t rows = (int64_t)p.T * p.Hq;
-  hipLaunchKernelGGL((chunk_combine_kernel<D, DT>), dim3((unsigned)((rows + RPW - 1) / RPW)), dim3(256), 0, stream, p);
+  if (p.P <= kFewSplits) {
+    constexpr int RPW = 256 / (D / 4);
+    hipLaunchKernelGGL((chunk_combine_few_kernel<D, DT>), dim3((unsigned)((rows + RPW - 1) / RPW)), dim3(256), 0,
+                       stream, p);
+  } else {
+    if (rows > 0x7fffffff) return set_error(kErrUnsupported, "chunk attention: launch too large");
+    hipLaunchKernelGGL((chunk_combine_kernel<D, DT>), dim3((unsigned)rows), dim3(256), 0, stream, p);
+  }
   return check_launch("chunk combine");
 }
 

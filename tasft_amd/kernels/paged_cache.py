@@ -16,6 +16,7 @@ vLLM, ``tasft/inference/vllm_patch.py:172-196``).
 """
 from __future__ import annotations
 
+import functools
 import math
 from typing import NamedTuple
 
@@ -141,15 +142,22 @@ def readable(t: torch.Tensor) -> torch.Tensor:
     return t if _native.kernel_layout(t) else t.clone(memory_format=torch.contiguous_format)
 
 
+@functools.lru_cache(maxsize=1024)
+def _overlaps(shape: tuple[int, ...], strides: tuple[int, ...]) -> bool:
+    expect = 1
+    for size, stride in sorted(((n, s) for n, s in zip(shape, strides) if n > 1), key=lambda x: x[1]):
+        if stride < expect:
+            return True
+        expect = stride * size
+    return False
+
+
 def writable_pool(t: torch.Tensor, what: str, rows16: bool) -> None:
     """Refuses pools that cannot be written in place: overlapping elements, or rows that the
     kernel does not address."""
-    expect = 1
-    for size, stride in sorted(((n, s) for n, s in zip(t.shape, t.stride()) if n > 1), key=lambda x: x[1]):
-        if stride < expect:
-            raise KernelError(f"{what} must not overlap itself (an expanded pool cannot be written)",
-                              context={"strides": list(t.stride())})
-        expect = stride * size
+    if _overlaps(t.shape, t.stride()):
+        raise KernelError(f"{what} must not overlap itself (an expanded pool cannot be written)",
+                          context={"strides": list(t.stride())})
     if t.stride(-1) != 1 or (rows16 and not _native.kernel_layout(t)):
         raise KernelError(f"{what} must have contiguous rows" + (", 16-byte aligned" if rows16 else ""),
                           context={"strides": list(t.stride())})
