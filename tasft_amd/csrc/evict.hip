@@ -94,18 +94,18 @@ __global__ void __launch_bounds__(THREADS) evict_select_kernel(const EvictParams
   }
 
   // Weights and positions of the first run, all loads in flight together. Up to 16 slots a thread
-  // they stay in registers, beyond that only the images do.
+  // they stay in registers, beyond that (HOLD false) only until the images are formed.
   constexpr bool HOLD = KPT <= 16 && !MANY;
   const int runs = MANY ? (len + RUN - 1) / RUN : 1;
-  float w[HOLD ? KPT : 1];
-  int32_t pos[HOLD ? KPT : 1];
+  float w[MANY ? 1 : KPT];
+  int32_t pos[MANY ? 1 : KPT];
   uint32_t img[KPT];
   int newest = -0x7fffffff - 1;
 #pragma unroll
   for (int r = 0; r < KPT; ++r) {
     const int i = min(r * THREADS + tid, len - 1);
     const int32_t x = po[i * sp];
-    if constexpr (HOLD) {
+    if constexpr (!MANY) {
       w[r] = sc[i * ss];
       pos[r] = x;
     }
@@ -137,10 +137,10 @@ __global__ void __launch_bounds__(THREADS) evict_select_kernel(const EvictParams
 #pragma unroll
       for (int r = r0; r < r0 + 8; ++r) {
         const int i = run * RUN + r * THREADS + t, j = min(i, len - 1);
-        const uint32_t x = HOLD ? image(w[HOLD ? r : 0], pos[HOLD ? r : 0]) : image(sc[j * ss], po[j * sp]);
+        const uint32_t x = MANY ? image(sc[j * ss], po[j * sp]) : image(w[MANY ? 0 : r], pos[MANY ? 0 : r]);
         img[r] = i < len ? x : 0u;
       }
-      if constexpr (!HOLD) asm volatile("" ::: "memory");  // eight slots' loads at a time: registers
+      if constexpr (MANY) asm volatile("" ::: "memory");  // eight slots' loads at a time: registers
     }
   };
   form_images(0);

@@ -169,8 +169,10 @@ class _Rotary(torch.autograd.Function):
         given = [g for g, want in ((gq, want_q), (gk, want_k)) if want and g is not None]
         if not given:
             return (None,) * 7
-        out = list(_Rotary.apply(given[0], given[1] if len(given) > 1 else None, positions, inv_freq,
-                                 interleaved, scale, not inverse))
+        # Through the function only where a graph of the gradients is being built.
+        turn = _Rotary.apply if torch.is_grad_enabled() else _rotate
+        out = list(turn(given[0], given[1] if len(given) > 1 else None, positions, inv_freq, interleaved, scale,
+                        not inverse))
         gq = out.pop(0) if want_q and gq is not None else None
         gk = out.pop(0) if want_k and gk is not None else None
         return gq, gk, None, None, None, None, None
