@@ -700,11 +700,14 @@ __global__ void __launch_bounds__(256) chunk_combine_kernel(const ChunkParams p)
 // adding exp2 of the scores to one register per key; lanes are summed once at the end. Fixed
 // order, no atomics.
 //
-// KW of the four waves hold different keys, 4 / KW share out the rows of the same. Many keys
-// (KW = 4) read Q less often, few keys (KW = 1) want four times as many workgroups. RING: the
-// waves walk the same rows, 64 a step, that come by DMA into a ring of four LDS stages, three steps
-// ahead (a step is shorter than a trip to L2); otherwise each wave loads its rows into registers,
-// the next tile's under the exponentials of one: few rows, or few keys.
+// KW of the waves hold different keys, the others share out the rows of the same. Many keys (KW = 4
+// of 4 waves) read Q less often, few keys (KW = 1) want four times as many workgroups. Where there
+// are many rows (RING) they come by DMA through LDS: as loads into a lane's registers the rows'
+// pieces of 16 bytes touch a line each, and the first-level cache bounds the kernel. KW = 4 walks the
+// same rows with all waves, 64 a step, in a ring of four stages filled three steps ahead (a step is
+// shorter than a trip to L2); KW = 1 gives each of eight waves two stages of 32 rows of its own,
+// without a barrier. With few rows each wave loads its own into registers, the next tile's under
+// the exponentials of one.
 // ---------------------------------------------------------------------------------------
 struct WeightParams {
   ChunkParams c;
@@ -729,20 +732,25 @@ struct RowPlace {
   }
 };
 
+constexpr int weight_waves(int kw, bool ring) { return kw == 1 && ring ? 8 : 4; }
+
 template <int D, int DT, int KW, bool RING, bool MASKED>
-__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(RING && D == 128 ? 2 : 3)))
+__global__ void __launch_bounds__(weight_waves(KW, RING) * kWave)
+    __attribute__((amdgpu_waves_per_eu(RING && (D == 128 || KW == 1) ? 2 : 3)))
 chunk_weights_kernel(const WeightParams wp) {
   constexpr int KSTEPS = D / 16;
   constexpr int ROWB = D * 2;
   constexpr int RPU = 1024 / ROWB;
-  constexpr int RW = 4 / KW;               // waves that share one of the KW sets of keys
-  constexpr int STAGE = RING ? kTile * ROWB : 16;
+  constexpr int WAVES = weight_waves(KW, RING);
+  constexpr int RW = WAVES / KW;           // waves that share one of the KW sets of keys
+  constexpr bool OWN = RING && KW == 1;    // two stages of its own for every wave
+  constexpr int STAGE = OWN ? WAVES * 32 * ROWB : RING ? kTile * ROWB : 16;
   const ChunkParams& p = wp.c;
   __shared__ __attribute__((aligned(1024))) uint8_t s0_lds[STAGE];
   __shared__ __attribute__((aligned(1024))) uint8_t s1_lds[STAGE];
-  __shared__ __attribute__((aligned(1024))) uint8_t s2_lds[STAGE];
-  __shared__ __attribute__((aligned(1024))) uint8_t s3_lds[STAGE];
-  __shared__ float lse_lds[4][4][kWave];   // stage, wave (its own copy), row; few keys: the sums
+  __shared__ __attribute__((aligned(1024))) uint8_t s2_lds[OWN ? 16 : STAGE];
+  __shared__ __attribute__((aligned(1024))) uint8_t s3_lds[OWN ? 16 : STAGE];
+  __shared__ float lse_lds[4][WAVES][kWave];   // stage, wave (its own copy), row; few keys: the sums
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int kg = wave % KW, rg = wave / KW;
@@ -829,11 +837,13 @@ chunk_weights_kernel(const WeightParams wp) {
     const int64_t head0 = (int64_t)kvh * p.G;
 
     if constexpr (RING) {
-      constexpr int UNITS = 16 / RPU;  // of a wave's 16 rows of a step
-      constexpr int IN_FLIGHT = 2 * (UNITS + 1);
-      const int di = kTile / p.G, dg = kTile - di * p.G;
-      const int r_start = r_first / kTile * kTile;
-      const int steps = (rows - r_start + kTile - 1) / kTile;
+      constexpr int STEP = OWN ? WAVES * 32 : kTile;   // rows of a step
+      constexpr int SHARE = OWN ? 32 : STEP / WAVES;   // of them, a wave's share of the copying
+      constexpr int UNITS = SHARE / RPU;
+      constexpr int TILES = OWN ? 1 : 2;               // 32 rows that a wave adds in a step
+      const int di = STEP / p.G, dg = STEP - di * p.G;
+      const int r_start = r_first / STEP * STEP;
+      const int steps = (rows - r_start + STEP - 1) / STEP;
       // Byte offsets of the rows a lane brings, moved a step at a time (the host sees to it that 32
       // bits hold them). The buffers end with the sequence's last row: rows past it are zeros.
       const int tokb = (int)p.sq[0] * 2, headb = (int)p.sq[1] * 2;
@@ -857,60 +867,78 @@ chunk_weights_kernel(const WeightParams wp) {
         }
       };
       Source src[UNITS], lsrc;
-      RowPlace tile[2];
+      RowPlace tile[TILES];
 #pragma unroll
       for (int u = 0; u < UNITS; ++u) {
-        const int row = wave * 16 + u * RPU + lane / (ROWB / 16);
+        const int row = wave * SHARE + u * RPU + lane / (ROWB / 16);
         const RowPlace at = place_of(r_start + row);
         src[u] = {at.i * tokb + at.g * headb + chunk_swz_k<D>(row, lane % (ROWB / 16)) * 16, at.g};
       }
       {
-        const RowPlace at = place_of(r_start + lane);
+        const RowPlace at = place_of(r_start + (OWN ? wave * SHARE + col : lane));
         lsrc = {at.i * tokl + at.g * headl, at.g};
       }
 #pragma unroll
-      for (int t = 0; t < 2; ++t) tile[t] = place_of(r_start + t * 32 + col);
+      for (int t = 0; t < TILES; ++t) tile[t] = place_of(r_start + (OWN ? wave * SHARE : t * 32) + col);
       auto dma_step = [&](uint8_t* stage, float* lstage) TASFT_INLINE {
 #pragma unroll
         for (int u = 0; u < UNITS; ++u) {
-          chunk_dma(qr, stage + (wave * 16 + u * RPU) * ROWB, src[u].off);
+          chunk_dma(qr, stage + (wave * SHARE + u * RPU) * ROWB, src[u].off);
           move(src[u], tokb, headb);
         }
         chunk_dma4(lr, lstage, lsrc.off);
         move(lsrc, tokl, headl);
       };
-      dma_step(s0_lds, lse_lds[0][wave]);
-      dma_step(s1_lds, lse_lds[1][wave]);
-      dma_step(s2_lds, lse_lds[2][wave]);
-      // Every step issues the DMA of the one three steps on (past the end: zeros that no step
-      // reads), so that the wait is for a fixed count. By the barrier every wave's share has
-      // landed, and every wave is done with the stage that is filled next.
-      auto step = [&](const uint8_t* now, const float* lnow, uint8_t* then, float* lthen) TASFT_INLINE {
-        __builtin_amdgcn_s_waitcnt(vm_wait(IN_FLIGHT));
-        __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
-        chunk_barrier();
-        if constexpr (!MASKED) dma_step(then, lthen);
+      // Adds the rows r .. r + 31 of a stage.
+      auto add_tile = [&](const uint8_t* now, const float* lnow, int r, RowPlace& at, auto between) TASFT_INLINE {
+        u32x4_t qf[KSTEPS];
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          u32x4_t qf[KSTEPS];
-          const int r = t * 32 + col;
-#pragma unroll
-          for (int ks = 0; ks < KSTEPS; ++ks)
-            qf[ks] = *(const u32x4_t*)(now + r * ROWB + chunk_swz_k<D>(r, ks * 2 + half) * 16);
-          add_rows(qf, tile[t], tile[t].i < sq.len, lnow[r], [] {});
-          tile[t].move(di, dg, p.G);
-        }
-        // Behind the mask bytes' loads: the wait for them would wait for it too.
-        if constexpr (MASKED) dma_step(then, lthen);
+        for (int ks = 0; ks < KSTEPS; ++ks)
+          qf[ks] = *(const u32x4_t*)(now + (r + col) * ROWB + chunk_swz_k<D>(r + col, ks * 2 + half) * 16);
+        add_rows(qf, at, at.i < sq.len, lnow[OWN ? lane : r + col], between);
+        at.move(di, dg, p.G);
       };
-      for (int s = 0; s < steps; s += 4) {
-        step(s0_lds, lse_lds[0][wave], s3_lds, lse_lds[3][wave]);
-        if (s + 1 >= steps) break;
-        step(s1_lds, lse_lds[1][wave], s0_lds, lse_lds[0][wave]);
-        if (s + 2 >= steps) break;
-        step(s2_lds, lse_lds[2][wave], s1_lds, lse_lds[1][wave]);
-        if (s + 3 >= steps) break;
-        step(s3_lds, lse_lds[3][wave], s2_lds, lse_lds[2][wave]);
+      if constexpr (OWN) {
+        // The stage is filled again, for two steps on, once its rows have been used.
+        auto step = [&](uint8_t* now, float* lnow) TASFT_INLINE {
+          __builtin_amdgcn_s_waitcnt(vm_wait(UNITS + 1));
+          add_tile(now, lnow, wave * SHARE, tile[0], [] {});
+          __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
+          dma_step(now, lnow);
+        };
+        dma_step(s0_lds, lse_lds[0][wave]);
+        dma_step(s1_lds, lse_lds[1][wave]);
+        for (int s = 0; s < steps; s += 2) {
+          step(s0_lds, lse_lds[0][wave]);
+          if (s + 1 >= steps) break;
+          step(s1_lds, lse_lds[1][wave]);
+        }
+      } else {
+        dma_step(s0_lds, lse_lds[0][wave]);
+        dma_step(s1_lds, lse_lds[1][wave]);
+        dma_step(s2_lds, lse_lds[2][wave]);
+        // Every step issues the DMA of the one three steps on (past the end: zeros that no step
+        // reads), so that the wait is for a fixed count. By the barrier every wave's share has
+        // landed, and every wave is done with the stage that is filled next.
+        auto step = [&](const uint8_t* now, const float* lnow, uint8_t* then, float* lthen) TASFT_INLINE {
+          __builtin_amdgcn_s_waitcnt(vm_wait(2 * (UNITS + 1)));
+          __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
+          chunk_barrier();
+          if constexpr (!MASKED) dma_step(then, lthen);
+#pragma unroll
+          for (int t = 0; t < TILES; ++t) add_tile(now, lnow, t * 32, tile[t], [] {});
+          // Behind the mask bytes' loads: the wait for them would wait for it too.
+          if constexpr (MASKED) dma_step(then, lthen);
+        };
+        for (int s = 0; s < steps; s += 4) {
+          step(s0_lds, lse_lds[0][wave], s3_lds, lse_lds[3][wave]);
+          if (s + 1 >= steps) break;
+          step(s1_lds, lse_lds[1][wave], s0_lds, lse_lds[0][wave]);
+          if (s + 2 >= steps) break;
+          step(s2_lds, lse_lds[2][wave], s1_lds, lse_lds[1][wave]);
+          if (s + 3 >= steps) break;
+          step(s3_lds, lse_lds[3][wave], s2_lds, lse_lds[2][wave]);
+        }
       }
       __builtin_amdgcn_s_waitcnt(0x0f70);  // no DMA into this workgroup's LDS outlives it
     } else {
@@ -959,6 +987,8 @@ chunk_weights_kernel(const WeightParams wp) {
       lse_lds[0][wave][lane] = total;
       __syncthreads();
       total = (lse_lds[0][0][lane] + lse_lds[0][1][lane]) + (lse_lds[0][2][lane] + lse_lds[0][3][lane]);
+      if constexpr (WAVES == 8)
+        total += (lse_lds[0][4][lane] + lse_lds[0][5][lane]) + (lse_lds[0][6][lane] + lse_lds[0][7][lane]);
     }
   }
   const int key = key0 + (col >> 4) * 32 + ((col & 15) >> 2) * 8 + (col & 3) + 4 * half;
@@ -1132,21 +1162,23 @@ static void launch_weights(const WeightParams& w, hipStream_t stream) {
   const ChunkParams& p = w.c;
   const int64_t heads = (int64_t)p.N * p.Hkv;
   auto grid = [&](int kw) { return heads * ((p.cap + kw * kTile - 1) / (kw * kTile)); };
-  // Byte offsets within a sequence's rows of Q and log-sums, a few steps past the end included.
-  const int64_t most = ((int64_t)1 << 31) - 1;
-  const bool small = ((int64_t)p.L + 5 * kTile) * p.sq[0] * 2 + p.G * p.sq[1] * 2 + D * 2 < most &&
-                     ((int64_t)p.L + 5 * kTile) * w.sl[0] * 4 + p.G * w.sl[1] * 4 + 4 < most;
-  auto run = [&](auto plain, auto masked, int64_t wgs) {
-    if (p.mask) hipLaunchKernelGGL(masked, dim3((unsigned)wgs), dim3(256), 0, stream, w);
-    else hipLaunchKernelGGL(plain, dim3((unsigned)wgs), dim3(256), 0, stream, w);
+  // Byte offsets within a sequence's rows of Q and log-sums, the steps past the end included.
+  const int64_t most = ((int64_t)1 << 31) - 1, past = (int64_t)p.L + 4 * 256;
+  const bool ring = (int64_t)p.L * p.G > 128 && past * p.sq[0] * 2 + p.G * p.sq[1] * 2 + D * 2 < most &&
+                    past * w.sl[0] * 4 + p.G * w.sl[1] * 4 + 4 < most;
+  auto run = [&](auto plain, auto masked, int kw, bool ringed) {
+    const dim3 wgs((unsigned)grid(kw)), threads(weight_waves(kw, ringed) * kWave);
+    if (p.mask) hipLaunchKernelGGL(masked, wgs, threads, 0, stream, w);
+    else hipLaunchKernelGGL(plain, wgs, threads, 0, stream, w);
   };
   // Few keys (not two workgroups of 256 keys per CU): four times as many workgroups.
-  if (grid(4) < 512)
-    run(chunk_weights_kernel<D, DT, 1, false, false>, chunk_weights_kernel<D, DT, 1, false, true>, grid(1));
-  else if ((int64_t)p.L * p.G <= 128 || !small)
-    run(chunk_weights_kernel<D, DT, 4, false, false>, chunk_weights_kernel<D, DT, 4, false, true>, grid(4));
-  else
-    run(chunk_weights_kernel<D, DT, 4, true, false>, chunk_weights_kernel<D, DT, 4, true, true>, grid(4));
+  if (grid(4) < 512) {
+    if (ring) run(chunk_weights_kernel<D, DT, 1, true, false>, chunk_weights_kernel<D, DT, 1, true, true>, 1, true);
+    else run(chunk_weights_kernel<D, DT, 1, false, false>, chunk_weights_kernel<D, DT, 1, false, true>, 1, false);
+  } else {
+    if (ring) run(chunk_weights_kernel<D, DT, 4, true, false>, chunk_weights_kernel<D, DT, 4, true, true>, 4, true);
+    else run(chunk_weights_kernel<D, DT, 4, false, false>, chunk_weights_kernel<D, DT, 4, false, true>, 4, false);
+  }
 }
 
 extern "C" int tasft_key_weights(

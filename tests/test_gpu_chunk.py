@@ -39,14 +39,14 @@ def _put(t, dev):
     return [x.to(dev) for x in t]
 
 
-def _mask(case, seed, bs, density, rows=None):
+def _mask(case, seed, bs, density, rows=None, blocks=None):
     lens, kv, hq = case[0], case[1], case[2]
     page = case[5]
     longest = max(lens)
     r = rows or (longest + bs - 2) // bs + 1
     cap = (max(max(1, -(-max(x, 1) // page)) for x in kv) + 1) * page
     g = torch.Generator().manual_seed(seed)
-    return torch.rand((len(lens), hq, r, -(-cap // bs)), generator=g) < density
+    return torch.rand((len(lens), hq, r, blocks or -(-cap // bs)), generator=g) < density
 
 
 def _check(out, lse, want, dtype, d, keys, what):
@@ -194,14 +194,26 @@ def test_lengths_are_clamped(lens):
 @pytest.mark.parametrize("masked", [0, 32, 64, 128])
 @pytest.mark.parametrize("index", range(len(CASES)))
 def test_key_weights(index, masked):
+    _check_weights(index, masked, None)
+
+
+@pytest.mark.parametrize("masked", [0, 32, 64, 128])
+@pytest.mark.parametrize("index", range(len(CASES)))
+def test_key_weights_of_a_wide_table(index, masked):
+    # Room for 512 workgroups of 256 keys: the kernel for many keys.
+    lens, _, _, hkv, _, page = CASES[index][:6]
+    _check_weights(index, masked, -(-512 // (len(lens) * hkv)) * 256 // page)
+
+
+def _check_weights(index, masked, max_pages):
     case = CASES[index]
     lens, kv, hq, hkv, d, page, dtype, causal = case
     dev = require_gpu()
-    t = ref.make(lens, kv, hq, hkv, d, page, dtype, seed=100 + index, pad=2)
+    t = ref.make(lens, kv, hq, hkv, d, page, dtype, seed=100 + index, pad=2, max_pages=max_pages)
     q, k, v, table, kvl, cu = t
-    mask = _mask(case, index, masked, 0.3) if masked else None
-    lse = ref.attention(*t, mask=mask, bs=masked or 64, causal=causal)[1].float()
     cap = table.shape[1] * page
+    mask = _mask(case, index, masked, 0.3, blocks=-(-cap // masked)) if masked else None
+    lse = ref.attention(*t, mask=mask, bs=masked or 64, causal=causal)[1].float()
     before = torch.rand((len(lens), hkv, cap), generator=torch.Generator().manual_seed(index))
     total, dot = ref.key_weights(q, k, table, kvl, cu, lse, before, mask, masked or 64, causal)
     weight = total - before.double()
