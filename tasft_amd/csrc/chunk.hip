@@ -18,8 +18,8 @@
 //
 // Masked scores are -inf before the exponential, and a key past kv_len is never read (its row
 // arrives as zeros). A tile in which only some rows see a key could still carry an infinity or
-// NaN of V into the others as 0 * inf: there V is looked over, and such a tile takes a slow
-// path that adds each key to the rows that see it.
+// NaN of V into the others as 0 * inf: there V is looked over and such values are left out of the
+// product; after the last tile they are added key by key to the rows that see them.
 #include <type_traits>
 
 #include "common.h"
@@ -70,7 +70,7 @@ __device__ __forceinline__ ChunkSeq chunk_seq(const ChunkParams& p, int n) {
   const int t1 = min(max(p.cu[n + 1], s.t0), p.T);
   s.len = min(t1 - s.t0, p.L);
   s.kv = min(max(p.kv_lens[n], 0), p.cap);
-  s.p0 = s.kv - s.len;
+  s.p0 = s.kv - (t1 - s.t0);  // of the whole chunk, also where L cuts it
   return s;
 }
 

@@ -201,7 +201,7 @@ def append_paged(
         positions: ``[T]`` int32 or int64 positions (default: the tokens' slots, right as long as
             nothing was evicted).
         slot_positions: ``[N, Hkv, max_pages * page_size]`` int32 contiguous, receives each new
-            token's position at its slot (what ``evict_paged`` reads).
+            token's position at its slot (what ``evict_paged`` reads; its low 32 bits).
 
     Returns:
         The rotated queries ``[T, Hq, D]`` (0 for tokens behind ``cu_seqlens[N]``, which are not
@@ -373,7 +373,8 @@ def evict_paged(
         raise KernelError("Tensors must be on one CUDA device",
                           context={"k_pages": str(dev), "v_pages": str(v_pages.device)})
     table, lens = int32_on(block_table, dev), int32_on(kv_lens, dev)
-    budget = min(budget, shape[2])
+    if budget >= shape[2]:  # nothing to evict
+        budget, recent, sinks = shape[2], 0, 0
     lib = _native.load_library()
     ws_bytes = lib.tasft_evict_workspace_bytes(n, Hkv, budget)
     workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
@@ -384,8 +385,7 @@ def evict_paged(
         status = lib.tasft_evict_paged(
             k_pages.data_ptr(), v_pages.data_ptr(), table.data_ptr(), lens.data_ptr(), scores.data_ptr(),
             slot_positions.data_ptr(), lens_out.data_ptr(), scores_out.data_ptr(), pos_out.data_ptr(),
-            workspace.data_ptr(), ws_bytes, n, Hkv, D, page_size, P, max_pages, budget, min(recent, budget),
-            min(sinks, budget), _native.strides(k_pages), _native.strides(v_pages), _native.strides(scores),
+            workspace.data_ptr(), ws_bytes, n, Hkv, D, page_size, P, max_pages, budget, recent, sinks, _native.strides(k_pages), _native.strides(v_pages), _native.strides(scores),
             _native.strides(slot_positions), table.stride(0), _native.stream_handle(dev))
     _native.check(status, "tasft_evict_paged", {"sequences": n, "slots": shape[2], "budget": budget})
     return lens_out, scores_out, pos_out

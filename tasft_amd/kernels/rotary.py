@@ -206,6 +206,8 @@ def apply_rotary(
     if q.ndim not in (3, 4):
         raise KernelError(f"Expected q of shape [B, H, S, D] or [T, H, D], got {tuple(q.shape)}",
                           context={"q_shape": list(q.shape)})
+    if q.shape[1] == 0:
+        raise KernelError("q must have at least one head", context={"q_shape": list(q.shape)})
     _native.dtype_code(q.dtype, "rotary")
     if k is not None:
         # All but the head counts are the same.

@@ -234,3 +234,54 @@ def _check_weights(index, masked, max_pages):
     # The weights of a row add up to one.
     rows = int((lse[:int(cu[-1])] != -math.inf).sum())
     assert abs(float(bare.double().sum()) - rows) <= (rel + 1e-5) * max(rows, 1)
+
+
+@pytest.mark.parametrize("masked", [0, 64])
+def test_longer_than_max_seqlen(masked):
+    """A sequence's tokens behind its first max_seqlen are left out; those before keep their place."""
+    dev = require_gpu()
+    lens, kv, cut = [150, 3, 40], [400, 90, 40], 70
+    t = ref.make(lens, kv, 4, 2, 128, 16, BF, seed=3)
+    case = (lens, kv, 4, 2, 128, 16)
+    rows = (cut + 62) // 64 + 1
+    mask = _mask(case, 1, 64, 0.4, blocks=-(-t[3].shape[1] * 16 // 64)) if masked else None
+    want = ref.attention(*t, mask=mask)
+    q, k, v, table, kvl, cu = _put(t, dev)
+    md = None if mask is None else mask[:, :, :rows].to(dev)
+    attn = BlockSparseFlashAttention(min_sparsity_for_speedup=0.0)
+    print(f"chunk longer than max_seqlen, masked={masked}", flush=True)
+    out, lse = attn.forward_chunk_paged(q, k, v, table, kvl, cu, md, max_seqlen=cut, return_lse=True)
+    kept = torch.cat([torch.arange(min(x, cut)) + int(a) for x, a in zip(lens, t[5])])
+    _check(out[kept], lse[kept], [x[kept] for x in want], BF, 128, max(kv), "kept")
+    # Their weights alone, each row's adding up to one.
+    w = accumulate_key_weights(q, k, table, kvl, cu, lse, block_mask=md, max_seqlen=cut)
+    short = want[1].float()
+    short[[i for i in range(sum(lens)) if i not in set(kept.tolist())]] = -math.inf
+    zeros = torch.zeros(w.shape)
+    total, dot = ref.key_weights(*[t[i] for i in (0, 1, 3, 4, 5)], short, zeros, mask)
+    rel = 4 * ((128 + 3) * dot + 8 * (1 + dot)) * 2.0 ** -24 + (cut * 2 + max(kv)) * 2.0 ** -24
+    assert bool(((w.cpu().double() - total).abs() <= rel * total).all())
+
+
+@pytest.mark.parametrize("masked", [0, 64])
+@pytest.mark.parametrize("lens", [[1, 1], [5, 300]])
+def test_offsets_past_32_bits(lens, masked):
+    """Pools whose pages lie 128 MB apart, 5 GB in all: the same bits as in close pools."""
+    dev = require_gpu()
+    kv, page = [300, 700], 32
+    t = ref.make(lens, kv, 4, 2, 128, page, BF, seed=4)
+    mask = _mask((lens, kv, 4, 2, 128, page), 2, 64, 0.5, blocks=-(-t[3].shape[1] * page // 64)) if masked else None
+    q, k, v, table, kvl, cu = _put(t, dev)
+    md = None if mask is None else mask.to(dev)
+    far = []
+    for x in (k, v):
+        room = torch.empty((x.shape[0], 1 << 26), dtype=BF, device=dev)
+        far.append(room[:, :x[0].numel()].view(x.shape).copy_(x))
+    assert (k.shape[0] - 1) << 26 > 1 << 31
+    attn = BlockSparseFlashAttention(min_sparsity_for_speedup=0.0)
+    print(f"chunk far pages lens={lens} masked={masked}", flush=True)
+    out, lse = attn.forward_chunk_paged(q, k, v, table, kvl, cu, md, max_seqlen=max(lens), return_lse=True)
+    o2, l2 = attn.forward_chunk_paged(q, *far, table, kvl, cu, md, max_seqlen=max(lens), return_lse=True)
+    assert torch.equal(out, o2) and torch.equal(lse, l2)
+    w = accumulate_key_weights(q, k, table, kvl, cu, lse, block_mask=md, max_seqlen=max(lens))
+    assert torch.equal(w, accumulate_key_weights(q, far[0], table, kvl, cu, lse, block_mask=md, max_seqlen=max(lens)))

@@ -171,6 +171,47 @@ def test_evict_views():
     assert all(torch.equal(x, y) for x, y in zip(a, b)) and torch.equal(k1, k2) and torch.equal(v1, v2)
 
 
+def test_evict_budget_of_more_than_the_table():
+    """What is always kept may be more than a small table holds, as long as it fits the budget."""
+    dev = require_gpu()
+    _, kp, vp, table, kvl, _ = ref.make([0, 0], [90, 60], 2, 2, 64, 16, HF, seed=8)
+    kp, vp = kp.nan_to_num(1.0), vp.nan_to_num(1.0, posinf=1.0)
+    cap = table.shape[1] * 16
+    scores, pos = torch.rand(2, 2, cap), torch.arange(cap, dtype=torch.int32).expand(2, 2, cap).contiguous()
+    for budget, recent, sinks in ((cap, cap - 1, 1), (cap + 1, cap, 1), (4096, 2000, 2000), (1 << 40, 1 << 39, 5)):
+        print(f"evict budget {budget} of {cap} slots", flush=True)
+        d = [x.to(dev) for x in (kp, vp, table, kvl, scores, pos)]
+        lens, s, p = evict_paged(*d, budget, recent=recent, sinks=sinks)
+        assert torch.equal(lens.cpu(), kvl) and torch.equal(d[0].cpu(), kp) and torch.equal(d[1].cpu(), vp)
+        for n in range(2):
+            x = int(kvl[n])
+            assert torch.equal(s[n, :, :x].cpu(), scores[n, :, :x]) and torch.equal(p[n, :, :x].cpu(), pos[n, :, :x])
+            assert not s[n, :, x:].any() and bool((p[n, :, x:] == -1).all())
+
+
+def test_cache_offsets_past_32_bits():
+    """Appending to and evicting from pools whose pages lie 128 MB apart."""
+    dev = require_gpu()
+    lens, kv, page = [3, 40], [300, 700], 32
+    _, kp, vp, table, kvl, cu = ref.make(lens, kv, 4, 2, 128, page, BF, seed=4)
+    kp, vp = kp.nan_to_num(2.0).to(dev), vp.nan_to_num(2.0, posinf=2.0).to(dev)
+    far = [torch.empty((kp.shape[0], 1 << 26), dtype=BF, device=dev)[:, :kp[0].numel()].view(kp.shape).copy_(x)
+           for x in (kp, vp)]
+    assert (kp.shape[0] - 1) << 26 > 1 << 31
+    cap = table.shape[1] * page
+    table, kvl, cu = table.to(dev), kvl.to(dev), cu.to(dev)
+    q, k, v = (x.to(dev) for x in _tokens(sum(lens), 4, 2, 128, BF, 1))
+    inv = rotary_frequencies(128, device=dev)[0]
+    scores = torch.rand((2, 2, cap), device=dev)
+    results = []
+    print("append and evict, far pages", flush=True)
+    for a, b in ((kp, vp), far):
+        pos = torch.arange(cap, dtype=torch.int32, device=dev).expand(2, 2, cap).contiguous()
+        out = append_paged(q, k, v, a, b, table, kvl, cu, inv, slot_positions=pos)
+        results.append((out, *evict_paged(a, b, table, kvl, scores, pos, 200, recent=20, sinks=2), a, b))
+    assert all(torch.equal(x, y) for x, y in zip(*results))
+
+
 @pytest.mark.parametrize(("dtype", "page", "hq", "hkv", "d"), [(BF, 16, 8, 2, 128), (HF, 8, 4, 4, 64)])
 def test_serving_steps(dtype, page, hq, hkv, d):
     """Two requests served in chunks and then token by token on a bounded cache: every step's

@@ -93,6 +93,7 @@ def _rope(**over):
 @pytest.mark.parametrize(("over", "match"), [
     ({}, "CUDA"),
     ({"q": torch.zeros(5, 64, dtype=BF)}, "Expected q"),
+    ({"q": torch.zeros(2, 0, 5, 64, dtype=BF)}, "one head"),
     ({"q": torch.zeros(2, 4, 5, 64)}, "bf16 or fp16"),
     ({"k": torch.zeros(2, 2, 5, 64, dtype=torch.float16)}, "one dtype"),
     ({"k": torch.zeros(2, 2, 6, 64, dtype=BF)}, "incompatible"),
