@@ -179,7 +179,8 @@ chunk_rows_kernel(const ChunkParams p) {
   const int n = (int)(group / p.Hkv), kvh = (int)(group % p.Hkv);
   const int split = member % p.P;
   member /= p.P;
-  const int qt = member % p.QT, gm = member / p.QT;
+  // The longest rows first, of all heads.
+  const int gm = MASKED ? member % p.G : 0, qt = p.QT - 1 - (MASKED ? member / p.G : member);
   const ChunkSeq sq = chunk_seq(p, n);
   if (sq.len == 0) return;
 
