@@ -1165,20 +1165,31 @@ static void launch_weights(const WeightParams& w, hipStream_t stream) {
   auto grid = [&](int kw) { return heads * ((p.cap + kw * kTile - 1) / (kw * kTile)); };
   // Byte offsets within a sequence's rows of Q and log-sums, the steps past the end included.
   const int64_t most = ((int64_t)1 << 31) - 1, past = (int64_t)p.L + 4 * 256;
-  const bool ring = (int64_t)p.L * p.G > 128 && past * p.sq[0] * 2 + p.G * p.sq[1] * 2 + D * 2 < most &&
-                    past * w.sl[0] * 4 + p.G * w.sl[1] * 4 + 4 < most;
+  const bool small = past * p.sq[0] * 2 + p.G * p.sq[1] * 2 + D * 2 < most &&
+                     past * w.sl[0] * 4 + p.G * w.sl[1] * 4 + 4 < most;
   auto run = [&](auto plain, auto masked, int kw, bool ringed) {
     const dim3 wgs((unsigned)grid(kw)), threads(weight_waves(kw, ringed) * kWave);
     if (p.mask) hipLaunchKernelGGL(masked, wgs, threads, 0, stream, w);
     else hipLaunchKernelGGL(plain, wgs, threads, 0, stream, w);
   };
-  // Few keys (not two workgroups of 256 keys per CU): four times as many workgroups.
+  const int64_t rows = (int64_t)p.L * p.G;
+  // Few keys (not two workgroups of 256 keys per CU): four times as many workgroups (8 heads, 2048
+  // keys: 512 new tokens 18 instead of 57 us, 2048 new tokens 44 instead of 193; where 64 heads have
+  // 4096 keys the other way round, 64 new tokens 115 instead of 35 us).
+  // Many rows: through LDS. With steps of 64 rows that pays from 33 on (8 requests of 16384 keys: 32
+  // rows 52 us without and 55 with it, 64 rows 69 and 58), with steps of 256 from about 1024 on (4096
+  // keys: 512 rows of one request 15 and 18 us, of two 30 and 33; 1024 of one 22 and 23, of two 56 and
+  // 43; 8192 of one, 2048 keys, 64 and 44).
   if (grid(4) < 512) {
-    if (ring) run(chunk_weights_kernel<D, DT, 1, true, false>, chunk_weights_kernel<D, DT, 1, true, true>, 1, true);
-    else run(chunk_weights_kernel<D, DT, 1, false, false>, chunk_weights_kernel<D, DT, 1, false, true>, 1, false);
+    if (small && rows >= 1024)
+      run(chunk_weights_kernel<D, DT, 1, true, false>, chunk_weights_kernel<D, DT, 1, true, true>, 1, true);
+    else
+      run(chunk_weights_kernel<D, DT, 1, false, false>, chunk_weights_kernel<D, DT, 1, false, true>, 1, false);
   } else {
-    if (ring) run(chunk_weights_kernel<D, DT, 4, true, false>, chunk_weights_kernel<D, DT, 4, true, true>, 4, true);
-    else run(chunk_weights_kernel<D, DT, 4, false, false>, chunk_weights_kernel<D, DT, 4, false, true>, 4, false);
+    if (small && rows > 32)
+      run(chunk_weights_kernel<D, DT, 4, true, false>, chunk_weights_kernel<D, DT, 4, true, true>, 4, true);
+    else
+      run(chunk_weights_kernel<D, DT, 4, false, false>, chunk_weights_kernel<D, DT, 4, false, true>, 4, false);
   }
 }
 

@@ -9,10 +9,12 @@
 // before the fp32 sine: positions of any size keep the sine's own accuracy (p f in fp32 would
 // be off by 0.03 rad at p = 10^6).
 //
-// Bound by memory: 4 bytes per element. A workgroup takes a few tokens: it computes their
-// sines once into LDS (shared by all heads; per head they would cost more than the traffic),
-// then every thread keeps one place within a row and walks the (token, head) rows, two
-// 16-byte vectors of the two halves at a time.
+// Bound by memory: 4 bytes per element (32768 tokens of 32 + 8 heads of 128: 117 us, 5.7 TB/s;
+// 64 tokens 4 us, the launch). A workgroup takes a token: it computes its sines once into LDS
+// (shared by all heads; per head they would cost more than the traffic), then every thread keeps
+// one place within a row and walks the heads, two 16-byte vectors of the two halves at a time.
+// (Four tokens a workgroup, one wait for the sines of all: 125 us for 32768, 9.1 instead of 8.6 for
+// 2048, 5.6 instead of 4.0 for 64.)
 #include "common.h"
 
 #include "../../include/tasft_amd.h"
@@ -20,7 +22,6 @@
 namespace tasft {
 
 constexpr int kRotaryThreads = 256;
-constexpr int kRotaryTok = 4;  // tokens per workgroup of large launches
 constexpr int kRotaryMaxHeadDim = 256;
 
 struct RotaryParams {
@@ -61,71 +62,62 @@ __device__ __forceinline__ float2 turn(float a, float b, float2 w) {
   return make_float2(fmaf(-b, w.y, a * w.x), fmaf(a, w.y, b * w.x));
 }
 
-// VEC elements per vector: 8 where strides, alignment and dims allow (the host decides), else 1.
+// VEC elements per vector: 8 where strides, alignment and dims allow (the host decides), else 1
+// (1024 tokens as above: 6 and 12 us, 32768: 117 and 225).
 // A place is one vector of each half (half layout), or one vector of whole pairs
 // (interleaved; at VEC 1 the pair's two elements), or VEC plain elements behind the pairs.
 template <int DT, int VEC, bool INTER, bool APPEND>
 __global__ void __launch_bounds__(kRotaryThreads)
-rotary_kernel(const RotaryParams p, int tok_per_wg) {
-  __shared__ float2 cs[kRotaryTok][kRotaryMaxHeadDim / 2];
-  __shared__ int64_t t_pos[kRotaryTok];
-  __shared__ int64_t t_slot[kRotaryTok];  // append: slot in the sequence's cache, -1: none
-  __shared__ int32_t t_seq[kRotaryTok];   // append: the token's sequence, N: padding
-  __shared__ int32_t t_page[kRotaryTok];  // append: its page, -1: none
-  __shared__ int32_t count[kRotaryTok];
+rotary_kernel(const RotaryParams p) {
+  __shared__ float2 cs[kRotaryMaxHeadDim / 2];
+  __shared__ int64_t t_pos;
+  __shared__ int64_t t_slot;  // append: slot in the sequence's cache
+  __shared__ int32_t t_seq;   // append: the token's sequence, N: padding
+  __shared__ int32_t t_page;  // append: its page, -1: none
   const int tid = threadIdx.x;
-  const int64_t tok0 = (int64_t)blockIdx.x * tok_per_wg;
-  const int ntok = (int)min((int64_t)tok_per_wg, p.tokens - tok0);
+  const int64_t tok = blockIdx.x;
 
   if constexpr (APPEND) {
     // A token's sequence: the number of ends at or before it (one load per thread and 256
     // sequences, instead of a search whose steps wait for each other).
-    if (tid < kRotaryTok) count[tid] = 0;
+    if (tid == 0) t_seq = 0;
     __syncthreads();
     for (int n0 = 0; n0 < p.N; n0 += kRotaryThreads) {
       const int n = n0 + tid;
-      const int64_t end = n < p.N ? p.cu[n + 1] : (int64_t)1 << 62;
-      for (int t = 0; t < ntok; ++t) {
-        const int c = __popcll(__ballot(end <= tok0 + t));
-        if ((tid & 63) == 0 && c) atomicAdd(&count[t], c);
-      }
+      const int c = __popcll(__ballot(n < p.N && p.cu[n + 1] <= tok));
+      if ((tid & 63) == 0 && c) atomicAdd(&t_seq, c);
     }
     __syncthreads();
-    if (tid < ntok) {
-      const int seq = count[tid];
+    if (tid == 0) {
+      const int seq = t_seq;
       int64_t slot = -1, pos = 0;
       int page = -1;
       if (seq < p.N) {
-        const int64_t t = tok0 + tid, start = p.cu[seq], len = p.cu[seq + 1] - start;
+        const int64_t start = p.cu[seq], len = p.cu[seq + 1] - start;
         const int64_t kv = min(max((int64_t)p.kv_lens[seq], (int64_t)0), p.cap);
-        slot = kv - len + (t - start);
+        slot = kv - len + (tok - start);
         // Outside the table, or a page outside the pool: rotated, but nothing is written.
         if (slot >= 0 && slot < p.cap) {
           page = p.table[(int64_t)seq * p.bt_stride + (slot >> p.ps_shift)];
           if (page < 0 || page >= p.num_pages) page = -1;
         }
-        pos = p.pos ? position_at(p, t * p.sp[1]) : slot;
+        pos = p.pos ? position_at(p, tok * p.sp[1]) : slot;
       }
-      t_seq[tid] = seq;
-      t_slot[tid] = slot;
-      t_page[tid] = page;
-      t_pos[tid] = pos;
+      t_slot = slot;
+      t_page = page;
+      t_pos = pos;
     }
-    __syncthreads();
-  } else {
-    if (tid < ntok) {
-      const int64_t t = tok0 + tid, b = t / p.S, s = t - b * p.S;
-      t_pos[tid] = position_at(p, b * p.sp[0] + s * p.sp[1]);
-    }
-    __syncthreads();
+  } else if (tid == 0) {
+    const int64_t b = tok / p.S, s = tok - b * p.S;
+    t_pos = position_at(p, b * p.sp[0] + s * p.sp[1]);
   }
-  for (int i = tid; i < ntok * p.pairs; i += kRotaryThreads) {
-    const int t = i / p.pairs, j = i - t * p.pairs;
-    double rev = (double)t_pos[t] * (p.inv_freq[j] * 0.15915494309189533577);
+  __syncthreads();
+  if (tid < p.pairs) {
+    double rev = (double)t_pos * (p.inv_freq[tid] * 0.15915494309189533577);
     rev -= rint(rev);
     float s, c;
     sincospif(2.f * (float)rev, &s, &c);
-    cs[t][j] = make_float2(c * p.scale, (p.inverse ? -s : s) * p.scale);
+    cs[tid] = make_float2(c * p.scale, (p.inverse ? -s : s) * p.scale);
   }
   __syncthreads();
 
@@ -134,8 +126,7 @@ rotary_kernel(const RotaryParams p, int tok_per_wg) {
   const int places = turned + (p.D - 2 * p.pairs) / VEC;
   const int rows_at_once = kRotaryThreads / places;
   const int place = tid % places;
-  int row = tid / places;
-  if (row >= rows_at_once) return;
+  if (tid / places >= rows_at_once) return;
   const bool turns = place < turned;
   // First element of the place's vector, and of its second one (half layout, pairs at VEC 1).
   int e0, e1 = -1, pair0 = 0;
@@ -151,31 +142,29 @@ rotary_kernel(const RotaryParams p, int tok_per_wg) {
     pair0 = e0;
   }
   const int heads = p.Hq + (APPEND ? 2 : 1) * p.Hkv;
-  int t = row / heads, h = row % heads;
-  while (t < ntok) {
+  const int64_t b = APPEND ? 0 : tok / p.S, s = tok - b * p.S;
+  for (int h = tid / places; h < heads; h += rows_at_once) {
     const uint16_t* src;
     uint16_t* dst;
     bool copy = !turns, zero = false, skip = false;
     if constexpr (APPEND) {
-      const int64_t tok = tok0 + t;
-      const int64_t in_page = t_slot[t] & ((1 << p.ps_shift) - 1);
+      const int64_t in_page = t_slot & ((1 << p.ps_shift) - 1);
       if (h < p.Hq) {
         src = p.q + tok * p.sq[2] + h * p.sq[1];
         dst = p.qo + tok * p.sqo[2] + h * p.sqo[1];
-        zero = t_seq[t] >= p.N;
+        zero = t_seq >= p.N;
       } else {
         const bool is_v = h >= p.Hq + p.Hkv;
         const int g = h - p.Hq - (is_v ? p.Hkv : 0);
         src = is_v ? p.v + tok * p.sv[2] + g * p.sv[1] : p.k + tok * p.sk[2] + g * p.sk[1];
         const int64_t* st = is_v ? p.svo : p.sko;
-        skip = t_page[t] < 0;
-        dst = (is_v ? p.vo : p.ko) + (int64_t)t_page[t] * st[0] + in_page * st[1] + g * st[2];
+        skip = t_page < 0;
+        dst = (is_v ? p.vo : p.ko) + (int64_t)t_page * st[0] + in_page * st[1] + g * st[2];
         copy = copy || is_v;
         if (!is_v && place == 0 && !skip && p.slot_pos)
-          p.slot_pos[((int64_t)t_seq[t] * p.Hkv + g) * p.cap + t_slot[t]] = (int32_t)t_pos[t];
+          p.slot_pos[((int64_t)t_seq * p.Hkv + g) * p.cap + t_slot] = (int32_t)t_pos;
       }
     } else {
-      const int64_t tok = tok0 + t, b = tok / p.S, s = tok - b * p.S;
       if (h < p.Hq) {
         src = p.q + b * p.sq[0] + h * p.sq[1] + s * p.sq[2];
         dst = p.qo + b * p.sqo[0] + h * p.sqo[1] + s * p.sqo[2];
@@ -197,7 +186,7 @@ rotary_kernel(const RotaryParams p, int tok_per_wg) {
             if constexpr (INTER) {
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
-                const float2 w = cs[t][pair0 + i];
+                const float2 w = cs[pair0 + i];
                 const float2 r = turn(a[2 * i], a[2 * i + 1], w);
                 x[i] = pack16x2<DT>(r.x, r.y);
               }
@@ -205,7 +194,7 @@ rotary_kernel(const RotaryParams p, int tok_per_wg) {
               unpack16x8<DT>(y, c);
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
-                const float2 w0 = cs[t][pair0 + 2 * i], w1 = cs[t][pair0 + 2 * i + 1];
+                const float2 w0 = cs[pair0 + 2 * i], w1 = cs[pair0 + 2 * i + 1];
                 const float2 r0 = turn(a[2 * i], c[2 * i], w0), r1 = turn(a[2 * i + 1], c[2 * i + 1], w1);
                 x[i] = pack16x2<DT>(r0.x, r1.x);
                 y[i] = pack16x2<DT>(r0.y, r1.y);
@@ -221,7 +210,7 @@ rotary_kernel(const RotaryParams p, int tok_per_wg) {
           x = src[e0];
           if (e1 >= 0) y = src[e1];
           if (!copy) {
-            const float2 r = turn(bits16_to_f32<DT>(x), bits16_to_f32<DT>(y), cs[t][pair0]);
+            const float2 r = turn(bits16_to_f32<DT>(x), bits16_to_f32<DT>(y), cs[pair0]);
             const uint32_t w = pack16x2<DT>(r.x, r.y);
             x = (uint16_t)(w & 0xffffu);
             y = (uint16_t)(w >> 16);
@@ -230,11 +219,6 @@ rotary_kernel(const RotaryParams p, int tok_per_wg) {
         dst[e0] = x;
         if (e1 >= 0) dst[e1] = y;
       }
-    }
-    h += rows_at_once;
-    while (h >= heads) {
-      h -= heads;
-      ++t;
     }
   }
 }
@@ -250,12 +234,9 @@ static bool vector_rows(const void* base, const int64_t* strides, int n) {
 template <bool APPEND>
 static int launch_rotary(const RotaryParams& p, bool vec, int interleaved, int dtype, hipStream_t stream,
                          const char* what) {
-  // Small launches: one token per workgroup (latency); larger ones share the sines' phase.
-  const int tok = p.tokens >= 4096 ? kRotaryTok : 1;
-  const int64_t grid = (p.tokens + tok - 1) / tok;
-  if (grid > 0x7fffffff) return set_error(kErrUnsupported, "%s: too many tokens", what);
-  const dim3 g((unsigned)grid), b(kRotaryThreads);
-  auto run = [&](auto kernel) { hipLaunchKernelGGL(kernel, g, b, 0, stream, p, tok); };
+  if (p.tokens > 0x7fffffff) return set_error(kErrUnsupported, "%s: too many tokens", what);
+  const dim3 g((unsigned)p.tokens), b(kRotaryThreads);
+  auto run = [&](auto kernel) { hipLaunchKernelGGL(kernel, g, b, 0, stream, p); };
   if (dtype == kF16) {
     if (vec) interleaved ? run(rotary_kernel<kF16, 8, true, APPEND>) : run(rotary_kernel<kF16, 8, false, APPEND>);
     else interleaved ? run(rotary_kernel<kF16, 1, true, APPEND>) : run(rotary_kernel<kF16, 1, false, APPEND>);

@@ -205,14 +205,30 @@ def test_key_weights_of_a_wide_table(index, masked):
     _check_weights(index, masked, -(-512 // (len(lens) * hkv)) * 256 // page)
 
 
-def _check_weights(index, masked, max_pages):
-    case = CASES[index]
+@pytest.mark.parametrize("masked", [0, 32, 64, 128])
+@pytest.mark.parametrize("index", range(len(CASES)))
+def test_key_weights_of_many_rows(index, masked):
+    # As many rows as the kernel for few keys and many rows asks for, most of them padding.
+    _check_weights(index, masked, None, pad=1024, longest=1024)
+
+
+@pytest.mark.parametrize("masked", [0, 64])
+@pytest.mark.parametrize("case", [([700, 513], [700, 1500], 4, 2, 128, 16, BF, True),
+                                  ([2100, 1], [2300, 900], 3, 3, 64, 64, HF, True)])
+def test_key_weights_of_long_chunks(case, masked):
+    _check_weights(case, masked, None)
+
+
+def _check_weights(index, masked, max_pages, pad=2, longest=None):
+    case = CASES[index] if isinstance(index, int) else index
+    index = index if isinstance(index, int) else 50
     lens, kv, hq, hkv, d, page, dtype, causal = case
     dev = require_gpu()
-    t = ref.make(lens, kv, hq, hkv, d, page, dtype, seed=100 + index, pad=2, max_pages=max_pages)
+    longest = longest or max(lens)
+    t = ref.make(lens, kv, hq, hkv, d, page, dtype, seed=100 + index, pad=pad, max_pages=max_pages)
     q, k, v, table, kvl, cu = t
     cap = table.shape[1] * page
-    mask = _mask(case, index, masked, 0.3, blocks=-(-cap // masked)) if masked else None
+    mask = _mask(case, index, masked, 0.3, (longest + masked - 2) // masked + 1, -(-cap // masked)) if masked else None
     lse = ref.attention(*t, mask=mask, bs=masked or 64, causal=causal)[1].float()
     before = torch.rand((len(lens), hkv, cap), generator=torch.Generator().manual_seed(index))
     total, dot = ref.key_weights(q, k, table, kvl, cu, lse, before, mask, masked or 64, causal)
@@ -221,7 +237,7 @@ def _check_weights(index, masked, max_pages):
     a = [x.to(dev) for x in (q, k, table, kvl, cu, lse)]
     md = None if mask is None else mask.to(dev)
     got = accumulate_key_weights(*a, before.to(dev), block_mask=md, block_size=masked or 64, causal=causal,
-                                 max_seqlen=max(lens))
+                                 max_seqlen=longest)
     torch.cuda.synchronize()
     # Scores as in the attention's bound, twice for the exponent's own rounding; fp32 sums over rows.
     rel = 2 * ((d + 3) * dot + 8 * (1 + dot)) * 2.0 ** -24 + (max(lens) * hq // hkv + 2) * 2.0 ** -24
@@ -229,7 +245,7 @@ def _check_weights(index, masked, max_pages):
     assert bool((err <= rel * weight + 2.0 ** -23 * total).all()), float((err - rel * weight).max())
     for n in range(len(lens)):
         assert torch.equal(got[n, :, max(kv[n], 0):].cpu(), before[n, :, max(kv[n], 0):])
-    bare = accumulate_key_weights(*a, block_mask=md, block_size=masked or 64, causal=causal, max_seqlen=max(lens))
+    bare = accumulate_key_weights(*a, block_mask=md, block_size=masked or 64, causal=causal, max_seqlen=longest)
     assert bool(((bare.cpu().double() - weight).abs() <= rel * weight + 2.0 ** -23 * weight).all())
     # The weights of a row add up to one.
     rows = int((lse[:int(cu[-1])] != -math.inf).sum())
