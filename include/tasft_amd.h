@@ -544,7 +544,8 @@ size_t tasft_chunk_workspace_bytes(int64_t tokens, int64_t num_q_heads, int64_t 
  * its last). out = softmax(q.k * scale) v over them, rows without keys 0; lse [T, Hq] fp32
  * contiguous (or NULL) the natural logarithm of the sum of exponentials, -inf without keys. Rows
  * of tokens at or after cu_seqlens[N] get 0 and -inf. What a row does not see does not reach it,
- * infinities and NaN included. Sequences are at most max_seqlen tokens of a call.
+ * infinities and NaN included. A sequence's tokens behind its first max_seqlen are left out: their
+ * rows are not written.
  * head_dim 64 or 128; block_size 32, 64 or 128; page_size a power of two >= 8; strides multiples
  * of 8 on 16-byte aligned bases. num_splits (1 to 1024) shares the keys of a row among
  * workgroups, joined by a second launch; workspace: tasft_chunk_workspace_bytes(...) bytes.
@@ -591,7 +592,7 @@ size_t tasft_evict_workspace_bytes(int64_t num_seqs, int64_t num_kv_heads, int64
  * place, nothing else of them is written. kv_lens_out[n] = n'; scores_out and positions_out
  * [N, Hkv, max_pages * page_size] contiguous hold the kept slots' values where they are now, and
  * 0 and -1 from n' on. scores fp32 and positions int32 have element strides (sequence, head,
- * slot); outputs must not overlap them. Sequences must not share pages that they evict from; a
+ * slot); outputs must not overlap them. No page may belong to two sequences, or twice to one; a
  * row whose page lies outside the pool is not moved. recent + sinks <= budget. head_dim a
  * multiple of 8 up to 256, page_size a power of two, 16-bit pools (any type) with strides of
  * multiples of 8. At most 65535 (sequence, KV head) pairs.

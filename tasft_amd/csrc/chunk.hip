@@ -20,6 +20,16 @@
 // arrives as zeros). A tile in which only some rows see a key could still carry an infinity or
 // NaN of V into the others as 0 * inf: there V is looked over and such values are left out of the
 // product; after the last tile they are added key by key to the rows that see them.
+//
+// Many rows: bound by the matrix cores and the exponentials of one wave not running beside the
+// other's (two waves per SIMD, all the registers allow). 2048 tokens of 32 / 8 heads over 32768 keys:
+// 1003 us, 1.07 PFLOP/s, 49% MFMA busy; a fifth of the blocks of 4 requests of 2048 over up to 16384:
+// 354 us, 0.71 PFLOP/s, 34% busy. Few rows: by the reads of the cache. 64 tokens of 64 requests of 8k
+// to 16k keys: 589 us, 5.5 TB/s.
+// Measured and not kept: three tiles in LDS for the masked form (a whole step's time for each DMA,
+// three workgroups a CU instead of four: 481 instead of 402 us); the same heads of every sequence on
+// one XCD (no gain, 376 instead of 362 us where a group's keys were then read twice); a higher wave
+// priority during the products (2% slower dense, 2% faster masked).
 #include <type_traits>
 
 #include "common.h"
@@ -143,7 +153,8 @@ constexpr int kMaskTile = 64;  // positions of a masked one: two waves
 // PIECES: runs of a wave's share of a tile that lie in one page each (one where pages are at least as
 // long as the share). A template: the general form's scalar registers spilled, at a fifth of the time.
 template <int D, int DT, bool MASKED, int PIECES>
-__global__ void __launch_bounds__(MASKED ? 128 : 256) __attribute__((amdgpu_waves_per_eu(D == 64 && MASKED ? 3 : 2, D == 64 && MASKED ? 3 : 2)))
+__global__ void __launch_bounds__(MASKED ? 128 : 256)
+    __attribute__((amdgpu_waves_per_eu(D == 64 && MASKED ? 3 : 2, D == 64 && MASKED ? 3 : 2)))
 chunk_rows_kernel(const ChunkParams p) {
   constexpr int WAVES = MASKED ? 2 : 4;
   constexpr int ROW_TILE = MASKED ? kMaskTile : kRowTile;
@@ -179,7 +190,8 @@ chunk_rows_kernel(const ChunkParams p) {
   const int n = (int)(group / p.Hkv), kvh = (int)(group % p.Hkv);
   const int split = member % p.P;
   member /= p.P;
-  // The longest rows first, of all heads.
+  // The longest rows first, of all heads: the short ones fill the launch's end (a prompt of 8192
+  // tokens 574 us in order, 513 so; masked 315 and 290).
   const int gm = MASKED ? member % p.G : 0, qt = p.QT - 1 - (MASKED ? member / p.G : member);
   const ChunkSeq sq = chunk_seq(p, n);
   if (sq.len == 0) return;
@@ -709,6 +721,11 @@ __global__ void __launch_bounds__(256) chunk_combine_kernel(const ChunkParams p)
 // shorter than a trip to L2); KW = 1 gives each of eight waves two stages of 32 rows of its own,
 // without a barrier. With few rows each wave loads its own into registers, the next tile's under
 // the exponentials of one.
+//
+// Many rows are bound by the exponentials: 32 rows and 64 keys are 512 cycles of products and 768 of
+// exponentials, multiply-adds and sums, on two waves per SIMD (256 tokens of 2 requests over 28k
+// keys on average: 120 us, 0.87 PFLOP/s, 34% MFMA busy). Few rows by the reads of K (one token of
+// 32 requests over 4097 keys, 28 / 4 heads: 28.5 us, 4.9 TB/s).
 // ---------------------------------------------------------------------------------------
 struct WeightParams {
   ChunkParams c;

@@ -334,7 +334,7 @@ def evict_paged(
 
     Args:
         k_pages, v_pages: the pools (bf16 or fp16, head_dim a multiple of 8), changed in place.
-            Sequences must not share pages.
+            No page may belong to two sequences, or twice to one.
         block_table: ``[N, max_pages]`` int32; kv_lens: ``[N]``.
         scores: ``[N, Hkv, max_pages * page_size]`` fp32 (``accumulate_key_weights``).
         slot_positions: the same shape, int32 (``append_paged``).
