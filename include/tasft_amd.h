@@ -579,8 +579,8 @@ int tasft_key_weights(
     const int64_t* lse_strides, const int64_t* score_strides, const int64_t* mask_strides,
     int64_t block_table_stride, float scale, int causal, int dtype, void* stream);
 
-/* Bytes of workspace tasft_evict_paged needs (budget at most max_pages * page_size). */
-size_t tasft_evict_workspace_bytes(int64_t num_seqs, int64_t num_kv_heads, int64_t budget);
+/* Bytes of workspace tasft_evict_paged needs; slots = max_pages * page_size. */
+size_t tasft_evict_workspace_bytes(int64_t num_seqs, int64_t num_kv_heads, int64_t slots, int64_t budget);
 
 /*
  * Eviction from a paged cache by accumulated weight. No reference counterpart.

@@ -166,7 +166,7 @@ _SIGNATURES: dict[str, tuple[object, list[object]]] = {
         [_P, _P, _P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64,
          _I64, _I64, _I64P, _I64P, _I64P, _I64P, _I64P, _I64, _F, _I, _I, _P],
     ),
-    "tasft_evict_workspace_bytes": (_SZ, [_I64, _I64, _I64]),
+    "tasft_evict_workspace_bytes": (_SZ, [_I64, _I64, _I64, _I64]),
     "tasft_evict_paged": (
         _I,
         [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _SZ, _I64, _I64, _I64, _I64, _I64, _I64, _I64,

@@ -376,7 +376,7 @@ def evict_paged(
     if budget >= shape[2]:  # nothing to evict
         budget, recent, sinks = shape[2], 0, 0
     lib = _native.load_library()
-    ws_bytes = lib.tasft_evict_workspace_bytes(n, Hkv, budget)
+    ws_bytes = lib.tasft_evict_workspace_bytes(n, Hkv, shape[2], budget)
     workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
     lens_out = torch.empty((n,), dtype=torch.int32, device=dev)
     scores_out = torch.empty(shape, dtype=torch.float32, device=dev)

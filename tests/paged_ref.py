@@ -182,15 +182,16 @@ def evict(k, v, table, kv_lens, scores, positions, budget, recent, sinks):
                 return (not guarded, not nan, 0.0 if guarded or nan else -w[j], j)
 
             kept = sorted(sorted(range(length), key=rank)[:keep])
-            holes = [j for j in range(keep) if j not in set(kept)]
+            held = set(kept)
+            holes = [j for j in range(keep) if j not in held]
             movers = [j for j in kept if j >= keep]
             src = list(range(keep))
             for a, b in zip(holes, movers):
                 src[a] = b
-            rows = [(int(table[i, j // page]), j % page) for j in range(length)]
+            pages = table[i].tolist()
+            rows = [(pages[j // page], j % page) for j in range(length)]
             for a, b in zip(holes, movers):
                 k[rows[a][0], rows[a][1], h] = k[rows[b][0], rows[b][1], h]
                 v[rows[a][0], rows[a][1], h] = v[rows[b][0], rows[b][1], h]
-            for a, b in enumerate(src):
-                s_out[i, h, a], p_out[i, h, a] = scores[i, h, b], positions[i, h, b]
+            s_out[i, h, :keep], p_out[i, h, :keep] = scores[i, h, src], positions[i, h, src]
     return k, v, lens.clamp(max=budget), s_out, p_out

@@ -113,7 +113,13 @@ def test_append_skips_pages_outside_the_pool_and_takes_views():
     ([150, 80], 40, 7, 2, 2, 64, 8, "odd"),               # NaN, infinities, negative weights, -0
     ([1500, 2048, 2049], 1000, 100, 4, 2, 64, 16, "random"),
     ([3000, 9000], 512, 50, 4, 1, 64, 64, "few"),         # few distinct weights
-    ([33000], 700, 20, 4, 1, 8, 128, "random"),           # more slots than the registers hold
+    ([33000], 700, 20, 4, 1, 8, 128, "random"),           # more slots than a workgroup holds
+    ([40000, 70001, 100, 0], 20000, 300, 4, 2, 8, 128, "random"),
+    ([40000, 24576, 16385], 9000, 0, 0, 2, 8, 64, "equal"),
+    ([50000, 49152], 30000, 30000, 0, 1, 8, 64, "odd"),
+    ([45000, 33000], 12345, 7, 2, 1, 8, 8, "zeros"),
+    ([66000], 66000 - 1, 9, 0, 2, 8, 32, "few"),
+    ([530000, 9000], 8200, 1000, 4, 1, 8, 128, "few"),    # parts of two runs
     ([500], 1000, 10, 4, 2, 64, 16, "random"),            # within the budget
 ])
 def test_evict(kv, budget, recent, sinks, hkv, d, page, kind):

@@ -291,8 +291,14 @@ def test_key_weight_entry_refusals():
 def test_evict_entry_refusals():
     lib = _native.load_library()
     pool, st = _i64(4096, 256, 128, 1), _i64(192, 96, 1, 0)
-    assert lib.tasft_evict_workspace_bytes(2, 2, 10) == 4 * 21 * 4
-    assert lib.tasft_evict_workspace_bytes(0, 2, 10) == 0
+    assert lib.tasft_evict_workspace_bytes(2, 2, 64, 10) == 4 * 21 * 4
+    assert lib.tasft_evict_workspace_bytes(2, 2, 8, 10) == 4 * 17 * 4
+    assert lib.tasft_evict_workspace_bytes(0, 2, 64, 10) == 0 == lib.tasft_evict_workspace_bytes(2, 2, 0, 10)
+    # In parts of 8192 slots: three words each, three digits of three, three times 2048 counts each.
+    assert lib.tasft_evict_workspace_bytes(2, 3, 40000, 10) == 6 * 4 * (21 + 15 + 9 + 15 * 2048)
+    # At most 64 parts, of whole runs.
+    assert lib.tasft_evict_workspace_bytes(1, 1, 1 << 20, 10) == 4 * (21 + 192 + 9 + 192 * 2048)
+    assert lib.tasft_evict_workspace_bytes(1, 1, (1 << 19) + 1, 10) == 4 * (21 + 99 + 9 + 99 * 2048)
 
     def call(k=FAKE, wb=1 << 20, n=2, d=128, page=16, budget=10, recent=2, sinks=1, kp=pool, ss=st, per=6):
         return lib.tasft_evict_paged(k, FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, wb, n, 2, d, page, 9, per,
