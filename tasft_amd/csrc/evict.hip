@@ -130,6 +130,15 @@ __device__ __forceinline__ int number_cells(const int* cells, int* base, int* wt
   return total;
 }
 
+// Slots from .. to of a head that keeps all its len keys: as they are, 0 and -1 behind them.
+__device__ __forceinline__ void copy_head(const EvictParams& p, const float* sc, const int32_t* po, float* so,
+                                          int32_t* pout, int len, int64_t from, int64_t to, int tid, int threads) {
+  for (int64_t i = from + tid; i < to; i += threads) {
+    so[i] = i < len ? sc[i * p.ss[2]] : 0.f;
+    pout[i] = i < len ? po[i * p.sp[2]] : -1;
+  }
+}
+
 // THREADS threads with KPT slots each, THREADS * KPT slots at the most: a thread's slots are
 // THREADS apart, so that a round of all threads is a run of slots in order.
 template <int THREADS, int KPT>
@@ -155,19 +164,8 @@ __global__ void __launch_bounds__(THREADS) evict_select_kernel(const EvictParams
   const int64_t ss = p.ss[2], sp = p.sp[2];
   if (h == 0 && tid == 0) p.kv_lens_out[n] = keep;
 
-  // Slots behind the kept ones; with nothing to evict the rest is copied as it is.
-  auto clear_rest = [&]() {
-    for (int64_t i = keep + tid; i < p.cap; i += THREADS) {
-      so[i] = 0.f;
-      pout[i] = -1;
-    }
-  };
-  if (len <= p.budget) {
-    for (int i = tid; i < keep; i += THREADS) {
-      so[i] = sc[i * ss];
-      pout[i] = po[i * sp];
-    }
-    clear_rest();
+  if (len <= p.budget) {  // nothing to evict
+    copy_head(p, sc, po, so, pout, len, 0, p.cap, tid, THREADS);
     if (tid == 0) moves[0] = 0;
     return;
   }
@@ -273,14 +271,6 @@ __global__ void __launch_bounds__(THREADS) evict_select_kernel(const EvictParams
     }
   }
   if (tid == 0) moves[0] = hole_count;  // as many movers as holes
-  clear_rest();
-  __threadfence_block();
-  __syncthreads();
-  for (int r = tid; r < hole_count; r += THREADS) {
-    const int to = holes[r], from = sources[r];
-    so[to] = sc[from * ss];
-    pout[to] = po[from * sp];
-  }
 }
 
 // The same selection where a head has more slots than one workgroup holds: its slots are cut into
@@ -322,15 +312,8 @@ __global__ void __launch_bounds__(kPartThreads) evict_part_kernel(const EvictPar
 
   if constexpr (PHASE == 4) {
     if (h == 0 && part == 0 && tid == 0) p.kv_lens_out[n] = keep;
-    for (int64_t i = max(from, (int64_t)keep) + tid; i < min(from + p.part_slots, p.cap); i += kPartThreads) {
-      so[i] = 0.f;
-      pout[i] = -1;
-    }
     if (len <= p.budget) {
-      for (int64_t i = from + tid; i < to; i += kPartThreads) {
-        so[i] = sc[i * ss];
-        pout[i] = po[i * sp];
-      }
+      copy_head(p, sc, po, so, pout, len, from, min(from + p.part_slots, p.cap), tid, kPartThreads);
       if (part == 0 && tid == 0) moves[0] = 0;
     }
   }
@@ -502,20 +485,27 @@ __global__ void __launch_bounds__(kPartThreads) evict_part_kernel(const EvictPar
 }
 
 // Rows of K and V from the movers' slots to the holes: D / 8 lanes move one key's K row and its
-// V row, 16 bytes a lane each (and, where the selection came in parts, its weight and position).
+// V row, 16 bytes a lane each, and its weight and position. Slots behind the kept ones are cleared.
 __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const EvictParams p) {
   const int nh = blockIdx.y, n = nh / p.Hkv, h = nh % p.Hkv;
   const int32_t* moves = p.moves + (int64_t)nh * (1 + 2 * (int64_t)p.budget);
   const int count = moves[0];
+  const int64_t head = (int64_t)nh * p.cap;
+  if (p.kv_lens[n] > p.budget)
+    for (int64_t i = p.budget + (int64_t)blockIdx.x * kMoveThreads + threadIdx.x; i < p.cap;
+         i += (int64_t)gridDim.x * kMoveThreads) {
+      p.scores_out[head + i] = 0.f;
+      p.positions_out[head + i] = -1;
+    }
   const int per = p.D / 8, at_once = kMoveThreads / per;
   const int sub = threadIdx.x / per, c = threadIdx.x % per;
   if (sub >= at_once) return;
   const int32_t* table = p.table + n * p.bt_stride;
   for (int r = blockIdx.x * at_once + sub; r < count; r += gridDim.x * at_once) {
     const int to = moves[1 + r], from = moves[1 + p.budget + r];
-    if (p.parts > 1 && c == 0) {
-      p.scores_out[nh * p.cap + to] = p.scores[n * p.ss[0] + h * p.ss[1] + from * p.ss[2]];
-      p.positions_out[nh * p.cap + to] = p.positions[n * p.sp[0] + h * p.sp[1] + from * p.sp[2]];
+    if (c == 0) {
+      p.scores_out[head + to] = p.scores[n * p.ss[0] + h * p.ss[1] + from * p.ss[2]];
+      p.positions_out[head + to] = p.positions[n * p.sp[0] + h * p.sp[1] + from * p.sp[2]];
     }
     const int pt = table[to >> p.ps_shift], pf = table[from >> p.ps_shift];
     if (pt < 0 || pt >= p.num_pages || pf < 0 || pf >= p.num_pages) continue;
@@ -643,7 +633,8 @@ extern "C" int tasft_evict_paged(void* k_pages, void* v_pages, const int32_t* bl
   }
   if (const int rc = check_launch("evict select")) return rc;
   // About 16 workgroups per CU over all heads, no more than a head's rows can use: each row is a
-  // chain of a table entry and two loads, so many have to be on their way.
+  // chain of a table entry and two loads, so many have to be on their way (four times as many: 512
+  // heads of 4096 slots 100 instead of 94 us, both launches, 32 of 32768 slots 48.5 and 48.7).
   const int64_t rows = kMoveThreads / (head_dim / 8);
   const int64_t most = budget < cap - budget ? budget : cap - budget;  // movers of a head at the most
   if (most <= 0) return kOk;
