@@ -12,9 +12,9 @@
 // prefix over those counts places them. The second copies rows, many workgroups per head. Heads of
 // more than 32768 slots are selected from in parts, in six launches.
 // Sources lie behind n', destinations before it: no row is read and written. The second is bound
-// by the bytes of the moved rows (20.8 us for 32 heads of 4096 kept of up to 32768 keys of 128, 118 MB
+// by the bytes of the moved rows (22.8 us for 32 heads of 4096 kept of up to 32768 keys of 128, 118 MB
 // in and out by the counters), the first by its chain of barriers: one workgroup a head, since the
-// digits follow each other (37.8 us for the same, 12.1 for 256 heads of 1040 slots).
+// digits follow each other (31.8 us for the same, 12.2 for 512 heads of 1040 slots).
 #include "common.h"
 
 #include "../../include/tasft_amd.h"
@@ -632,13 +632,15 @@ extern "C" int tasft_evict_paged(void* k_pages, void* v_pages, const int32_t* bl
     phase(evict_part_kernel<5>);
   }
   if (const int rc = check_launch("evict select")) return rc;
-  // About 16 workgroups per CU over all heads, no more than a head's rows can use: each row is a
-  // chain of a table entry and two loads, so many have to be on their way (four times as many: 512
-  // heads of 4096 slots 100 instead of 94 us, both launches, 32 of 32768 slots 48.5 and 48.7).
+  // About 16 workgroups per CU over all heads, no more than a head's rows (and the slots to clear, 16
+  // a thread) can use: each row is a chain of a table entry and two loads, so many have to be on their
+  // way (four times as many: 512 heads of 4096 slots 100 instead of 94 us, both launches, 32 of 32768
+  // slots 48.5 and 48.7).
   const int64_t rows = kMoveThreads / (head_dim / 8);
   const int64_t most = budget < cap - budget ? budget : cap - budget;  // movers of a head at the most
   if (most <= 0) return kOk;
-  const int64_t want = (4096 + heads - 1) / heads, need = (most + rows - 1) / rows;
+  const int64_t want = (4096 + heads - 1) / heads, clear = (cap - budget) / (16 * kMoveThreads);
+  const int64_t need = (most + rows - 1) / rows > clear ? (most + rows - 1) / rows : clear;
   hipLaunchKernelGGL(evict_move_kernel, dim3((unsigned)(need < want ? need : want), heads), dim3(kMoveThreads), 0, st,
                      p);
   return check_launch("evict move");
