@@ -798,14 +798,20 @@ def default_decode_splits(batch: int, num_kv_heads: int, num_blocks: int,
 
 def default_chunk_splits(num_seqs: int, num_kv_heads: int, q_per_kv: int, chunk: int, slots: int,
                          masked: bool = False) -> int:
-    """Key splits of ``forward_chunk_paged``: one where its row tiles (128 rows of a KV head's
-    tokens and query heads, two workgroups per CU; with a mask 64 positions of a head, four per CU)
-    fill three quarters of the GPU's 256 CUs, else as many as it holds at once, at least four 64-key
-    tiles each (a workgroup more takes a round of its own: 300 tokens of 8 heads over 131072 keys 202
-    us with 26 splits, 256 with 27). Few rows (a wave's 32) over long caches are read by 2048 workgroups, 2048 keys or more
-    each: requests of different lengths end together (one token of 64 requests of 8k to 16k keys:
-    574 us with one split, 554 with 4; of 48 of 4k to 8k: 139 with 3, 129 with 4; where all have
-    4096 keys it costs 3%)."""
+    """Key splits of ``forward_chunk_paged``, by its row tiles: 128 rows of a KV head's tokens and
+    query heads, two workgroups per CU, or with a mask 64 positions of a head, four per CU.
+
+    * Tiles that fill three quarters of the GPU's 256 CUs: one split. Fewer: as many splits as the
+      GPU holds at once, at least four 64-key tiles each (a workgroup more takes a round of its own:
+      300 tokens of 8 heads over 131072 keys 202 us with 26 splits, 256 with 27).
+    * Few rows (a wave's 32) over long caches: 2048 workgroups, 2048 keys or more each, so that
+      requests of different lengths end together (one token of 64 requests of 8k to 16k keys 574 us
+      with one split, 554 with 4; of 48 of 4k to 8k 139 with 3, 129 with 4; where all have 4096 keys
+      it costs 3%).
+    * Many rows whose last round leaves a seventh of all rounds idle, over caches of four times
+      their chunk: three (32 / 8 heads over 32768 keys: 2100 tokens 1456 and 1142 us, 4200 tokens 2378
+      and 2103; where most keys are the chunk's own, 4200 tokens over 8192, it would cost 10%).
+    """
     if masked:
         tiles, full = num_seqs * num_kv_heads * q_per_kv * math.ceil(chunk / 64), 1024
     else:
@@ -813,6 +819,9 @@ def default_chunk_splits(num_seqs: int, num_kv_heads: int, q_per_kv: int, chunk:
     splits = 1 if tiles >= 0.75 * full else min(full // tiles, math.ceil(slots / 256), 64)
     if not masked and chunk * q_per_kv <= 32:
         splits = max(splits, min(math.ceil(2048 / tiles), slots // 2048, 64))
+    elif not masked and 0.75 * full <= tiles < 4 * full and slots >= max(4 * chunk, 16384):
+        if tiles < 0.85 * full * math.ceil(tiles / full):
+            splits = 3
     return max(1, splits)
 
 

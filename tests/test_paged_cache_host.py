@@ -194,6 +194,8 @@ def test_evict_refusals(over, error, match):
 def test_chunk_splits():
     assert default_chunk_splits(1, 8, 4, 2048, 32768) == 1
     assert default_chunk_splits(1, 8, 4, 1, 64) == 1
+    assert default_chunk_splits(1, 8, 4, 2100, 32768) == 3 and default_chunk_splits(1, 8, 4, 2100, 4096) == 1
+    assert default_chunk_splits(1, 1, 8, 300, 131072) == 26 and default_chunk_splits(64, 8, 4, 1, 16384) == 4
     for n, hkv, g, chunk, slots in ((1, 8, 4, 1, 32768), (64, 8, 4, 1, 16384), (2, 4, 7, 256, 32768), (1, 1, 1, 1, 8)):
         for masked in (False, True):
             s = default_chunk_splits(n, hkv, g, chunk, slots, masked)
