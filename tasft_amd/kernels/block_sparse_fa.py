@@ -675,7 +675,7 @@ class BlockSparseFlashAttention:
         mask = None if block_mask is None else chunk_mask(block_mask, b, H, self.block_size, dev)
         if num_splits is None:
             num_splits = default_chunk_splits(b.num_seqs, Hkv, H // Hkv, min(b.max_seqlen, T), b.slots,
-                                              mask is not None)
+                                              mask is not None, D)
         elif not 1 <= num_splits <= 1024:
             raise KernelError(f"num_splits must be in [1, 1024], got {num_splits}",
                               context={"num_splits": num_splits})
@@ -797,13 +797,16 @@ def default_decode_splits(batch: int, num_kv_heads: int, num_blocks: int,
 
 
 def default_chunk_splits(num_seqs: int, num_kv_heads: int, q_per_kv: int, chunk: int, slots: int,
-                         masked: bool = False) -> int:
+                         masked: bool = False, head_dim: int = 128) -> int:
     """Key splits of ``forward_chunk_paged``, by its row tiles: 128 rows of a KV head's tokens and
-    query heads, two workgroups per CU, or with a mask 64 positions of a head, four per CU.
+    query heads, two workgroups per CU, or with a mask 64 positions of a head, four per CU (six with
+    heads of 64: 3 x 700 tokens of 16 of them 59 us with one split, 49 with two).
 
     * Tiles that fill three quarters of the GPU's 256 CUs: one split. Fewer: as many splits as the
       GPU holds at once, at least four 64-key tiles each (a workgroup more takes a round of its own:
-      300 tokens of 8 heads over 131072 keys 202 us with 26 splits, 256 with 27).
+      300 tokens of 8 heads over 131072 keys 202 us with 26 splits, 256 with 27). More than 8 are
+      joined by a workgroup a row, which costs more than it gives past 8192 rows (a mask, 600 tokens
+      of 16 heads of 64: 39 us with 9, 28 with 6).
     * Few rows (a wave's 32) over long caches: 2048 workgroups, 2048 keys or more each, so that
       requests of different lengths end together (one token of 64 requests of 8k to 16k keys 574 us
       with one split, 554 with 4; of 48 of 4k to 8k 139 with 3, 129 with 4; where all have 4096 keys
@@ -813,10 +816,12 @@ def default_chunk_splits(num_seqs: int, num_kv_heads: int, q_per_kv: int, chunk:
       and 2103; where most keys are the chunk's own, 4200 tokens over 8192, it would cost 10%).
     """
     if masked:
-        tiles, full = num_seqs * num_kv_heads * q_per_kv * math.ceil(chunk / 64), 1024
+        tiles, full = num_seqs * num_kv_heads * q_per_kv * math.ceil(chunk / 64), 1024 if head_dim > 64 else 1536
     else:
         tiles, full = num_seqs * num_kv_heads * math.ceil(chunk * q_per_kv / 128), 512
     splits = 1 if tiles >= 0.75 * full else min(full // tiles, math.ceil(slots / 256), 64)
+    if num_seqs * chunk * num_kv_heads * q_per_kv > 8192:
+        splits = min(splits, 8)
     if not masked and chunk * q_per_kv <= 32:
         splits = max(splits, min(math.ceil(2048 / tiles), slots // 2048, 64))
     elif not masked and 0.75 * full <= tiles < 4 * full and slots >= max(4 * chunk, 16384):
