@@ -11,14 +11,16 @@
 // each and share 64-key tiles of K and V in LDS, brought by DMA through the page table a tile
 // ahead: two stages, one barrier a tile. Masked: neighbouring heads and blocks see different keys,
 // so a workgroup takes 64 positions of one head aligned to the mask's blocks, two waves, with one
-// K and one V tile. S^T = K Q^T with v_mfma_f32_32x32x16, so a lane owns one row: its
+// K and one V tile; but where all rows of a KV head fit one wave, the dense form goes over the tiles
+// that any of them selects, each row with its own bits of the mask. S^T = K Q^T with v_mfma_f32_32x32x16, so a lane owns one row: its
 // running maximum and sum stay in the lane (and the one 32 away), and the accumulator of S^T is
 // the B operand of O^T = V^T P^T. P is rounded to the input type for that product (as the MFMA
 // takes it); maxima, sums, O and the log-sum are fp32.
 //
 // Masked scores are -inf before the exponential, and a key past kv_len is never read (its row
 // arrives as zeros). A tile in which only some rows see a key could still carry an infinity or
-// NaN of V into the others as 0 * inf: there V is looked over and such values are left out of the
+// NaN of V into the others as 0 * inf: there V's largest magnitude is looked for (every value by
+// itself took as long as the rest of the tile) and, if it is not finite, such values are left out of the
 // product; after the last tile they are added key by key to the rows that see them.
 //
 // Many rows: bound by the matrix cores and the exponentials of one wave not running beside the
@@ -125,6 +127,8 @@ __device__ __forceinline__ int chunk_swz_v(int r, int cc) {
   return cc ^ (D == 128 ? ((r & 3) << 2) : (((r >> 1) & 1) << 2));
 }
 
+typedef uint16_t u16x2_t __attribute__((ext_vector_type(2)));
+
 // A pair of 16-bit values with infinities and NaN replaced by 0.
 template <int DT>
 __device__ __forceinline__ uint32_t finite2(uint32_t w) {
@@ -152,10 +156,13 @@ constexpr int kMaskTile = 64;  // positions of a masked one: two waves
 
 // PIECES: runs of a wave's share of a tile that lie in one page each (one where pages are at least as
 // long as the share). A template: the general form's scalar registers spilled, at a fifth of the time.
-template <int D, int DT, bool MASKED, int PIECES>
-__global__ void __launch_bounds__(MASKED ? 128 : 256)
-    __attribute__((amdgpu_waves_per_eu(D == 64 && MASKED ? 3 : 2, D == 64 && MASKED ? 3 : 2)))
+// MASK: kDense, kPositions (64 positions of a head), kRows (a mask, the dense form's rows).
+enum ChunkMask { kDense = 0, kPositions = 1, kRows = 2 };
+template <int D, int DT, int MASK, int PIECES>
+__global__ void __launch_bounds__(MASK == kPositions ? 128 : 256)
+    __attribute__((amdgpu_waves_per_eu(D == 64 && MASK == kPositions ? 3 : 2, D == 64 && MASK == kPositions ? 3 : 2)))
 chunk_rows_kernel(const ChunkParams p) {
+  constexpr bool MASKED = MASK == kPositions, ROWMASK = MASK == kRows;
   constexpr int WAVES = MASKED ? 2 : 4;
   constexpr int ROW_TILE = MASKED ? kMaskTile : kRowTile;
   constexpr int ROW_SHIFT = MASKED ? 6 : 7;
@@ -247,7 +254,15 @@ chunk_rows_kernel(const ChunkParams p) {
   int cursor = tile_a, chunk = tile_a - kWave, own_next = 0;
   uint64_t ubits = 0, own0 = 0, own1 = 0;
   const uint8_t* mseq = nullptr;
-  int row_lo = 0, row_hi = 0, row_own = 0;
+  int row_lo = 0, row_hi = 0, row_own = 0;  // mask rows; row_own: the wave's (positions), the lane's (rows)
+  if constexpr (ROWMASK) {
+    mseq = p.mask + n * p.sm[0] + (int64_t)kvh * p.G * p.sm[1];
+    const int block0 = sq.p0 >> p.bs_shift;
+    auto row_of = [&](int j) { return min(max(((sq.p0 + j) >> p.bs_shift) - block0, 0), p.mask_rows - 1); };
+    row_lo = row_of(0);
+    row_hi = row_of(i_end);
+    row_own = row_of(i);
+  }
   if constexpr (MASKED) {
     mseq = p.mask + n * p.sm[0] + (int64_t)(kvh * p.G + gm) * p.sm[1];
     const int block0 = sq.p0 >> p.bs_shift;
@@ -257,8 +272,42 @@ chunk_rows_kernel(const ChunkParams p) {
     row_own = wave_on ? row_of(i_first) : -1;
   }
   auto next_tile = [&]() TASFT_INLINE -> int {
-    if constexpr (!MASKED) {
+    if constexpr (MASK == kDense) {
       return cursor < tile_b ? cursor++ : -1;
+    } else if constexpr (ROWMASK) {
+      while (ubits == 0) {
+        chunk += kWave;
+        if (chunk >= tile_b) return -1;
+        const int kt = min(chunk + lane, tile_b - 1);
+        const int b0 = p.bs_shift == 5 ? 2 * kt : kt >> (p.bs_shift - 6);
+        const int b1 = p.bs_shift == 5 ? min(2 * kt + 1, (p.cap - 1) >> 5) : b0;
+        // Every head's rows of the mask, four heads' loads in flight; a lane keeps its own row's.
+        uint32_t any = 0;
+        own0 = own1 = 0;
+        for (int g0 = 0; g0 < p.G; g0 += 4)
+          for (int r = row_lo; r <= row_hi; ++r) {
+            uint32_t x[4], y[4];
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+              const uint8_t* m = mseq + min(g0 + g, p.G - 1) * p.sm[1] + r * p.sm[2];
+              x[g] = m[b0 * p.sm[3]];
+              y[g] = m[b1 * p.sm[3]];
+            }
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+              const bool mine = h - kvh * p.G == g0 + g && row_own == r;
+              const uint64_t bx = __ballot(x[g] != 0), by = __ballot(y[g] != 0);
+              own0 = mine ? bx : own0;
+              own1 = mine ? by : own1;
+              any |= x[g] | y[g];
+            }
+          }
+        ubits = __ballot(any != 0 && chunk + lane < tile_b);
+      }
+      const int b = __builtin_ctzll(ubits);
+      ubits &= ubits - 1;
+      own_next = (int)((own0 >> b) & 1) | (int)((own1 >> b) & 1) << 1;
+      return chunk + b;
     } else {
       while (ubits == 0) {
         chunk += kWave;
@@ -338,7 +387,10 @@ chunk_rows_kernel(const ChunkParams p) {
   int fix_from = 0x7fffffff;  // first tile whose infinities or NaN of V were left out
 
   // Whether this wave has anything to do with a tile.
-  auto takes_part = [&](int kt, int own) { return kt * kTile <= any_see && (!MASKED || own != 0); };
+  auto takes_part = [&](int kt, int own) {
+    if constexpr (ROWMASK) return kt * kTile <= any_see && __ballot(row_ok && own != 0) != 0;
+    return kt * kTile <= any_see && (!MASKED || own != 0);
+  };
   // S^T of a tile. Register rr of s0 / s1 is key 4 half + off(rr) (+ 32), off = 8 (rr / 4) + rr % 4.
   auto scores = [&](const uint8_t* kS, f32x16_t& s0, f32x16_t& s1) TASFT_INLINE {
     u32x4_t kf[2][KSTEPS];
@@ -357,12 +409,15 @@ chunk_rows_kernel(const ChunkParams p) {
     }
   };
   // Whether some row of the wave does not see some key of the tile.
-  auto is_mixed = [&](int kt, int own) { return kt * kTile + kTile - 1 > all_see || (MASKED && own != 3); };
+  auto is_mixed = [&](int kt, int own) {
+    if constexpr (ROWMASK) return kt * kTile + kTile - 1 > all_see || __ballot(own != 3) != 0;
+    return kt * kTile + kTile - 1 > all_see || (MASKED && own != 3);
+  };
   // The softmax step: P^T as the B operand of the second product.
   auto softmax = [&](f32x16_t& s0, f32x16_t& s1, int kt, int own, bool mixed, u32x4_t (&pb)[4]) TASFT_INLINE {
     const int key0 = kt * kTile;
-    const int lim0 = MASKED && !(own & 1) ? -1 : lim - key0 - 4 * half;
-    const int lim1 = MASKED && !(own & 2) ? -1 : lim - key0 - 4 * half - 32;
+    const int lim0 = MASK != kDense && !(own & 1) ? -1 : lim - key0 - 4 * half;
+    const int lim1 = MASK != kDense && !(own & 2) ? -1 : lim - key0 - 4 * half - 32;
     if (mixed) {
 #pragma unroll
       for (int rr = 0; rr < 16; ++rr) {
@@ -422,19 +477,30 @@ chunk_rows_kernel(const ChunkParams p) {
       }
     }
     if (mixed) {
-      bool bad = false;
+      // The largest magnitudes tell whether there is one (two instructions a pair of values).
+      u16x2_t top = {0, 0};
 #pragma unroll
       for (int pp = 0; pp < 4; ++pp)
 #pragma unroll
         for (int dt = 0; dt < DTILES; ++dt)
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
-            const uint32_t a = vlo[pp][dt][j], b = vhi[pp][dt][j];
-            vlo[pp][dt][j] = finite2<DT>(a);
-            vhi[pp][dt][j] = finite2<DT>(b);
-            bad = bad || ((vlo[pp][dt][j] ^ a) | (vhi[pp][dt][j] ^ b)) != 0u;
+            top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2_t, vlo[pp][dt][j] & 0x7fff7fffu));
+            top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2_t, vhi[pp][dt][j] & 0x7fff7fffu));
           }
-      if (__ballot(bad)) fix_from = min(fix_from, kt);
+      constexpr uint16_t E = DT == kF16 ? 0x7c00 : 0x7f80;
+      if (__ballot(top[0] >= E || top[1] >= E)) {
+        fix_from = min(fix_from, kt);
+#pragma unroll
+        for (int pp = 0; pp < 4; ++pp)
+#pragma unroll
+          for (int dt = 0; dt < DTILES; ++dt)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              vlo[pp][dt][j] = finite2<DT>(vlo[pp][dt][j]);
+              vhi[pp][dt][j] = finite2<DT>(vhi[pp][dt][j]);
+            }
+      }
     }
 #pragma unroll
     for (int pp = 0; pp < 4; ++pp)
@@ -447,13 +513,14 @@ chunk_rows_kernel(const ChunkParams p) {
 
   int cur = next_tile(), own_cur = own_next;
   if constexpr (!MASKED) {
-    int nxt = -1;
+    int nxt = -1, own_nxt = 0;
     Pages pg = {};
     if (cur >= 0) {
       const Pages first = load_pages(cur);
       dma_k(k0_lds, cur, first);
       dma_v(v0_lds, cur, first);
       nxt = next_tile();
+      own_nxt = own_next;
       if (nxt >= 0) pg = load_pages(nxt);
     }
     // One tile from a stage while the next one's DMA fills the other: by the barrier every wave's
@@ -461,24 +528,28 @@ chunk_rows_kernel(const ChunkParams p) {
     auto step = [&](uint8_t* ka, uint8_t* va, uint8_t* kb, uint8_t* vb) TASFT_INLINE {
       __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0)
       chunk_barrier();
-      int nn = -1;
+      int nn = -1, own_nn = 0;
       Pages pn = pg;
       if (nxt >= 0) {
         dma_k(kb, nxt, pg);
         dma_v(vb, nxt, pg);
         nn = next_tile();
+        own_nn = own_next;
         if (nn >= 0) pn = load_pages(nn);
       }
-      if (takes_part(cur, 3)) {
-        const bool mixed = is_mixed(cur, 3);
+      const int own = ROWMASK ? own_cur : 3;
+      if (takes_part(cur, own)) {
+        const bool mixed = is_mixed(cur, own);
         f32x16_t s0, s1;
         u32x4_t pb[4];
         scores(ka, s0, s1);
-        softmax(s0, s1, cur, 3, mixed, pb);
+        softmax(s0, s1, cur, own, mixed, pb);
         add_values(va, cur, mixed, pb);
       }
       cur = nxt;
+      own_cur = own_nxt;
       nxt = nn;
+      own_nxt = own_nn;
       pg = pn;
     };
     while (cur >= 0) {
@@ -535,8 +606,9 @@ chunk_rows_kernel(const ChunkParams p) {
       const uint32_t w = *(const uint32_t*)(vr + (lane * 2) % D);
       if (!__ballot(finite2<DT>(w) != w)) continue;
       bool sees = row_ok && key <= lim;
-      if constexpr (MASKED) {
-        const uint8_t* m = pe->mask + n * pe->sm[0] + (int64_t)(kvh * pe->G + gm) * pe->sm[1] + row_own * pe->sm[2];
+      if constexpr (MASK != kDense) {
+        const int head = MASKED ? kvh * pe->G + gm : h;
+        const uint8_t* m = pe->mask + n * pe->sm[0] + (int64_t)head * pe->sm[1] + row_own * pe->sm[2];
         sees = sees && m[(key >> pe->bs_shift) * pe->sm[3]] != 0;
       }
       const uint16_t* kr = pe->k + kvh * pe->sk[2] + page * pe->sk[0] + in_page * pe->sk[1] + half * 8;
@@ -1095,17 +1167,20 @@ extern "C" size_t tasft_chunk_workspace_bytes(int64_t tokens, int64_t num_q_head
 }
 
 template <int D, int DT>
-static int launch_chunk(const ChunkParams& p, int64_t grid, hipStream_t stream) {
+static int launch_chunk(const ChunkParams& p, int mask, int64_t grid, hipStream_t stream) {
   auto run = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(p.mask ? 128 : 256), 0, stream, p);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(mask == kPositions ? 128 : 256), 0, stream, p);
   };
-  if (p.mask) {
-    if (p.ps_shift >= 5) run(chunk_rows_kernel<D, DT, true, 1>);
-    else if (p.ps_shift == 4) run(chunk_rows_kernel<D, DT, true, 2>);
-    else run(chunk_rows_kernel<D, DT, true, 4>);
+  if (mask == kPositions) {
+    if (p.ps_shift >= 5) run(chunk_rows_kernel<D, DT, kPositions, 1>);
+    else if (p.ps_shift == 4) run(chunk_rows_kernel<D, DT, kPositions, 2>);
+    else run(chunk_rows_kernel<D, DT, kPositions, 4>);
+  } else if (mask == kRows) {
+    if (p.ps_shift >= 4) run(chunk_rows_kernel<D, DT, kRows, 1>);
+    else run(chunk_rows_kernel<D, DT, kRows, 2>);
   } else {
-    if (p.ps_shift >= 4) run(chunk_rows_kernel<D, DT, false, 1>);
-    else run(chunk_rows_kernel<D, DT, false, 2>);
+    if (p.ps_shift >= 4) run(chunk_rows_kernel<D, DT, kDense, 1>);
+    else run(chunk_rows_kernel<D, DT, kDense, 2>);
   }
   if (const int rc = check_launch("chunk attention")) return rc;
   if (p.P == 1) return kOk;
@@ -1164,15 +1239,20 @@ extern "C" int tasft_chunk_paged_fwd(
   p.ws_o = (float*)workspace;
   p.ws_ml = (float*)workspace + tokens * num_q_heads * num_splits * head_dim;
   // Row tiles: masked ones are aligned to positions, so a chunk can touch one more.
-  const int64_t rows = p.mask ? (int64_t)p.L + kMaskTile - 1 : (int64_t)p.L * p.G;
-  const int tile = p.mask ? kMaskTile : kRowTile;
+  // Up to a wave's rows the heads of a group share K and V: 61 sequences of 1099 keys, 4 heads a KV head,
+  // a fourth of the blocks of 32, 26 us and as positions of each head 44; 32 sequences of 4096, 32 heads
+  // a KV head, 28 and 93; a tenth of the blocks of 64 sequences of 16384, 4 heads, 297 both ways, of 8
+  // sequences of 8192 33 and 30.
+  const int form = !p.mask ? kDense : (int64_t)p.L * p.G <= 32 ? kRows : kPositions;
+  const int64_t rows = form == kPositions ? (int64_t)p.L + kMaskTile - 1 : (int64_t)p.L * p.G;
+  const int tile = form == kPositions ? kMaskTile : kRowTile;
   p.QT = (int)((rows + tile - 1) / tile);
-  const int64_t grid = (int64_t)p.N * p.Hkv * p.QT * (p.mask ? p.G : 1) * p.P;
+  const int64_t grid = (int64_t)p.N * p.Hkv * p.QT * (form == kPositions ? p.G : 1) * p.P;
   if (grid > 0x7fffffff) return set_error(kErrUnsupported, "chunk attention: launch too large");
   const hipStream_t st = (hipStream_t)stream;
   if (head_dim == 128)
-    return dtype == kF16 ? launch_chunk<128, kF16>(p, grid, st) : launch_chunk<128, kBf16>(p, grid, st);
-  return dtype == kF16 ? launch_chunk<64, kF16>(p, grid, st) : launch_chunk<64, kBf16>(p, grid, st);
+    return dtype == kF16 ? launch_chunk<128, kF16>(p, form, grid, st) : launch_chunk<128, kBf16>(p, form, grid, st);
+  return dtype == kF16 ? launch_chunk<64, kF16>(p, form, grid, st) : launch_chunk<64, kBf16>(p, form, grid, st);
 }
 
 template <int D, int DT>

@@ -799,8 +799,8 @@ def default_decode_splits(batch: int, num_kv_heads: int, num_blocks: int,
 def default_chunk_splits(num_seqs: int, num_kv_heads: int, q_per_kv: int, chunk: int, slots: int,
                          masked: bool = False, head_dim: int = 128) -> int:
     """Key splits of ``forward_chunk_paged``, by its row tiles: 128 rows of a KV head's tokens and
-    query heads, two workgroups per CU, or with a mask 64 positions of a head, four per CU (six with
-    heads of 64: 3 x 700 tokens of 16 of them 59 us with one split, 49 with two).
+    query heads, two workgroups per CU, or with a mask and more than 32 rows 64 positions of a head,
+    four per CU (six with heads of 64: 3 x 700 tokens of 16 of them 59 us with one split, 49 with two).
 
     * Tiles that fill three quarters of the GPU's 256 CUs: one split. Fewer: as many splits as the
       GPU holds at once, at least four 64-key tiles each (a workgroup more takes a round of its own:
@@ -815,6 +815,7 @@ def default_chunk_splits(num_seqs: int, num_kv_heads: int, q_per_kv: int, chunk:
       their chunk: three (32 / 8 heads over 32768 keys: 2100 tokens 1456 and 1142 us, 4200 tokens 2378
       and 2103; where most keys are the chunk's own, 4200 tokens over 8192, it would cost 10%).
     """
+    masked = masked and chunk * q_per_kv > 32
     if masked:
         tiles, full = num_seqs * num_kv_heads * q_per_kv * math.ceil(chunk / 64), 1024 if head_dim > 64 else 1536
     else:
