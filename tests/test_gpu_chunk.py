@@ -98,6 +98,27 @@ def test_block_mask(index, bs):
             _check(out, lse, want, dtype, d, max(kv), f"block {bs} splits {splits}")
 
 
+@pytest.mark.parametrize("bs", [32, 64, 128])
+@pytest.mark.parametrize(("lens", "hq", "hkv", "d"), [([1, 1], 14, 2, 128), ([5, 2], 8, 2, 64), ([1, 0], 32, 1, 64),
+                                                       ([40, 3], 4, 2, 128)])
+def test_block_mask_of_a_long_cache(lens, hq, hkv, d, bs):
+    """More key tiles than a wave looks over at once, whole stretches of them left out."""
+    dev = require_gpu()
+    kv, page = [9500, 13000], 16
+    t = ref.make(lens, kv, hq, hkv, d, page, BF, seed=bs)
+    mask = _mask((lens, kv, hq, hkv, d, page), bs, bs, 0.05, blocks=-(-t[3].shape[1] * page // bs))
+    mask[:, :, :, 4200 // bs:8400 // bs] = False
+    mask[0, 0] = False
+    want = ref.attention(*t, mask=mask, bs=bs)
+    q, k, v, table, kvl, cu = _put(t, dev)
+    attn = BlockSparseFlashAttention(block_size=bs, min_sparsity_for_speedup=0.0)
+    for splits in (None, 1, 5):
+        print(f"chunk long masked lens={lens} heads={hq}/{hkv} block={bs} splits={splits}", flush=True)
+        out, lse = attn.forward_chunk_paged(q, k, v, table, kvl, cu, mask.to(dev), max_seqlen=max(lens), return_lse=True,
+                                            num_splits=splits)
+        _check(out, lse, want, BF, d, max(kv), f"splits {splits}")
+
+
 @pytest.mark.parametrize("dtype", [BF, HF])
 @pytest.mark.parametrize("masked", [False, True])
 @pytest.mark.parametrize(("lens", "kv"), [([100], [230]), ([6], [200]), ([1], [100])])
