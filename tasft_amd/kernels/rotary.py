@@ -201,7 +201,9 @@ def apply_rotary(
         scale: factor on the rotated dims (the second value of ``rotary_frequencies``).
 
     Returns:
-        The rotated q and k (None without k), new tensors of q's and k's layout.
+        The rotated q and k (None without k), new tensors of q's and k's layout. As for every
+        operator of a graph of gradients: to capture a backward pass into a HIP graph, drop eager
+        results of the same leaves first (torch ends the process otherwise).
     """
     if q.ndim not in (3, 4):
         raise KernelError(f"Expected q of shape [B, H, S, D] or [T, H, D], got {tuple(q.shape)}",

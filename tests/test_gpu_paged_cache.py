@@ -316,3 +316,36 @@ def test_serving_step_in_a_graph():
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, want))
         assert all(torch.equal(a, b) for a, b in zip((kp, vp, slots), copies))
+
+
+def test_calls_on_two_streams_at_once():
+    """Splits, weights and evictions (one head in parts) of two requests on streams of their own, queued
+    together: what each gives alone."""
+    dev = require_gpu()
+    attn = BlockSparseFlashAttention(min_sparsity_for_speedup=0.0)
+    work = []
+    for i, (lens, kv) in enumerate((([3, 1], [900, 2500]), ([2], [40000]))):
+        q, kp, vp, table, kvl, cu = (x.to(dev) for x in ref.make(lens, kv, 8, 2, 64, 16, BF, seed=30 + i))
+        cap = table.shape[1] * 16
+        scores = torch.rand((len(lens), 2, cap), generator=torch.Generator().manual_seed(i)).to(dev)
+        pos = torch.arange(cap, dtype=torch.int32, device=dev).expand(len(lens), 2, cap).contiguous()
+        work.append((q, kp.nan_to_num(1.0), vp.nan_to_num(1.0, posinf=1.0), table, kvl, cu, scores, pos, max(lens)))
+
+    def step(q, kp, vp, table, kvl, cu, scores, pos, longest):
+        kp, vp = kp.clone(), vp.clone()
+        out, lse = attn.forward_chunk_paged(q, kp, vp, table, kvl, cu, max_seqlen=longest, return_lse=True, num_splits=12)
+        w = accumulate_key_weights(q, kp, table, kvl, cu, lse, scores, max_seqlen=longest)
+        return (out, lse, w, *evict_paged(kp, vp, table, kvl, w, pos, 500, recent=20, sinks=2), kp, vp)
+
+    alone = [step(*x) for x in work]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in work]
+    print("two streams", flush=True)
+    for _ in range(4):
+        got = []
+        for x, s in zip(work, streams):
+            with torch.cuda.stream(s):
+                got.append(step(*x))
+        torch.cuda.synchronize()
+        for a, b in zip(alone, got):
+            assert all(torch.equal(x, y) for x, y in zip(a, b))
