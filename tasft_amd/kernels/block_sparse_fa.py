@@ -810,7 +810,8 @@ def default_chunk_splits(num_seqs: int, num_kv_heads: int, q_per_kv: int, chunk:
     * Few rows (a wave's 32) over long caches: 2048 workgroups, 2048 keys or more each, so that
       requests of different lengths end together (one token of 64 requests of 8k to 16k keys 574 us
       with one split, 554 with 4; of 48 of 4k to 8k 139 with 3, 129 with 4; where all have 4096 keys
-      it costs 3%).
+      it costs 3%). Over short ones down to a tile a split, until every CU has a workgroup (one token
+      over 1000 keys, 4 KV heads, 13 us with 4 splits, 10 with 16).
     * Many rows whose last round leaves a seventh of all rounds idle, over caches of four times
       their chunk: three (32 / 8 heads over 32768 keys: 2100 tokens 1456 and 1142 us, 4200 tokens 2378
       and 2103; where most keys are the chunk's own, 4200 tokens over 8192, it would cost 10%).
@@ -824,7 +825,8 @@ def default_chunk_splits(num_seqs: int, num_kv_heads: int, q_per_kv: int, chunk:
     if num_seqs * chunk * num_kv_heads * q_per_kv > 8192:
         splits = min(splits, 8)
     if not masked and chunk * q_per_kv <= 32:
-        splits = max(splits, min(math.ceil(2048 / tiles), slots // 2048, 64))
+        splits = max(splits, min(math.ceil(2048 / tiles), slots // 2048, 64),
+                     min(256 // tiles, math.ceil(slots / 64), 64))
     elif not masked and 0.75 * full <= tiles < 4 * full and slots >= max(4 * chunk, 16384):
         if tiles < 0.85 * full * math.ceil(tiles / full):
             splits = 3
