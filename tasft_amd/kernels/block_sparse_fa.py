@@ -680,11 +680,11 @@ class BlockSparseFlashAttention:
             raise KernelError(f"num_splits must be in [1, 1024], got {num_splits}",
                               context={"num_splits": num_splits})
         q, k_pages, v_pages = readable(q), readable(k_pages), readable(v_pages)
-        out = torch.empty((T, H, D), dtype=q.dtype, device=dev)
+        out = torch.empty_like(q) if q.is_contiguous() else torch.empty((T, H, D), dtype=q.dtype, device=dev)
         lse = torch.empty((T, H), dtype=torch.float32, device=dev) if return_lse else None
         if T > 0:
             lib = _native.load_library()
-            ws_bytes = lib.tasft_chunk_workspace_bytes(T, H, D, num_splits)
+            ws_bytes = lib.tasft_chunk_workspace_bytes(T, H, D, num_splits) if num_splits > 1 else 0
             workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
             with _native.on_device(dev):
                 status = lib.tasft_chunk_paged_fwd(
@@ -694,8 +694,7 @@ class BlockSparseFlashAttention:
                     0 if mask is None else mask.shape[2], b.page_size, k_pages.shape[0], b.max_pages, num_splits,
                     _native.strides(q), _native.strides(k_pages), _native.strides(v_pages), _native.strides(out),
                     None if mask is None else _native.strides(mask), b.table.stride(0), 1.0 / math.sqrt(D),
-                    1 if causal else 0, _native.dtype_code(q.dtype, "chunk attention"),
-                    _native.stream_handle(dev))
+                    1 if causal else 0, b.dtype, _native.stream_handle(dev))
             _native.check(status, "tasft_chunk_paged_fwd", {"tokens": T, "sequences": b.num_seqs})
         return (out, lse) if return_lse else out
 

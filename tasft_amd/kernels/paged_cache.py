@@ -40,10 +40,8 @@ class PagedBatch(NamedTuple):
     cu: torch.Tensor
     kv_lens: torch.Tensor
     table: torch.Tensor
-
-    @property
-    def slots(self) -> int:
-        return self.max_pages * self.page_size
+    slots: int   # max_pages * page_size
+    dtype: int   # the C interface's code
 
 
 def int32_on(t: torch.Tensor, device: torch.device) -> torch.Tensor:
@@ -66,34 +64,34 @@ def check_batch(q: torch.Tensor, k_pages: torch.Tensor, block_table: torch.Tenso
                 cu_seqlens: torch.Tensor, max_seqlen: int | None, min_page: int = 8,
                 need_max: bool = True) -> PagedBatch:
     """The checks shared by the calls on a packed chunk over page pools."""
-    if q.ndim != 3:
-        raise KernelError(f"Expected packed q of shape [T, H, D], got {tuple(q.shape)}",
-                          context={"q_shape": list(q.shape)})
-    T, H, D = q.shape
+    qs, ks, cs, bs = q.shape, k_pages.shape, cu_seqlens.shape, block_table.shape
+    if len(qs) != 3:
+        raise KernelError(f"Expected packed q of shape [T, H, D], got {tuple(qs)}", context={"q_shape": list(qs)})
+    T, H, D = qs
     if k_pages.dtype != q.dtype:
         raise KernelError(f"page pools are {k_pages.dtype} but q is {q.dtype}",
                           context={"q": str(q.dtype), "pages": str(k_pages.dtype)})
-    _native.dtype_code(q.dtype, "paged cache")
-    _, page_size, Hkv, Dk = k_pages.shape
+    code = _native.dtype_code(q.dtype, "paged cache")
+    _, page_size, Hkv, Dk = ks
     if Dk != D or H == 0 or H % Hkv != 0:
         raise KernelError("page pools must have q's head_dim and Hq % Hkv == 0",
-                          context={"q": list(q.shape), "pages": list(k_pages.shape)})
+                          context={"q": list(qs), "pages": list(ks)})
     if page_size < min_page or page_size & (page_size - 1):
         raise KernelError(f"page_size must be a power of two >= {min_page}, got {page_size}",
                           context={"page_size": page_size})
-    if cu_seqlens.ndim != 1 or cu_seqlens.numel() < 2:
+    if len(cs) != 1 or cs[0] < 2:
         raise KernelError("cu_seqlens must be a 1-D tensor of N + 1 >= 2 offsets",
-                          context={"cu_seqlens_shape": list(cu_seqlens.shape)})
-    n = cu_seqlens.numel() - 1
-    if block_table.ndim != 2 or block_table.shape[0] != n or block_table.shape[1] == 0:
-        raise KernelError(f"block_table must have shape [{n}, max_pages], got {tuple(block_table.shape)}",
-                          context={"block_table": list(block_table.shape)})
+                          context={"cu_seqlens_shape": list(cs)})
+    n = cs[0] - 1
+    if len(bs) != 2 or bs[0] != n or bs[1] == 0:
+        raise KernelError(f"block_table must have shape [{n}, max_pages], got {tuple(bs)}",
+                          context={"block_table": list(bs)})
     if kv_lens.shape != (n,):
         raise KernelError(f"kv_lens must have shape ({n},), got {tuple(kv_lens.shape)}",
                           context={"kv_lens": list(kv_lens.shape)})
-    slots = block_table.shape[1] * page_size
+    slots = bs[1] * page_size
     lens = None
-    if cu_seqlens.device.type == "cpu":
+    if cu_seqlens.is_cpu:
         cu = cu_seqlens.to(torch.int64)
         lens = cu[1:] - cu[:-1]
         if int(cu[0]) != 0 or bool((lens < 0).any()) or int(cu[-1]) > T:
@@ -108,18 +106,18 @@ def check_batch(q: torch.Tensor, k_pages: torch.Tensor, block_table: torch.Tenso
     elif max_seqlen is None and need_max:
         raise KernelError("max_seqlen is required when cu_seqlens is on the device",
                           context={"device": str(cu_seqlens.device)})
-    if kv_lens.device.type == "cpu":
+    if kv_lens.is_cpu:
         kv = kv_lens.to(torch.int64)
         if bool((kv < 0).any()) or int(kv.max()) > slots or (lens is not None and bool((kv < lens).any())):
             raise KernelError(f"kv_lens must hold the chunk and be at most max_pages * page_size = {slots}",
                               context={"kv_lens": kv.tolist()[:16], "slots": slots})
     if max_seqlen is not None and max_seqlen <= 0:
         raise KernelError(f"max_seqlen must be positive, got {max_seqlen}", context={"max_seqlen": max_seqlen})
-    if not q.is_cuda or k_pages.device != q.device:
-        raise KernelError("Tensors must be on one CUDA device",
-                          context={"q": str(q.device), "pages": str(k_pages.device)})
-    return PagedBatch(n, T, max_seqlen or 0, page_size, block_table.shape[1], int32_on(cu_seqlens, q.device),
-                      int32_on(kv_lens, q.device), int32_on(block_table, q.device))
+    dev = q.device
+    if not q.is_cuda or k_pages.device != dev:
+        raise KernelError("Tensors must be on one CUDA device", context={"q": str(dev), "pages": str(k_pages.device)})
+    return PagedBatch(n, T, max_seqlen or 0, page_size, bs[1], int32_on(cu_seqlens, dev), int32_on(kv_lens, dev),
+                      int32_on(block_table, dev), slots, code)
 
 
 def chunk_mask(block_mask: torch.Tensor, batch: PagedBatch, heads: int, block_size: int,
@@ -244,7 +242,7 @@ def append_paged(
             k_pages.shape[0], b.max_pages, _native.strides(q), _native.strides(k), _native.strides(v),
             _native.strides(out), _native.strides(k_pages), _native.strides(v_pages), b.table.stride(0),
             positions.stride(0) if positions is not None else 0, 1 if interleaved else 0, float(scale),
-            _native.dtype_code(q.dtype, "append"), _native.stream_handle(dev))
+            b.dtype, _native.stream_handle(dev))
     _native.check(status, "tasft_rotary_append_paged", {"tokens": T, "sequences": b.num_seqs})
     return out
 
@@ -297,7 +295,8 @@ def accumulate_key_weights(
     if T == 0:
         return torch.zeros(shape, dtype=torch.float32, device=dev) if scores is None else scores.clone()
     q, k_pages = readable(q), readable(k_pages)
-    out = torch.empty(shape, dtype=torch.float32, device=dev)
+    out = (torch.empty_like(scores) if scores is not None and scores.is_contiguous()
+           else torch.empty(shape, dtype=torch.float32, device=dev))
     lib = _native.load_library()
     with _native.on_device(dev):
         status = lib.tasft_key_weights(
@@ -306,8 +305,7 @@ def accumulate_key_weights(
             b.max_seqlen, D, block_size, 0 if mask is None else mask.shape[2], b.page_size, k_pages.shape[0],
             b.max_pages, _native.strides(q), _native.strides(k_pages), _native.strides(lse),
             None if scores is None else _native.strides(scores), None if mask is None else _native.strides(mask),
-            b.table.stride(0), 1.0 / math.sqrt(D), 1 if causal else 0, _native.dtype_code(q.dtype, "key weights"),
-            _native.stream_handle(dev))
+            b.table.stride(0), 1.0 / math.sqrt(D), 1 if causal else 0, b.dtype, _native.stream_handle(dev))
     _native.check(status, "tasft_key_weights", {"tokens": T, "sequences": b.num_seqs})
     return out
 
@@ -379,8 +377,9 @@ def evict_paged(
     ws_bytes = lib.tasft_evict_workspace_bytes(n, Hkv, shape[2], budget)
     workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
     lens_out = torch.empty((n,), dtype=torch.int32, device=dev)
-    scores_out = torch.empty(shape, dtype=torch.float32, device=dev)
-    pos_out = torch.empty(shape, dtype=torch.int32, device=dev)
+    contiguous = scores.is_contiguous() and slot_positions.is_contiguous()
+    scores_out = torch.empty_like(scores) if contiguous else torch.empty(shape, dtype=torch.float32, device=dev)
+    pos_out = torch.empty_like(slot_positions) if contiguous else torch.empty(shape, dtype=torch.int32, device=dev)
     with _native.on_device(dev):
         status = lib.tasft_evict_paged(
             k_pages.data_ptr(), v_pages.data_ptr(), table.data_ptr(), lens.data_ptr(), scores.data_ptr(),

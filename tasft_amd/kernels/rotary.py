@@ -102,6 +102,8 @@ def check_frequencies(inv_freq: torch.Tensor, head_dim: int, device: torch.devic
                           context={"dtype": str(inv_freq.dtype)})
     if inv_freq.requires_grad:
         raise KernelError("inv_freq must not require grad: the rotation has no gradient for it", context={})
+    if inv_freq.dtype == torch.float64 and inv_freq.device == device and inv_freq.is_contiguous():
+        return inv_freq
     return inv_freq.to(device=device, dtype=torch.float64).contiguous()
 
 
@@ -119,7 +121,7 @@ def _unit_last(t: torch.Tensor) -> torch.Tensor:
 def _strides4(t: torch.Tensor):
     """(b, h, s, d) strides of ``[B, H, S, D]``, or of packed ``[T, H, D]`` as one batch entry."""
     st = t.stride()
-    return _native.kept_strides(st if t.ndim == 4 else (0, st[1], st[0], st[2]))
+    return _native.kept_strides(st if len(st) == 4 else (0, st[1], st[0], st[2]))
 
 
 def _rotate(q, k, positions, inv_freq, interleaved, scale, inverse):
@@ -128,13 +130,13 @@ def _rotate(q, k, positions, inv_freq, interleaved, scale, inverse):
     k = None if k is None else _unit_last(k)
     q_out = torch.empty_like(q)
     k_out = None if k is None else torch.empty_like(k)
+    ps = positions.stride()
     if q.ndim == 4:
         B, Hq, S, D = q.shape
-        ps = positions.stride()
-        pos_strides = (0 if positions.ndim == 1 or positions.shape[0] == 1 else ps[0], ps[-1])
+        pos_strides = (0 if len(ps) == 1 or positions.shape[0] == 1 else ps[0], ps[-1])
     else:
         S, Hq, D = q.shape
-        B, pos_strides = 1, (0, positions.stride(0))
+        B, pos_strides = 1, (0, ps[0])
     if q.numel() == 0:
         return q_out, k_out
     lib = _native.load_library()
@@ -205,32 +207,26 @@ def apply_rotary(
         operator of a graph of gradients: to capture a backward pass into a HIP graph, drop eager
         results of the same leaves first (torch ends the process otherwise).
     """
-    if q.ndim not in (3, 4):
-        raise KernelError(f"Expected q of shape [B, H, S, D] or [T, H, D], got {tuple(q.shape)}",
-                          context={"q_shape": list(q.shape)})
-    if q.shape[1] == 0:
-        raise KernelError("q must have at least one head", context={"q_shape": list(q.shape)})
+    qs, dev = tuple(q.shape), q.device
+    if len(qs) not in (3, 4):
+        raise KernelError(f"Expected q of shape [B, H, S, D] or [T, H, D], got {qs}", context={"q_shape": list(qs)})
+    if qs[1] == 0:
+        raise KernelError("q must have at least one head", context={"q_shape": list(qs)})
     _native.dtype_code(q.dtype, "rotary")
     if k is not None:
-        # All but the head counts are the same.
-        if k.ndim != q.ndim or k.shape[1] == 0 or k.shape[:1] + k.shape[2:] != q.shape[:1] + q.shape[2:]:
-            raise KernelError("q and k shapes are incompatible",
-                              context={"q": list(q.shape), "k": list(k.shape)})
-        if k.dtype != q.dtype or k.device != q.device:
+        ks = tuple(k.shape)  # all but the head count as q's
+        if len(ks) != len(qs) or ks[1] == 0 or ks[0] != qs[0] or ks[2:] != qs[2:]:
+            raise KernelError("q and k shapes are incompatible", context={"q": list(qs), "k": list(ks)})
+        if k.dtype != q.dtype or k.device != dev:
             raise KernelError("q and k must have one dtype and device",
-                              context={"q": [str(q.dtype), str(q.device)], "k": [str(k.dtype), str(k.device)]})
-    if q.ndim == 4:
-        B, S = q.shape[0], q.shape[2]
-        fits = tuple(positions.shape) in ((S,), (1, S), (B, S))
-    else:
-        fits = tuple(positions.shape) == (q.shape[0],)
-    if not fits:
-        raise KernelError(f"positions of shape {tuple(positions.shape)} do not fit q {tuple(q.shape)}",
-                          context={"positions": list(positions.shape), "q": list(q.shape)})
-    positions = check_positions(positions, q.device)
-    inv_freq = check_frequencies(inv_freq, q.shape[-1], q.device)
+                              context={"q": [str(q.dtype), str(dev)], "k": [str(k.dtype), str(k.device)]})
+    at = tuple(positions.shape)
+    if at != ((qs[0],) if len(qs) == 3 else (qs[2],)) and (len(qs) == 3 or at not in ((1, qs[2]), (qs[0], qs[2]))):
+        raise KernelError(f"positions of shape {at} do not fit q {qs}", context={"positions": list(at), "q": list(qs)})
+    positions = check_positions(positions, dev)
+    inv_freq = check_frequencies(inv_freq, qs[-1], dev)
     if not q.is_cuda:
-        raise KernelError("Tensors must be on CUDA device", context={"device": str(q.device)})
+        raise KernelError("Tensors must be on CUDA device", context={"device": str(dev)})
     args = (q, k, positions, inv_freq, bool(interleaved), float(scale), False)
     if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
         return _Rotary.apply(*args)
