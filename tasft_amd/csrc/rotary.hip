@@ -94,8 +94,9 @@ rotary_kernel(const RotaryParams p) {
       int page = -1;
       if (seq < p.N) {
         const int64_t start = p.cu[seq], len = p.cu[seq + 1] - start;
-        const int64_t kv = min(max((int64_t)p.kv_lens[seq], (int64_t)0), p.cap);
-        slot = kv - len + (tok - start);
+        // From the length as it is given: clamped to the table, tokens past its end would land on the
+        // live keys before them.
+        slot = max(p.kv_lens[seq], 0) - len + (tok - start);
         // Outside the table, or a page outside the pool: rotated, but nothing is written.
         if (slot >= 0 && slot < p.cap) {
           page = p.table[(int64_t)seq * p.bt_stride + (slot >> p.ps_shift)];

@@ -349,3 +349,45 @@ def test_calls_on_two_streams_at_once():
         torch.cuda.synchronize()
         for a, b in zip(alone, got):
             assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+@pytest.mark.parametrize("given", [False, True])
+@pytest.mark.parametrize(("lens", "over"), [([1], [1]), ([4, 1, 6], [2, 1, 6]), ([40, 300, 2], [9, 0, 2 ** 31 - 1 - 80])])
+def test_append_past_the_table(lens, over, given):
+    """Lengths (on the device) that pass the table: a token whose slot lies behind it is rotated at its
+    own position and written nowhere, and no live key of the table changes."""
+    dev = require_gpu()
+    page, cap, hq, hkv, d = 16, 80, 4, 2, 64
+    _, kp, vp, table, _, cu = ref.make(lens, [cap] * len(lens), hq, hkv, d, page, BF, seed=6, max_pages=cap // page)
+    kvl = torch.tensor([cap + x for x in over], dtype=torch.int32)
+    t = sum(lens)
+    q, k, v = _tokens(t, hq, hkv, d, BF, 5)
+    inv, _ = rotary_frequencies(d)
+    pos = torch.randint(0, 1 << 20, (t,), generator=torch.Generator().manual_seed(9)) if given else None
+    slots = torch.full((len(lens), hkv, cap), -5, dtype=torch.int32)
+    a = [x.to(dev) for x in (q, k, v, kp, vp, table, kvl, cu, inv)]
+    slots_d = slots.to(dev)
+    print(f"append past the table lens={lens} over={over}", flush=True)
+    out = append_paged(*a, positions=None if pos is None else pos.to(dev), slot_positions=slots_d)
+    torch.cuda.synchronize()
+    want_k, want_v = kp.clone(), vp.clone()
+    for n, length in enumerate(lens):
+        rows = slice(int(cu[n]), int(cu[n + 1]))
+        slot = int(kvl[n]) - length + torch.arange(length)
+        p = slot if pos is None else pos[rows]
+        turned = []
+        for got, x in ((out, q), (None, k)):
+            want = ref.rotate(x[rows], p[:, None], inv)
+            bound = ref.rotate_bound(x[rows], want, inv, 1.0, False, BF)
+            turned.append((want, bound))
+            if got is not None:
+                assert bool(((got[rows].cpu().double() - want).abs() <= bound).all())
+        on = (slot >= 0) & (slot < cap)
+        pg, row = table[n, slot[on] // page].long(), slot[on] % page
+        got = a[3].cpu()[pg, row]
+        assert bool(((got.double() - turned[1][0][on]).abs() <= turned[1][1][on]).all())
+        want_k[pg, row], want_v[pg, row] = got, v[rows][on]
+        slots[n, :, slot[on]] = p[on].to(torch.int32)
+    assert torch.equal(slots_d.cpu(), slots)
+    assert torch.equal(a[3].cpu().view(torch.int16), want_k.view(torch.int16))  # bits: spare pages hold NaN
+    assert torch.equal(a[4].cpu().view(torch.int16), want_v.view(torch.int16))
