@@ -536,9 +536,10 @@ size_t tasft_chunk_workspace_bytes(int64_t tokens, int64_t num_q_heads, int64_t 
  * tasft/inference/vllm_patch.py:172-176, or to one new token).
  *
  * q, out [T, Hq, D] (strides token, head, dim); sequences, pools, block_table and kv_lens as in
- * tasft_rotary_append_paged (kv_lens clamped to [0, max_pages * page_size], table entries into
- * the pool). Token i of sequence n is at position p = kv_lens[n] - len + i and sees the keys
- * j < kv_lens[n], j <= p when causal, of the blocks that block_mask selects:
+ * tasft_rotary_append_paged (a negative length counts as 0, table entries are clamped into the
+ * pool). Token i of sequence n is at position p = kv_lens[n] - len + i and sees the keys
+ * j < min(kv_lens[n], max_pages * page_size), j <= p when causal, of the blocks that block_mask
+ * selects:
  * [N, Hq, mask_rows, ceil(max_pages * page_size / block_size)] bytes (byte strides; NULL: all),
  * row r for the query block floor((kv_lens[n] - len) / block_size) + r (rows past mask_rows use
  * its last). out = softmax(q.k * scale) v over them, rows without keys 0; lse [T, Hq] fp32

@@ -71,7 +71,8 @@ struct ChunkParams {
   int causal;
 };
 
-// A sequence's chunk: its first token, length, cache length and first position.
+// A sequence's chunk: its first token, length, cached keys and first position. A length past the table
+// (its keys are not there) leaves the tokens at the positions that the append gave them.
 struct ChunkSeq {
   int t0, len, kv, p0;
 };
@@ -81,8 +82,9 @@ __device__ __forceinline__ ChunkSeq chunk_seq(const ChunkParams& p, int n) {
   s.t0 = min(max(p.cu[n], 0), p.T);
   const int t1 = min(max(p.cu[n + 1], s.t0), p.T);
   s.len = min(t1 - s.t0, p.L);
-  s.kv = min(max(p.kv_lens[n], 0), p.cap);
-  s.p0 = s.kv - (t1 - s.t0);  // of the whole chunk, also where L cuts it
+  const int full = min(max(p.kv_lens[n], 0), 0x7fffffff - 255);
+  s.kv = min(full, p.cap);
+  s.p0 = full - (t1 - s.t0);  // of the whole chunk, also where L cuts it
   return s;
 }
 
@@ -165,8 +167,7 @@ chunk_rows_kernel(const ChunkParams p) {
   constexpr bool MASKED = MASK == kPositions, ROWMASK = MASK == kRows;
   constexpr int WAVES = MASKED ? 2 : 4;
   constexpr int ROW_TILE = MASKED ? kMaskTile : kRowTile;
-  constexpr int ROW_SHIFT = MASKED ? 6 : 7;
-  static_assert(ROW_TILE == 1 << ROW_SHIFT && ROW_TILE == 32 * WAVES, "row tile");
+  static_assert(ROW_TILE == 32 * WAVES && (ROW_TILE & (ROW_TILE - 1)) == 0, "row tile");
   constexpr int KSTEPS = D / 16;
   constexpr int DTILES = D / 32;
   constexpr int ROWB = D * 2;
@@ -209,7 +210,7 @@ chunk_rows_kernel(const ChunkParams p) {
   bool row_ok;
   if constexpr (MASKED) {
     // Positions aligned to the row tile: a wave's 32 rows lie in one mask block.
-    const int base = ((sq.p0 >> ROW_SHIFT) << ROW_SHIFT) + qt * ROW_TILE - sq.p0;
+    const int base = qt * ROW_TILE - (sq.p0 & (ROW_TILE - 1));
     if (base >= sq.len) return;
     i_first = max(base + wave * 32, 0);
     i_last = min(base + wave * 32 + 31, sq.len - 1);
@@ -267,7 +268,7 @@ chunk_rows_kernel(const ChunkParams p) {
     mseq = p.mask + n * p.sm[0] + (int64_t)(kvh * p.G + gm) * p.sm[1];
     const int block0 = sq.p0 >> p.bs_shift;
     auto row_of = [&](int j) { return min(max(((sq.p0 + j) >> p.bs_shift) - block0, 0), p.mask_rows - 1); };
-    row_lo = row_of(max(((sq.p0 >> ROW_SHIFT) << ROW_SHIFT) + qt * ROW_TILE - sq.p0, 0));
+    row_lo = row_of(max(qt * ROW_TILE - (sq.p0 & (ROW_TILE - 1)), 0));
     row_hi = row_of(i_end);
     row_own = wave_on ? row_of(i_first) : -1;
   }

@@ -645,8 +645,8 @@ class BlockSparseFlashAttention:
                 ``cu_seqlens[n] .. cu_seqlens[n + 1] - 1``.
             k_pages, v_pages, block_table: the pools and table of ``forward_decode_paged``.
             kv_lens: ``[N]`` cached lengths, the chunk's tokens included (they are the last ones).
-                On the device it is trusted to be at most ``max_pages * page_size`` (the kernel
-                clamps it); on the CPU it is checked.
+                On the CPU it is checked to be at most ``max_pages * page_size``; on the device a
+                longer one leaves the tokens their positions, and the keys are the table's.
             cu_seqlens: ``[N + 1]`` offsets; on the CPU they are checked, on the device trusted,
                 and ``max_seqlen`` must be given (a sequence's tokens behind its first
                 ``max_seqlen`` are not computed).

@@ -322,3 +322,33 @@ def test_offsets_past_32_bits(lens, masked):
     assert torch.equal(out, o2) and torch.equal(lse, l2)
     w = accumulate_key_weights(q, k, table, kvl, cu, lse, block_mask=md, max_seqlen=max(lens))
     assert torch.equal(w, accumulate_key_weights(q, far[0], table, kvl, cu, lse, block_mask=md, max_seqlen=max(lens)))
+
+
+@pytest.mark.parametrize("masked", [0, 64])
+@pytest.mark.parametrize(("lens", "over"), [([1, 1], [1, 0]), ([5, 3], [2, 300]), ([70, 130], [33, 1])])
+def test_lengths_past_the_table(lens, over, masked):
+    """Lengths (on the device) that pass the table: the chunk's tokens keep the positions they were
+    written at, and the keys are those that the table holds. The oracle has a longer table, whose blocks
+    behind the short one's end no row sees."""
+    dev = require_gpu()
+    hq, hkv, d, page, cap = 4, 2, 128, 16, 256
+    kv = [cap + x for x in over]
+    t = ref.make(lens, kv, hq, hkv, d, page, BF, seed=12)
+    rows, blocks = (max(lens) + 62) // 64 + 1, -(-t[3].shape[1] * page // 64)
+    mask = _mask((lens, kv, hq, hkv, d, page), 4, 64, 0.5 if masked else 2.0, blocks=blocks)
+    mask[..., cap // 64:] = False
+    want = ref.attention(*t, mask=mask)
+    q, k, v, table, kvl, cu = _put(t, dev)
+    short = table[:, :cap // page].contiguous()
+    md = mask[..., :cap // 64].contiguous().to(dev) if masked else None
+    attn = BlockSparseFlashAttention(min_sparsity_for_speedup=0.0)
+    for splits in (None, 3):
+        print(f"chunk past the table lens={lens} over={over} masked={masked} splits={splits}", flush=True)
+        out, lse = attn.forward_chunk_paged(q, k, v, short, kvl, cu, md, max_seqlen=max(lens), return_lse=True,
+                                            num_splits=splits)
+        _check(out, lse, want, BF, d, cap, f"splits {splits}")
+    exact = want[1].float()
+    got = accumulate_key_weights(q, k, short, kvl, cu, exact.to(dev), block_mask=md, max_seqlen=max(lens))
+    total, dot = ref.key_weights(t[0], t[1], *t[3:], exact, torch.zeros(len(lens), hkv, t[3].shape[1] * page), mask)
+    rel = 2 * ((d + 3) * dot + 8 * (1 + dot)) * 2.0 ** -24 + (max(lens) * hq // hkv + 2) * 2.0 ** -24
+    assert bool(((got.cpu().double() - total[..., :cap]).abs() <= (rel + 2.0 ** -23) * total[..., :cap]).all())
