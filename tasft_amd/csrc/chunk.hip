@@ -851,7 +851,10 @@ chunk_weights_kernel(const WeightParams wp) {
   int member;
   xcd_group_map(blockIdx.x, (int64_t)p.N * p.Hkv, per, &group, &member);
   const int n = (int)(group / p.Hkv), kvh = (int)(group % p.Hkv);
-  const ChunkSeq sq = chunk_seq(p, n);
+  ChunkSeq sq = chunk_seq(p, n);
+  // Scalars: as the loads' own vector registers they spilled beside the masked form's.
+  sq.kv = __builtin_amdgcn_readfirstlane(sq.kv);
+  sq.p0 = __builtin_amdgcn_readfirstlane(sq.p0);
   const int key0 = (member * KW + kg) * kTile;
   const int wg0 = member * KW * kTile;
 
