@@ -100,6 +100,17 @@ __device__ __forceinline__ void chunk_zero_tail(const ChunkParams& p, int64_t wg
     }
 }
 
+// Rows of a KV head behind the first L tokens of a sequence: the join leaves out what has such a sum.
+constexpr uint32_t kCutRow = 0xbf800000u;  // -1: no sum of exponentials
+__device__ __forceinline__ void chunk_mark_cut(const ChunkParams& p, const ChunkSeq& s, int n, int kvh, int tid,
+                                               int threads) {
+  const int rows = (min(max(p.cu[n + 1], s.t0), p.T) - s.t0 - s.len) * p.G;
+  for (int r = tid; r < rows; r += threads) {
+    const int64_t t = s.t0 + s.len + r / p.G;
+    p.ws_ml[((t * p.Hq + kvh * p.G + r % p.G) * p.P) * 2 + 1] = __uint_as_float(kCutRow);
+  }
+}
+
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_rsrc(const uint16_t* base, int rows, int64_t stride, int d) {
   const int n = rows > 0 ? (int)(((rows - 1) * stride + d) * 2) : 0;
   return __builtin_amdgcn_make_buffer_rsrc((void*)base, (short)0, n, 0x00020000);
@@ -203,6 +214,7 @@ chunk_rows_kernel(const ChunkParams p) {
   const int gm = MASKED ? member % p.G : 0, qt = p.QT - 1 - (MASKED ? member / p.G : member);
   const ChunkSeq sq = chunk_seq(p, n);
   if (sq.len == 0) return;
+  if (p.P > 1 && split == 0 && qt == 0 && gm == 0) chunk_mark_cut(p, sq, n, kvh, tid, WAVES * kWave);
 
   // This lane's row (token i of the chunk, head h), the wave's range of tokens and the workgroup's
   // last token.
@@ -703,6 +715,7 @@ __global__ void __launch_bounds__(256) chunk_combine_few_kernel(const ChunkParam
   const int c = threadIdx.x % LPR;
   if (row >= (int64_t)min(max(p.cu[p.N], 0), p.T) * p.Hq) return;
   const float* ml = p.ws_ml + row * p.P * 2;
+  if (__float_as_uint(ml[1]) == kCutRow) return;
   const float* os = p.ws_o + row * p.P * D + c * 4;
   float m[kFewSplits], l[kFewSplits];
   f32x4_t o[kFewSplits];
@@ -739,6 +752,7 @@ __global__ void __launch_bounds__(256) chunk_combine_kernel(const ChunkParams p)
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = tid % LPR, grp = tid / LPR;
   if (row >= (int64_t)min(max(p.cu[p.N], 0), p.T) * p.Hq) return;
   const float* ml = p.ws_ml + row * p.P * 2;
+  if (__float_as_uint(ml[1]) == kCutRow) return;
   const float* os = p.ws_o + row * p.P * D + c * 4;
   float M = -INFINITY;
   for (int s = tid; s < p.P; s += 256) M = fmaxf(M, ml[2 * s]);

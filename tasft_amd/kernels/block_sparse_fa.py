@@ -649,7 +649,7 @@ class BlockSparseFlashAttention:
                 longer one leaves the tokens their positions, and the keys are the table's.
             cu_seqlens: ``[N + 1]`` offsets; on the CPU they are checked, on the device trusted,
                 and ``max_seqlen`` must be given (a sequence's tokens behind its first
-                ``max_seqlen`` are not computed).
+                ``max_seqlen`` are not computed: their rows of the results are not defined).
             block_mask: ``[N, Hq, R, NB]`` with ``NB = ceil(max_pages * page_size / block_size)``
                 and ``R = (max_seqlen + block_size - 2) // block_size + 1``: row r of sequence n is
                 query block ``(kv_lens[n] - len_n) // block_size + r``, the rows of

@@ -8,6 +8,7 @@ import torch
 
 import paged_ref as ref
 from helpers import require_gpu
+from tasft_amd import _native
 from tasft_amd.kernels import BlockSparseFlashAttention, accumulate_key_weights
 
 pytestmark = pytest.mark.gpu
@@ -352,3 +353,36 @@ def test_lengths_past_the_table(lens, over, masked):
     total, dot = ref.key_weights(t[0], t[1], *t[3:], exact, torch.zeros(len(lens), hkv, t[3].shape[1] * page), mask)
     rel = 2 * ((d + 3) * dot + 8 * (1 + dot)) * 2.0 ** -24 + (max(lens) * hq // hkv + 2) * 2.0 ** -24
     assert bool(((got.cpu().double() - total[..., :cap]).abs() <= (rel + 2.0 ** -23) * total[..., :cap]).all())
+
+
+@pytest.mark.parametrize("splits", [1, 3, 9])
+@pytest.mark.parametrize(("hq", "cut", "masked"), [(4, 70, 0), (4, 70, 64), (4, 8, 64), (32, 8, 0)])
+def test_rows_behind_max_seqlen_are_not_written(hq, cut, masked, splits):
+    """The C entry leaves the output rows of tokens behind max_seqlen as they were, with one split and with
+    several joined."""
+    dev = require_gpu()
+    lens, kv, hkv, d, page = [150, 3, 75, 1], [400, 90, 75, 30], 2, 128, 16
+    t = ref.make(lens, kv, hq, hkv, d, page, BF, seed=3, pad=2)
+    blocks = -(-t[3].shape[1] * page // 64)
+    mask = _mask((lens, kv, hq, hkv, d, page), 1, 64, 0.4, blocks=blocks) if masked else None
+    want = ref.attention(*t, mask=mask)
+    q, k, v, table, kvl, cu = _put(t, dev)
+    md = None if mask is None else mask[:, :, :(cut + 62) // 64 + 1].contiguous().to(dev)
+    out, lse = torch.full_like(q, 7.0), torch.full(q.shape[:2], 7.0, device=dev)
+    lib = _native.load_library()
+    size = lib.tasft_chunk_workspace_bytes(q.shape[0], hq, d, splits)
+    ws = torch.full((max(size, 4) // 4,), 3.0, device=dev)
+    print(f"chunk cut at {cut}, heads {hq}, masked={masked} splits={splits}", flush=True)
+    status = lib.tasft_chunk_paged_fwd(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), _native.ptr(md), table.data_ptr(),
+        kvl.data_ptr(), cu.data_ptr(), ws.data_ptr(), size, len(lens), q.shape[0], hq, hkv, cut, d, 64,
+        0 if md is None else md.shape[2], page, k.shape[0], table.shape[1], splits, _native.strides(q),
+        _native.strides(k), _native.strides(v), _native.strides(out), None if md is None else _native.strides(md),
+        table.stride(0), 1.0 / math.sqrt(d), 1, _native.DTYPE_BF16, _native.stream_handle(q.device))
+    _native.check(status, "tasft_chunk_paged_fwd")
+    torch.cuda.synchronize()
+    kept = torch.cat([torch.arange(min(x, cut)) + int(a) for x, a in zip(lens, t[5])] + [torch.arange(2) + sum(lens)])
+    _check(out[kept], lse[kept], [x[kept] for x in want], BF, d, max(kv), "kept")
+    rest = torch.ones(q.shape[0], dtype=torch.bool)
+    rest[kept] = False
+    assert rest.any() and bool((out.cpu()[rest] == 7.0).all()) and bool((lse.cpu()[rest] == 7.0).all())
