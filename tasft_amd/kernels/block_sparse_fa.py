@@ -814,7 +814,11 @@ def default_chunk_splits(num_seqs: int, num_kv_heads: int, q_per_kv: int, chunk:
     * Many rows whose last round leaves a seventh of all rounds idle, over caches of four times
       their chunk: three (32 / 8 heads over 32768 keys: 2100 tokens 1456 and 1142 us, 4200 tokens 2378
       and 2103; where most keys are the chunk's own, 4200 tokens over 8192, it would cost 10%).
+
+    An empty chunk takes one.
     """
+    if num_seqs * num_kv_heads * q_per_kv * chunk == 0:
+        return 1
     masked = masked and chunk * q_per_kv > 32
     if masked:
         tiles, full = num_seqs * num_kv_heads * q_per_kv * math.ceil(chunk / 64), 1024 if head_dim > 64 else 1536

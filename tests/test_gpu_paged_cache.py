@@ -391,3 +391,26 @@ def test_append_past_the_table(lens, over, given):
     assert torch.equal(slots_d.cpu(), slots)
     assert torch.equal(a[3].cpu().view(torch.int16), want_k.view(torch.int16))  # bits: spare pages hold NaN
     assert torch.equal(a[4].cpu().view(torch.int16), want_v.view(torch.int16))
+
+
+@pytest.mark.parametrize("masked", [False, True])
+def test_no_new_tokens(masked):
+    """A step without new tokens: empty results, scores as they were, pages untouched."""
+    dev = require_gpu()
+    _, kp, vp, table, kvl, cu = ref.make([0, 0], [70, 33], 8, 2, 64, 16, BF, seed=2)
+    q, k, v = (torch.empty((0, h, 64), dtype=BF, device=dev) for h in (8, 2, 2))
+    a = [x.to(dev) for x in (kp, vp, table, kvl, cu)]
+    cap = table.shape[1] * 16
+    scores = torch.rand((2, 2, cap), device=dev)
+    inv = rotary_frequencies(64, device=dev)[0]
+    mask = torch.ones((2, 8, 1, -(-cap // 64)), dtype=torch.bool, device=dev) if masked else None
+    print(f"no new tokens, masked={masked}", flush=True)
+    qr = append_paged(q, k, v, *a, inv)
+    attn = BlockSparseFlashAttention(min_sparsity_for_speedup=0.0)
+    for splits in (None, 1, 4):
+        out, lse = attn.forward_chunk_paged(qr, *a, mask, max_seqlen=1, return_lse=True, num_splits=splits)
+        assert out.shape == (0, 8, 64) and out.dtype == BF and lse.shape == (0, 8) and lse.dtype == torch.float32
+    w = accumulate_key_weights(qr, a[0], *a[2:], lse, scores, block_mask=mask, max_seqlen=1)
+    assert torch.equal(w, scores)
+    assert not accumulate_key_weights(qr, a[0], *a[2:], lse, block_mask=mask, max_seqlen=1).any()
+    assert torch.equal(a[0].cpu().view(torch.int16), kp.view(torch.int16))

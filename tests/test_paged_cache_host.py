@@ -202,6 +202,12 @@ def test_chunk_splits():
             assert 1 <= s <= 64 and s <= max(1, math.ceil(slots / 64))
 
 
+def test_chunk_splits_of_an_empty_chunk():
+    for masked in (False, True):
+        assert default_chunk_splits(1, 8, 4, 0, 4096, masked) == 1
+        assert default_chunk_splits(64, 2, 1, 0, 1 << 20, masked, 64) == 1
+
+
 # ------------------------------------------------------------------------- the C entries
 def _i64(*vals):
     return (ctypes.c_int64 * 4)(*vals)
