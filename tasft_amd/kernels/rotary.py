@@ -11,6 +11,7 @@ from __future__ import annotations
 import math
 
 import torch
+from torch.autograd import forward_ad
 
 from tasft_amd import _native
 from tasft_amd.exceptions import KernelError
@@ -153,31 +154,52 @@ def _rotate(q, k, positions, inv_freq, interleaved, scale, inverse):
 
 
 class _Rotary(torch.autograd.Function):
-    """The rotation is linear and its gradient is the inverse rotation of the outputs' gradients
-    (with the same factor), itself this function: derivatives of any order."""
+    """The rotation is linear: its gradient is the inverse rotation of the outputs' gradients (with the
+    same factor), its forward derivative the rotation of the tangents; both are this function again,
+    so derivatives of any order."""
 
     @staticmethod
     def forward(ctx, q, k, positions, inv_freq, interleaved, scale, inverse):
         ctx.save_for_backward(positions, inv_freq)
+        ctx.save_for_forward(positions, inv_freq)
         ctx.cfg = (interleaved, scale, inverse)
+        ctx.heads = (q.shape[1], None if k is None else k.shape[1])
         ctx.set_materialize_grads(False)
         return _rotate(q, k, positions, inv_freq, interleaved, scale, inverse)
 
     @staticmethod
     def backward(ctx, gq, gk):
-        positions, inv_freq = ctx.saved_tensors
-        interleaved, scale, inverse = ctx.cfg
         want_q, want_k = ctx.needs_input_grad[:2]
-        given = [g for g, want in ((gq, want_q), (gk, want_k)) if want and g is not None]
-        if not given:
-            return (None,) * 7
-        # Through the function only where a graph of the gradients is being built.
-        turn = _Rotary.apply if torch.is_grad_enabled() else _rotate
-        out = list(turn(given[0], given[1] if len(given) > 1 else None, positions, inv_freq, interleaved, scale,
-                        not inverse))
-        gq = out.pop(0) if want_q and gq is not None else None
-        gk = out.pop(0) if want_k and gk is not None else None
+        gq, gk = _turn_given(ctx, gq if want_q else None, gk if want_k else None, not ctx.cfg[2])
         return gq, gk, None, None, None, None, None
+
+    @staticmethod
+    def jvp(ctx, tq, tk, *_):
+        out = _turn_given(ctx, tq, tk, ctx.cfg[2])
+        there = tq if tq is not None else tk
+        # torch takes no None for the tangent of a tensor.
+        return tuple(there.new_zeros((there.shape[0], h, *there.shape[2:])) if t is None and h is not None else t
+                     for t, h in zip(out, ctx.heads))
+
+
+def _turn_given(ctx, a, b, inverse):
+    """Those of the two that are there, rotated as ``ctx``'s operator or its inverse does."""
+    given = [x for x in (a, b) if x is not None]
+    if not given:
+        return None, None
+    positions, inv_freq = ctx.saved_tensors
+    interleaved, scale, _ = ctx.cfg
+    out = list(_turn(given[0], given[1] if len(given) > 1 else None, positions, inv_freq, interleaved, scale, inverse))
+    return out.pop(0) if a is not None else None, out.pop(0) if b is not None else None
+
+
+def _turn(q, k, *args):
+    """Through the function only where a graph is being built or tangents are carried along (a dual
+    tensor does not require grad)."""
+    if forward_ad._current_level >= 0 or (torch.is_grad_enabled() and
+                                          (q.requires_grad or (k is not None and k.requires_grad))):
+        return _Rotary.apply(q, k, *args)
+    return _rotate(q, k, *args)
 
 
 def apply_rotary(
@@ -189,7 +211,8 @@ def apply_rotary(
     interleaved: bool = False,
     scale: float = 1.0,
 ) -> tuple[torch.Tensor, torch.Tensor | None]:
-    """Queries and keys rotated by their positions, in one launch; differentiable in q and k.
+    """Queries and keys rotated by their positions, in one launch; differentiable in q and k, also in
+    forward mode.
 
     Args:
         q: ``[B, Hq, S, D]`` or packed ``[T, Hq, D]``, bf16 or fp16, any strides (a transposed view
@@ -227,10 +250,7 @@ def apply_rotary(
     inv_freq = check_frequencies(inv_freq, qs[-1], dev)
     if not q.is_cuda:
         raise KernelError("Tensors must be on CUDA device", context={"device": str(dev)})
-    args = (q, k, positions, inv_freq, bool(interleaved), float(scale), False)
-    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
-        return _Rotary.apply(*args)
-    return _rotate(*args)
+    return _turn(q, k, positions, inv_freq, bool(interleaved), float(scale), False)
 
 
 __all__ = ["apply_rotary", "rotary_frequencies"]

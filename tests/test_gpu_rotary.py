@@ -3,6 +3,7 @@ from __future__ import annotations
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fwAD
 
 import paged_ref as ref
 from helpers import require_gpu
@@ -148,3 +149,46 @@ def test_graph_replay_and_streams():
         torch.cuda.synchronize()
         assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1])
     assert on_side[0].shape == q.shape
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("inter", [False, True])
+def test_forward_mode(inter, dtype):
+    """Forward-mode derivatives: the operator is linear, so a tangent is rotated as its value is; with
+    and without gradients recorded, and of a gradient."""
+    dev = require_gpu()
+    print(f"rotary forward mode interleaved={inter} {dtype}", flush=True)
+    g = torch.Generator().manual_seed(21)
+    B, S, D, R = 2, 19, 64, 32
+    inv, _ = rotary_frequencies(R, device=dev)
+    q, k, tq, tk = (torch.randn((B, h, S, D), generator=g).to(dtype).to(dev) for h in (4, 2, 4, 2))
+    pos = torch.randint(0, 5000, (B, S), generator=g).to(dev)
+    kw = {"interleaved": inter, "scale": 1.25}
+    want = apply_rotary(q, k, pos, inv, **kw)
+    moved = apply_rotary(tq, tk, pos, inv, **kw)
+    _check(moved[0], tq, pos[:, None], inv, 1.25, inter, what="tangent")
+    for grads in (False, True):
+        a, b = q.clone().requires_grad_(grads), k.clone().requires_grad_(grads)
+        for on in ((True, True), (True, False), (False, True)):
+            with fwAD.dual_level():
+                da, db = (fwAD.make_dual(x, t) if yes else x for x, t, yes in ((a, tq, on[0]), (b, tk, on[1])))
+                got = [fwAD.unpack_dual(x) for x in apply_rotary(da, db, pos, inv, **kw)]
+                for yes, (value, tangent), x, t in zip(on, got, want, moved):
+                    assert torch.equal(value, x)
+                    assert torch.equal(tangent, t) if yes else tangent is None or not tangent.any()
+            with fwAD.dual_level(), torch.no_grad():
+                only, none = apply_rotary(fwAD.make_dual(q, tq), None, pos, inv, **kw)
+                assert none is None and torch.equal(fwAD.unpack_dual(only).tangent, moved[0])
+    # Reverse over forward: a tangent that needs a gradient.
+    t = tq.clone().requires_grad_(True)
+    with fwAD.dual_level():
+        out, _ = apply_rotary(fwAD.make_dual(q, t), None, pos, inv, **kw)
+        (back,) = torch.autograd.grad(fwAD.unpack_dual(out).tangent, t, tq)
+    _check(back, tq, pos[:, None], inv, 1.25, inter, inverse=True, what="gradient of the tangent")
+    # Forward over reverse: a gradient's tangent.
+    x = q.clone().requires_grad_(True)
+    out, _ = apply_rotary(x, None, pos, inv, **kw)
+    with fwAD.dual_level():
+        (gx,) = torch.autograd.grad(out, x, fwAD.make_dual(q, tq))
+        tangent = fwAD.unpack_dual(gx).tangent
+    assert tangent is not None and torch.equal(tangent, back)
