@@ -38,6 +38,7 @@ struct RotaryParams {
   int pos64;
   const double* inv_freq;  // [pairs]
   int64_t tokens;          // B * S (apply), T (append)
+  int64_t first;           // token of the launch's first workgroup
   int S, Hq, Hkv, D, pairs;
   float scale;
   int inverse;
@@ -75,7 +76,7 @@ rotary_kernel(const RotaryParams p) {
   __shared__ int32_t t_seq;   // append: the token's sequence, N: padding
   __shared__ int32_t t_page;  // append: its page, -1: none
   const int tid = threadIdx.x;
-  const int64_t tok = blockIdx.x;
+  const int64_t tok = p.first + blockIdx.x;
 
   if constexpr (APPEND) {
     // A token's sequence: the number of ends at or before it (one load per thread and 256
@@ -233,11 +234,17 @@ static bool vector_rows(const void* base, const int64_t* strides, int n) {
 }
 
 template <bool APPEND>
-static int launch_rotary(const RotaryParams& p, bool vec, int interleaved, int dtype, hipStream_t stream,
+static int launch_rotary(RotaryParams& p, bool vec, int interleaved, int dtype, hipStream_t stream,
                          const char* what) {
   if (p.tokens > 0x7fffffff) return set_error(kErrUnsupported, "%s: too many tokens", what);
-  const dim3 g((unsigned)p.tokens), b(kRotaryThreads);
-  auto run = [&](auto kernel) { hipLaunchKernelGGL(kernel, g, b, 0, stream, p); };
+  // A launch holds fewer than 2^32 threads: more tokens in several.
+  constexpr int64_t kMost = ((int64_t)1 << 32) / kRotaryThreads - 1;
+  auto run = [&](auto kernel) {
+    for (p.first = 0; p.first < p.tokens; p.first += kMost) {
+      const int64_t left = p.tokens - p.first;
+      hipLaunchKernelGGL(kernel, dim3((unsigned)(left < kMost ? left : kMost)), dim3(kRotaryThreads), 0, stream, p);
+    }
+  };
   if (dtype == kF16) {
     if (vec) interleaved ? run(rotary_kernel<kF16, 8, true, APPEND>) : run(rotary_kernel<kF16, 8, false, APPEND>);
     else interleaved ? run(rotary_kernel<kF16, 1, true, APPEND>) : run(rotary_kernel<kF16, 1, false, APPEND>);

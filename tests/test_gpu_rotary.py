@@ -7,7 +7,7 @@ import torch.autograd.forward_ad as fwAD
 
 import paged_ref as ref
 from helpers import require_gpu
-from tasft_amd.kernels import apply_rotary, rotary_frequencies
+from tasft_amd.kernels import append_paged, apply_rotary, rotary_frequencies
 
 pytestmark = pytest.mark.gpu
 
@@ -192,3 +192,34 @@ def test_forward_mode(inter, dtype):
         (gx,) = torch.autograd.grad(out, x, fwAD.make_dual(q, tq))
         tangent = fwAD.unpack_dual(gx).tangent
     assert tangent is not None and torch.equal(tangent, back)
+
+
+def test_more_tokens_than_one_launch_takes():
+    """A launch holds fewer than 2^32 threads, 2^24 tokens of a workgroup each."""
+    dev = require_gpu()
+    t, d = (1 << 24) + 700, 8
+    inv, _ = rotary_frequencies(d, device=dev)
+    q = torch.randn((t, 1, d), device=dev).bfloat16()
+    k = torch.randn((t, 1, d), device=dev).bfloat16()
+    pos = torch.arange(t, device=dev) * 3 + 1
+    print("rotary of 2^24 + 700 tokens", flush=True)
+    a, b = apply_rotary(q, k, pos, inv)
+    for part in (slice(0, 1000), slice((1 << 24) - 1500, (1 << 24) + 600), slice(t - 50, t)):
+        x, y = apply_rotary(q[part], k[part], pos[part], inv)
+        assert torch.equal(a[part], x) and torch.equal(b[part], y)
+        _check(x, q[part], pos[part][:, None], inv, 1.0, False)
+    # Appended: two sequences, the second's tokens in the second launch.
+    page, first = 1 << 12, (1 << 24) + 100
+    lens = [first, t - first]
+    per = -(-first // page)
+    table = torch.arange(2 * per, dtype=torch.int32, device=dev).view(2, per)
+    kp = torch.zeros((2 * per, page, 1, d), dtype=q.dtype, device=dev)
+    vp = torch.zeros_like(kp)
+    cu = torch.tensor([0, first, t], dtype=torch.int32, device=dev)
+    kvl = torch.tensor(lens, dtype=torch.int32, device=dev)
+    print("append of 2^24 + 700 tokens", flush=True)
+    out = append_paged(q, k, q, kp, vp, table, kvl, cu, inv, positions=pos)
+    assert torch.equal(out, a)
+    for n, (s0, s1) in enumerate(((0, first), (first, t))):
+        rows = slice(n * per * page, n * per * page + s1 - s0)
+        assert torch.equal(kp.view(-1, 1, d)[rows], b[s0:s1]) and torch.equal(vp.view(-1, 1, d)[rows], q[s0:s1])
