@@ -1110,6 +1110,12 @@ chunk_weights_kernel(const WeightParams wp) {
 
 using namespace tasft;
 
+// Whether a launch of `groups` times `each` workgroups holds fewer than 2^32 threads, as it must.
+static bool launch_fits(int64_t groups, int64_t each, int threads) {
+  const int64_t most = (int64_t)0xffffffff / threads;
+  return groups <= most && each <= most && groups * each <= most;
+}
+
 // Checks shared by both entry points; fills the parameters that they share.
 static int chunk_params(ChunkParams& p, const char* what, const void* q, const void* k_pages, const uint8_t* mask,
                         const int32_t* table, const int32_t* kv_lens, const int32_t* cu, int64_t num_seqs,
@@ -1184,6 +1190,9 @@ extern "C" size_t tasft_chunk_workspace_bytes(int64_t tokens, int64_t num_q_head
   return (size_t)(tokens * num_q_heads * num_splits) * (size_t)(head_dim + 2) * sizeof(float);
 }
 
+// Rows of a workgroup that joins few splits.
+constexpr int join_rows(int64_t head_dim) { return 256 / (int)(head_dim / 4); }
+
 template <int D, int DT>
 static int launch_chunk(const ChunkParams& p, int mask, int64_t grid, hipStream_t stream) {
   auto run = [&](auto kernel) {
@@ -1204,11 +1213,10 @@ static int launch_chunk(const ChunkParams& p, int mask, int64_t grid, hipStream_
   if (p.P == 1) return kOk;
   const int64_t rows = (int64_t)p.T * p.Hq;
   if (p.P <= kFewSplits) {
-    constexpr int RPW = 256 / (D / 4);
+    constexpr int RPW = join_rows(D);
     hipLaunchKernelGGL((chunk_combine_few_kernel<D, DT>), dim3((unsigned)((rows + RPW - 1) / RPW)), dim3(256), 0,
                        stream, p);
   } else {
-    if (rows > 0x7fffffff) return set_error(kErrUnsupported, "chunk attention: launch too large");
     hipLaunchKernelGGL((chunk_combine_kernel<D, DT>), dim3((unsigned)rows), dim3(256), 0, stream, p);
   }
   return check_launch("chunk combine");
@@ -1265,8 +1273,12 @@ extern "C" int tasft_chunk_paged_fwd(
   const int64_t rows = form == kPositions ? (int64_t)p.L + kMaskTile - 1 : (int64_t)p.L * p.G;
   const int tile = form == kPositions ? kMaskTile : kRowTile;
   p.QT = (int)((rows + tile - 1) / tile);
-  const int64_t grid = (int64_t)p.N * p.Hkv * p.QT * (form == kPositions ? p.G : 1) * p.P;
-  if (grid > 0x7fffffff) return set_error(kErrUnsupported, "chunk attention: launch too large");
+  const int64_t groups = (int64_t)p.N * p.Hkv, each = (int64_t)p.QT * (form == kPositions ? p.G : 1) * p.P;
+  const int64_t out_rows = (int64_t)p.T * p.Hq, joined = p.P <= kFewSplits ? join_rows(head_dim) : 1;
+  if (!launch_fits(groups, each, form == kPositions ? 128 : 256) ||
+      (p.P > 1 && !launch_fits((out_rows + joined - 1) / joined, 1, 256)))
+    return set_error(kErrUnsupported, "chunk attention: launch too large");
+  const int64_t grid = groups * each;
   const hipStream_t st = (hipStream_t)stream;
   if (head_dim == 128)
     return dtype == kF16 ? launch_chunk<128, kF16>(p, form, grid, st) : launch_chunk<128, kBf16>(p, form, grid, st);
@@ -1327,7 +1339,8 @@ extern "C" int tasft_key_weights(
     return rc;
   if (!strides_nonneg(lse_strides, 2) || (scores && !strides_nonneg(score_strides, 3)))
     return set_error(kErrInvalidArgument, "key weights: strides must be non-negative");
-  if (num_seqs * num_kv_heads * ((int64_t)w.c.cap / kTile + 1) > 0x7fffffff)
+  // At the workgroups of many keys: those of few are fewer than 2048.
+  if (!launch_fits(num_seqs * num_kv_heads, ((int64_t)w.c.cap + 4 * kTile - 1) / (4 * kTile), 256))
     return set_error(kErrUnsupported, "key weights: launch too large");
   w.scores = scores;
   if (scores)

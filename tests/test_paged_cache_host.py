@@ -319,3 +319,25 @@ def test_evict_entry_refusals():
                            ({"kp": _i64(4096, 256, 128, 2)}, -1, b"contiguous"), ({"k": ODD}, -1, b"aligned"),
                            ({"ss": _i64(0, 0, -1, 0)}, -1, b"non-negative"), ({"wb": 100}, -4, b"workspace")):
         assert call(**args) == rc and text in _err(), args
+
+
+def test_launches_of_too_many_threads_are_refused():
+    """A launch holds fewer than 2^32 threads: refused before anything is launched."""
+    lib = _native.load_library()
+    st, pool = _i64(64, 64, 1, 0), _i64(4096, 256, 128, 1)
+
+    def chunk(n, t, longest, splits, heads=1):
+        size = lib.tasft_chunk_workspace_bytes(t, heads, 64, splits)
+        return lib.tasft_chunk_paged_fwd(FAKE, FAKE, FAKE, FAKE, None, None, FAKE, FAKE, FAKE, FAKE, size, n, t, heads,
+                                         heads, longest, 64, 64, 0, 16, 9, 6, splits, st, pool, pool, st, None, 6, 1.0,
+                                         1, 0, None)
+
+    assert chunk(1 << 14, 1 << 17, 1 << 17, 1) == -2 and b"launch too large" in _err()      # 2^24 row tiles
+    assert chunk(1, 1 << 20, 1, 9, 16) == -2 and b"launch too large" in _err()              # joined, a workgroup a row
+    assert chunk(1, 1 << 20, 1, 8, 2048) == -2 and b"launch too large" in _err()            # joined, 16 rows a workgroup
+
+    def weights(n, per):
+        return lib.tasft_key_weights(FAKE, FAKE, None, FAKE, FAKE, FAKE, FAKE, None, FAKE, n, 8, 1, 1, 5, 64, 64, 0, 256,
+                                     9, per, st, pool, _i64(4, 1), None, None, 6, 1.0, 1, 0, None)
+
+    assert weights(1 << 14, 1 << 10) == -2 and b"launch too large" in _err()                # 2^24 times 256 keys
