@@ -36,9 +36,13 @@ def rotary_frequencies(
             frequencies of fewer than ``low_freq_factor`` turns over the original length divided by
             the factor, of more than ``high_freq_factor`` kept, those between blended; ``"yarn"``
             (``factor``, ``original_max_position_embeddings``, optional ``beta_fast`` 32,
-            ``beta_slow`` 1, ``attention_factor``): blended by dimension between the dims that make
-            ``beta_fast`` and ``beta_slow`` turns, with the factor ``0.1 ln(factor) + 1`` on the
-            result. Types whose frequencies follow the running length are refused.
+            ``beta_slow`` 1, ``truncate``, ``attention_factor``, ``mscale`` with
+            ``mscale_all_dim``): blended by dimension between the dims that make ``beta_fast`` and
+            ``beta_slow`` turns (whole dims unless ``truncate`` is false), with a factor on the
+            result: ``attention_factor``, or ``0.1 mscale ln(factor) + 1`` over the same of
+            ``mscale_all_dim`` (without them ``0.1 ln(factor) + 1``; what such a model multiplies
+            its softmax by is the caller's). Types whose frequencies follow the running length, and
+            entries that none of these types has, are refused.
         device: of the returned tensor.
     """
     if rotary_dim <= 0 or rotary_dim % 2 != 0:
@@ -48,16 +52,24 @@ def rotary_frequencies(
     inv = torch.tensor([base ** (-2.0 * j / rotary_dim) for j in range(rotary_dim // 2)], dtype=torch.float64)
     kind = "default" if scaling is None else scaling.get("rope_type", scaling.get("type", "default"))
     attention = 1.0
+    if kind not in ("default", "linear", "llama3", "yarn"):
+        raise ValueError(f"rope_type must be default, linear, llama3 or yarn, got {kind!r}")
+    unknown = sorted(name for name, value in (scaling or {}).items() if name not in _ENTRIES and value is not None)
+    if unknown:
+        raise ValueError(f"rope_type {kind!r}: no such entries: {', '.join(map(str, unknown))}")
+    theta = (scaling or {}).get("rope_theta")
+    if theta is not None and float(theta) != float(base):
+        raise ValueError(f"rope_theta is {theta} but base is {base}")
     if kind != "default":
-        if kind not in ("linear", "llama3", "yarn"):
-            raise ValueError(f"rope_type must be default, linear, llama3 or yarn, got {kind!r}")
         factor = _entry(scaling, "factor", kind)
-        if not factor > 0.0:
-            raise ValueError(f"factor must be positive, got {factor}")
+        if not 0.0 < factor < math.inf:
+            raise ValueError(f"factor must be positive and finite, got {factor}")
         if kind == "linear":
             inv = inv / factor
         else:
             original = _entry(scaling, "original_max_position_embeddings", kind)
+            if not 0.0 < original < math.inf:
+                raise ValueError(f"original_max_position_embeddings must be positive and finite, got {original}")
             if kind == "llama3":
                 low, high = _entry(scaling, "low_freq_factor", kind), _entry(scaling, "high_freq_factor", kind)
                 if not 0.0 < low < high:
@@ -65,10 +77,18 @@ def rotary_frequencies(
                 keep = ((original * inv / (2.0 * math.pi) - low) / (high - low)).clamp(0.0, 1.0)
             else:
                 keep = 1.0 - _yarn_ramp(rotary_dim, base, original, scaling)
-                given = scaling.get("attention_factor")
-                attention = float(given) if given is not None else (0.1 * math.log(factor) + 1.0 if factor > 1.0 else 1.0)
+                attention = _yarn_factor(factor, scaling)
             inv = inv / factor * (1.0 - keep) + inv * keep
     return inv.to(device) if device is not None else inv, attention
+
+
+# What the configurations of these types hold. Of no effect here: "finetuned" (describes the weights),
+# "partial_rotary_factor" (the caller's rotary_dim), "mrope_section" (one position a token, so that its
+# sections turn alike).
+_ENTRIES = frozenset({
+    "rope_type", "type", "rope_theta", "factor", "original_max_position_embeddings", "low_freq_factor",
+    "high_freq_factor", "beta_fast", "beta_slow", "attention_factor", "mscale", "mscale_all_dim", "truncate",
+    "finetuned", "partial_rotary_factor", "mrope_section"})
 
 
 def _entry(scaling: dict, name: str, kind: str) -> float:
@@ -77,15 +97,33 @@ def _entry(scaling: dict, name: str, kind: str) -> float:
     return float(scaling[name])
 
 
+def _yarn_factor(factor: float, scaling: dict) -> float:
+    """The factor on cosine and sine."""
+    if scaling.get("attention_factor") is not None:
+        return float(scaling["attention_factor"])
+    given = [scaling.get(name) for name in ("mscale", "mscale_all_dim")]
+    if (given[0] is None) != (given[1] is None):
+        raise ValueError("mscale and mscale_all_dim are given together or not at all")
+    over, under = (1.0, 0.0) if given[0] is None else (float(x) for x in given)
+    growth = 0.1 * math.log(factor) if factor > 1.0 else 0.0
+    return (growth * over + 1.0) / (growth * under + 1.0)
+
+
 def _yarn_ramp(dim: int, base: float, original: float, scaling: dict) -> torch.Tensor:
     """0 for the pairs that keep their frequency, 1 for those divided by the factor."""
+    if not base > 1.0:
+        raise ValueError(f"rope_type 'yarn' needs a base above 1, got {base}")
     fast, slow = float(scaling.get("beta_fast") or 32.0), float(scaling.get("beta_slow") or 1.0)
+    if not (0.0 < fast < math.inf and 0.0 < slow < math.inf):
+        raise ValueError(f"beta_fast and beta_slow must be positive and finite, got {fast} and {slow}")
 
     def pair_with_turns(turns: float) -> float:
         return dim * math.log(original / (turns * 2.0 * math.pi)) / (2.0 * math.log(base))
 
-    low = max(math.floor(pair_with_turns(fast)), 0)
-    high = min(math.ceil(pair_with_turns(slow)), dim - 1)
+    low, high = pair_with_turns(fast), pair_with_turns(slow)
+    if scaling.get("truncate") is None or scaling["truncate"]:
+        low, high = math.floor(low), math.ceil(high)
+    low, high = max(low, 0), min(high, dim - 1)
     at = torch.arange(dim // 2, dtype=torch.float64)
     return ((at - low) / (high - low if high != low else 0.001)).clamp(0.0, 1.0)
 

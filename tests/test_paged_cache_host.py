@@ -82,6 +82,66 @@ def test_frequency_refusals(args, match):
         rotary_frequencies(*args)
 
 
+def test_yarn_factor_of_mscale():
+    """The published factor on cosine and sine: (0.1 m ln(factor) + 1) of mscale over that of
+    mscale_all_dim."""
+    cfg = {"type": "yarn", "factor": 40.0, "original_max_position_embeddings": 4096, "beta_fast": 32, "beta_slow": 1}
+    both = {**cfg, "mscale": 1.0, "mscale_all_dim": 1.0}
+    assert rotary_frequencies(64, 10000.0, both)[1] == 1.0
+    assert rotary_frequencies(64, 10000.0, {**cfg, "mscale": 0.707, "mscale_all_dim": 0.707})[1] == 1.0
+    got = rotary_frequencies(64, 10000.0, {**cfg, "mscale": 1.0, "mscale_all_dim": 0.5})[1]
+    assert abs(got - (0.1 * math.log(40.0) + 1.0) / (0.05 * math.log(40.0) + 1.0)) < 1e-15
+    assert abs(rotary_frequencies(64, 10000.0, {**cfg, "mscale": 1.0, "mscale_all_dim": 0.0})[1]
+               - (0.1 * math.log(40.0) + 1.0)) < 1e-15
+    assert rotary_frequencies(64, 10000.0, {**both, "attention_factor": 1.25})[1] == 1.25  # given: taken as it is
+    assert rotary_frequencies(64, 10000.0, {**both, "factor": 1.0, "mscale": 2.0})[1] == 1.0
+    assert torch.equal(rotary_frequencies(64, 10000.0, both)[0], rotary_frequencies(64, 10000.0, cfg)[0])
+
+
+def test_yarn_range_without_rounding():
+    cfg = {"rope_type": "yarn", "factor": 4.0, "original_max_position_embeddings": 4096, "truncate": False}
+    plain, _ = rotary_frequencies(128, 10000.0)
+    got, a = rotary_frequencies(128, 10000.0, cfg)
+    assert abs(a - (0.1 * math.log(4.0) + 1.0)) < 1e-15
+    low, high = (128 * math.log(4096 / (t * 2 * math.pi)) / (2 * math.log(10000.0)) for t in (32.0, 1.0))
+    for j, (f, x) in enumerate(zip(plain.tolist(), got.tolist())):
+        r = min(1.0, max(0.0, (j - low) / (high - low)))
+        assert abs(x - (f / 4.0 * r + f * (1 - r))) <= 1e-15
+    rounded = rotary_frequencies(128, 10000.0, {**cfg, "truncate": True})[0]
+    assert not torch.equal(got, rounded)
+    assert torch.equal(rounded, rotary_frequencies(128, 10000.0, {k: v for k, v in cfg.items() if k != "truncate"})[0])
+
+
+_YARN = {"rope_type": "yarn", "factor": 4.0, "original_max_position_embeddings": 4096}
+
+
+@pytest.mark.parametrize(("base", "scaling", "match"), [
+    (1.0, _YARN, "base"), (0.5, _YARN, "base"),
+    (1e4, {**_YARN, "mscale": 0.707}, "mscale"), (1e4, {**_YARN, "mscale_all_dim": 1.0}, "mscale"),
+    (1e4, {**_YARN, "original_max_position_embeddings": 0}, "original_max"),
+    (1e4, {**_YARN, "beta_fast": -1.0}, "beta"),
+    (1e4, {**_YARN, "beta_slow": math.inf}, "beta"),
+    (1e4, {**_YARN, "factor": math.inf}, "factor"),
+    (1e4, {**_YARN, "short_factor": [1.0]}, "short_factor"),
+    (1e4, {"rope_type": "default", "long_factor": [1.0, 2.0]}, "long_factor"),
+    (1e4, {"rope_type": "linear", "factor": 2.0, "rope_theta": 5e5}, "rope_theta"),
+])
+def test_scaling_entries_that_would_be_ignored(base, scaling, match):
+    with pytest.raises(ValueError, match=match):
+        rotary_frequencies(64, base, scaling)
+
+
+def test_scaling_entries_without_effect():
+    """Entries of other types, and those that only describe, are read past as before."""
+    plain = rotary_frequencies(64, 1e4, {"rope_type": "linear", "factor": 2.0})
+    more = {"rope_type": "linear", "factor": 2.0, "original_max_position_embeddings": 4096, "rope_theta": 1e4,
+            "finetuned": True, "attention_factor": None, "partial_rotary_factor": 0.5, "mrope_section": [8, 12, 12],
+            "short_factor": None}
+    got = rotary_frequencies(64, 1e4, more)
+    assert torch.equal(got[0], plain[0]) and got[1] == plain[1]
+    assert torch.equal(rotary_frequencies(64, 1e4, {})[0], rotary_frequencies(64, 1e4)[0])
+
+
 # ------------------------------------------------------------------------------ refusals
 def _rope(**over):
     a = {"q": torch.zeros(2, 4, 5, 64, dtype=BF), "k": torch.zeros(2, 2, 5, 64, dtype=BF),
