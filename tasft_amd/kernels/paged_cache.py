@@ -24,7 +24,7 @@ import torch
 
 from tasft_amd import _native
 from tasft_amd.exceptions import KernelError
-from tasft_amd.kernels.rotary import _unit_last, check_frequencies, check_positions
+from tasft_amd.kernels.rotary import _new_like, _unit_last, check_frequencies, check_positions
 
 _VALID_HEAD_DIMS = frozenset({64, 128})
 
@@ -229,7 +229,7 @@ def append_paged(
         if not slot_positions.is_contiguous():
             raise KernelError("slot_positions must be contiguous", context={"strides": list(slot_positions.stride())})
     q, k, v = _unit_last(q), _unit_last(k), _unit_last(v)
-    out = torch.empty_like(q)
+    out = _new_like(q)
     if T == 0:
         return out
     lib = _native.load_library()

@@ -157,6 +157,13 @@ def _unit_last(t: torch.Tensor) -> torch.Tensor:
     return t if t.stride(-1) == 1 else t.contiguous()
 
 
+def _new_like(t: torch.Tensor) -> torch.Tensor:
+    """A new tensor of t's layout, of contiguous rows in any case (rows that overlap can make torch put
+    another dim innermost)."""
+    out = torch.empty_like(t)
+    return out if out.stride(-1) == 1 else torch.empty(t.shape, dtype=t.dtype, device=t.device)
+
+
 def _strides4(t: torch.Tensor):
     """(b, h, s, d) strides of ``[B, H, S, D]``, or of packed ``[T, H, D]`` as one batch entry."""
     st = t.stride()
@@ -167,8 +174,8 @@ def _rotate(q, k, positions, inv_freq, interleaved, scale, inverse):
     """``tasft_rotary`` on checked tensors; ``k`` may be None."""
     q = _unit_last(q)
     k = None if k is None else _unit_last(k)
-    q_out = torch.empty_like(q)
-    k_out = None if k is None else torch.empty_like(k)
+    q_out = _new_like(q)
+    k_out = None if k is None else _new_like(k)
     ps = positions.stride()
     if q.ndim == 4:
         B, Hq, S, D = q.shape

@@ -223,3 +223,29 @@ def test_more_tokens_than_one_launch_takes():
     for n, (s0, s1) in enumerate(((0, first), (first, t))):
         rows = slice(n * per * page, n * per * page + s1 - s0)
         assert torch.equal(kp.view(-1, 1, d)[rows], b[s0:s1]) and torch.equal(vp.view(-1, 1, d)[rows], q[s0:s1])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_overlapping_rows(dtype):
+    """Rows that overlap (windows one element apart), and heads or tokens one element apart: torch lays a
+    tensor like such a one out with another dim innermost."""
+    dev = require_gpu()
+    g = torch.Generator().manual_seed(4)
+    base = torch.randn(20000, generator=g).to(dtype).to(dev)
+    inv, _ = rotary_frequencies(64, device=dev)
+    for shape, strides in (((1, 2, 37, 64), (0, 128, 1, 1)), ((2, 2, 80, 64), (700, 1, 64, 1)), ((5, 4, 64), (1, 96, 1))):
+        q = base.as_strided(shape, strides)
+        s = shape[-2] if len(shape) == 4 else shape[0]
+        pos = torch.arange(s, device=dev)
+        print(f"rotary overlapping {shape} {strides}", flush=True)
+        want, _ = apply_rotary(q.contiguous(), None, pos, inv)
+        a, b = apply_rotary(q, q, pos, inv)
+        assert torch.equal(a, want) and torch.equal(b, want)
+    # Packed rows as new tokens of a cache.
+    q = base.as_strided((5, 4, 64), (1, 96, 1))
+    pools = [torch.zeros((2, 8, 4, 64), dtype=dtype, device=dev) for _ in range(4)]
+    table = torch.tensor([[1]], dtype=torch.int32, device=dev)
+    kvl, cu = torch.tensor([6], dtype=torch.int32, device=dev), torch.tensor([0, 5], dtype=torch.int32, device=dev)
+    got = append_paged(q, q, q, *pools[:2], table, kvl, cu, inv)
+    want = append_paged(*(q.contiguous() for _ in range(3)), *pools[2:], table, kvl, cu, inv)
+    assert torch.equal(got, want) and torch.equal(pools[0], pools[2]) and torch.equal(pools[1], pools[3])
