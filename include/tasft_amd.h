@@ -593,10 +593,10 @@ size_t tasft_evict_workspace_bytes(int64_t num_seqs, int64_t num_kv_heads, int64
  * place, nothing else of them is written. kv_lens_out[n] = n'; scores_out and positions_out
  * [N, Hkv, max_pages * page_size] contiguous hold the kept slots' values where they are now, and
  * 0 and -1 from n' on. scores fp32 and positions int32 have element strides (sequence, head,
- * slot); outputs must not overlap them. No page may belong to two sequences, or twice to one; a
- * row whose page lies outside the pool is not moved. recent + sinks <= budget. head_dim a
- * multiple of 8 up to 256, page_size a power of two, 16-bit pools (any type) with strides of
- * multiples of 8. At most 65535 (sequence, KV head) pairs.
+ * slot); outputs must not overlap them, nor kv_lens_out kv_lens. No page may belong to two
+ * sequences, or twice to one; a row whose page lies outside the pool is not moved.
+ * recent + sinks <= budget. head_dim a multiple of 8 up to 256, page_size a power of two, 16-bit
+ * pools (any type) with strides of multiples of 8. At most 65535 (sequence, KV head) pairs.
  */
 int tasft_evict_paged(void* k_pages, void* v_pages, const int32_t* block_table, const int32_t* kv_lens,
                       const float* scores, const int32_t* positions, int32_t* kv_lens_out,

@@ -575,6 +575,9 @@ extern "C" int tasft_evict_paged(void* k_pages, void* v_pages, const int32_t* bl
   budget = budget < cap ? budget : cap;
   if (workspace_bytes < tasft_evict_workspace_bytes(num_seqs, num_kv_heads, cap, budget))
     return set_error(kErrWorkspace, "evict: workspace too small");
+  // Later launches (and other workgroups) read the lengths, weights and positions again.
+  if (kv_lens_out == kv_lens || scores_out == scores || positions_out == positions)
+    return set_error(kErrInvalidArgument, "evict: outputs may not be the inputs");
   EvictParams p = {};
   p.scores = scores;
   p.positions = positions;

@@ -401,3 +401,17 @@ def test_launches_of_too_many_threads_are_refused():
                                      9, per, st, pool, _i64(4, 1), None, None, 6, 1.0, 1, 0, None)
 
     assert weights(1 << 14, 1 << 10) == -2 and b"launch too large" in _err()                # 2^24 times 256 keys
+
+
+def test_evict_entry_refuses_outputs_that_are_inputs():
+    """Lengths cut in place would be read again, shorter, by the launches behind."""
+    lib = _native.load_library()
+    pool, st = _i64(4096, 256, 128, 1), _i64(192, 96, 1, 0)
+    a = [ctypes.c_void_p(16 * (i + 1)) for i in range(10)]  # never dereferenced
+
+    def call(kv, scores, pos, kv_out, scores_out, pos_out):
+        return lib.tasft_evict_paged(a[0], a[1], a[2], kv, scores, pos, kv_out, scores_out, pos_out, a[9], 1 << 20, 2, 2,
+                                     128, 16, 9, 6, 10, 2, 1, pool, pool, st, st, 6, None)
+
+    for same in ((3, 4, 5, 3, 7, 8), (3, 4, 5, 6, 4, 8), (3, 4, 5, 6, 7, 5)):
+        assert call(*(a[i] for i in same)) == -1 and b"outputs" in _err(), same
