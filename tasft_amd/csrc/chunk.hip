@@ -111,11 +111,6 @@ __device__ __forceinline__ void chunk_mark_cut(const ChunkParams& p, const Chunk
   }
 }
 
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_rsrc(const uint16_t* base, int rows, int64_t stride, int d) {
-  const int n = rows > 0 ? (int)(((rows - 1) * stride + d) * 2) : 0;
-  return __builtin_amdgcn_make_buffer_rsrc((void*)base, (short)0, n, 0x00020000);
-}
-
 __device__ __forceinline__ void chunk_dma(__amdgpu_buffer_rsrc_t r, uint8_t* dst, int voff) {
   __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (TASFT_LDS void*)dst, 16, voff, 0, 0, 0);
 }

@@ -189,7 +189,9 @@ def append_paged(
     Args:
         q, k, v: ``[T, Hq, D]`` and ``[T, Hkv, D]`` of the packed new tokens, before the rotation
             (bf16 or fp16, the pools' dtype).
-        k_pages, v_pages: ``[num_pages, page_size, Hkv, D]`` pools, written in place.
+        k_pages, v_pages: ``[num_pages, page_size, Hkv, D]`` pools, written in place, in any layout of
+            contiguous rows. (The attention and the key weights copy, at every call, pools whose base
+            is not 16-byte aligned or whose strides are not multiples of 8.)
         block_table: ``[N, max_pages]`` int32. A token whose page lies outside the pool (or whose
             slot outside the table) is rotated but not written.
         kv_lens: ``[N]`` lengths with the new tokens: token i of a sequence's ``len`` goes to slot
@@ -384,7 +386,8 @@ def evict_paged(
         status = lib.tasft_evict_paged(
             k_pages.data_ptr(), v_pages.data_ptr(), table.data_ptr(), lens.data_ptr(), scores.data_ptr(),
             slot_positions.data_ptr(), lens_out.data_ptr(), scores_out.data_ptr(), pos_out.data_ptr(),
-            workspace.data_ptr(), ws_bytes, n, Hkv, D, page_size, P, max_pages, budget, recent, sinks, _native.strides(k_pages), _native.strides(v_pages), _native.strides(scores),
+            workspace.data_ptr(), ws_bytes, n, Hkv, D, page_size, P, max_pages, budget, recent, sinks,
+            _native.strides(k_pages), _native.strides(v_pages), _native.strides(scores),
             _native.strides(slot_positions), table.stride(0), _native.stream_handle(dev))
     _native.check(status, "tasft_evict_paged", {"sequences": n, "slots": shape[2], "budget": budget})
     return lens_out, scores_out, pos_out
