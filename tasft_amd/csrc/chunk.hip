@@ -12,10 +12,11 @@
 // ahead: two stages, one barrier a tile. Masked: neighbouring heads and blocks see different keys,
 // so a workgroup takes 64 positions of one head aligned to the mask's blocks, two waves, with one
 // K and one V tile; but where all rows of a KV head fit one wave, the dense form goes over the tiles
-// that any of them selects, each row with its own bits of the mask. S^T = K Q^T with v_mfma_f32_32x32x16, so a lane owns one row: its
-// running maximum and sum stay in the lane (and the one 32 away), and the accumulator of S^T is
-// the B operand of O^T = V^T P^T. P is rounded to the input type for that product (as the MFMA
-// takes it); maxima, sums, O and the log-sum are fp32.
+// that any of them selects, each row with its own bits of the mask. S^T = K Q^T with
+// v_mfma_f32_32x32x16, so a lane owns one row: its running maximum and sum stay in the lane (and the
+// one 32 away), and the accumulator of S^T is the B operand of O^T = V^T P^T. P is rounded to the
+// input type for that product (as the MFMA takes it): outputs are off by up to half a step of their
+// weighted magnitudes more than with P in 32 bits. Maxima, sums, O and the log-sum are fp32.
 //
 // Masked scores are -inf before the exponential, and a key past kv_len is never read (its row
 // arrives as zeros). A tile in which only some rows see a key could still carry an infinity or
