@@ -164,18 +164,30 @@ def _new_like(t: torch.Tensor) -> torch.Tensor:
     return out if out.stride(-1) == 1 else torch.empty(t.shape, dtype=t.dtype, device=t.device)
 
 
-def _strides4(t: torch.Tensor):
+def _strides4(st: tuple[int, ...]):
     """(b, h, s, d) strides of ``[B, H, S, D]``, or of packed ``[T, H, D]`` as one batch entry."""
-    st = t.stride()
     return _native.kept_strides(st if len(st) == 4 else (0, st[1], st[0], st[2]))
+
+
+def _rows_and_new(t: torch.Tensor):
+    """``t`` with contiguous rows and a new tensor like it (``_unit_last``, ``_new_like``), each with its
+    strides for the library: looked up once."""
+    st = t.stride()
+    if st[-1] != 1:
+        t = t.contiguous()
+        st = t.stride()
+    out = torch.empty_like(t)
+    so = out.stride()
+    if so[-1] != 1:
+        out = _new_like(t)
+        so = out.stride()
+    return t, _strides4(st), out, _strides4(so)
 
 
 def _rotate(q, k, positions, inv_freq, interleaved, scale, inverse):
     """``tasft_rotary`` on checked tensors; ``k`` may be None."""
-    q = _unit_last(q)
-    k = None if k is None else _unit_last(k)
-    q_out = _new_like(q)
-    k_out = None if k is None else _new_like(k)
+    q, qs, q_out, qos = _rows_and_new(q)
+    k, ks, k_out, kos = (None,) * 4 if k is None else _rows_and_new(k)
     ps = positions.stride()
     if q.ndim == 4:
         B, Hq, S, D = q.shape
@@ -190,8 +202,7 @@ def _rotate(q, k, positions, inv_freq, interleaved, scale, inverse):
         status = lib.tasft_rotary(
             q.data_ptr(), _native.ptr(k), q_out.data_ptr(), _native.ptr(k_out), positions.data_ptr(),
             1 if positions.dtype == torch.int64 else 0, inv_freq.data_ptr(), B, Hq,
-            0 if k is None else k.shape[1], S, D, 2 * inv_freq.numel(), _strides4(q),
-            None if k is None else _strides4(k), _strides4(q_out), None if k is None else _strides4(k_out),
+            0 if k is None else k.shape[1], S, D, 2 * inv_freq.numel(), qs, ks, qos, kos,
             _native.kept_strides(pos_strides), 1 if interleaved else 0, 1 if inverse else 0, scale,
             _native.dtype_code(q.dtype, "rotary"), _native.stream_handle(q.device))
     _native.check(status, "tasft_rotary", {"shape": list(q.shape)})
@@ -206,9 +217,10 @@ class _Rotary(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, positions, inv_freq, interleaved, scale, inverse):
         ctx.save_for_backward(positions, inv_freq)
-        ctx.save_for_forward(positions, inv_freq)
         ctx.cfg = (interleaved, scale, inverse)
-        ctx.heads = (q.shape[1], None if k is None else k.shape[1])
+        if forward_ad._current_level >= 0:
+            ctx.save_for_forward(positions, inv_freq)
+            ctx.heads = (q.shape[1], None if k is None else k.shape[1])
         ctx.set_materialize_grads(False)
         return _rotate(q, k, positions, inv_freq, interleaved, scale, inverse)
 
