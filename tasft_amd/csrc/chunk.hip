@@ -83,7 +83,7 @@ __device__ __forceinline__ ChunkSeq chunk_seq(const ChunkParams& p, int n) {
   s.t0 = min(max(p.cu[n], 0), p.T);
   const int t1 = min(max(p.cu[n + 1], s.t0), p.T);
   s.len = min(t1 - s.t0, p.L);
-  const int full = min(max(p.kv_lens[n], 0), 0x7fffffff - 255);
+  const int full = max(p.kv_lens[n], 0);
   s.kv = min(full, p.cap);
   s.p0 = full - (t1 - s.t0);  // of the whole chunk, also where L cuts it
   return s;
@@ -861,10 +861,7 @@ chunk_weights_kernel(const WeightParams wp) {
   int member;
   xcd_group_map(blockIdx.x, (int64_t)p.N * p.Hkv, per, &group, &member);
   const int n = (int)(group / p.Hkv), kvh = (int)(group % p.Hkv);
-  ChunkSeq sq = chunk_seq(p, n);
-  // Scalars: as the loads' own vector registers they spilled beside the masked form's.
-  sq.kv = __builtin_amdgcn_readfirstlane(sq.kv);
-  sq.p0 = __builtin_amdgcn_readfirstlane(sq.p0);
+  const ChunkSeq sq = chunk_seq(p, n);
   const int key0 = (member * KW + kg) * kTile;
   const int wg0 = member * KW * kTile;
 
@@ -891,13 +888,14 @@ chunk_weights_kernel(const WeightParams wp) {
     // Adds a tile of 32 rows: Q as the B operand; this lane's row is at `at`, its log-sum `lse`.
     // between() runs when Q has been used.
     auto add_rows = [&](const u32x4_t* qf, RowPlace at, bool ok, float lse, auto between) TASFT_INLINE {
-      const int lim = p.causal ? min(sq.p0 + at.i, sq.kv - 1) : sq.kv - 1;
+      const int pos = (int)((uint32_t)sq.p0 + (uint32_t)at.i);  // of a row past the last one any number
+      const int lim = p.causal ? min(pos, sq.kv - 1) : sq.kv - 1;
       // How far the row sees into the two halves of the keys, in the lane's count. A row without
       // keys (lse -inf) or behind the last one adds nothing.
       int lim0 = ok && lse != -INFINITY ? lim - key0 - 4 * half : -1, lim1 = lim0 - 32;
       if constexpr (MASKED) {
         // (A row past the last one stays within the mask, by its row's and head's limits.)
-        const int mr = min(max(((sq.p0 + at.i) >> p.bs_shift) - block0, 0), p.mask_rows - 1);
+        const int mr = min(max((pos >> p.bs_shift) - block0, 0), p.mask_rows - 1);
         const uint8_t* m = p.mask + n * p.sm[0] + (int64_t)(kvh * p.G + at.g) * p.sm[1] + mr * p.sm[2];
         const int last_block = (p.cap - 1) >> p.bs_shift;
         if (m[min(key0 >> p.bs_shift, last_block) * p.sm[3]] == 0) lim0 = -1;
