@@ -711,7 +711,6 @@ __global__ void __launch_bounds__(256) chunk_combine_few_kernel(const ChunkParam
   const int c = threadIdx.x % LPR;
   if (row >= (int64_t)min(max(p.cu[p.N], 0), p.T) * p.Hq) return;
   const float* ml = p.ws_ml + row * p.P * 2;
-  if (__float_as_uint(ml[1]) == kCutRow) return;
   const float* os = p.ws_o + row * p.P * D + c * 4;
   float m[kFewSplits], l[kFewSplits];
   f32x4_t o[kFewSplits];
@@ -722,6 +721,7 @@ __global__ void __launch_bounds__(256) chunk_combine_few_kernel(const ChunkParam
     l[s] = ml[2 * at + 1];
     o[s] = *(const f32x4_t*)(os + (int64_t)at * D);
   }
+  if (__float_as_uint(l[0]) == kCutRow) return;  // behind the loads: not one more wait before them
   float M = -INFINITY;
 #pragma unroll
   for (int s = 0; s < kFewSplits; ++s) M = fmaxf(M, m[s]);
@@ -748,7 +748,7 @@ __global__ void __launch_bounds__(256) chunk_combine_kernel(const ChunkParams p)
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = tid % LPR, grp = tid / LPR;
   if (row >= (int64_t)min(max(p.cu[p.N], 0), p.T) * p.Hq) return;
   const float* ml = p.ws_ml + row * p.P * 2;
-  if (__float_as_uint(ml[1]) == kCutRow) return;
+  const bool cut = __float_as_uint(ml[1]) == kCutRow;
   const float* os = p.ws_o + row * p.P * D + c * 4;
   float M = -INFINITY;
   for (int s = tid; s < p.P; s += 256) M = fmaxf(M, ml[2 * s]);
@@ -783,7 +783,7 @@ __global__ void __launch_bounds__(256) chunk_combine_kernel(const ChunkParams p)
   }
   part[grp][c] = O;
   __syncthreads();
-  if (grp != 0) return;
+  if (grp != 0 || cut) return;
 #pragma unroll
   for (int g = 1; g < GROUPS; ++g) O += part[g][c];
   chunk_store<D, DT>(p, row, c, O, L, M);
