@@ -26,9 +26,9 @@
 //
 // Many rows: bound by the matrix cores and the exponentials of one wave not running beside the
 // other's (two waves per SIMD, all the registers allow). 2048 tokens of 32 / 8 heads over 32768 keys:
-// 1003 us, 1.07 PFLOP/s, 49% MFMA busy; a fifth of the blocks of 4 requests of 2048 over up to 16384:
-// 354 us, 0.71 PFLOP/s, 34% busy. Few rows: by the reads of the cache. 64 tokens of 64 requests of 8k
-// to 16k keys: 589 us, 5.5 TB/s.
+// 1045 us, 1.02 PFLOP/s, 49% MFMA busy (1003 to 1082 by the card); a fifth of the blocks of 4 requests
+// of 2048 over up to 16384: 360 us, 0.69 PFLOP/s, 34% busy (354 to 414 by masks and card). Few rows: by
+// the reads of the cache. 64 tokens of 64 requests of 8k to 16k keys: 586 us, 5.5 TB/s.
 // Measured and not kept: three tiles in LDS for the masked form (a whole step's time for each DMA,
 // three workgroups a CU instead of four: 481 instead of 402 us); the same heads of every sequence on
 // one XCD (no gain, 376 instead of 362 us where a group's keys were then read twice); a higher wave
@@ -805,10 +805,11 @@ __global__ void __launch_bounds__(256) chunk_combine_kernel(const ChunkParams p)
 // without a barrier. With few rows each wave loads its own into registers, the next tile's under
 // the exponentials of one.
 //
-// Many rows are bound by the exponentials: 32 rows and 64 keys are 512 cycles of products and 768 of
-// exponentials, multiply-adds and sums, on two waves per SIMD (256 tokens of 2 requests over 28k
-// keys on average: 120 us, 0.87 PFLOP/s, 34% MFMA busy). Few rows by the reads of K (one token of
-// 32 requests over 4097 keys, 28 / 4 heads: 28.5 us, 4.9 TB/s).
+// Many rows: 32 rows and 64 keys are 512 cycles of products and 768 of exponentials, multiply-adds and
+// sums, on two waves per SIMD, of which one's products hardly run beside the other's exponentials: 256
+// tokens of 2 requests over 28k keys on average take 125 us (0.84 PFLOP/s, 34% MFMA busy), one after the
+// other they would take 105. Few rows: by the reads of K (one token of 32 requests over 4097 keys,
+// 28 / 4 heads: 28.5 us, 4.9 TB/s).
 // ---------------------------------------------------------------------------------------
 struct WeightParams {
   ChunkParams c;

@@ -9,12 +9,14 @@
 // before the fp32 sine: positions of any size keep the sine's own accuracy (p f in fp32 would
 // be off by 0.03 rad at p = 10^6).
 //
-// Bound by memory: 4 bytes per element (32768 tokens of 32 + 8 heads of 128: 117 us, 5.7 TB/s;
-// 64 tokens 4 us, the launch). A workgroup takes a token: it computes its sines once into LDS
-// (shared by all heads; per head they would cost more than the traffic), then every thread keeps
-// one place within a row and walks the heads, two 16-byte vectors of the two halves at a time.
-// (Four tokens a workgroup, one wait for the sines of all: 125 us for 32768, 9.1 instead of 8.6 for
-// 2048, 5.6 instead of 4.0 for 64.)
+// Bound by memory: 4 bytes per element (32768 tokens of 32 + 8 heads of 128: 113 us one after the
+// other, 5.9 TB/s, 124 as the forward or backward of a training pass; 64 tokens 3 us, the launch). A
+// workgroup takes a token: it computes its sines once into LDS (shared by all heads; per head they
+// would cost more than the traffic), then every thread keeps one place within a row and walks the
+// heads, two 16-byte vectors of the two halves at a time. (Four tokens a workgroup, one wait for the
+// sines of all: 125 us where one took 117, 9.1 and 8.6 for 2048 tokens, 5.6 and 4.0 for 64.) Measured
+// at 10 KB a token; tokens of few or short heads leave threads without a row, behind the same wait for
+// the sines: 16384 tokens of 8 + 2 heads of 64 take 18.3 us, 2.3 TB/s, of 128 23.1 us, 3.6 TB/s.
 #include "common.h"
 
 #include "../../include/tasft_amd.h"
