@@ -231,7 +231,9 @@ class _Rotary(torch.autograd.Function):
         return gq, gk, None, None, None, None, None
 
     @staticmethod
-    def jvp(ctx, tq, tk, *_):
+    def jvp(ctx, tq, tk, positions, inv_freq, *_):
+        if inv_freq is not None:
+            raise KernelError("inv_freq must not carry a tangent: the rotation has no derivative for it", context={})
         out = _turn_given(ctx, tq, tk, ctx.cfg[2])
         there = tq if tq is not None else tk
         # torch takes no None for the tangent of a tensor.

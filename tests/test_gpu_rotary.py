@@ -7,6 +7,7 @@ import torch.autograd.forward_ad as fwAD
 
 import paged_ref as ref
 from helpers import require_gpu
+from tasft_amd.exceptions import KernelError
 from tasft_amd.kernels import append_paged, apply_rotary, rotary_frequencies
 
 pytestmark = pytest.mark.gpu
@@ -249,3 +250,17 @@ def test_overlapping_rows(dtype):
     got = append_paged(q, q, q, *pools[:2], table, kvl, cu, inv)
     want = append_paged(*(q.contiguous() for _ in range(3)), *pools[2:], table, kvl, cu, inv)
     assert torch.equal(got, want) and torch.equal(pools[0], pools[2]) and torch.equal(pools[1], pools[3])
+
+
+def test_forward_mode_of_frequencies():
+    """The rotation has no derivative for its frequencies: a tangent of theirs is refused, not dropped."""
+    dev = require_gpu()
+    inv, _ = rotary_frequencies(32, device=dev)
+    q, t = (torch.randn(2, 3, 9, 32, device=dev).bfloat16() for _ in range(2))
+    pos = torch.arange(9, device=dev)
+    print("rotary forward mode of frequencies", flush=True)
+    for x in (q, None):
+        with fwAD.dual_level():
+            dual = fwAD.make_dual(inv, torch.ones_like(inv))
+            with pytest.raises(KernelError, match="inv_freq"):
+                apply_rotary(q if x is None else fwAD.make_dual(x, t), None, pos, dual)
