@@ -101,10 +101,11 @@ def _yarn_factor(factor: float, scaling: dict) -> float:
     """The factor on cosine and sine."""
     if scaling.get("attention_factor") is not None:
         return float(scaling["attention_factor"])
-    given = [scaling.get(name) for name in ("mscale", "mscale_all_dim")]
-    if (given[0] is None) != (given[1] is None):
+    over, under = scaling.get("mscale"), scaling.get("mscale_all_dim")
+    # Alone, and not at the value that leaving it out means, an entry is read in two ways.
+    if (under is None and over not in (None, 1)) or (over is None and under not in (None, 0)):
         raise ValueError("mscale and mscale_all_dim are given together or not at all")
-    over, under = (1.0, 0.0) if given[0] is None else (float(x) for x in given)
+    over, under = 1.0 if over is None else float(over), 0.0 if under is None else float(under)
     growth = 0.1 * math.log(factor) if factor > 1.0 else 0.0
     return (growth * over + 1.0) / (growth * under + 1.0)
 

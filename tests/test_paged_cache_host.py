@@ -142,6 +142,14 @@ def test_scaling_entries_without_effect():
     assert torch.equal(rotary_frequencies(64, 1e4, {})[0], rotary_frequencies(64, 1e4)[0])
 
 
+def test_a_lone_mscale_of_its_default():
+    """One of the two entries at the value that leaving it out means: the plain factor."""
+    cfg = {"rope_type": "yarn", "factor": 40.0, "original_max_position_embeddings": 4096}
+    plain = rotary_frequencies(64, 10000.0, cfg)[1]
+    assert rotary_frequencies(64, 10000.0, {**cfg, "mscale": 1.0})[1] == plain
+    assert rotary_frequencies(64, 10000.0, {**cfg, "mscale_all_dim": 0})[1] == plain
+
+
 # ------------------------------------------------------------------------------ refusals
 def _rope(**over):
     a = {"q": torch.zeros(2, 4, 5, 64, dtype=BF), "k": torch.zeros(2, 2, 5, 64, dtype=BF),
