@@ -545,7 +545,8 @@ size_t tasft_chunk_workspace_bytes(int64_t tokens, int64_t num_q_heads, int64_t 
  * its last). out = softmax(q.k * scale) v over them, rows without keys 0; lse [T, Hq] fp32
  * contiguous (or NULL) the natural logarithm of the sum of exponentials, -inf without keys. Rows
  * of tokens at or after cu_seqlens[N] get 0 and -inf. What a row does not see does not reach it,
- * infinities and NaN included. A sequence's tokens behind its first max_seqlen are left out: their
+ * infinities and NaN included; an infinity of V that it sees gives that infinity, or NaN where its
+ * weight, taken in the input type, is 0. A sequence's tokens behind its first max_seqlen are left out: their
  * rows are not written.
  * head_dim 64 or 128; block_size 32, 64 or 128; page_size a power of two >= 8; strides multiples
  * of 8 on 16-byte aligned bases. num_splits (1 to 1024) shares the keys of a row among

@@ -22,7 +22,8 @@
 // arrives as zeros). A tile in which only some rows see a key could still carry an infinity or
 // NaN of V into the others as 0 * inf: there V's largest magnitude is looked for (every value by
 // itself took as long as the rest of the tile) and, if it is not finite, such values are left out of the
-// product; after the last tile they are added key by key to the rows that see them.
+// product; after the last tile they are added key by key to the rows that see them. (A row that sees
+// an infinity whose weight rounds to 0, in fp16 below 2^-25 of the row's largest, gets NaN.)
 //
 // Many rows: bound by the matrix cores and the exponentials of one wave not running beside the
 // other's (two waves per SIMD, all the registers allow). 2048 tokens of 32 / 8 heads over 32768 keys:
