@@ -607,6 +607,44 @@ int tasft_evict_paged(void* k_pages, void* v_pages, const int32_t* block_table, 
                       const int64_t* kp_strides, const int64_t* vp_strides, const int64_t* score_strides,
                       const int64_t* position_strides, int64_t block_table_stride, void* stream);
 
+/*
+ * Dense attention of a training step. Replaces the dense branch of
+ * TASFTAttention._training_forward (tasft/modules/tasft_attention.py:427-466), whose scores are stored.
+ *
+ * Sequence n: with cu_seqlens ([N + 1] int32) tokens cu_seqlens[n] .. cu_seqlens[n + 1] - 1 of `tokens`
+ * packed ones (at most max_seqlen of them; batch strides are ignored for the offset 0); without, the first
+ * seq_lens[n] (NULL: all) of `tokens` of batch entry n. Token i sees key j of its sequence if j <= i or
+ * j < prefix_lens[n] (NULL: 0), or with causal 0 every key. With s = q_i.k_j * scale, then
+ * softcap tanh(s / softcap) if softcap > 0, then s - alibi_slopes[h] |i - j| (NULL: none):
+ * out_i = softmax_j(s) v_j, lse_i = log sum_j exp(s) (NULL: not wanted). Rows without a token of a
+ * sequence: 0 and -inf. head_dim 64 or 128; strides (b, h, s, d) of q, k, v, out and (b, h, s) of lse.
+ */
+int tasft_dense_fwd(const void* q, const void* k, const void* v, void* out, float* lse,
+                    const int32_t* cu_seqlens, const int32_t* seq_lens, const int32_t* prefix_lens,
+                    const float* alibi_slopes, int64_t num_seqs, int64_t tokens, int64_t num_q_heads,
+                    int64_t num_kv_heads, int64_t max_seqlen, int64_t head_dim, const int64_t* q_strides,
+                    const int64_t* k_strides, const int64_t* v_strides, const int64_t* o_strides,
+                    const int64_t* lse_strides, float scale, float softcap, int causal, int dtype, void* stream);
+
+/* Bytes of workspace tasft_dense_bwd needs; rows: tokens if packed, else num_seqs * tokens. */
+size_t tasft_dense_bwd_workspace_bytes(int64_t num_seqs, int64_t rows, int64_t num_q_heads,
+                                       int64_t num_kv_heads, int64_t max_seqlen, int64_t head_dim);
+
+/*
+ * Its backward: grad_q, grad_k (summed over the query heads of a KV head) and grad_v from out and lse of the
+ * forward, grad_out and grad_lse (NULL: none). Every sum has a fixed order. Rows without a token of a
+ * sequence get 0. Gradients must not overlap anything else.
+ */
+int tasft_dense_bwd(const void* q, const void* k, const void* v, const void* out, const float* lse,
+                    const void* grad_out, const float* grad_lse, void* grad_q, void* grad_k, void* grad_v,
+                    void* workspace, size_t workspace_bytes, const int32_t* cu_seqlens, const int32_t* seq_lens,
+                    const int32_t* prefix_lens, const float* alibi_slopes, int64_t num_seqs, int64_t tokens,
+                    int64_t num_q_heads, int64_t num_kv_heads, int64_t max_seqlen, int64_t head_dim,
+                    const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides,
+                    const int64_t* o_strides, const int64_t* lse_strides, const int64_t* go_strides,
+                    const int64_t* glse_strides, const int64_t* gq_strides, const int64_t* gk_strides,
+                    const int64_t* gv_strides, float scale, float softcap, int causal, int dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -56,6 +56,9 @@ EXPORTED_SYMBOLS = (
     "tasft_key_weights",
     "tasft_evict_workspace_bytes",
     "tasft_evict_paged",
+    "tasft_dense_fwd",
+    "tasft_dense_bwd_workspace_bytes",
+    "tasft_dense_bwd",
 )
 
 _lock = threading.Lock()
@@ -171,6 +174,17 @@ _SIGNATURES: dict[str, tuple[object, list[object]]] = {
         _I,
         [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _SZ, _I64, _I64, _I64, _I64, _I64, _I64, _I64,
          _I64, _I64, _I64P, _I64P, _I64P, _I64P, _I64, _P],
+    ),
+    "tasft_dense_fwd": (
+        _I,
+        [_P, _P, _P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I64P, _I64P, _I64P,
+         _I64P, _I64P, _F, _F, _I, _I, _P],
+    ),
+    "tasft_dense_bwd_workspace_bytes": (_SZ, [_I64, _I64, _I64, _I64, _I64, _I64]),
+    "tasft_dense_bwd": (
+        _I,
+        [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _SZ, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64,
+         _I64, _I64P, _I64P, _I64P, _I64P, _I64P, _I64P, _I64P, _I64P, _I64P, _I64P, _F, _F, _I, _I, _P],
     ),
 }
 

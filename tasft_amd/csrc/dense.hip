@@ -1,0 +1,949 @@
+// Dense attention of a training step, forward and backward.
+//
+// Sequence n has len tokens (packed: tokens cu[n] .. cu[n + 1] - 1 of [T, H, D]; batched: the first
+// seq_lens[n] of [B, H, S, D]). Token i sees key j of its own sequence if j <= i or j < prefix[n]
+// (causal), or every key. With s = scale q_i . k_j, then cap tanh(s / cap), then - slope_h |i - j|:
+//   o_i = sum_j P_ij v_j,  P_ij = exp(s_ij - lse_i),  lse_i = log sum_j exp(s_ij).
+// Backward, with dP_ij = do_i . v_j and D_i = do_i . o_i - dlse_i:
+//   dv_j = sum_i P_ij do_i,  dS_ij = P_ij (dP_ij - D_i) (1 - tanh^2),
+//   dq_i = scale sum_j dS_ij k_j,  dk_j = scale sum_i dS_ij q_i.
+// Two kernels: one owns queries (dq, and D_i on the way), one owns keys (dk, dv of a KV head over the
+// query heads of its group). Each forms S and dP for itself, seven products instead of five, and no
+// sum depends on the order in which workgroups run.
+//
+// All three use v_mfma_f32_32x32x16 with the owned rows as columns of the result: a lane owns one row,
+// the accumulator of S^T (or S) is the B operand of the product that follows, and the tiles that the
+// workgroup walks over lie in LDS, brought by DMA a tile ahead, read in rows and (transposed) in
+// columns. A workgroup owns 128 rows, four waves 32 each; tiles have 64 rows. P and dS are rounded to
+// the input type for their products (as the MFMA takes them): results are off by up to half a step of
+// their weighted magnitudes more than with P and dS in 32 bits. Maxima, sums and accumulators are fp32.
+//
+// Tokens that a row does not see do not reach it: where only some rows of a tile see a key, infinities
+// and NaN of what the zero weights would multiply are left out of the product and added to the rows
+// that see them after the last tile.
+#include <type_traits>
+
+#include "scores.h"
+
+#include "../../include/tasft_amd.h"
+
+namespace tasft {
+
+#define TASFT_INLINE __attribute__((always_inline))
+
+constexpr int kDenseRows = 128;  // rows that a workgroup owns
+constexpr int kDenseTile = 64;   // rows of a tile that it walks over
+constexpr float kDenseMove = 8.f;  // a new maximum moves the exp2 reference only if this far above it
+constexpr float kDenseLn2 = 0.69314718055994531f;
+
+// A [batch, token, head] view of contiguous rows: element strides.
+struct DenseRows {
+  uint16_t* p;
+  int64_t s[3];
+};
+
+struct DenseParams {
+  DenseRows q, k, v, o, go, gq, gk, gv;
+  float* lse;         // strides (batch, token, head)
+  int64_t sl[3];
+  const float* glse;  // or null
+  int64_t sgl[3];
+  float2* stats;      // [head][row]: lse log2(e) and D
+  float* part_k;      // [SG][row][Hkv][D], or null
+  float* part_v;
+  const int32_t* cu;        // packed, or null
+  const int32_t* seq_lens;  // batched, or null
+  const int32_t* prefix;    // or null
+  ScoreParams sc;
+  float scale;
+  int64_t rows;  // rows of a head in all: T, or B S
+  int N, T, Hq, Hkv, G, L;  // T: tokens packed, or of a batch entry
+  int tiles;                // workgroups along a sequence
+  int SG;                   // workgroups that share a KV head's query heads
+  int causal;
+};
+
+struct DenseSeq {
+  int b;      // batch entry
+  int t0, t1; // its tokens, the last ones without a sequence's part
+  int len, pre;
+};
+
+__device__ __forceinline__ DenseSeq dense_seq(const DenseParams& p, int n) {
+  DenseSeq s;
+  if (p.cu) {
+    s.b = 0;
+    s.t0 = min(max(p.cu[n], 0), p.T);
+    s.t1 = min(max(p.cu[n + 1], s.t0), p.T);
+    s.len = min(s.t1 - s.t0, p.L);
+  } else {
+    s.b = n;
+    s.t0 = 0;
+    s.t1 = p.T;
+    s.len = p.seq_lens ? min(max(p.seq_lens[n], 0), p.T) : p.T;
+  }
+  s.pre = p.causal && p.prefix ? min(max(p.prefix[n], 0), s.len) : 0;
+  return s;
+}
+
+__device__ __forceinline__ uint16_t* dense_at(const DenseRows& r, const DenseSeq& s, int i, int h) {
+  return r.p + s.b * r.s[0] + (int64_t)(s.t0 + i) * r.s[1] + h * r.s[2];
+}
+
+// Rows of a head that no sequence has: those behind its length in tile `tile` of the workgroup's
+// sequence, those that max_seqlen cuts off, and those behind the last sequence, shared out.
+template <class F>
+__device__ __forceinline__ void dense_rest(const DenseParams& p, const DenseSeq& s, int n, int tile, int tid, F&& clear) {
+  if (!p.cu) {
+    const int from = max(tile * kDenseRows, s.len), to = min((tile + 1) * kDenseRows, p.T);
+    for (int t = from; t < to; ++t) clear(s.b, t);
+    return;
+  }
+  if (tile == 0)
+    for (int t = s.t0 + s.len; t < s.t1; ++t) clear(0, t);
+  const int64_t end = min(max(p.cu[p.N], 0), p.T);
+  for (int64_t t = end + (int64_t)n * p.tiles + tile; t < p.T; t += (int64_t)p.N * p.tiles) clear(0, (int)t);
+}
+
+// A row of D values of a head set to 0 by D / 8 lanes.
+template <int D>
+__device__ __forceinline__ void dense_clear(const DenseRows& r, int b, int t, int h, int tid) {
+  if (tid < D / 8) *(u32x4_t*)(r.p + b * r.s[0] + (int64_t)t * r.s[1] + h * r.s[2] + tid * 8) = (u32x4_t){0u, 0u, 0u, 0u};
+}
+
+// Position of 16-byte chunk cc of row r in LDS: of 16 consecutive rows the same chunk, and of 4
+// consecutive rows (from a multiple of 4) any 64 bytes, lie in different banks.
+template <int D>
+__device__ __forceinline__ int dense_swz(int r, int cc) {
+  return cc ^ (D == 128 ? ((r & 3) << 2 | ((r >> 2) & 3)) : (((r >> 1) & 1) << 2 | ((r >> 2) & 3)));
+}
+
+__device__ __forceinline__ void dense_barrier() { asm volatile("s_barrier" ::: "memory"); }
+
+// A pair of 16-bit values with infinities and NaN replaced by 0.
+template <int DT>
+__device__ __forceinline__ uint32_t dense_finite2(uint32_t w) {
+  constexpr uint32_t E = DT == kF16 ? 0x7c00u : 0x7f80u;
+  if ((w & E) == E) w &= 0xffff0000u;
+  if ((w & (E << 16)) == (E << 16)) w &= 0xffffu;
+  return w;
+}
+
+typedef uint16_t dense_u16x2_t __attribute__((ext_vector_type(2)));
+
+// What a wave does with the tiles of 64 rows in LDS. A tile's share of a wave: 16 rows.
+template <int D, int DT>
+struct DenseTiles {
+  static constexpr int KSTEPS = D / 16;
+  static constexpr int DTILES = D / 32;
+  static constexpr int ROWB = D * 2;
+  static constexpr int TILE = kDenseTile * ROWB;
+  static constexpr int RPU = 1024 / ROWB;            // rows of a 1 KB DMA unit
+  static constexpr int UPW = kDenseTile / 4 / RPU;   // units of a wave's share
+  static constexpr int CPR = ROWB / 16;
+
+  // Byte offsets, from the tile's first row, of what a lane brings.
+  static __device__ __forceinline__ void offsets(int (&off)[UPW], int64_t stride, int wave, int lane) {
+#pragma unroll
+    for (int u = 0; u < UPW; ++u) {
+      const int row = wave * (kDenseTile / 4) + u * RPU + lane / CPR;
+      off[u] = (row * (int)stride + dense_swz<D>(row, lane % CPR) * 8) * 2;
+    }
+  }
+  // Rows `first` .. of a head's tensor into a tile; rows from `len` on arrive as zeros.
+  static __device__ __forceinline__ void dma(uint8_t* tile, const uint16_t* base, int64_t stride, const int (&off)[UPW],
+                                             int first, int len, int wave) {
+    const int rows = min(len - first, kDenseTile);
+    const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
+        (void*)(base + (int64_t)first * stride), (short)0, rows > 0 ? (rows - 1) * (int)stride * 2 + ROWB : 0, 0x00020000);
+#pragma unroll
+    for (int u = 0; u < UPW; ++u)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (TASFT_LDS void*)(tile + (wave * UPW + u) * 1024), 16, off[u], 0, 0, 0);
+  }
+  // Rows r0 .. r0 + 31 as the A operand, times b: 32 x 32 products.
+  static __device__ __forceinline__ f32x16_t rows_times(const uint8_t* tile, int r0, const u32x4_t (&b)[KSTEPS], int col,
+                                                        int half) {
+    u32x4_t a[KSTEPS];
+    const int r = r0 + col;
+#pragma unroll
+    for (int ks = 0; ks < KSTEPS; ++ks)
+      a[ks] = *(const u32x4_t*)(tile + r * ROWB + dense_swz<D>(r, ks * 2 + half) * 16);
+    f32x16_t s = (f32x16_t){};
+#pragma unroll
+    for (int ks = 0; ks < KSTEPS; ++ks) s = mfma16<DT>(a[ks], b[ks], s);
+    return s;
+  }
+  // acc [D x 32] += (rows r0 .. r0 + 31)^T b, b in the order of an accumulator's registers. With
+  // `mixed` infinities and NaN are left out; returns whether there was one.
+  static __device__ __forceinline__ bool columns_times(const uint8_t* tile, int r0, const u32x4_t (&b)[2], bool mixed,
+                                                       f32x16_t (&acc)[DTILES], int lane) {
+    const int grp16 = lane >> 4, t16 = lane & 15, tr_row = t16 >> 2, tr_cb = t16 & 3;
+    u32x2_t lo[2][DTILES], hi[2][DTILES];
+#pragma unroll
+    for (int pp = 0; pp < 2; ++pp) {
+      const int r1 = r0 + 16 * pp + 4 * (grp16 >> 1) + tr_row, r2 = r1 + 8;
+#pragma unroll
+      for (int dt = 0; dt < DTILES; ++dt) {
+        const int d0 = dt * 32 + 16 * (grp16 & 1) + 4 * tr_cb;
+        const int cc = d0 >> 3, sub = (d0 & 7) * 2;
+        lo[pp][dt] = ds_read_tr16_b64((const void*)(tile + r1 * ROWB + dense_swz<D>(r1, cc) * 16 + sub));
+        hi[pp][dt] = ds_read_tr16_b64((const void*)(tile + r2 * ROWB + dense_swz<D>(r2, cc) * 16 + sub));
+      }
+    }
+    bool found = false;
+    if (mixed) {
+      dense_u16x2_t top = {0, 0};  // the largest magnitudes tell whether there is one
+#pragma unroll
+      for (int pp = 0; pp < 2; ++pp)
+#pragma unroll
+        for (int dt = 0; dt < DTILES; ++dt)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            top = __builtin_elementwise_max(top, __builtin_bit_cast(dense_u16x2_t, lo[pp][dt][j] & 0x7fff7fffu));
+            top = __builtin_elementwise_max(top, __builtin_bit_cast(dense_u16x2_t, hi[pp][dt][j] & 0x7fff7fffu));
+          }
+      constexpr uint16_t E = DT == kF16 ? 0x7c00 : 0x7f80;
+      if (__ballot(top[0] >= E || top[1] >= E)) {
+        found = true;
+#pragma unroll
+        for (int pp = 0; pp < 2; ++pp)
+#pragma unroll
+          for (int dt = 0; dt < DTILES; ++dt)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              lo[pp][dt][j] = dense_finite2<DT>(lo[pp][dt][j]);
+              hi[pp][dt][j] = dense_finite2<DT>(hi[pp][dt][j]);
+            }
+      }
+    }
+#pragma unroll
+    for (int pp = 0; pp < 2; ++pp)
+#pragma unroll
+      for (int dt = 0; dt < DTILES; ++dt) {
+        const u32x4_t a = {lo[pp][dt][0], lo[pp][dt][1], hi[pp][dt][0], hi[pp][dt][1]};
+        acc[dt] = mfma16<DT>(a, b[pp], acc[dt]);
+      }
+    return found;
+  }
+  // A wave's 32 rows of the transposed accumulators times f, to `out` (row `col` at element `at`, < 0:
+  // not there), whole rows through 32 rows of LDS of its own.
+  static __device__ __forceinline__ void store(uint8_t* lds, const f32x16_t (&acc)[DTILES], float f, uint16_t* out,
+                                               int64_t at, int lane) {
+    const int col = lane & 31, half = lane >> 5;
+#pragma unroll
+    for (int dt = 0; dt < DTILES; ++dt)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int d0 = dt * 32 + 8 * g + 4 * half;
+        const u32x2_t w = {pack16x2<DT>(acc[dt][4 * g] * f, acc[dt][4 * g + 1] * f),
+                           pack16x2<DT>(acc[dt][4 * g + 2] * f, acc[dt][4 * g + 3] * f)};
+        *(u32x2_t*)(lds + col * ROWB + (((d0 >> 3) ^ (col & (CPR - 1))) << 4) + (d0 & 7) * 2) = w;
+      }
+#pragma unroll
+    for (int j = 0; j < 32 * CPR / kWave; ++j) {
+      const int r = j * (kWave / CPR) + lane / CPR, c = lane % CPR;
+      const u32x4_t x = *(const u32x4_t*)(lds + r * ROWB + ((c ^ (r & (CPR - 1))) << 4));
+      const int64_t to = __shfl(at, r, kWave);
+      if (to >= 0) *(u32x4_t*)(out + to + c * 8) = x;
+    }
+  }
+  // A row as the B operand: dims 16 ks + 8 half .. + 7.
+  static __device__ __forceinline__ void load_row(u32x4_t (&f)[KSTEPS], const uint16_t* row, int half) {
+#pragma unroll
+    for (int ks = 0; ks < KSTEPS; ++ks) f[ks] = *(const u32x4_t*)(row + half * 8 + ks * 16);
+  }
+  // The product of a row in memory and one held as the B operand.
+  static __device__ __forceinline__ float dot(const uint16_t* row, const u32x4_t (&f)[KSTEPS], int half) {
+    float sum = 0.f;
+#pragma unroll
+    for (int ks = 0; ks < KSTEPS; ++ks) {
+      float x[8], y[8];
+      unpack16x8<DT>(*(const u32x4_t*)(row + half * 8 + ks * 16), x);
+      unpack16x8<DT>(f[ks], y);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) sum = fmaf(x[j], y[j], sum);
+    }
+    return pair_sum32(sum);
+  }
+  // acc += w (the infinities and NaN of a row), for the lanes with `sees`.
+  static __device__ __forceinline__ void add_nonfinite(f32x16_t (&acc)[DTILES], const uint16_t* row, float w, bool sees,
+                                                       int half) {
+#pragma unroll
+    for (int dt = 0; dt < DTILES; ++dt) {
+      asm volatile("" ::: "memory");  // not all loads at once: they would take the main loop's registers
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const uint32_t x = row[dt * 32 + 8 * (e >> 2) + 4 * half + (e & 3)];
+        acc[dt][e] += sees && dense_finite2<DT>(x) != x ? w * bits16_to_f32<DT>(x) : 0.f;
+      }
+    }
+  }
+  static __device__ __forceinline__ bool has_nonfinite(const uint16_t* row, int lane) {
+    const uint32_t w = *(const uint32_t*)(row + (lane * 2) % D);
+    return __ballot(dense_finite2<DT>(w) != w) != 0;
+  }
+};
+
+// Scores in units of log2 from the products s of 32 rows; distance of register rr: |d + off(rr)|. gate
+// holds what the cap's derivative needs.
+template <bool CAP, bool BIAS, bool GATE>
+__device__ __forceinline__ void dense_scores(f32x16_t& s, f32x16_t& gate, const ScoreParams& sc, float slope2, float d) {
+  if constexpr (CAP) {
+#pragma unroll
+    for (int rr = 0; rr < 16; ++rr) {
+      const float r = cap_gate(s[rr], sc);
+      if constexpr (GATE) gate[rr] = r;
+      if (sc.cap_wide) s[rr] = cap_score_wide(s[rr], r, sc);
+      else s[rr] = cap_score(s[rr], r, sc);
+    }
+  } else {
+#pragma unroll
+    for (int rr = 0; rr < 16; ++rr) s[rr] *= sc.scale_log2;
+  }
+  if constexpr (BIAS) {
+#pragma unroll
+    for (int rr = 0; rr < 16; ++rr) s[rr] = fmaf(-slope2, fabsf(d + (float)(8 * (rr >> 2) + (rr & 3))), s[rr]);
+  }
+}
+
+// One score as above.
+template <bool CAP, bool BIAS>
+__device__ __forceinline__ float dense_score(float s, float& gate, const ScoreParams& sc, float slope2, float d) {
+  float x = s * sc.scale_log2;
+  if constexpr (CAP) {
+    gate = cap_gate(s, sc);
+    x = sc.cap_wide ? cap_score_wide(s, gate, sc) : cap_score(s, gate, sc);
+  }
+  return BIAS ? fmaf(-slope2, fabsf(d), x) : x;
+}
+
+// ------------------------------------------------------------------------------------ forward
+template <int D, int DT, bool CAP, bool BIAS>
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) dense_fwd_kernel(const DenseParams p) {
+  using X = DenseTiles<D, DT>;
+  constexpr bool UNITS = CAP || BIAS;  // scores are in units of log2 before their maximum
+  __shared__ __attribute__((aligned(1024))) uint8_t k0_lds[X::TILE];
+  __shared__ __attribute__((aligned(1024))) uint8_t v0_lds[X::TILE];
+  __shared__ __attribute__((aligned(1024))) uint8_t k1_lds[X::TILE];
+  __shared__ __attribute__((aligned(1024))) uint8_t v1_lds[X::TILE];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int col = lane & 31, half = lane >> 5;
+  int64_t group;
+  int member;
+  xcd_group_map(blockIdx.x, (int64_t)p.N * p.Hkv, p.tiles * p.G, &group, &member);
+  const int n = (int)(group / p.Hkv), kvh = (int)(group % p.Hkv);
+  const int h = kvh * p.G + member % p.G;
+  const int tile = p.tiles - 1 - member / p.G;  // the longest rows first
+  const DenseSeq sq = dense_seq(p, n);
+  dense_rest(p, sq, n, tile, tid, [&](int b, int t) {
+    dense_clear<D>(p.o, b, t, h, tid);
+    if (tid == 0 && p.lse) p.lse[b * p.sl[0] + t * p.sl[1] + h * p.sl[2]] = -INFINITY;
+  });
+  const int r0 = tile * kDenseRows;
+  if (r0 >= sq.len) return;
+  const int i_first = r0 + wave * 32, i_last = min(i_first + 31, sq.len - 1), i_end = min(r0 + kDenseRows, sq.len) - 1;
+  const bool row_ok = i_first + col < sq.len;
+  const int i = min(i_first + col, sq.len - 1);
+  // Keys a row sees: 0 .. lim. All rows of the wave see the keys to all_see, none one past any_see.
+  auto sees = [&](int row) { return p.causal ? max(row, sq.pre - 1) : sq.len - 1; };
+  const int lim = sees(i), all_see = sees(min(i_first, i_last)), any_see = i_first <= i_last ? sees(i_last) : -1;
+  const int tiles = sees(i_end) / kDenseTile + 1;
+
+  u32x4_t qf[X::KSTEPS];
+  X::load_row(qf, dense_at(p.q, sq, i, h), half);
+  const float slope2 = BIAS ? p.sc.slopes[h] * kLog2e : 0.f;
+  const uint16_t* kbase = dense_at(p.k, sq, 0, kvh);
+  const uint16_t* vbase = dense_at(p.v, sq, 0, kvh);
+  int koff[X::UPW], voff[X::UPW];
+  X::offsets(koff, p.k.s[1], wave, lane);
+  X::offsets(voff, p.v.s[1], wave, lane);
+  auto bring = [&](uint8_t* kt, uint8_t* vt, int t) TASFT_INLINE {
+    X::dma(kt, kbase, p.k.s[1], koff, t * kDenseTile, sq.len, wave);
+    X::dma(vt, vbase, p.v.s[1], voff, t * kDenseTile, sq.len, wave);
+  };
+
+  f32x16_t oacc[X::DTILES];
+#pragma unroll
+  for (int dt = 0; dt < X::DTILES; ++dt) oacc[dt] = (f32x16_t){};
+  float m_ref = -INFINITY, l_run = 0.f;
+  int fix_from = 0x7fffffff;  // first tile whose infinities or NaN of V were left out
+
+  auto step = [&](const uint8_t* ka, const uint8_t* va, uint8_t* kb, uint8_t* vb, int t) TASFT_INLINE {
+    __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0)
+    dense_barrier();
+    if (t + 1 < tiles) bring(kb, vb, t + 1);
+    const int key0 = t * kDenseTile;
+    if (key0 > any_see) return;
+    const bool mixed = key0 + kDenseTile - 1 > all_see;
+    f32x16_t s0 = X::rows_times(ka, 0, qf, col, half), s1 = X::rows_times(ka, 32, qf, col, half);
+    f32x16_t none;
+    if constexpr (UNITS) {
+      const float d = (float)(key0 + 4 * half - i);
+      dense_scores<CAP, BIAS, false>(s0, none, p.sc, slope2, d);
+      dense_scores<CAP, BIAS, false>(s1, none, p.sc, slope2, d + 32.f);
+    }
+    if (mixed) {
+      const int lim0 = lim - key0 - 4 * half, lim1 = lim0 - 32;
+#pragma unroll
+      for (int rr = 0; rr < 16; ++rr) {
+        const int off = 8 * (rr >> 2) + (rr & 3);
+        s0[rr] = off > lim0 ? -INFINITY : s0[rr];
+        s1[rr] = off > lim1 ? -INFINITY : s1[rr];
+      }
+    }
+    float ma = fmaxf(fmaxf(s0[0], s0[1]), s0[2]), mb = fmaxf(fmaxf(s1[0], s1[1]), s1[2]);
+#pragma unroll
+    for (int rr = 3; rr < 15; rr += 2) {
+      ma = fmaxf(fmaxf(ma, s0[rr]), s0[rr + 1]);
+      mb = fmaxf(fmaxf(mb, s1[rr]), s1[rr + 1]);
+    }
+    const float mloc = pair_max32(fmaxf(fmaxf(ma, s0[15]), fmaxf(mb, s1[15]))) * (UNITS ? 1.f : p.sc.scale_log2);
+    const bool move = mloc > m_ref + kDenseMove;
+    if (__ballot(move)) {
+      const float alpha = move ? __builtin_amdgcn_exp2f(m_ref - mloc) : 1.f;
+      l_run *= alpha;
+#pragma unroll
+      for (int dt = 0; dt < X::DTILES; ++dt) oacc[dt] *= alpha;
+      m_ref = move ? mloc : m_ref;
+    }
+    const float m_use = m_ref == -INFINITY ? 0.f : m_ref;
+    float sum0 = 0.f, sum1 = 0.f;
+#pragma unroll
+    for (int rr = 0; rr < 16; ++rr) {
+      s0[rr] = __builtin_amdgcn_exp2f(UNITS ? s0[rr] - m_use : fmaf(s0[rr], p.sc.scale_log2, -m_use));
+      s1[rr] = __builtin_amdgcn_exp2f(UNITS ? s1[rr] - m_use : fmaf(s1[rr], p.sc.scale_log2, -m_use));
+      sum0 += s0[rr];
+      sum1 += s1[rr];
+    }
+    l_run += sum0 + sum1;
+#pragma unroll
+    for (int t2 = 0; t2 < 2; ++t2) {
+      const f32x16_t& sv = t2 ? s1 : s0;
+      u32x4_t pb[2];
+#pragma unroll
+      for (int pp = 0; pp < 2; ++pp)
+        pb[pp] = (u32x4_t){pack16x2<DT>(sv[8 * pp], sv[8 * pp + 1]), pack16x2<DT>(sv[8 * pp + 2], sv[8 * pp + 3]),
+                           pack16x2<DT>(sv[8 * pp + 4], sv[8 * pp + 5]), pack16x2<DT>(sv[8 * pp + 6], sv[8 * pp + 7])};
+      if (X::columns_times(va, 32 * t2, pb, mixed, oacc, lane)) fix_from = min(fix_from, t);
+    }
+  };
+  bring(k0_lds, v0_lds, 0);
+  for (int t = 0; t < tiles; t += 2) {
+    step(k0_lds, v0_lds, k1_lds, v1_lds, t);
+    if (t + 1 >= tiles) break;
+    step(k1_lds, v1_lds, k0_lds, v0_lds, t + 1);
+  }
+
+  if (fix_from != 0x7fffffff) {
+    // Key by key, from memory, to the rows that see the key. (Where another tile had them in its
+    // product, once more changes nothing.)
+    const float m_use = m_ref == -INFINITY ? 0.f : m_ref;
+#pragma nounroll
+    for (int key = fix_from * kDenseTile; key <= any_see; ++key) {
+      const uint16_t* vr = vbase + (int64_t)key * p.v.s[1];
+      if (!X::has_nonfinite(vr, lane)) continue;
+      float gate;
+      const float s = dense_score<CAP, BIAS>(X::dot(kbase + (int64_t)key * p.k.s[1], qf, half), gate, p.sc, slope2,
+                                             (float)(key - i));
+      X::add_nonfinite(oacc, vr, __builtin_amdgcn_exp2f(s - m_use), row_ok && key <= lim, half);
+    }
+  }
+
+  const float l_tot = pair_sum32(l_run);
+  if (p.lse && row_ok && half == 0)
+    p.lse[sq.b * p.sl[0] + (sq.t0 + i) * p.sl[1] + h * p.sl[2]] = (m_ref + __builtin_amdgcn_logf(l_tot)) * kDenseLn2;
+  __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
+  dense_barrier();                     // every wave is done with the tiles
+  uint8_t* ost = ((wave & 2) ? v0_lds : k0_lds) + (wave & 1) * (32 * X::ROWB);
+  X::store(ost, oacc, 1.f / (l_tot > 0.f ? l_tot : 1.f), dense_at(p.o, sq, 0, h), row_ok ? (int64_t)i * p.o.s[1] : -1, lane);
+}
+
+// ------------------------------------------------------------------------- backward: queries
+template <int D, int DT, bool CAP, bool BIAS>
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) dense_dq_kernel(const DenseParams p) {
+  using X = DenseTiles<D, DT>;
+  __shared__ __attribute__((aligned(1024))) uint8_t k0_lds[X::TILE];
+  __shared__ __attribute__((aligned(1024))) uint8_t v0_lds[X::TILE];
+  __shared__ __attribute__((aligned(1024))) uint8_t k1_lds[X::TILE];
+  __shared__ __attribute__((aligned(1024))) uint8_t v1_lds[X::TILE];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int col = lane & 31, half = lane >> 5;
+  int64_t group;
+  int member;
+  xcd_group_map(blockIdx.x, (int64_t)p.N * p.Hkv, p.tiles * p.G, &group, &member);
+  const int n = (int)(group / p.Hkv), kvh = (int)(group % p.Hkv);
+  const int h = kvh * p.G + member % p.G;
+  const int tile = p.tiles - 1 - member / p.G;
+  const DenseSeq sq = dense_seq(p, n);
+  dense_rest(p, sq, n, tile, tid, [&](int b, int t) { dense_clear<D>(p.gq, b, t, h, tid); });
+  const int r0 = tile * kDenseRows;
+  if (r0 >= sq.len) return;
+  const int i_first = r0 + wave * 32, i_last = min(i_first + 31, sq.len - 1), i_end = min(r0 + kDenseRows, sq.len) - 1;
+  const bool row_ok = i_first + col < sq.len;
+  const int i = min(i_first + col, sq.len - 1);
+  auto sees = [&](int row) { return p.causal ? max(row, sq.pre - 1) : sq.len - 1; };
+  const int lim = sees(i), all_see = sees(min(i_first, i_last)), any_see = i_first <= i_last ? sees(i_last) : -1;
+  const int tiles = sees(i_end) / kDenseTile + 1;
+
+  const uint16_t* kbase = dense_at(p.k, sq, 0, kvh);
+  const uint16_t* vbase = dense_at(p.v, sq, 0, kvh);
+  int koff[X::UPW], voff[X::UPW];
+  X::offsets(koff, p.k.s[1], wave, lane);
+  X::offsets(voff, p.v.s[1], wave, lane);
+  auto bring = [&](uint8_t* kt, uint8_t* vt, int t) TASFT_INLINE {
+    X::dma(kt, kbase, p.k.s[1], koff, t * kDenseTile, sq.len, wave);
+    X::dma(vt, vbase, p.v.s[1], voff, t * kDenseTile, sq.len, wave);
+  };
+  bring(k0_lds, v0_lds, 0);
+
+  u32x4_t qf[X::KSTEPS], gf[X::KSTEPS];
+  X::load_row(qf, dense_at(p.q, sq, i, h), half);
+  X::load_row(gf, dense_at(p.go, sq, i, h), half);
+  const int64_t li = sq.b * p.sl[0] + (sq.t0 + i) * p.sl[1] + h * p.sl[2];
+  const float lse2 = p.lse[li] * kLog2e;
+  float D_i = X::dot(dense_at(p.o, sq, i, h), gf, half);
+  if (p.glse) D_i -= p.glse[sq.b * p.sgl[0] + (sq.t0 + i) * p.sgl[1] + h * p.sgl[2]];
+  if (row_ok && half == 0) p.stats[h * p.rows + (int64_t)sq.b * p.T + sq.t0 + i] = make_float2(lse2, D_i);
+  const float slope2 = BIAS ? p.sc.slopes[h] * kLog2e : 0.f;
+
+  f32x16_t acc[X::DTILES];
+#pragma unroll
+  for (int dt = 0; dt < X::DTILES; ++dt) acc[dt] = (f32x16_t){};
+  int fix_from = 0x7fffffff;
+
+  auto step = [&](const uint8_t* ka, const uint8_t* va, uint8_t* kb, uint8_t* vb, int t) TASFT_INLINE {
+    __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0)
+    dense_barrier();
+    if (t + 1 < tiles) bring(kb, vb, t + 1);
+#pragma unroll
+    for (int t2 = 0; t2 < 2; ++t2) {
+      const int key0 = t * kDenseTile + 32 * t2;
+      if (key0 > any_see) continue;
+      const bool mixed = key0 + 31 > all_see;
+      f32x16_t s = X::rows_times(ka, 32 * t2, qf, col, half);
+      f32x16_t dp = X::rows_times(va, 32 * t2, gf, col, half);
+      f32x16_t gate;
+      dense_scores<CAP, BIAS, true>(s, gate, p.sc, slope2, (float)(key0 + 4 * half - i));
+#pragma unroll
+      for (int rr = 0; rr < 16; ++rr) {
+        float ds = __builtin_amdgcn_exp2f(s[rr] - lse2) * (dp[rr] - D_i);
+        if constexpr (CAP) ds *= 4.f * (gate[rr] - gate[rr] * gate[rr]);
+        s[rr] = ds;
+      }
+      if (mixed) {
+        const int lim0 = lim - key0 - 4 * half;
+#pragma unroll
+        for (int rr = 0; rr < 16; ++rr) s[rr] = 8 * (rr >> 2) + (rr & 3) > lim0 ? 0.f : s[rr];
+      }
+      u32x4_t sb[2];
+#pragma unroll
+      for (int pp = 0; pp < 2; ++pp)
+        sb[pp] = (u32x4_t){pack16x2<DT>(s[8 * pp], s[8 * pp + 1]), pack16x2<DT>(s[8 * pp + 2], s[8 * pp + 3]),
+                           pack16x2<DT>(s[8 * pp + 4], s[8 * pp + 5]), pack16x2<DT>(s[8 * pp + 6], s[8 * pp + 7])};
+      if (X::columns_times(ka, 32 * t2, sb, mixed, acc, lane)) fix_from = min(fix_from, t);
+    }
+  };
+  for (int t = 0; t < tiles; t += 2) {
+    step(k0_lds, v0_lds, k1_lds, v1_lds, t);
+    if (t + 1 >= tiles) break;
+    step(k1_lds, v1_lds, k0_lds, v0_lds, t + 1);
+  }
+
+  if (fix_from != 0x7fffffff) {
+#pragma nounroll
+    for (int key = fix_from * kDenseTile; key <= any_see; ++key) {
+      const uint16_t* kr = kbase + (int64_t)key * p.k.s[1];
+      if (!X::has_nonfinite(kr, lane)) continue;
+      float gate;
+      const float s = dense_score<CAP, BIAS>(X::dot(kr, qf, half), gate, p.sc, slope2, (float)(key - i));
+      float ds = __builtin_amdgcn_exp2f(s - lse2) * (X::dot(vbase + (int64_t)key * p.v.s[1], gf, half) - D_i);
+      if constexpr (CAP) ds *= 4.f * (gate - gate * gate);
+      X::add_nonfinite(acc, kr, ds, row_ok && key <= lim, half);
+    }
+  }
+
+  __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
+  dense_barrier();                     // every wave is done with the tiles
+  uint8_t* ost = ((wave & 2) ? v0_lds : k0_lds) + (wave & 1) * (32 * X::ROWB);
+  X::store(ost, acc, p.scale, dense_at(p.gq, sq, 0, h), row_ok ? (int64_t)i * p.gq.s[1] : -1, lane);
+}
+
+// ---------------------------------------------------------------------------- backward: keys
+template <int D, int DT, bool CAP, bool BIAS>
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) dense_dkv_kernel(const DenseParams p) {
+  using X = DenseTiles<D, DT>;
+  __shared__ __attribute__((aligned(1024))) uint8_t q0_lds[X::TILE];
+  __shared__ __attribute__((aligned(1024))) uint8_t g0_lds[X::TILE];
+  __shared__ __attribute__((aligned(1024))) uint8_t q1_lds[X::TILE];
+  __shared__ __attribute__((aligned(1024))) uint8_t g1_lds[X::TILE];
+  __shared__ __attribute__((aligned(1024))) float2 st0_lds[kDenseTile], st1_lds[kDenseTile];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int col = lane & 31, half = lane >> 5;
+  int64_t group;
+  int member;
+  xcd_group_map(blockIdx.x, (int64_t)p.N * p.Hkv, p.tiles * p.SG, &group, &member);
+  const int n = (int)(group / p.Hkv), kvh = (int)(group % p.Hkv);
+  const int sg = member % p.SG, tile = member / p.SG;  // causal: the first keys are seen by the most rows
+  const DenseSeq sq = dense_seq(p, n);
+  if (sg == 0)
+    dense_rest(p, sq, n, tile, tid, [&](int b, int t) {
+      dense_clear<D>(p.gk, b, t, kvh, tid);
+      dense_clear<D>(p.gv, b, t, kvh, tid);
+    });
+  const int r0 = tile * kDenseRows;
+  if (r0 >= sq.len) return;
+  const int j_first = r0 + wave * 32, j_last = min(j_first + 31, sq.len - 1), j_end = min(r0 + kDenseRows, sq.len) - 1;
+  const bool row_ok = j_first + col < sq.len;
+  const int j = min(j_first + col, sq.len - 1);
+  // The first query that sees a key. All of the wave's keys are seen by the rows from all_from on, none
+  // by one before any_from.
+  auto seen_from = [&](int key) { return p.causal && key >= sq.pre ? key : 0; };
+  const int from = seen_from(j), all_from = seen_from(j_last), any_from = j_first <= j_last ? seen_from(j_first) : 0x7fffffff;
+  const int t_first = seen_from(r0) / kDenseTile, t_end = (sq.len - 1) / kDenseTile + 1;
+  const int g_first = kvh * p.G + sg * (p.G / p.SG), heads = p.G / p.SG;
+  (void)j_end;
+
+  u32x4_t kf[X::KSTEPS], vf[X::KSTEPS];
+  X::load_row(kf, dense_at(p.k, sq, j, kvh), half);
+  X::load_row(vf, dense_at(p.v, sq, j, kvh), half);
+  int qoff[X::UPW], goff[X::UPW];
+  X::offsets(qoff, p.q.s[1], wave, lane);
+  X::offsets(goff, p.go.s[1], wave, lane);
+  const float2* stats = p.stats + (int64_t)sq.b * p.T + sq.t0;
+  auto bring = [&](uint8_t* qt, uint8_t* gt, float2* st, int h, int t) TASFT_INLINE {
+    X::dma(qt, dense_at(p.q, sq, 0, h), p.q.s[1], qoff, t * kDenseTile, sq.len, wave);
+    X::dma(gt, dense_at(p.go, sq, 0, h), p.go.s[1], goff, t * kDenseTile, sq.len, wave);
+    if (wave < 2) {  // 32 rows' statistics each, a word a lane: past the sequence's end zeros
+      const int rows = min(sq.len - t * kDenseTile, kDenseTile);
+      const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
+          (void*)(stats + h * p.rows + t * kDenseTile), (short)0, rows * 8, 0x00020000);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (TASFT_LDS void*)(st + 32 * wave), 4, wave * 256 + lane * 4, 0, 0, 0);
+    }
+  };
+
+  f32x16_t ka[X::DTILES], va[X::DTILES];
+#pragma unroll
+  for (int dt = 0; dt < X::DTILES; ++dt) ka[dt] = va[dt] = (f32x16_t){};
+  bool fix = false;
+
+  auto step = [&](const uint8_t* qa, const uint8_t* ga, const float2* sa, uint8_t* qb, uint8_t* gb, float2* sb_, int h,
+                  int t, int hn, int tn) TASFT_INLINE {
+    __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0)
+    dense_barrier();
+    if (hn >= 0) bring(qb, gb, sb_, hn, tn);
+    const float slope2 = BIAS ? p.sc.slopes[h] * kLog2e : 0.f;
+#pragma unroll
+    for (int t2 = 0; t2 < 2; ++t2) {
+      const int i0 = t * kDenseTile + 32 * t2;
+      if (i0 + 31 < any_from || i0 >= sq.len) continue;
+      const bool mixed = i0 < all_from;
+      f32x16_t s = X::rows_times(qa, 32 * t2, kf, col, half);
+      f32x16_t dp = X::rows_times(ga, 32 * t2, vf, col, half);
+      f32x16_t gate;
+      dense_scores<CAP, BIAS, true>(s, gate, p.sc, slope2, (float)(i0 + 4 * half - j));
+#pragma unroll
+      for (int rr = 0; rr < 16; ++rr) {
+        const float2 st = sa[32 * t2 + 4 * half + 8 * (rr >> 2) + (rr & 3)];
+        s[rr] = __builtin_amdgcn_exp2f(s[rr] - st.x);
+        dp[rr] = s[rr] * (dp[rr] - st.y);
+        if constexpr (CAP) dp[rr] *= 4.f * (gate[rr] - gate[rr] * gate[rr]);
+      }
+      if (mixed) {
+        const int from0 = from - i0 - 4 * half;
+#pragma unroll
+        for (int rr = 0; rr < 16; ++rr) {
+          const bool off = 8 * (rr >> 2) + (rr & 3) < from0;
+          s[rr] = off ? 0.f : s[rr];
+          dp[rr] = off ? 0.f : dp[rr];
+        }
+      }
+      u32x4_t pb[2], sb[2];
+#pragma unroll
+      for (int pp = 0; pp < 2; ++pp) {
+        pb[pp] = (u32x4_t){pack16x2<DT>(s[8 * pp], s[8 * pp + 1]), pack16x2<DT>(s[8 * pp + 2], s[8 * pp + 3]),
+                           pack16x2<DT>(s[8 * pp + 4], s[8 * pp + 5]), pack16x2<DT>(s[8 * pp + 6], s[8 * pp + 7])};
+        sb[pp] = (u32x4_t){pack16x2<DT>(dp[8 * pp], dp[8 * pp + 1]), pack16x2<DT>(dp[8 * pp + 2], dp[8 * pp + 3]),
+                           pack16x2<DT>(dp[8 * pp + 4], dp[8 * pp + 5]), pack16x2<DT>(dp[8 * pp + 6], dp[8 * pp + 7])};
+      }
+      fix |= X::columns_times(ga, 32 * t2, pb, mixed, va, lane);
+      fix |= X::columns_times(qa, 32 * t2, sb, mixed, ka, lane);
+    }
+  };
+  int h = g_first, t = t_first;
+  bring(q0_lds, g0_lds, st0_lds, h, t);
+  const int steps = heads * (t_end - t_first);
+  for (int done = 0; done < steps; done += 2) {
+    int hn = h, tn = t + 1;
+    if (tn == t_end) tn = t_first, ++hn;
+    step(q0_lds, g0_lds, st0_lds, q1_lds, g1_lds, st1_lds, h, t, done + 1 < steps ? hn : -1, tn);
+    if (done + 1 >= steps) break;
+    h = hn, t = tn + 1;
+    if (t == t_end) t = t_first, ++h;
+    step(q1_lds, g1_lds, st1_lds, q0_lds, g0_lds, st0_lds, hn, tn, done + 2 < steps ? h : -1, t);
+  }
+
+  if (fix) {
+    // Row by row, from memory, the rows before all_from (with the tiles' rows behind it).
+    const int end = min((all_from + 31) / 32 * 32, sq.len);
+#pragma nounroll
+    for (int gh = g_first; gh < g_first + heads; ++gh) {
+      const float slope2 = BIAS ? p.sc.slopes[gh] * kLog2e : 0.f;
+#pragma nounroll
+      for (int i = any_from / 32 * 32; i < end; ++i) {
+        const uint16_t* qr = dense_at(p.q, sq, i, gh);
+        const uint16_t* gr = dense_at(p.go, sq, i, gh);
+        const bool bad_q = X::has_nonfinite(qr, lane), bad_g = X::has_nonfinite(gr, lane);
+        if (!bad_q && !bad_g) continue;
+        const float2 st = stats[gh * p.rows + i];
+        float gate;
+        const float s = dense_score<CAP, BIAS>(X::dot(qr, kf, half), gate, p.sc, slope2, (float)(i - j));
+        const float pr = __builtin_amdgcn_exp2f(s - st.x);
+        float ds = pr * (X::dot(gr, vf, half) - st.y);
+        if constexpr (CAP) ds *= 4.f * (gate - gate * gate);
+        if (bad_g) X::add_nonfinite(va, gr, pr, row_ok && i >= from, half);
+        if (bad_q) X::add_nonfinite(ka, qr, ds, row_ok && i >= from, half);
+      }
+    }
+  }
+
+  if (p.SG > 1) {  // sums of these heads, joined by dense_join_kernel
+    if (!row_ok) return;
+    const int64_t at = (((int64_t)sg * p.rows + (int64_t)sq.b * p.T + sq.t0 + j) * p.Hkv + kvh) * D + 4 * half;
+#pragma unroll
+    for (int dt = 0; dt < X::DTILES; ++dt)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int d0 = dt * 32 + 8 * g;
+        *(f32x4_t*)(p.part_k + at + d0) = (f32x4_t){ka[dt][4 * g], ka[dt][4 * g + 1], ka[dt][4 * g + 2], ka[dt][4 * g + 3]};
+        *(f32x4_t*)(p.part_v + at + d0) = (f32x4_t){va[dt][4 * g], va[dt][4 * g + 1], va[dt][4 * g + 2], va[dt][4 * g + 3]};
+      }
+    return;
+  }
+  __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
+  dense_barrier();                     // every wave is done with the tiles
+  const int64_t kat = row_ok ? (int64_t)j * p.gk.s[1] : -1, vat = row_ok ? (int64_t)j * p.gv.s[1] : -1;
+  uint8_t* kst = ((wave & 2) ? q1_lds : q0_lds) + (wave & 1) * (32 * X::ROWB);
+  uint8_t* vst = ((wave & 2) ? g1_lds : g0_lds) + (wave & 1) * (32 * X::ROWB);
+  X::store(kst, ka, p.scale, dense_at(p.gk, sq, 0, kvh), kat, lane);
+  X::store(vst, va, 1.f, dense_at(p.gv, sq, 0, kvh), vat, lane);
+}
+
+// Joins the SG partial sums of every key's gradients: D / 4 lanes a row.
+template <int D, int DT>
+__global__ void __launch_bounds__(256) dense_join_kernel(const DenseParams p) {
+  constexpr int LPR = D / 4;
+  const int64_t row = ((int64_t)blockIdx.x * 256 + threadIdx.x) / LPR;
+  const int c = threadIdx.x % LPR;
+  const int64_t all = p.rows * p.Hkv;
+  if (row >= all) return;
+  const int64_t tok = row / p.Hkv;
+  const int kvh = (int)(row - tok * p.Hkv);
+  const int b = p.cu ? 0 : (int)(tok / p.T), t = p.cu ? (int)tok : (int)(tok - (int64_t)b * p.T);
+  // Rows that no workgroup computed are zeros already; their partial sums are not written. (A packed row
+  // that max_seqlen cuts off is found by its sequence.)
+  if (!p.cu) {
+    if (p.seq_lens && t >= p.seq_lens[b]) return;
+  } else {
+    int lo = 0, hi = p.N;  // the last sequence that starts at or before t
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) / 2;
+      (p.cu[mid] <= t ? lo : hi) = mid;
+    }
+    const int t0 = max(p.cu[lo], 0);
+    if (t >= min(p.cu[lo + 1], t0 + p.L) || t < t0) return;
+  }
+  const int64_t at = row * D + c * 4, step = all * D;
+  f32x4_t k = *(const f32x4_t*)(p.part_k + at), v = *(const f32x4_t*)(p.part_v + at);
+  for (int s = 1; s < p.SG; ++s) {
+    k += *(const f32x4_t*)(p.part_k + at + s * step);
+    v += *(const f32x4_t*)(p.part_v + at + s * step);
+  }
+  k *= p.scale;
+  *(u32x2_t*)(p.gk.p + b * p.gk.s[0] + (int64_t)t * p.gk.s[1] + kvh * p.gk.s[2] + c * 4) =
+      (u32x2_t){pack16x2<DT>(k[0], k[1]), pack16x2<DT>(k[2], k[3])};
+  *(u32x2_t*)(p.gv.p + b * p.gv.s[0] + (int64_t)t * p.gv.s[1] + kvh * p.gv.s[2] + c * 4) =
+      (u32x2_t){pack16x2<DT>(v[0], v[1]), pack16x2<DT>(v[2], v[3])};
+}
+
+}  // namespace tasft
+
+using namespace tasft;
+
+static int dense_rows(DenseRows& r, const char* what, const char* name, const void* ptr, const int64_t* s) {
+  if (!ptr || !s) return set_error(kErrInvalidArgument, "%s: null pointer argument", what);
+  if (!strides_nonneg(s, 4)) return set_error(kErrInvalidArgument, "%s: strides of %s must be non-negative", what, name);
+  if (s[3] != 1) return set_error(kErrInvalidArgument, "%s: head dims of %s must be contiguous", what, name);
+  if ((s[0] & 7) || (s[1] & 7) || (s[2] & 7) || ((uintptr_t)ptr & 15))
+    return set_error(kErrInvalidArgument, "%s: strides of %s must be multiples of 8 on a 16-byte aligned base", what, name);
+  if (s[2] >= (int64_t)1 << 24) return set_error(kErrUnsupported, "%s: token stride of %s too large", what, name);
+  r.p = (uint16_t*)ptr;
+  r.s[0] = s[0];
+  r.s[1] = s[2];
+  r.s[2] = s[1];
+  return kOk;
+}
+
+// Workgroups that share a KV head's query heads: a divisor of the group that gives four rounds of two
+// workgroups on every CU, so that causal rows of unequal length even out.
+static int dense_head_splits(int64_t num_seqs, int64_t num_kv_heads, int64_t group, int64_t max_seqlen) {
+  const int64_t wgs = num_seqs * num_kv_heads * ((max_seqlen + kDenseRows - 1) / kDenseRows);
+  int64_t sg = 1;
+  while (sg < group && (group % sg != 0 || wgs * sg < 2048)) ++sg;
+  return (int)sg;
+}
+
+extern "C" size_t tasft_dense_bwd_workspace_bytes(int64_t num_seqs, int64_t rows, int64_t num_q_heads,
+                                                  int64_t num_kv_heads, int64_t max_seqlen, int64_t head_dim) {
+  if (num_seqs <= 0 || rows <= 0 || num_q_heads <= 0 || num_kv_heads <= 0 || max_seqlen <= 0 || head_dim <= 0 ||
+      num_q_heads % num_kv_heads != 0)
+    return 0;
+  const int sg = dense_head_splits(num_seqs, num_kv_heads, num_q_heads / num_kv_heads, max_seqlen);
+  const size_t stats = ((size_t)rows * num_q_heads * 8 + 15) / 16 * 16;
+  return stats + (sg > 1 ? (size_t)sg * rows * num_kv_heads * head_dim * 8 : 0);
+}
+
+static int dense_params(DenseParams& p, const char* what, const int32_t* cu, const int32_t* seq_lens,
+                        const int32_t* prefix, const float* slopes, int64_t num_seqs, int64_t tokens,
+                        int64_t num_q_heads, int64_t num_kv_heads, int64_t max_seqlen, int64_t head_dim, float scale,
+                        float softcap, int causal, int dtype) {
+  if (dtype != kBf16 && dtype != kF16)
+    return set_error(kErrUnsupported, "%s: dtype must be bf16 (0) or fp16 (1), got %d", what, dtype);
+  if (num_seqs <= 0 || tokens <= 0 || num_q_heads <= 0 || num_kv_heads <= 0 || max_seqlen <= 0)
+    return set_error(kErrInvalidArgument, "%s: sizes must be positive", what);
+  if (num_q_heads % num_kv_heads != 0)
+    return set_error(kErrInvalidArgument, "%s: num_q_heads must be a multiple of num_kv_heads", what);
+  if (head_dim != 64 && head_dim != 128)
+    return set_error(kErrUnsupported, "%s: head_dim must be 64 or 128, got %lld", what, (long long)head_dim);
+  if (!(scale > 0.f) || !(softcap >= 0.f))
+    return set_error(kErrInvalidArgument, "%s: scale must be positive and softcap not negative", what);
+  if (cu && seq_lens) return set_error(kErrInvalidArgument, "%s: cu_seqlens or seq_lens, not both", what);
+  const int64_t lim = 0x7fffffff - 255;
+  if (num_seqs > lim || tokens > lim || num_q_heads > 65535 || (!cu && num_seqs * tokens > ((int64_t)1 << 40)))
+    return set_error(kErrUnsupported, "%s: sizes exceed 32 bits", what);
+  p.cu = cu;
+  p.seq_lens = seq_lens;
+  p.prefix = prefix;
+  p.sc = score_params(scale, softcap, slopes);
+  p.scale = scale;
+  p.rows = cu ? tokens : num_seqs * tokens;
+  p.N = (int)num_seqs;
+  p.T = (int)tokens;
+  p.Hq = (int)num_q_heads;
+  p.Hkv = (int)num_kv_heads;
+  p.G = (int)(num_q_heads / num_kv_heads);
+  p.L = (int)(max_seqlen < tokens && cu ? max_seqlen : tokens);
+  p.tiles = (p.L + kDenseRows - 1) / kDenseRows;
+  p.SG = 1;
+  p.causal = causal;
+  // Launches of fewer than 2^32 threads.
+  const int64_t most = 0xffffffffll / 256;
+  if (num_seqs * num_q_heads > most || num_seqs * num_q_heads * p.tiles > most ||
+      p.rows > most * 4 / num_kv_heads)
+    return set_error(kErrUnsupported, "%s: launch too large", what);
+  return kOk;
+}
+
+// Calls run(std::integral_constant D, DT, CAP, BIAS).
+template <class F>
+static void dense_dispatch(int64_t head_dim, int dtype, bool cap, bool bias, F&& run) {
+  auto with_bias = [&](auto d, auto dt, auto c) {
+    if (bias) run(d, dt, c, std::true_type{});
+    else run(d, dt, c, std::false_type{});
+  };
+  auto with_cap = [&](auto d, auto dt) {
+    if (cap) with_bias(d, dt, std::true_type{});
+    else with_bias(d, dt, std::false_type{});
+  };
+  auto with_dtype = [&](auto d) {
+    if (dtype == kF16) with_cap(d, std::integral_constant<int, kF16>{});
+    else with_cap(d, std::integral_constant<int, kBf16>{});
+  };
+  if (head_dim == 128) with_dtype(std::integral_constant<int, 128>{});
+  else with_dtype(std::integral_constant<int, 64>{});
+}
+
+extern "C" int tasft_dense_fwd(const void* q, const void* k, const void* v, void* out, float* lse,
+                               const int32_t* cu_seqlens, const int32_t* seq_lens, const int32_t* prefix_lens,
+                               const float* alibi_slopes, int64_t num_seqs, int64_t tokens, int64_t num_q_heads,
+                               int64_t num_kv_heads, int64_t max_seqlen, int64_t head_dim, const int64_t* q_strides,
+                               const int64_t* k_strides, const int64_t* v_strides, const int64_t* o_strides,
+                               const int64_t* lse_strides, float scale, float softcap, int causal, int dtype,
+                               void* stream) {
+  const char* what = "dense attention";
+  DenseParams p = {};
+  if (const int rc = dense_params(p, what, cu_seqlens, seq_lens, prefix_lens, alibi_slopes, num_seqs, tokens, num_q_heads,
+                                  num_kv_heads, max_seqlen, head_dim, scale, softcap, causal, dtype))
+    return rc;
+  if (const int rc = dense_rows(p.q, what, "q", q, q_strides)) return rc;
+  if (const int rc = dense_rows(p.k, what, "k", k, k_strides)) return rc;
+  if (const int rc = dense_rows(p.v, what, "v", v, v_strides)) return rc;
+  if (const int rc = dense_rows(p.o, what, "out", out, o_strides)) return rc;
+  if (lse && (!lse_strides || !strides_nonneg(lse_strides, 3)))
+    return set_error(kErrInvalidArgument, "dense attention: strides of lse must be non-negative");
+  p.lse = lse;
+  if (lse) p.sl[0] = lse_strides[0], p.sl[2] = lse_strides[1], p.sl[1] = lse_strides[2];
+  const dim3 grid((unsigned)((int64_t)p.N * p.Hq * p.tiles));
+  dense_dispatch(head_dim, dtype, softcap > 0.f, alibi_slopes != nullptr, [&](auto d, auto dt, auto c, auto b) {
+    hipLaunchKernelGGL((dense_fwd_kernel<d.value, dt.value, c.value, b.value>), grid, dim3(256), 0, (hipStream_t)stream, p);
+  });
+  return check_launch(what);
+}
+
+extern "C" int tasft_dense_bwd(const void* q, const void* k, const void* v, const void* out, const float* lse,
+                               const void* grad_out, const float* grad_lse, void* grad_q, void* grad_k, void* grad_v,
+                               void* workspace, size_t workspace_bytes, const int32_t* cu_seqlens,
+                               const int32_t* seq_lens, const int32_t* prefix_lens, const float* alibi_slopes,
+                               int64_t num_seqs, int64_t tokens, int64_t num_q_heads, int64_t num_kv_heads,
+                               int64_t max_seqlen, int64_t head_dim, const int64_t* q_strides, const int64_t* k_strides,
+                               const int64_t* v_strides, const int64_t* o_strides, const int64_t* lse_strides,
+                               const int64_t* go_strides, const int64_t* glse_strides, const int64_t* gq_strides,
+                               const int64_t* gk_strides, const int64_t* gv_strides, float scale, float softcap,
+                               int causal, int dtype, void* stream) {
+  const char* what = "dense attention backward";
+  DenseParams p = {};
+  if (const int rc = dense_params(p, what, cu_seqlens, seq_lens, prefix_lens, alibi_slopes, num_seqs, tokens, num_q_heads,
+                                  num_kv_heads, max_seqlen, head_dim, scale, softcap, causal, dtype))
+    return rc;
+  if (const int rc = dense_rows(p.q, what, "q", q, q_strides)) return rc;
+  if (const int rc = dense_rows(p.k, what, "k", k, k_strides)) return rc;
+  if (const int rc = dense_rows(p.v, what, "v", v, v_strides)) return rc;
+  if (const int rc = dense_rows(p.o, what, "out", out, o_strides)) return rc;
+  if (const int rc = dense_rows(p.go, what, "grad_out", grad_out, go_strides)) return rc;
+  if (const int rc = dense_rows(p.gq, what, "grad_q", grad_q, gq_strides)) return rc;
+  if (const int rc = dense_rows(p.gk, what, "grad_k", grad_k, gk_strides)) return rc;
+  if (const int rc = dense_rows(p.gv, what, "grad_v", grad_v, gv_strides)) return rc;
+  if (!lse || !lse_strides || (grad_lse && !glse_strides))
+    return set_error(kErrInvalidArgument, "dense attention backward: null pointer argument");
+  if (!strides_nonneg(lse_strides, 3) || (grad_lse && !strides_nonneg(glse_strides, 3)))
+    return set_error(kErrInvalidArgument, "dense attention backward: strides must be non-negative");
+  if (!workspace || workspace_bytes < tasft_dense_bwd_workspace_bytes(num_seqs, p.rows, num_q_heads, num_kv_heads, p.L,
+                                                                      head_dim))
+    return set_error(kErrWorkspace, "dense attention backward: workspace too small");
+  if ((uintptr_t)workspace & 15)
+    return set_error(kErrInvalidArgument, "dense attention backward: workspace must be 16-byte aligned");
+  p.lse = (float*)lse;
+  p.sl[0] = lse_strides[0], p.sl[2] = lse_strides[1], p.sl[1] = lse_strides[2];
+  p.glse = grad_lse;
+  if (grad_lse) p.sgl[0] = glse_strides[0], p.sgl[2] = glse_strides[1], p.sgl[1] = glse_strides[2];
+  p.SG = dense_head_splits(num_seqs, num_kv_heads, p.G, p.L);
+  p.stats = (float2*)workspace;
+  const size_t stats = ((size_t)p.rows * p.Hq * 8 + 15) / 16 * 16;
+  if (p.SG > 1) {
+    p.part_k = (float*)((uint8_t*)workspace + stats);
+    p.part_v = p.part_k + (int64_t)p.SG * p.rows * p.Hkv * head_dim;
+  }
+  const dim3 grid_q((unsigned)((int64_t)p.N * p.Hq * p.tiles)), grid_k((unsigned)((int64_t)p.N * p.Hkv * p.tiles * p.SG));
+  const hipStream_t st = (hipStream_t)stream;
+  dense_dispatch(head_dim, dtype, softcap > 0.f, alibi_slopes != nullptr, [&](auto d, auto dt, auto c, auto b) {
+    hipLaunchKernelGGL((dense_dq_kernel<d.value, dt.value, c.value, b.value>), grid_q, dim3(256), 0, st, p);
+    hipLaunchKernelGGL((dense_dkv_kernel<d.value, dt.value, c.value, b.value>), grid_k, dim3(256), 0, st, p);
+    if (p.SG > 1) {
+      const int64_t lanes = p.rows * p.Hkv * (d.value / 4);
+      hipLaunchKernelGGL((dense_join_kernel<d.value, dt.value>), dim3((unsigned)((lanes + 255) / 256)), dim3(256), 0, st, p);
+    }
+  });
+  return check_launch(what);
+}

@@ -10,6 +10,7 @@ from tasft_amd.kernels.block_sparse_fa import (
     indices_to_mask,
     mask_to_csr,
 )
+from tasft_amd.kernels.dense_attention import dense_attention
 from tasft_amd.kernels.kernel_config import KernelConfig, LayerKernelConfig
 from tasft_amd.kernels.paged_cache import accumulate_key_weights, append_paged, evict_paged
 from tasft_amd.kernels.rotary import apply_rotary, rotary_frequencies
@@ -25,6 +26,7 @@ __all__ = [
     "apply_rotary",
     "default_chunk_splits",
     "default_decode_splits",
+    "dense_attention",
     "detect_kernels",
     "evict_paged",
     "executed_blocks",
