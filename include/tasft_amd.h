@@ -563,6 +563,26 @@ int tasft_chunk_paged_fwd(
     int64_t block_table_stride, float scale, int causal, int dtype, void* stream);
 
 /*
+ * The same with capped or biased scores, or over a tree of new tokens. With s = q.k * scale:
+ * softcap tanh(s / softcap) if softcap > 0, then s - alibi_slopes[h] distance ([Hq] fp32, NULL: none), the
+ * distance between slots. ancestors (NULL: a chain): [T][ancestor_words] 64-bit words; token i of a chunk
+ * sees the keys before the chunk, and of the chunk's tokens j <= i those whose bit (j % 64 of word j / 64) is
+ * set; the distance is then between positions, a token's being the first new slot's plus the bits set in its
+ * row, less one. ancestors need causal and no block_mask, and a bit for each of max_seqlen tokens. The other
+ * arguments as above.
+ */
+int tasft_chunk_scored_fwd(
+    const void* q, const void* k_pages, const void* v_pages, void* out, float* lse,
+    const uint8_t* block_mask, const int32_t* block_table, const int32_t* kv_lens,
+    const int32_t* cu_seqlens, const float* alibi_slopes, const void* ancestors, int64_t ancestor_words,
+    void* workspace, size_t workspace_bytes, int64_t num_seqs, int64_t tokens, int64_t num_q_heads,
+    int64_t num_kv_heads, int64_t max_seqlen, int64_t head_dim, int64_t block_size, int64_t mask_rows,
+    int64_t page_size, int64_t num_pages, int64_t max_pages, int64_t num_splits, const int64_t* q_strides,
+    const int64_t* kp_strides, const int64_t* vp_strides, const int64_t* o_strides,
+    const int64_t* mask_strides, int64_t block_table_stride, float scale, float softcap, int causal, int dtype,
+    void* stream);
+
+/*
  * The attention weight that each cached key received from a chunk: scores_out[n, g, j] =
  * scores[n, g, j] (0 if NULL) + sum over the chunk's tokens and the query heads of KV head g
  * that see key j of exp(q.k_j * scale - lse), in a fixed order. No reference counterpart.
@@ -644,6 +664,40 @@ int tasft_dense_bwd(const void* q, const void* k, const void* v, const void* out
                     const int64_t* o_strides, const int64_t* lse_strides, const int64_t* go_strides,
                     const int64_t* glse_strides, const int64_t* gq_strides, const int64_t* gk_strides,
                     const int64_t* gv_strides, float scale, float softcap, int causal, int dtype, void* stream);
+
+/*
+ * Trees of drafted tokens (no reference counterpart). Sequence n's nodes are the packed tokens
+ * cu_seqlens[n] .. cu_seqlens[n + 1] - 1; parents holds each node's parent as an index within its
+ * sequence, smaller than its own (anything else: a root). At most max_nodes <= 4096 nodes of a tree are read.
+ *
+ * tasft_draft_tree: ancestors [tokens][ceil(max_nodes / 64)] 64-bit words, bit a % 64 of word a / 64 set for
+ * node a itself and its ancestors; positions[t] = kv_lens[n] - (nodes of n) + the number of ancestors. 0 for
+ * tokens that no tree has.
+ *
+ * tasft_draft_accept: a node is kept if its parent is and its token is targets[parent]; a root if
+ * first_targets is NULL or its token is first_targets[n]. path [num_seqs][max_nodes]: the nodes down to the
+ * deepest kept one (the lowest of several), -1 behind them; counts; next_tokens: targets[last], or where
+ * nothing is kept first_targets[n] (-1 if NULL). wide: 64-bit tokens, else 32-bit.
+ *
+ * tasft_draft_commit_paged: the keys and values of node path[n][j] go from slot start + path[n][j] to
+ * start + j, start = kv_lens[n] - (nodes of n), j < counts[n], in the pools and table of
+ * tasft_chunk_paged_fwd (16-bit, strides (page, token, head, d)); slot_positions ([N][Hkv][slots], NULL: none)
+ * alike; kv_lens_out[n] = start + counts[n]. max_nodes: the width of path. An index below its place or no
+ * node's, a slot outside the table and a page outside the pool are not moved.
+ */
+int tasft_draft_tree(const int32_t* parents, const int32_t* cu_seqlens, const int32_t* kv_lens,
+                     void* ancestors, int32_t* positions, int64_t num_seqs, int64_t tokens,
+                     int64_t max_nodes, void* stream);
+int tasft_draft_accept(const int32_t* parents, const void* draft_tokens, const void* targets,
+                       const void* first_targets, const int32_t* cu_seqlens, int32_t* path, int32_t* counts,
+                       void* next_tokens, int64_t num_seqs, int64_t tokens, int64_t max_nodes, int wide,
+                       void* stream);
+int tasft_draft_commit_paged(void* k_pages, void* v_pages, const int32_t* block_table, const int32_t* kv_lens,
+                             const int32_t* cu_seqlens, const int32_t* path, const int32_t* counts,
+                             int32_t* kv_lens_out, int32_t* slot_positions, int64_t num_seqs,
+                             int64_t max_nodes, int64_t num_kv_heads, int64_t head_dim, int64_t page_size,
+                             int64_t num_pages, int64_t max_pages, const int64_t* kp_strides,
+                             const int64_t* vp_strides, int64_t block_table_stride, void* stream);
 
 #ifdef __cplusplus
 }

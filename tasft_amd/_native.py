@@ -53,12 +53,16 @@ EXPORTED_SYMBOLS = (
     "tasft_rotary_append_paged",
     "tasft_chunk_workspace_bytes",
     "tasft_chunk_paged_fwd",
+    "tasft_chunk_scored_fwd",
     "tasft_key_weights",
     "tasft_evict_workspace_bytes",
     "tasft_evict_paged",
     "tasft_dense_fwd",
     "tasft_dense_bwd_workspace_bytes",
     "tasft_dense_bwd",
+    "tasft_draft_tree",
+    "tasft_draft_accept",
+    "tasft_draft_commit_paged",
 )
 
 _lock = threading.Lock()
@@ -164,6 +168,11 @@ _SIGNATURES: dict[str, tuple[object, list[object]]] = {
         [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _SZ, _I64, _I64, _I64, _I64, _I64, _I64, _I64,
          _I64, _I64, _I64, _I64, _I64, _I64P, _I64P, _I64P, _I64P, _I64P, _I64, _F, _I, _I, _P],
     ),
+    "tasft_chunk_scored_fwd": (
+        _I,
+        [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I64, _P, _SZ, _I64, _I64, _I64, _I64, _I64, _I64, _I64,
+         _I64, _I64, _I64, _I64, _I64, _I64P, _I64P, _I64P, _I64P, _I64P, _I64, _F, _F, _I, _I, _P],
+    ),
     "tasft_key_weights": (
         _I,
         [_P, _P, _P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64,
@@ -185,6 +194,12 @@ _SIGNATURES: dict[str, tuple[object, list[object]]] = {
         _I,
         [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _SZ, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64,
          _I64, _I64P, _I64P, _I64P, _I64P, _I64P, _I64P, _I64P, _I64P, _I64P, _I64P, _F, _F, _I, _I, _P],
+    ),
+    "tasft_draft_tree": (_I, [_P, _P, _P, _P, _P, _I64, _I64, _I64, _P]),
+    "tasft_draft_accept": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I, _P]),
+    "tasft_draft_commit_paged": (
+        _I,
+        [_P, _P, _P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64P, _I64P, _I64, _P],
     ),
 }
 

@@ -16,7 +16,7 @@ HERE = Path(__file__).resolve().parent
 OUT_DIR = HERE.parent / "_lib"
 LIB_NAME = "libtasft_amd.so"
 SOURCES = ["capi.cpp", "prefill.hip", "decode.hip", "gate.hip", "gate_grads.hip", "gate_target.hip", "mask.hip",
-           "rotary.hip", "chunk.hip", "evict.hip", "dense.hip"]
+           "rotary.hip", "chunk.hip", "evict.hip", "dense.hip", "draft.hip"]
 ARCH = "gfx950"
 
 

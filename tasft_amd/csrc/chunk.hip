@@ -36,7 +36,7 @@
 // priority during the products (2% slower dense, 2% faster masked).
 #include <type_traits>
 
-#include "common.h"
+#include "scores.h"
 
 #include "../../include/tasft_amd.h"
 
@@ -71,6 +71,9 @@ struct ChunkParams {
   int QT, P;                     // row tiles per sequence and KV head (or head), key splits
   float scale_log2;
   int causal;
+  ScoreParams sc;            // SCORED: a cap (cap_out not 0) and slopes, or neither
+  const uint64_t* ancestors; // SCORED: [T][words] or null
+  int words;
 };
 
 // A sequence's chunk: its first token, length, cached keys and first position. A length past the table
@@ -168,11 +171,16 @@ constexpr int kMaskTile = 64;  // positions of a masked one: two waves
 // long as the share). A template: the general form's scalar registers spilled, at a fifth of the time.
 // MASK: kDense, kPositions (64 positions of a head), kRows (a mask, the dense form's rows).
 enum ChunkMask { kDense = 0, kPositions = 1, kRows = 2 };
-template <int D, int DT, int MASK, int PIECES>
+// SCORES: kPlain, kScored (capped or biased scores, by uniform branches: they are brought to units of log2
+// before their maximum), kTree (these, and the new tokens are the nodes of a tree).
+enum ChunkScores { kPlain = 0, kScored = 1, kTree = 2 };
+template <int D, int DT, int MASK, int PIECES, int SCORES>
 __global__ void __launch_bounds__(MASK == kPositions ? 128 : 256)
     __attribute__((amdgpu_waves_per_eu(D == 64 && MASK == kPositions ? 3 : 2, D == 64 && MASK == kPositions ? 3 : 2)))
 chunk_rows_kernel(const ChunkParams p) {
   constexpr bool MASKED = MASK == kPositions, ROWMASK = MASK == kRows;
+  constexpr bool SCORED = SCORES != kPlain, TREE = SCORES == kTree;
+  static_assert(!TREE || MASK == kDense, "a tree without a block mask");
   constexpr int WAVES = MASKED ? 2 : 4;
   constexpr int ROW_TILE = MASKED ? kMaskTile : kRowTile;
   static_assert(ROW_TILE == 32 * WAVES && (ROW_TILE & (ROW_TILE - 1)) == 0, "row tile");
@@ -245,7 +253,7 @@ chunk_rows_kernel(const ChunkParams p) {
   }
   // Keys a row sees: 0 .. lim. All rows of the wave see the keys to all_see, none one past any_see.
   const int lim = p.causal ? min(sq.p0 + i, sq.kv - 1) : sq.kv - 1;
-  const int all_see = p.causal ? min(sq.p0 + i_first, sq.kv - 1) : sq.kv - 1;
+  const int all_see = TREE ? min(sq.p0, sq.kv) - 1 : p.causal ? min(sq.p0 + i_first, sq.kv - 1) : sq.kv - 1;
   const int any_see = !wave_on ? -1 : (p.causal ? min(sq.p0 + i_last, sq.kv - 1) : sq.kv - 1);
   const int wg_see = p.causal ? min(sq.p0 + i_end, sq.kv - 1) : sq.kv - 1;
   const int tiles = wg_see < 0 ? 0 : wg_see / kTile + 1;
@@ -258,6 +266,87 @@ chunk_rows_kernel(const ChunkParams p) {
 #pragma unroll
     for (int ks = 0; ks < KSTEPS; ++ks) qf[ks] = *(const u32x4_t*)(qr + ks * 16);
   }
+
+  // A tree's row: its node's words of ancestors (bit a of word w: node 64 w + a), and where the node is.
+  const uint64_t* words = nullptr;
+  float pos = 0.f, slope2 = 0.f;
+  if constexpr (SCORED) {
+    if (p.sc.slopes) {
+      slope2 = p.sc.slopes[h] * kLog2e;
+      pos = (float)(sq.p0 + i);
+    }
+    if constexpr (TREE) {
+      words = p.ancestors + (int64_t)(sq.t0 + i) * p.words;
+      if (p.sc.slopes) {
+        int above = -1;
+        for (int w = 0; w < p.words; ++w) above += __popcll(words[w]);
+        pos = (float)(sq.p0 + above);
+      }
+    }
+  }
+  // The keys key0 .. key0 + 63 that a tree's row sees, of those that are nodes (bits of the tile).
+  auto nodes_seen = [&](int key0) TASFT_INLINE -> uint64_t {
+    const int rel = key0 - sq.p0;  // the node that the tile's first key is
+    if (rel <= -64) return 0;
+    const int w = max(rel, 0) >> 6, sh = rel & 63;
+    const uint64_t a = w < p.words ? words[w] : 0;
+    if (rel < 0) return a << -rel;
+    const uint64_t b = sh && w + 1 < p.words ? words[w + 1] : 0;
+    return sh ? a >> sh | b << (64 - sh) : a;
+  };
+  // How many of a tree's row's ancestors lie before a key.
+  auto nodes_before = [&](int key) TASFT_INLINE {
+    int count = 0;
+    for (int w = 0; w < p.words && 64 * w < key - sq.p0; ++w) {
+      const int n = key - sq.p0 - 64 * w;
+      count += __popcll(n < 64 ? words[w] & (((uint64_t)1 << n) - 1) : words[w]);
+    }
+    return count;
+  };
+  // Brings the scores of a tile to units of log2: capped, biased by the distance.
+  auto modify = [&](f32x16_t& s0, f32x16_t& s1, int key0, bool mixed) TASFT_INLINE {
+    if (p.sc.cap_out != 0.f) {
+#pragma unroll
+      for (int rr = 0; rr < 16; ++rr) {
+        const float g0 = cap_gate(s0[rr], p.sc), g1 = cap_gate(s1[rr], p.sc);
+        if (p.sc.cap_wide) {
+          s0[rr] = cap_score_wide(s0[rr], g0, p.sc);
+          s1[rr] = cap_score_wide(s1[rr], g1, p.sc);
+        } else {
+          s0[rr] = cap_score(s0[rr], g0, p.sc);
+          s1[rr] = cap_score(s1[rr], g1, p.sc);
+        }
+      }
+    } else {
+      s0 *= p.scale_log2;
+      s1 *= p.scale_log2;
+    }
+    if (!p.sc.slopes) return;
+    const float d = (float)(key0 + 4 * half) - pos;
+    if (TREE && mixed) {
+      // A node's position is behind the cache by the number of its ancestors: of this row's, those with
+      // a lower bit.
+      const uint64_t bits = nodes_seen(key0);
+      const int before = nodes_before(key0);
+#pragma unroll
+      for (int rr = 0; rr < 16; ++rr) {
+        const int b0 = 4 * half + 8 * (rr >> 2) + (rr & 3), b1 = b0 + 32;
+        const int up0 = before + __popcll(bits & (((uint64_t)1 << b0) - 1));
+        const int up1 = before + __popcll(bits & (((uint64_t)1 << b1) - 1));
+        const float d0 = (float)(key0 + b0 < sq.p0 ? key0 + b0 : sq.p0 + up0) - pos;
+        const float d1 = (float)(key0 + b1 < sq.p0 ? key0 + b1 : sq.p0 + up1) - pos;
+        s0[rr] = fmaf(-slope2, fabsf(d0), s0[rr]);
+        s1[rr] = fmaf(-slope2, fabsf(d1), s1[rr]);
+      }
+      return;
+    }
+#pragma unroll
+    for (int rr = 0; rr < 16; ++rr) {
+      const float off = (float)(8 * (rr >> 2) + (rr & 3));
+      s0[rr] = fmaf(-slope2, fabsf(d + off), s0[rr]);
+      s1[rr] = fmaf(-slope2, fabsf(d + (off + 32.f)), s1[rr]);
+    }
+  };
 
   // The tiles of the split in order; masked: those that any row's block mask selects, with this
   // wave's own two bits (the 32-key halves, which differ at mask blocks of 32 only).
@@ -428,6 +517,19 @@ chunk_rows_kernel(const ChunkParams p) {
     const int key0 = kt * kTile;
     const int lim0 = MASK != kDense && !(own & 1) ? -1 : lim - key0 - 4 * half;
     const int lim1 = MASK != kDense && !(own & 2) ? -1 : lim - key0 - 4 * half - 32;
+    if constexpr (SCORED) modify(s0, s1, key0, mixed);
+    if (TREE && mixed) {
+      const int cached = sq.p0 - key0;  // keys of the tile before the tree
+      const uint64_t below = cached >= 64 ? ~(uint64_t)0 : cached > 0 ? ((uint64_t)1 << cached) - 1 : 0;
+      const uint64_t bits = (nodes_seen(key0) | below) >> (4 * half);
+      const uint32_t lo = (uint32_t)bits, hi = (uint32_t)(bits >> 32);
+#pragma unroll
+      for (int rr = 0; rr < 16; ++rr) {
+        const int off = 8 * (rr >> 2) + (rr & 3);
+        s0[rr] = lo >> off & 1 ? s0[rr] : -INFINITY;
+        s1[rr] = hi >> off & 1 ? s1[rr] : -INFINITY;
+      }
+    }
     if (mixed) {
 #pragma unroll
       for (int rr = 0; rr < 16; ++rr) {
@@ -442,7 +544,8 @@ chunk_rows_kernel(const ChunkParams p) {
       ma = fmaxf(fmaxf(ma, s0[rr]), s0[rr + 1]);
       mb = fmaxf(fmaxf(mb, s1[rr]), s1[rr + 1]);
     }
-    const float mloc = pair_max32(fmaxf(fmaxf(ma, s0[15]), fmaxf(mb, s1[15]))) * p.scale_log2;
+    float mloc = pair_max32(fmaxf(fmaxf(ma, s0[15]), fmaxf(mb, s1[15])));
+    if constexpr (!SCORED) mloc *= p.scale_log2;
     const bool move = mloc > m_ref + kChunkMove;
     if (__ballot(move)) {
       const float alpha = move ? __builtin_amdgcn_exp2f(m_ref - mloc) : 1.f;
@@ -455,8 +558,8 @@ chunk_rows_kernel(const ChunkParams p) {
     float lsum0 = 0.f, lsum1 = 0.f;
 #pragma unroll
     for (int rr = 0; rr < 16; ++rr) {
-      const float e0 = __builtin_amdgcn_exp2f(fmaf(s0[rr], p.scale_log2, -m_use));
-      const float e1 = __builtin_amdgcn_exp2f(fmaf(s1[rr], p.scale_log2, -m_use));
+      const float e0 = __builtin_amdgcn_exp2f(SCORED ? s0[rr] - m_use : fmaf(s0[rr], p.scale_log2, -m_use));
+      const float e1 = __builtin_amdgcn_exp2f(SCORED ? s1[rr] - m_use : fmaf(s1[rr], p.scale_log2, -m_use));
       s0[rr] = e0;
       s1[rr] = e1;
       lsum0 += e0;
@@ -621,6 +724,11 @@ chunk_rows_kernel(const ChunkParams p) {
         const uint8_t* m = pe->mask + n * pe->sm[0] + (int64_t)head * pe->sm[1] + row_own * pe->sm[2];
         sees = sees && m[(key >> pe->bs_shift) * pe->sm[3]] != 0;
       }
+      const bool node = TREE && key >= sq.p0;
+      if (node) {
+        const int a = key - sq.p0;
+        sees = sees && a < 64 * p.words && (words[a >> 6] >> (a & 63) & 1);
+      }
       const uint16_t* kr = pe->k + kvh * pe->sk[2] + page * pe->sk[0] + in_page * pe->sk[1] + half * 8;
       float dot = 0.f;
 #pragma unroll
@@ -631,7 +739,16 @@ chunk_rows_kernel(const ChunkParams p) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) dot = fmaf(x[j], y[j], dot);
       }
-      const float pk = __builtin_amdgcn_exp2f(fmaf(pair_sum32(dot), pe->scale_log2, -m_use));
+      float score = pair_sum32(dot);
+      if constexpr (SCORED) {
+        const float gate = cap_gate(score, p.sc);
+        score = p.sc.cap_out == 0.f ? score * p.scale_log2
+                : p.sc.cap_wide     ? cap_score_wide(score, gate, p.sc)
+                                    : cap_score(score, gate, p.sc);
+        // (A node's position is behind the cache by the number of its ancestors.)
+        if (p.sc.slopes) score = fmaf(-slope2, fabsf((float)(node ? sq.p0 + nodes_before(key) : key) - pos), score);
+      }
+      const float pk = __builtin_amdgcn_exp2f(SCORED ? score - m_use : fmaf(score, pe->scale_log2, -m_use));
 #pragma unroll
       for (int dt = 0; dt < DTILES; ++dt)
 #pragma unroll
@@ -1189,21 +1306,24 @@ extern "C" size_t tasft_chunk_workspace_bytes(int64_t tokens, int64_t num_q_head
 // Rows of a workgroup that joins few splits.
 constexpr int join_rows(int64_t head_dim) { return 256 / (int)(head_dim / 4); }
 
-template <int D, int DT>
+template <int D, int DT, int SCORES>
 static int launch_chunk(const ChunkParams& p, int mask, int64_t grid, hipStream_t stream) {
   auto run = [&](auto kernel) {
     hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(mask == kPositions ? 128 : 256), 0, stream, p);
   };
-  if (mask == kPositions) {
-    if (p.ps_shift >= 5) run(chunk_rows_kernel<D, DT, kPositions, 1>);
-    else if (p.ps_shift == 4) run(chunk_rows_kernel<D, DT, kPositions, 2>);
-    else run(chunk_rows_kernel<D, DT, kPositions, 4>);
+  if constexpr (SCORES == kTree) {
+    if (p.ps_shift >= 4) run(chunk_rows_kernel<D, DT, kDense, 1, SCORES>);
+    else run(chunk_rows_kernel<D, DT, kDense, 2, SCORES>);
+  } else if (mask == kPositions) {
+    if (p.ps_shift >= 5) run(chunk_rows_kernel<D, DT, kPositions, 1, SCORES>);
+    else if (p.ps_shift == 4) run(chunk_rows_kernel<D, DT, kPositions, 2, SCORES>);
+    else run(chunk_rows_kernel<D, DT, kPositions, 4, SCORES>);
   } else if (mask == kRows) {
-    if (p.ps_shift >= 4) run(chunk_rows_kernel<D, DT, kRows, 1>);
-    else run(chunk_rows_kernel<D, DT, kRows, 2>);
+    if (p.ps_shift >= 4) run(chunk_rows_kernel<D, DT, kRows, 1, SCORES>);
+    else run(chunk_rows_kernel<D, DT, kRows, 2, SCORES>);
   } else {
-    if (p.ps_shift >= 4) run(chunk_rows_kernel<D, DT, kDense, 1>);
-    else run(chunk_rows_kernel<D, DT, kDense, 2>);
+    if (p.ps_shift >= 4) run(chunk_rows_kernel<D, DT, kDense, 1, SCORES>);
+    else run(chunk_rows_kernel<D, DT, kDense, 2, SCORES>);
   }
   if (const int rc = check_launch("chunk attention")) return rc;
   if (p.P == 1) return kOk;
@@ -1218,16 +1338,15 @@ static int launch_chunk(const ChunkParams& p, int mask, int64_t grid, hipStream_
   return check_launch("chunk combine");
 }
 
-extern "C" int tasft_chunk_paged_fwd(
+static int chunk_run(
     const void* q, const void* k_pages, const void* v_pages, void* out, float* lse, const uint8_t* block_mask,
     const int32_t* block_table, const int32_t* kv_lens, const int32_t* cu_seqlens, void* workspace,
     size_t workspace_bytes, int64_t num_seqs, int64_t tokens, int64_t num_q_heads, int64_t num_kv_heads,
     int64_t max_seqlen, int64_t head_dim, int64_t block_size, int64_t mask_rows, int64_t page_size,
     int64_t num_pages, int64_t max_pages, int64_t num_splits, const int64_t* q_strides, const int64_t* kp_strides,
     const int64_t* vp_strides, const int64_t* o_strides, const int64_t* mask_strides, int64_t block_table_stride,
-    float scale, int causal, int dtype, void* stream) {
+    float scale, int causal, int dtype, void* stream, ChunkParams p, bool scored) {
   const char* what = "chunk attention";
-  ChunkParams p = {};
   if (!v_pages || !out || !vp_strides || !o_strides)
     return set_error(kErrInvalidArgument, "chunk attention: null pointer argument");
   if (const int rc = chunk_params(p, what, q, k_pages, block_mask, block_table, kv_lens, cu_seqlens, num_seqs, tokens,
@@ -1276,10 +1395,57 @@ extern "C" int tasft_chunk_paged_fwd(
     return set_error(kErrUnsupported, "chunk attention: launch too large");
   const int64_t grid = groups * each;
   const hipStream_t st = (hipStream_t)stream;
-  if (head_dim == 128)
-    return dtype == kF16 ? launch_chunk<128, kF16>(p, form, grid, st) : launch_chunk<128, kBf16>(p, form, grid, st);
-  return dtype == kF16 ? launch_chunk<64, kF16>(p, form, grid, st) : launch_chunk<64, kBf16>(p, form, grid, st);
+  if (scored) {
+    if (p.ancestors && (p.mask || !p.causal || (int64_t)p.words * 64 < p.L))
+      return set_error(kErrInvalidArgument, "chunk attention: ancestors need causal, no block mask and a bit a token");
+  }
+  auto launch = [&](auto scores) {
+    constexpr int S = decltype(scores)::value;
+    if (head_dim == 128)
+      return dtype == kF16 ? launch_chunk<128, kF16, S>(p, form, grid, st) : launch_chunk<128, kBf16, S>(p, form, grid, st);
+    return dtype == kF16 ? launch_chunk<64, kF16, S>(p, form, grid, st) : launch_chunk<64, kBf16, S>(p, form, grid, st);
+  };
+  if (p.ancestors) return launch(std::integral_constant<int, kTree>{});
+  return scored ? launch(std::integral_constant<int, kScored>{}) : launch(std::integral_constant<int, kPlain>{});
 }
+
+extern "C" int tasft_chunk_paged_fwd(
+    const void* q, const void* k_pages, const void* v_pages, void* out, float* lse, const uint8_t* block_mask,
+    const int32_t* block_table, const int32_t* kv_lens, const int32_t* cu_seqlens, void* workspace,
+    size_t workspace_bytes, int64_t num_seqs, int64_t tokens, int64_t num_q_heads, int64_t num_kv_heads,
+    int64_t max_seqlen, int64_t head_dim, int64_t block_size, int64_t mask_rows, int64_t page_size,
+    int64_t num_pages, int64_t max_pages, int64_t num_splits, const int64_t* q_strides, const int64_t* kp_strides,
+    const int64_t* vp_strides, const int64_t* o_strides, const int64_t* mask_strides, int64_t block_table_stride,
+    float scale, int causal, int dtype, void* stream) {
+  return chunk_run(q, k_pages, v_pages, out, lse, block_mask, block_table, kv_lens, cu_seqlens, workspace,
+                   workspace_bytes, num_seqs, tokens, num_q_heads, num_kv_heads, max_seqlen, head_dim, block_size,
+                   mask_rows, page_size, num_pages, max_pages, num_splits, q_strides, kp_strides, vp_strides, o_strides,
+                   mask_strides, block_table_stride, scale, causal, dtype, stream, ChunkParams{}, false);
+}
+
+extern "C" int tasft_chunk_scored_fwd(
+    const void* q, const void* k_pages, const void* v_pages, void* out, float* lse, const uint8_t* block_mask,
+    const int32_t* block_table, const int32_t* kv_lens, const int32_t* cu_seqlens, const float* alibi_slopes,
+    const void* ancestors, int64_t ancestor_words, void* workspace, size_t workspace_bytes, int64_t num_seqs,
+    int64_t tokens, int64_t num_q_heads, int64_t num_kv_heads, int64_t max_seqlen, int64_t head_dim,
+    int64_t block_size, int64_t mask_rows, int64_t page_size, int64_t num_pages, int64_t max_pages,
+    int64_t num_splits, const int64_t* q_strides, const int64_t* kp_strides, const int64_t* vp_strides,
+    const int64_t* o_strides, const int64_t* mask_strides, int64_t block_table_stride, float scale, float softcap,
+    int causal, int dtype, void* stream) {
+  if (!(scale > 0.f) || !(softcap >= 0.f))
+    return set_error(kErrInvalidArgument, "chunk attention: scale must be positive and softcap not negative");
+  if (ancestors && (ancestor_words <= 0 || ancestor_words > 1 << 20 || ((uintptr_t)ancestors & 7)))
+    return set_error(kErrInvalidArgument, "chunk attention: ancestors must be 8-byte aligned rows of 1 to 2^20 words");
+  ChunkParams p = {};
+  p.sc = score_params(scale, softcap, alibi_slopes);
+  p.ancestors = (const uint64_t*)ancestors;
+  p.words = ancestors ? (int)ancestor_words : 0;
+  return chunk_run(q, k_pages, v_pages, out, lse, block_mask, block_table, kv_lens, cu_seqlens, workspace,
+                   workspace_bytes, num_seqs, tokens, num_q_heads, num_kv_heads, max_seqlen, head_dim, block_size,
+                   mask_rows, page_size, num_pages, max_pages, num_splits, q_strides, kp_strides, vp_strides, o_strides,
+                   mask_strides, block_table_stride, scale, causal, dtype, stream, p, true);
+}
+
 
 template <int D, int DT>
 static void launch_weights(const WeightParams& w, hipStream_t stream) {

@@ -28,6 +28,7 @@ from torch.nn import functional
 
 from tasft_amd import _native
 from tasft_amd.exceptions import KernelError
+from tasft_amd.kernels.dense_attention import check_slopes, check_softcap
 from tasft_amd.kernels.paged_cache import check_batch, check_pools, chunk_mask, readable
 from tasft_amd.types import VALID_BLOCK_SIZES
 
@@ -634,9 +635,12 @@ class BlockSparseFlashAttention:
         causal: bool = True,
         return_lse: bool = False,
         num_splits: int | None = None,
+        softcap: float | None = None,
+        alibi_slopes: torch.Tensor | None = None,
+        ancestors: torch.Tensor | None = None,
     ) -> torch.Tensor | tuple[torch.Tensor, torch.Tensor]:
         """Attention of a chunk of new tokens of each sequence over its paged cache: a piece of a
-        long prompt, drafted tokens to be checked, or one token each. The cache already holds the
+        long prompt, drafted tokens (a chain or a tree) to be checked, or one token each. The cache already holds the
         new tokens (``append_paged``). The reference has no such call (its vLLM backend attends
         within the tokens of a call, ``tasft/inference/vllm_patch.py:172-176``).
 
@@ -657,6 +661,13 @@ class BlockSparseFlashAttention:
             causal: a token sees no key behind its own position.
             return_lse: also return the log-sum-exp of every row.
             num_splits: workgroups that share the keys of a row (default: enough to fill the GPU).
+            softcap: scores s = q . k / sqrt(D) become ``softcap * tanh(s / softcap)``, as in
+                ``dense_attention``.
+            alibi_slopes: ``[Hq]``: then ``s -= alibi_slopes[h] * distance``, between slots (so not over
+                a cache that ``evict_paged`` has thinned out), in a tree between its nodes' positions.
+            ancestors: ``[T, W]`` int64 bits of ``draft_tree``, ``64 * W >= max_seqlen``: the new tokens are the
+                nodes of a tree, and a token sees the cache before them, and of them itself and its
+                ancestors alone. With ``causal``, without ``block_mask``.
 
         Returns:
             ``[T, Hq, D]``: rows that see no key, and rows of tokens behind ``cu_seqlens[N]``, are
@@ -679,6 +690,16 @@ class BlockSparseFlashAttention:
         elif not 1 <= num_splits <= 1024:
             raise KernelError(f"num_splits must be in [1, 1024], got {num_splits}",
                               context={"num_splits": num_splits})
+        cap, slopes = check_softcap(softcap), check_slopes(alibi_slopes, H, dev)
+        if ancestors is not None:
+            if not causal or block_mask is not None:
+                raise ValueError("ancestors go with causal=True and without a block_mask")
+            if (ancestors.ndim != 2 or ancestors.shape[0] != T or 64 * ancestors.shape[1] < min(b.max_seqlen, T)
+                    or ancestors.dtype != torch.int64 or ancestors.device != dev):
+                raise KernelError(f"ancestors must be int64 of shape [{T}, W] on {dev} with a bit for each of "
+                                  f"max_seqlen={b.max_seqlen} tokens, got {ancestors.dtype} {tuple(ancestors.shape)} on "
+                                  f"{ancestors.device}", context={"ancestors": list(ancestors.shape)})
+            ancestors = ancestors.contiguous()
         q, k_pages, v_pages = readable(q), readable(k_pages), readable(v_pages)
         out = torch.empty_like(q) if q.is_contiguous() else torch.empty((T, H, D), dtype=q.dtype, device=dev)
         lse = torch.empty((T, H), dtype=torch.float32, device=dev) if return_lse else None
@@ -686,15 +707,20 @@ class BlockSparseFlashAttention:
             lib = _native.load_library()
             ws_bytes = lib.tasft_chunk_workspace_bytes(T, H, D, num_splits) if num_splits > 1 else 0
             workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
+            where = (q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr(), _native.ptr(lse),
+                     _native.ptr(mask), b.table.data_ptr(), b.kv_lens.data_ptr(), b.cu.data_ptr())
+            sizes = (_native.ptr(workspace), ws_bytes, b.num_seqs, T, H, Hkv, b.max_seqlen, D, self.block_size,
+                     0 if mask is None else mask.shape[2], b.page_size, k_pages.shape[0], b.max_pages, num_splits,
+                     _native.strides(q), _native.strides(k_pages), _native.strides(v_pages), _native.strides(out),
+                     None if mask is None else _native.strides(mask), b.table.stride(0), 1.0 / math.sqrt(D))
+            last = (1 if causal else 0, b.dtype, _native.stream_handle(dev))
             with _native.on_device(dev):
-                status = lib.tasft_chunk_paged_fwd(
-                    q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr(), _native.ptr(lse),
-                    _native.ptr(mask), b.table.data_ptr(), b.kv_lens.data_ptr(), b.cu.data_ptr(),
-                    _native.ptr(workspace), ws_bytes, b.num_seqs, T, H, Hkv, b.max_seqlen, D, self.block_size,
-                    0 if mask is None else mask.shape[2], b.page_size, k_pages.shape[0], b.max_pages, num_splits,
-                    _native.strides(q), _native.strides(k_pages), _native.strides(v_pages), _native.strides(out),
-                    None if mask is None else _native.strides(mask), b.table.stride(0), 1.0 / math.sqrt(D),
-                    1 if causal else 0, b.dtype, _native.stream_handle(dev))
+                if cap == 0.0 and slopes is None and ancestors is None:
+                    status = lib.tasft_chunk_paged_fwd(*where, *sizes, *last)
+                else:
+                    words = 0 if ancestors is None else ancestors.shape[1]
+                    status = lib.tasft_chunk_scored_fwd(*where, _native.ptr(slopes), _native.ptr(ancestors), words,
+                                                        *sizes, cap, *last)
             _native.check(status, "tasft_chunk_paged_fwd", {"tokens": T, "sequences": b.num_seqs})
         return (out, lse) if return_lse else out
 
