@@ -48,7 +48,8 @@ struct DenseParams {
   int64_t sl[3];
   const float* glse;  // or null
   int64_t sgl[3];
-  float2* stats;      // [head][row]: lse log2(e) and D
+  float* lse2;        // [head][row]: lse log2(e)
+  float* di;          // and D
   float* part_k;      // [SG][row][Hkv][D], or null
   float* part_v;
   const int32_t* cu;        // packed, or null
@@ -86,8 +87,18 @@ __device__ __forceinline__ DenseSeq dense_seq(const DenseParams& p, int n) {
   return s;
 }
 
-__device__ __forceinline__ uint16_t* dense_at(const DenseRows& r, const DenseSeq& s, int i, int h) {
+template <class R>
+__device__ __forceinline__ uint16_t* dense_at(R& r, const DenseSeq& s, int i, int h) {
   return r.p + s.b * r.s[0] + (int64_t)(s.t0 + i) * r.s[1] + h * r.s[2];
+}
+
+// The kernel's argument read again: what only the end of a kernel uses is not kept in scalar registers over
+// its main loop (they spilled).
+typedef const __attribute__((address_space(4))) DenseParams* DenseParamsPtr;
+__device__ __forceinline__ DenseParamsPtr dense_params_again() {
+  DenseParamsPtr p = (DenseParamsPtr)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  return p;
 }
 
 // Rows of a head that no sequence has: those behind its length in tile `tile` of the workgroup's
@@ -131,7 +142,7 @@ __device__ __forceinline__ uint32_t dense_finite2(uint32_t w) {
 
 typedef uint16_t dense_u16x2_t __attribute__((ext_vector_type(2)));
 
-// What a wave does with the tiles of 64 rows in LDS. A tile's share of a wave: 16 rows.
+// What one of four waves does with the tiles of 64 rows in LDS.
 template <int D, int DT>
 struct DenseTiles {
   static constexpr int KSTEPS = D / 16;
@@ -139,91 +150,124 @@ struct DenseTiles {
   static constexpr int ROWB = D * 2;
   static constexpr int TILE = kDenseTile * ROWB;
   static constexpr int RPU = 1024 / ROWB;            // rows of a 1 KB DMA unit
-  static constexpr int UPW = kDenseTile / 4 / RPU;   // units of a wave's share
+  static constexpr int UPW = kDenseTile / 4 / RPU;  // units of a wave's share of the copying
   static constexpr int CPR = ROWB / 16;
 
-  // Byte offsets, from the tile's first row, of what a lane brings.
-  static __device__ __forceinline__ void offsets(int (&off)[UPW], int64_t stride, int wave, int lane) {
-#pragma unroll
-    for (int u = 0; u < UPW; ++u) {
-      const int row = wave * (kDenseTile / 4) + u * RPU + lane / CPR;
-      off[u] = (row * (int)stride + dense_swz<D>(row, lane % CPR) * 8) * 2;
+  // What a lane brings of a tile: its part of row `row` (of the first of the wave's units), in chunk `chunk`.
+  struct Share {
+    int row;    // in bytes, from the tile's first row
+    int chunk;
+    __device__ __forceinline__ Share(int64_t stride, int wave, int lane) {
+      const int r = wave * UPW * RPU + lane / CPR;
+      row = r * (int)stride * 2;
+      chunk = dense_swz<D>(r, lane % CPR);
     }
-  }
+  };
   // Rows `first` .. of a head's tensor into a tile; rows from `len` on arrive as zeros.
-  static __device__ __forceinline__ void dma(uint8_t* tile, const uint16_t* base, int64_t stride, const int (&off)[UPW],
-                                             int first, int len, int wave) {
+  static __device__ __forceinline__ void dma(uint8_t* tile, const uint16_t* base, int64_t stride, Share at, int first,
+                                             int len, int wave) {
     const int rows = min(len - first, kDenseTile);
     const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
         (void*)(base + (int64_t)first * stride), (short)0, rows > 0 ? (rows - 1) * (int)stride * 2 + ROWB : 0, 0x00020000);
+    asm volatile("" : "+v"(at.chunk));  // formed again for every tile: the units' offsets are not kept
 #pragma unroll
-    for (int u = 0; u < UPW; ++u)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (TASFT_LDS void*)(tile + (wave * UPW + u) * 1024), 16, off[u], 0, 0, 0);
+    for (int u = 0; u < UPW; ++u) {  // RPU rows on the swizzle changes by an exclusive or
+      const int off = at.row + u * RPU * (int)stride * 2 + ((at.chunk ^ (D == 128 ? u : 2 * u)) << 4);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (TASFT_LDS void*)(tile + (wave * UPW + u) * 1024), 16, off, 0, 0, 0);
+    }
   }
-  // Rows r0 .. r0 + 31 as the A operand, times b: 32 x 32 products.
-  static __device__ __forceinline__ f32x16_t rows_times(const uint8_t* tile, int r0, const u32x4_t (&b)[KSTEPS], int col,
-                                                        int half) {
-    u32x4_t a[KSTEPS];
-    const int r = r0 + col;
-#pragma unroll
-    for (int ks = 0; ks < KSTEPS; ++ks)
-      a[ks] = *(const u32x4_t*)(tile + r * ROWB + dense_swz<D>(r, ks * 2 + half) * 16);
+  // Where a lane reads in a tile. The swizzle moves 16-byte chunks by exclusive or within a row and repeats
+  // every 16 rows, so that every other place is this one with constants: xor within the row, plus whole rows.
+  struct Place {
+    int rows;     // row lane % 32, chunk lane / 32
+    int columns;  // row 4 (lane / 32) + (lane % 16) / 4, dims 16 (lane / 16 % 2) + 4 (lane % 4) .. + 3
+    __device__ __forceinline__ Place(int lane) {
+      const int col = lane & 31, half = lane >> 5, row = 4 * half + ((lane & 15) >> 2);
+      rows = col * ROWB + dense_swz<D>(col, half) * 16;
+      columns = row * ROWB + dense_swz<D>(row, 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) * 16 + (lane & 1) * 8;
+    }
+  };
+  // Rows r0 .. r0 + 31 as the A operand, times b: 32 x 32 products. PARTS > 1: for kernels short of registers;
+  // the operand is read in as many pieces, and its places are formed again for each use.
+  template <int PARTS = 1>
+  static __device__ __forceinline__ f32x16_t rows_times(const uint8_t* tile, int r0, const u32x4_t (&b)[KSTEPS], Place at) {
+    constexpr int N = KSTEPS / PARTS;
+    if (PARTS > 1) asm volatile("" : "+v"(at.rows));
     f32x16_t s = (f32x16_t){};
 #pragma unroll
-    for (int ks = 0; ks < KSTEPS; ++ks) s = mfma16<DT>(a[ks], b[ks], s);
+    for (int part = 0; part < PARTS; ++part) {
+      u32x4_t a[N];
+#pragma unroll
+      for (int k = 0; k < N; ++k)
+        a[k] = *(const u32x4_t*)(tile + (at.rows ^ (part * N + k) << 5) + r0 * ROWB);
+#pragma unroll
+      for (int k = 0; k < N; ++k) s = mfma16<DT>(a[k], b[part * N + k], s);
+      if (PARTS > 1) __builtin_amdgcn_sched_barrier(0);
+    }
     return s;
   }
   // acc [D x 32] += (rows r0 .. r0 + 31)^T b, b in the order of an accumulator's registers. With
-  // `mixed` infinities and NaN are left out; returns whether there was one.
-  static __device__ __forceinline__ bool columns_times(const uint8_t* tile, int r0, const u32x4_t (&b)[2], bool mixed,
-                                                       f32x16_t (&acc)[DTILES], int lane) {
-    const int grp16 = lane >> 4, t16 = lane & 15, tr_row = t16 >> 2, tr_cb = t16 & 3;
-    u32x2_t lo[2][DTILES], hi[2][DTILES];
+  // `mixed` infinities and NaN are left out, and noted in `found` (in LDS: as a value it had the compiler
+  // make a second copy of the loop for it, and spill).
+  template <int PARTS = 1>
+  static __device__ __forceinline__ void columns_times(const uint8_t* tile, int r0, const u32x4_t (&b)[2], bool mixed,
+                                                       f32x16_t (&acc)[DTILES], Place at, int* found) {
+    constexpr int N = 2 / PARTS;
+    if (PARTS > 1) asm volatile("" : "+v"(at.columns));
 #pragma unroll
-    for (int pp = 0; pp < 2; ++pp) {
-      const int r1 = r0 + 16 * pp + 4 * (grp16 >> 1) + tr_row, r2 = r1 + 8;
+    for (int part = 0; part < PARTS; ++part) {
+      u32x2_t lo[N][DTILES], hi[N][DTILES];
 #pragma unroll
-      for (int dt = 0; dt < DTILES; ++dt) {
-        const int d0 = dt * 32 + 16 * (grp16 & 1) + 4 * tr_cb;
-        const int cc = d0 >> 3, sub = (d0 & 7) * 2;
-        lo[pp][dt] = ds_read_tr16_b64((const void*)(tile + r1 * ROWB + dense_swz<D>(r1, cc) * 16 + sub));
-        hi[pp][dt] = ds_read_tr16_b64((const void*)(tile + r2 * ROWB + dense_swz<D>(r2, cc) * 16 + sub));
+      for (int e = 0; e < N; ++e) {
+        const uint8_t* from = tile + (r0 + 16 * (part * N + e)) * ROWB;
+#pragma unroll
+        for (int dt = 0; dt < DTILES; ++dt) {  // 8 rows on the swizzle's bit 1 changes too
+          lo[e][dt] = ds_read_tr16_b64((const void*)(from + (at.columns ^ dt << 6)));
+          hi[e][dt] = ds_read_tr16_b64((const void*)(from + (at.columns ^ (dt << 6 | 32)) + 8 * ROWB));
+        }
       }
-    }
-    bool found = false;
-    if (mixed) {
-      dense_u16x2_t top = {0, 0};  // the largest magnitudes tell whether there is one
+      if (mixed) {
+        asm volatile("");
+        dense_u16x2_t top = {0, 0};  // the largest magnitudes tell whether there is one
 #pragma unroll
-      for (int pp = 0; pp < 2; ++pp)
-#pragma unroll
-        for (int dt = 0; dt < DTILES; ++dt)
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            top = __builtin_elementwise_max(top, __builtin_bit_cast(dense_u16x2_t, lo[pp][dt][j] & 0x7fff7fffu));
-            top = __builtin_elementwise_max(top, __builtin_bit_cast(dense_u16x2_t, hi[pp][dt][j] & 0x7fff7fffu));
-          }
-      constexpr uint16_t E = DT == kF16 ? 0x7c00 : 0x7f80;
-      if (__ballot(top[0] >= E || top[1] >= E)) {
-        found = true;
-#pragma unroll
-        for (int pp = 0; pp < 2; ++pp)
+        for (int e = 0; e < N; ++e)
 #pragma unroll
           for (int dt = 0; dt < DTILES; ++dt)
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-              lo[pp][dt][j] = dense_finite2<DT>(lo[pp][dt][j]);
-              hi[pp][dt][j] = dense_finite2<DT>(hi[pp][dt][j]);
+              top = __builtin_elementwise_max(top, __builtin_bit_cast(dense_u16x2_t, lo[e][dt][j] & 0x7fff7fffu));
+              top = __builtin_elementwise_max(top, __builtin_bit_cast(dense_u16x2_t, hi[e][dt][j] & 0x7fff7fffu));
             }
+        constexpr uint16_t E = DT == kF16 ? 0x7c00 : 0x7f80;
+        if (__ballot(top[0] >= E || top[1] >= E)) {
+          *found = 1;
+#pragma unroll
+          for (int e = 0; e < N; ++e)
+#pragma unroll
+            for (int dt = 0; dt < DTILES; ++dt)
+#pragma unroll
+              for (int j = 0; j < 2; ++j) {
+                lo[e][dt][j] = dense_finite2<DT>(lo[e][dt][j]);
+                hi[e][dt][j] = dense_finite2<DT>(hi[e][dt][j]);
+              }
+        }
       }
+#pragma unroll
+      for (int e = 0; e < N; ++e)
+#pragma unroll
+        for (int dt = 0; dt < DTILES; ++dt) {
+          const u32x4_t a = {lo[e][dt][0], lo[e][dt][1], hi[e][dt][0], hi[e][dt][1]};
+          acc[dt] = mfma16<DT>(a, b[part * N + e], acc[dt]);
+        }
+      if (PARTS > 1) __builtin_amdgcn_sched_barrier(0);
     }
+  }
+  // The registers of a 32 x 32 product as the B operand of columns_times.
+  static __device__ __forceinline__ void pack(u32x4_t (&b)[2], const f32x16_t& s) {
 #pragma unroll
     for (int pp = 0; pp < 2; ++pp)
-#pragma unroll
-      for (int dt = 0; dt < DTILES; ++dt) {
-        const u32x4_t a = {lo[pp][dt][0], lo[pp][dt][1], hi[pp][dt][0], hi[pp][dt][1]};
-        acc[dt] = mfma16<DT>(a, b[pp], acc[dt]);
-      }
-    return found;
+      b[pp] = (u32x4_t){pack16x2<DT>(s[8 * pp], s[8 * pp + 1]), pack16x2<DT>(s[8 * pp + 2], s[8 * pp + 3]),
+                        pack16x2<DT>(s[8 * pp + 4], s[8 * pp + 5]), pack16x2<DT>(s[8 * pp + 6], s[8 * pp + 7])};
   }
   // A wave's 32 rows of the transposed accumulators times f, to `out` (row `col` at element `at`, < 0:
   // not there), whole rows through 32 rows of LDS of its own.
@@ -265,45 +309,60 @@ struct DenseTiles {
     }
     return pair_sum32(sum);
   }
-  // acc += w (the infinities and NaN of a row), for the lanes with `sees`.
-  static __device__ __forceinline__ void add_nonfinite(f32x16_t (&acc)[DTILES], const uint16_t* row, float w, bool sees,
-                                                       int half) {
-#pragma unroll
-    for (int dt = 0; dt < DTILES; ++dt) {
-      asm volatile("" ::: "memory");  // not all loads at once: they would take the main loop's registers
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const uint32_t x = row[dt * 32 + 8 * (e >> 2) + 4 * half + (e & 3)];
-        acc[dt][e] += sees && dense_finite2<DT>(x) != x ? w * bits16_to_f32<DT>(x) : 0.f;
-      }
-    }
-  }
   static __device__ __forceinline__ bool has_nonfinite(const uint16_t* row, int lane) {
     const uint32_t w = *(const uint32_t*)(row + (lane * 2) % D);
     return __ballot(dense_finite2<DT>(w) != w) != 0;
   }
 };
 
-// Scores in units of log2 from the products s of 32 rows; distance of register rr: |d + off(rr)|. gate
-// holds what the cap's derivative needs.
-template <bool CAP, bool BIAS, bool GATE>
-__device__ __forceinline__ void dense_scores(f32x16_t& s, f32x16_t& gate, const ScoreParams& sc, float slope2, float d) {
-  if constexpr (CAP) {
+// What follows the last tile where infinities or NaN were left out of a product: they are added to the stored
+// results, key by key, from memory, for the rows that see them. (The sum is infinite or NaN, whatever its
+// finite part; where another tile had them in its product, once more changes nothing.) Rolled loops: in the
+// registers of the main loop's sums this took hundreds of spills there.
+template <int D, int DT>
+__device__ __forceinline__ float dense_dot(const uint16_t* a, const uint16_t* b) {
+  float sum = 0.f;
+#pragma nounroll
+  for (int c = 0; c < D; c += 2) {
+    const uint32_t x = *(const uint32_t*)(a + c), y = *(const uint32_t*)(b + c);
+    sum = fmaf(bits16_to_f32<DT>(x & 0xffffu), bits16_to_f32<DT>(y & 0xffffu), sum);
+    sum = fmaf(bits16_to_f32<DT>(x >> 16), bits16_to_f32<DT>(y >> 16), sum);
+  }
+  return sum;
+}
+// out (16-bit, or fp32 sums) += w x where x is infinite or NaN.
+template <int D, int DT, class T>
+__device__ __forceinline__ void dense_patch(T* out, const uint16_t* x, float w, int half) {
+#pragma nounroll
+  for (int d = half * (D / 2); d < (half + 1) * (D / 2); ++d) {
+    const uint32_t b = x[d];
+    if (dense_finite2<DT>(b) == b) continue;
+    if constexpr (sizeof(T) == 2) out[d] = f32_to16<DT>(bits16_to_f32<DT>(out[d]) + w * bits16_to_f32<DT>(b));
+    else out[d] += w * bits16_to_f32<DT>(b);
+  }
+}
+
+// For each of the products s of 32 rows f(register, score in units of log2, derivative of the cap), into s.
+// Distance of register rr: |d + off(rr)|.
+template <bool CAP, bool BIAS, class F>
+__device__ __forceinline__ void dense_weights(f32x16_t& s, const ScoreParams& sc, float slope2, float d, F&& f) {
+  auto each = [&](auto score) TASFT_INLINE {
 #pragma unroll
     for (int rr = 0; rr < 16; ++rr) {
-      const float r = cap_gate(s[rr], sc);
-      if constexpr (GATE) gate[rr] = r;
-      if (sc.cap_wide) s[rr] = cap_score_wide(s[rr], r, sc);
-      else s[rr] = cap_score(s[rr], r, sc);
+      float g = 1.f, x;
+      if constexpr (CAP) {
+        const float r = cap_gate(s[rr], sc);
+        x = score(s[rr], r, sc);
+        g = 4.f * (r - r * r);
+      } else {
+        x = s[rr] * sc.scale_log2;
+      }
+      if constexpr (BIAS) x = fmaf(-slope2, fabsf(d + (float)(8 * (rr >> 2) + (rr & 3))), x);
+      s[rr] = f(rr, x, g);
     }
-  } else {
-#pragma unroll
-    for (int rr = 0; rr < 16; ++rr) s[rr] *= sc.scale_log2;
-  }
-  if constexpr (BIAS) {
-#pragma unroll
-    for (int rr = 0; rr < 16; ++rr) s[rr] = fmaf(-slope2, fabsf(d + (float)(8 * (rr >> 2) + (rr & 3))), s[rr]);
-  }
+  };
+  if (CAP && sc.cap_wide) each([](float a, float r, const ScoreParams& q) { return cap_score_wide(a, r, q); });
+  else each([](float a, float r, const ScoreParams& q) { return cap_score(a, r, q); });
 }
 
 // One score as above.
@@ -326,9 +385,12 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
   __shared__ __attribute__((aligned(1024))) uint8_t v0_lds[X::TILE];
   __shared__ __attribute__((aligned(1024))) uint8_t k1_lds[X::TILE];
   __shared__ __attribute__((aligned(1024))) uint8_t v1_lds[X::TILE];
+  __shared__ int found;
   const int tid = threadIdx.x, lane = tid & 63;
+  if (tid == 0) found = 0;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 31, half = lane >> 5;
+  const typename X::Place place(lane);
   int64_t group;
   int member;
   xcd_group_map(blockIdx.x, (int64_t)p.N * p.Hkv, p.tiles * p.G, &group, &member);
@@ -355,9 +417,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
   const float slope2 = BIAS ? p.sc.slopes[h] * kLog2e : 0.f;
   const uint16_t* kbase = dense_at(p.k, sq, 0, kvh);
   const uint16_t* vbase = dense_at(p.v, sq, 0, kvh);
-  int koff[X::UPW], voff[X::UPW];
-  X::offsets(koff, p.k.s[1], wave, lane);
-  X::offsets(voff, p.v.s[1], wave, lane);
+  const typename X::Share koff(p.k.s[1], wave, lane), voff(p.v.s[1], wave, lane);
   auto bring = [&](uint8_t* kt, uint8_t* vt, int t) TASFT_INLINE {
     X::dma(kt, kbase, p.k.s[1], koff, t * kDenseTile, sq.len, wave);
     X::dma(vt, vbase, p.v.s[1], voff, t * kDenseTile, sq.len, wave);
@@ -367,7 +427,6 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
 #pragma unroll
   for (int dt = 0; dt < X::DTILES; ++dt) oacc[dt] = (f32x16_t){};
   float m_ref = -INFINITY, l_run = 0.f;
-  int fix_from = 0x7fffffff;  // first tile whose infinities or NaN of V were left out
 
   auto step = [&](const uint8_t* ka, const uint8_t* va, uint8_t* kb, uint8_t* vb, int t) TASFT_INLINE {
     __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0)
@@ -376,14 +435,15 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
     const int key0 = t * kDenseTile;
     if (key0 > any_see) return;
     const bool mixed = key0 + kDenseTile - 1 > all_see;
-    f32x16_t s0 = X::rows_times(ka, 0, qf, col, half), s1 = X::rows_times(ka, 32, qf, col, half);
-    f32x16_t none;
+    f32x16_t s0 = X::rows_times(ka, 0, qf, place), s1 = X::rows_times(ka, 32, qf, place);
     if constexpr (UNITS) {
       const float d = (float)(key0 + 4 * half - i);
-      dense_scores<CAP, BIAS, false>(s0, none, p.sc, slope2, d);
-      dense_scores<CAP, BIAS, false>(s1, none, p.sc, slope2, d + 32.f);
+      auto same = [](int, float x, float) { return x; };
+      dense_weights<CAP, BIAS>(s0, p.sc, slope2, d, same);
+      dense_weights<CAP, BIAS>(s1, p.sc, slope2, d + 32.f, same);
     }
     if (mixed) {
+      asm volatile("");  // a branch, no selections in other tiles
       const int lim0 = lim - key0 - 4 * half, lim1 = lim0 - 32;
 #pragma unroll
       for (int rr = 0; rr < 16; ++rr) {
@@ -419,13 +479,9 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
     l_run += sum0 + sum1;
 #pragma unroll
     for (int t2 = 0; t2 < 2; ++t2) {
-      const f32x16_t& sv = t2 ? s1 : s0;
       u32x4_t pb[2];
-#pragma unroll
-      for (int pp = 0; pp < 2; ++pp)
-        pb[pp] = (u32x4_t){pack16x2<DT>(sv[8 * pp], sv[8 * pp + 1]), pack16x2<DT>(sv[8 * pp + 2], sv[8 * pp + 3]),
-                           pack16x2<DT>(sv[8 * pp + 4], sv[8 * pp + 5]), pack16x2<DT>(sv[8 * pp + 6], sv[8 * pp + 7])};
-      if (X::columns_times(va, 32 * t2, pb, mixed, oacc, lane)) fix_from = min(fix_from, t);
+      X::pack(pb, t2 ? s1 : s0);
+      X::columns_times(va, 32 * t2, pb, mixed, oacc, place, &found);
     }
   };
   bring(k0_lds, v0_lds, 0);
@@ -435,28 +491,28 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
     step(k1_lds, v1_lds, k0_lds, v0_lds, t + 1);
   }
 
-  if (fix_from != 0x7fffffff) {
-    // Key by key, from memory, to the rows that see the key. (Where another tile had them in its
-    // product, once more changes nothing.)
-    const float m_use = m_ref == -INFINITY ? 0.f : m_ref;
-#pragma nounroll
-    for (int key = fix_from * kDenseTile; key <= any_see; ++key) {
-      const uint16_t* vr = vbase + (int64_t)key * p.v.s[1];
-      if (!X::has_nonfinite(vr, lane)) continue;
-      float gate;
-      const float s = dense_score<CAP, BIAS>(X::dot(kbase + (int64_t)key * p.k.s[1], qf, half), gate, p.sc, slope2,
-                                             (float)(key - i));
-      X::add_nonfinite(oacc, vr, __builtin_amdgcn_exp2f(s - m_use), row_ok && key <= lim, half);
-    }
-  }
-
+  const DenseParamsPtr pe = dense_params_again();
   const float l_tot = pair_sum32(l_run);
-  if (p.lse && row_ok && half == 0)
-    p.lse[sq.b * p.sl[0] + (sq.t0 + i) * p.sl[1] + h * p.sl[2]] = (m_ref + __builtin_amdgcn_logf(l_tot)) * kDenseLn2;
+  if (pe->lse && row_ok && half == 0)
+    pe->lse[sq.b * pe->sl[0] + (sq.t0 + i) * pe->sl[1] + h * pe->sl[2]] = (m_ref + __builtin_amdgcn_logf(l_tot)) * kDenseLn2;
   __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
   dense_barrier();                     // every wave is done with the tiles
   uint8_t* ost = ((wave & 2) ? v0_lds : k0_lds) + (wave & 1) * (32 * X::ROWB);
-  X::store(ost, oacc, 1.f / (l_tot > 0.f ? l_tot : 1.f), dense_at(p.o, sq, 0, h), row_ok ? (int64_t)i * p.o.s[1] : -1, lane);
+  X::store(ost, oacc, 1.f / (l_tot > 0.f ? l_tot : 1.f), dense_at(pe->o, sq, 0, h), row_ok ? (int64_t)i * pe->o.s[1] : -1, lane);
+
+  if (found) {
+    __threadfence();
+    const float lse2 = m_ref + __builtin_amdgcn_logf(l_tot);
+#pragma nounroll
+    for (int key = (all_see + 1) / kDenseTile * kDenseTile; key <= any_see; ++key) {
+      const uint16_t* vr = vbase + (int64_t)key * pe->v.s[1];
+      if (!X::has_nonfinite(vr, lane) || !row_ok || key > lim) continue;
+      float gate;
+      const float s = dense_score<CAP, BIAS>(dense_dot<D, DT>(dense_at(pe->q, sq, i, h), kbase + (int64_t)key * pe->k.s[1]),
+                                             gate, p.sc, slope2, (float)(key - i));
+      dense_patch<D, DT>(dense_at(pe->o, sq, i, h), vr, __builtin_amdgcn_exp2f(s - lse2), half);
+    }
+  }
 }
 
 // ------------------------------------------------------------------------- backward: queries
@@ -467,9 +523,12 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
   __shared__ __attribute__((aligned(1024))) uint8_t v0_lds[X::TILE];
   __shared__ __attribute__((aligned(1024))) uint8_t k1_lds[X::TILE];
   __shared__ __attribute__((aligned(1024))) uint8_t v1_lds[X::TILE];
+  __shared__ int found;
   const int tid = threadIdx.x, lane = tid & 63;
+  if (tid == 0) found = 0;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 31, half = lane >> 5;
+  const typename X::Place place(lane);
   int64_t group;
   int member;
   xcd_group_map(blockIdx.x, (int64_t)p.N * p.Hkv, p.tiles * p.G, &group, &member);
@@ -489,9 +548,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
 
   const uint16_t* kbase = dense_at(p.k, sq, 0, kvh);
   const uint16_t* vbase = dense_at(p.v, sq, 0, kvh);
-  int koff[X::UPW], voff[X::UPW];
-  X::offsets(koff, p.k.s[1], wave, lane);
-  X::offsets(voff, p.v.s[1], wave, lane);
+  const typename X::Share koff(p.k.s[1], wave, lane), voff(p.v.s[1], wave, lane);
   auto bring = [&](uint8_t* kt, uint8_t* vt, int t) TASFT_INLINE {
     X::dma(kt, kbase, p.k.s[1], koff, t * kDenseTile, sq.len, wave);
     X::dma(vt, vbase, p.v.s[1], voff, t * kDenseTile, sq.len, wave);
@@ -505,14 +562,16 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
   const float lse2 = p.lse[li] * kLog2e;
   float D_i = X::dot(dense_at(p.o, sq, i, h), gf, half);
   if (p.glse) D_i -= p.glse[sq.b * p.sgl[0] + (sq.t0 + i) * p.sgl[1] + h * p.sgl[2]];
-  if (row_ok && half == 0) p.stats[h * p.rows + (int64_t)sq.b * p.T + sq.t0 + i] = make_float2(lse2, D_i);
+  if (row_ok && half == 0) {
+    const int64_t at = h * p.rows + (int64_t)sq.b * p.T + sq.t0 + i;
+    p.lse2[at] = lse2;
+    p.di[at] = D_i;
+  }
   const float slope2 = BIAS ? p.sc.slopes[h] * kLog2e : 0.f;
 
   f32x16_t acc[X::DTILES];
 #pragma unroll
   for (int dt = 0; dt < X::DTILES; ++dt) acc[dt] = (f32x16_t){};
-  int fix_from = 0x7fffffff;
-
   auto step = [&](const uint8_t* ka, const uint8_t* va, uint8_t* kb, uint8_t* vb, int t) TASFT_INLINE {
     __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0)
     dense_barrier();
@@ -522,27 +581,19 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
       const int key0 = t * kDenseTile + 32 * t2;
       if (key0 > any_see) continue;
       const bool mixed = key0 + 31 > all_see;
-      f32x16_t s = X::rows_times(ka, 32 * t2, qf, col, half);
-      f32x16_t dp = X::rows_times(va, 32 * t2, gf, col, half);
-      f32x16_t gate;
-      dense_scores<CAP, BIAS, true>(s, gate, p.sc, slope2, (float)(key0 + 4 * half - i));
-#pragma unroll
-      for (int rr = 0; rr < 16; ++rr) {
-        float ds = __builtin_amdgcn_exp2f(s[rr] - lse2) * (dp[rr] - D_i);
-        if constexpr (CAP) ds *= 4.f * (gate[rr] - gate[rr] * gate[rr]);
-        s[rr] = ds;
-      }
+      f32x16_t s = X::rows_times(ka, 32 * t2, qf, place), dp = X::rows_times(va, 32 * t2, gf, place);
+      dense_weights<CAP, BIAS>(s, p.sc, slope2, (float)(key0 + 4 * half - i), [&](int rr, float x, float g) {
+        return __builtin_amdgcn_exp2f(x - lse2) * g * (dp[rr] - D_i);
+      });
       if (mixed) {
+        asm volatile("");  // a branch, no selections in other tiles
         const int lim0 = lim - key0 - 4 * half;
 #pragma unroll
         for (int rr = 0; rr < 16; ++rr) s[rr] = 8 * (rr >> 2) + (rr & 3) > lim0 ? 0.f : s[rr];
       }
       u32x4_t sb[2];
-#pragma unroll
-      for (int pp = 0; pp < 2; ++pp)
-        sb[pp] = (u32x4_t){pack16x2<DT>(s[8 * pp], s[8 * pp + 1]), pack16x2<DT>(s[8 * pp + 2], s[8 * pp + 3]),
-                           pack16x2<DT>(s[8 * pp + 4], s[8 * pp + 5]), pack16x2<DT>(s[8 * pp + 6], s[8 * pp + 7])};
-      if (X::columns_times(ka, 32 * t2, sb, mixed, acc, lane)) fix_from = min(fix_from, t);
+      X::pack(sb, s);
+      X::columns_times(ka, 32 * t2, sb, mixed, acc, place, &found);
     }
   };
   for (int t = 0; t < tiles; t += 2) {
@@ -551,23 +602,27 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
     step(k1_lds, v1_lds, k0_lds, v0_lds, t + 1);
   }
 
-  if (fix_from != 0x7fffffff) {
-#pragma nounroll
-    for (int key = fix_from * kDenseTile; key <= any_see; ++key) {
-      const uint16_t* kr = kbase + (int64_t)key * p.k.s[1];
-      if (!X::has_nonfinite(kr, lane)) continue;
-      float gate;
-      const float s = dense_score<CAP, BIAS>(X::dot(kr, qf, half), gate, p.sc, slope2, (float)(key - i));
-      float ds = __builtin_amdgcn_exp2f(s - lse2) * (X::dot(vbase + (int64_t)key * p.v.s[1], gf, half) - D_i);
-      if constexpr (CAP) ds *= 4.f * (gate - gate * gate);
-      X::add_nonfinite(acc, kr, ds, row_ok && key <= lim, half);
-    }
-  }
-
+  const DenseParamsPtr pe = dense_params_again();
   __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
   dense_barrier();                     // every wave is done with the tiles
   uint8_t* ost = ((wave & 2) ? v0_lds : k0_lds) + (wave & 1) * (32 * X::ROWB);
-  X::store(ost, acc, p.scale, dense_at(p.gq, sq, 0, h), row_ok ? (int64_t)i * p.gq.s[1] : -1, lane);
+  X::store(ost, acc, pe->scale, dense_at(pe->gq, sq, 0, h), row_ok ? (int64_t)i * pe->gq.s[1] : -1, lane);
+
+  if (found) {
+    __threadfence();
+#pragma nounroll
+    for (int key = (all_see + 1) / kDenseTile * kDenseTile; key <= any_see; ++key) {
+      const uint16_t* kr = kbase + (int64_t)key * pe->k.s[1];
+      if (!X::has_nonfinite(kr, lane) || !row_ok || key > lim) continue;
+      float gate;
+      const float s = dense_score<CAP, BIAS>(dense_dot<D, DT>(dense_at(pe->q, sq, i, h), kr), gate, p.sc, slope2,
+                                             (float)(key - i));
+      float ds = __builtin_amdgcn_exp2f(s - lse2) *
+                 (dense_dot<D, DT>(dense_at(pe->go, sq, i, h), vbase + (int64_t)key * pe->v.s[1]) - D_i);
+      if constexpr (CAP) ds *= 4.f * (gate - gate * gate);
+      dense_patch<D, DT>(dense_at(pe->gq, sq, i, h), kr, ds * pe->scale, half);
+    }
+  }
 }
 
 // ---------------------------------------------------------------------------- backward: keys
@@ -578,10 +633,13 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
   __shared__ __attribute__((aligned(1024))) uint8_t g0_lds[X::TILE];
   __shared__ __attribute__((aligned(1024))) uint8_t q1_lds[X::TILE];
   __shared__ __attribute__((aligned(1024))) uint8_t g1_lds[X::TILE];
-  __shared__ __attribute__((aligned(1024))) float2 st0_lds[kDenseTile], st1_lds[kDenseTile];
+  __shared__ __attribute__((aligned(1024))) float st0_lds[2][kDenseTile], st1_lds[2][kDenseTile];  // lse, D
+  __shared__ int found;
   const int tid = threadIdx.x, lane = tid & 63;
+  if (tid == 0) found = 0;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 31, half = lane >> 5;
+  const typename X::Place place(lane);
   int64_t group;
   int member;
   xcd_group_map(blockIdx.x, (int64_t)p.N * p.Hkv, p.tiles * p.SG, &group, &member);
@@ -595,7 +653,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
     });
   const int r0 = tile * kDenseRows;
   if (r0 >= sq.len) return;
-  const int j_first = r0 + wave * 32, j_last = min(j_first + 31, sq.len - 1), j_end = min(r0 + kDenseRows, sq.len) - 1;
+  const int j_first = r0 + wave * 32, j_last = min(j_first + 31, sq.len - 1);
   const bool row_ok = j_first + col < sq.len;
   const int j = min(j_first + col, sq.len - 1);
   // The first query that sees a key. All of the wave's keys are seen by the rows from all_from on, none
@@ -604,76 +662,76 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
   const int from = seen_from(j), all_from = seen_from(j_last), any_from = j_first <= j_last ? seen_from(j_first) : 0x7fffffff;
   const int t_first = seen_from(r0) / kDenseTile, t_end = (sq.len - 1) / kDenseTile + 1;
   const int g_first = kvh * p.G + sg * (p.G / p.SG), heads = p.G / p.SG;
-  (void)j_end;
+
+  const typename X::Share qoff(p.q.s[1], wave, lane), goff(p.go.s[1], wave, lane);
+  const int64_t row0 = (int64_t)sq.b * p.T + sq.t0;
+  auto bring = [&](uint8_t* qt, uint8_t* gt, float (*st)[kDenseTile], int h, int t) TASFT_INLINE {
+    X::dma(qt, dense_at(p.q, sq, 0, h), p.q.s[1], qoff, t * kDenseTile, sq.len, wave);
+    X::dma(gt, dense_at(p.go, sq, 0, h), p.go.s[1], goff, t * kDenseTile, sq.len, wave);
+    if (wave < 2) {  // a row a lane; past the sequence's end zeros
+      const int rows = min(sq.len - t * kDenseTile, kDenseTile);
+      const float* from = (wave == 0 ? p.lse2 : p.di) + h * p.rows + row0 + t * kDenseTile;
+      const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)from, (short)0, rows * 4, 0x00020000);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (TASFT_LDS void*)st[wave], 4, lane * 4, 0, 0, 0);
+    }
+  };
+  bring(q0_lds, g0_lds, st0_lds, g_first, t_first);
 
   u32x4_t kf[X::KSTEPS], vf[X::KSTEPS];
   X::load_row(kf, dense_at(p.k, sq, j, kvh), half);
   X::load_row(vf, dense_at(p.v, sq, j, kvh), half);
-  int qoff[X::UPW], goff[X::UPW];
-  X::offsets(qoff, p.q.s[1], wave, lane);
-  X::offsets(goff, p.go.s[1], wave, lane);
-  const float2* stats = p.stats + (int64_t)sq.b * p.T + sq.t0;
-  auto bring = [&](uint8_t* qt, uint8_t* gt, float2* st, int h, int t) TASFT_INLINE {
-    X::dma(qt, dense_at(p.q, sq, 0, h), p.q.s[1], qoff, t * kDenseTile, sq.len, wave);
-    X::dma(gt, dense_at(p.go, sq, 0, h), p.go.s[1], goff, t * kDenseTile, sq.len, wave);
-    if (wave < 2) {  // 32 rows' statistics each, a word a lane: past the sequence's end zeros
-      const int rows = min(sq.len - t * kDenseTile, kDenseTile);
-      const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
-          (void*)(stats + h * p.rows + t * kDenseTile), (short)0, rows * 8, 0x00020000);
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (TASFT_LDS void*)(st + 32 * wave), 4, wave * 256 + lane * 4, 0, 0, 0);
-    }
-  };
-
   f32x16_t ka[X::DTILES], va[X::DTILES];
 #pragma unroll
   for (int dt = 0; dt < X::DTILES; ++dt) ka[dt] = va[dt] = (f32x16_t){};
-  bool fix = false;
-
-  auto step = [&](const uint8_t* qa, const uint8_t* ga, const float2* sa, uint8_t* qb, uint8_t* gb, float2* sb_, int h,
-                  int t, int hn, int tn) TASFT_INLINE {
+  auto step = [&](const uint8_t* qa, const uint8_t* ga, const float (*st)[kDenseTile], uint8_t* qb, uint8_t* gb,
+                  float (*stb)[kDenseTile], int h, int t, int hn, int tn) TASFT_INLINE {
     __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0)
     dense_barrier();
-    if (hn >= 0) bring(qb, gb, sb_, hn, tn);
+    if (hn >= 0) bring(qb, gb, stb, hn, tn);
     const float slope2 = BIAS ? p.sc.slopes[h] * kLog2e : 0.f;
 #pragma unroll
     for (int t2 = 0; t2 < 2; ++t2) {
       const int i0 = t * kDenseTile + 32 * t2;
       if (i0 + 31 < any_from || i0 >= sq.len) continue;
       const bool mixed = i0 < all_from;
-      f32x16_t s = X::rows_times(qa, 32 * t2, kf, col, half);
-      f32x16_t dp = X::rows_times(ga, 32 * t2, vf, col, half);
-      f32x16_t gate;
-      dense_scores<CAP, BIAS, true>(s, gate, p.sc, slope2, (float)(i0 + 4 * half - j));
+      const float* lse2 = st[0] + 32 * t2 + 4 * half;
+      const float* di = st[1] + 32 * t2 + 4 * half;
+      const int from0 = from - i0 - 4 * half;
+      // S, then dv, then dP, then dk: two of the four products' operands at a time. The registers hold no
+      // more beside dk, dv and the wave's K and V.
+      f32x16_t s = X::template rows_times<D == 128 ? 2 : 1>(qa, 32 * t2, kf, place);
+      u32x4_t b[2];
+      {
+        f32x16_t w;
+        dense_weights<CAP, BIAS>(s, p.sc, slope2, (float)(i0 + 4 * half - j), [&](int rr, float x, float g) {
+          w[rr] = __builtin_amdgcn_exp2f(x - lse2[8 * (rr >> 2) + (rr & 3)]);
+          return w[rr] * g;
+        });
+        if (mixed) {
+          asm volatile("");  // a branch, no selections in other tiles
 #pragma unroll
-      for (int rr = 0; rr < 16; ++rr) {
-        const float2 st = sa[32 * t2 + 4 * half + 8 * (rr >> 2) + (rr & 3)];
-        s[rr] = __builtin_amdgcn_exp2f(s[rr] - st.x);
-        dp[rr] = s[rr] * (dp[rr] - st.y);
-        if constexpr (CAP) dp[rr] *= 4.f * (gate[rr] - gate[rr] * gate[rr]);
-      }
-      if (mixed) {
-        const int from0 = from - i0 - 4 * half;
-#pragma unroll
-        for (int rr = 0; rr < 16; ++rr) {
-          const bool off = 8 * (rr >> 2) + (rr & 3) < from0;
-          s[rr] = off ? 0.f : s[rr];
-          dp[rr] = off ? 0.f : dp[rr];
+          for (int rr = 0; rr < 16; ++rr) w[rr] = 8 * (rr >> 2) + (rr & 3) < from0 ? 0.f : w[rr];
         }
+        X::pack(b, w);
       }
-      u32x4_t pb[2], sb[2];
+      __builtin_amdgcn_sched_barrier(0);
+      X::template columns_times<D == 128 ? 2 : 1>(ga, 32 * t2, b, mixed, va, place, &found);
+      __builtin_amdgcn_sched_barrier(0);
+      const f32x16_t dp = X::template rows_times<D == 128 ? 2 : 1>(ga, 32 * t2, vf, place);
 #pragma unroll
-      for (int pp = 0; pp < 2; ++pp) {
-        pb[pp] = (u32x4_t){pack16x2<DT>(s[8 * pp], s[8 * pp + 1]), pack16x2<DT>(s[8 * pp + 2], s[8 * pp + 3]),
-                           pack16x2<DT>(s[8 * pp + 4], s[8 * pp + 5]), pack16x2<DT>(s[8 * pp + 6], s[8 * pp + 7])};
-        sb[pp] = (u32x4_t){pack16x2<DT>(dp[8 * pp], dp[8 * pp + 1]), pack16x2<DT>(dp[8 * pp + 2], dp[8 * pp + 3]),
-                           pack16x2<DT>(dp[8 * pp + 4], dp[8 * pp + 5]), pack16x2<DT>(dp[8 * pp + 6], dp[8 * pp + 7])};
+      for (int rr = 0; rr < 16; ++rr) s[rr] *= dp[rr] - di[8 * (rr >> 2) + (rr & 3)];
+      if (mixed) {
+        asm volatile("");
+#pragma unroll
+        for (int rr = 0; rr < 16; ++rr) s[rr] = 8 * (rr >> 2) + (rr & 3) < from0 ? 0.f : s[rr];
       }
-      fix |= X::columns_times(ga, 32 * t2, pb, mixed, va, lane);
-      fix |= X::columns_times(qa, 32 * t2, sb, mixed, ka, lane);
+      X::pack(b, s);
+      __builtin_amdgcn_sched_barrier(0);
+      X::template columns_times<D == 128 ? 2 : 1>(qa, 32 * t2, b, mixed, ka, place, &found);
+      __builtin_amdgcn_sched_barrier(0);
     }
   };
   int h = g_first, t = t_first;
-  bring(q0_lds, g0_lds, st0_lds, h, t);
   const int steps = heads * (t_end - t_first);
   for (int done = 0; done < steps; done += 2) {
     int hn = h, tn = t + 1;
@@ -685,50 +743,62 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
     step(q1_lds, g1_lds, st1_lds, q0_lds, g0_lds, st0_lds, hn, tn, done + 2 < steps ? h : -1, t);
   }
 
-  if (fix) {
-    // Row by row, from memory, the rows before all_from (with the tiles' rows behind it).
+  const DenseParamsPtr pe = dense_params_again();
+  __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
+  dense_barrier();                     // every wave is done with the tiles
+  if (pe->SG > 1) {  // sums of these heads, joined by dense_join_kernel
+    if (row_ok) {
+      const int64_t at = (((int64_t)sg * pe->rows + row0 + j) * pe->Hkv + kvh) * D + 4 * half;
+#pragma unroll
+      for (int dt = 0; dt < X::DTILES; ++dt)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const int d0 = dt * 32 + 8 * g;
+          const f32x16_t &x = ka[dt], &y = va[dt];
+          *(f32x4_t*)(pe->part_k + at + d0) = (f32x4_t){x[4 * g], x[4 * g + 1], x[4 * g + 2], x[4 * g + 3]};
+          *(f32x4_t*)(pe->part_v + at + d0) = (f32x4_t){y[4 * g], y[4 * g + 1], y[4 * g + 2], y[4 * g + 3]};
+        }
+    }
+  } else {
+    uint8_t* kst = ((wave & 2) ? q1_lds : q0_lds) + (wave & 1) * (32 * X::ROWB);
+    uint8_t* vst = ((wave & 2) ? g1_lds : g0_lds) + (wave & 1) * (32 * X::ROWB);
+    X::store(kst, ka, pe->scale, dense_at(pe->gk, sq, 0, kvh), row_ok ? (int64_t)j * pe->gk.s[1] : -1, lane);
+    X::store(vst, va, 1.f, dense_at(pe->gv, sq, 0, kvh), row_ok ? (int64_t)j * pe->gv.s[1] : -1, lane);
+  }
+
+  if (found) {
+    __threadfence();
+    // The rows before all_from, with those behind it in the last 32 of them.
     const int end = min((all_from + 31) / 32 * 32, sq.len);
 #pragma nounroll
     for (int gh = g_first; gh < g_first + heads; ++gh) {
-      const float slope2 = BIAS ? p.sc.slopes[gh] * kLog2e : 0.f;
+      const float slope2 = BIAS ? pe->sc.slopes[gh] * kLog2e : 0.f;
 #pragma nounroll
       for (int i = any_from / 32 * 32; i < end; ++i) {
-        const uint16_t* qr = dense_at(p.q, sq, i, gh);
-        const uint16_t* gr = dense_at(p.go, sq, i, gh);
+        const uint16_t* qr = dense_at(pe->q, sq, i, gh);
+        const uint16_t* gr = dense_at(pe->go, sq, i, gh);
         const bool bad_q = X::has_nonfinite(qr, lane), bad_g = X::has_nonfinite(gr, lane);
         if (!bad_q && !bad_g) continue;
-        const float2 st = stats[gh * p.rows + i];
+        const float lse2 = pe->lse2[gh * pe->rows + row0 + i], di = pe->di[gh * pe->rows + row0 + i];
+        if (!row_ok || i < from) continue;
         float gate;
-        const float s = dense_score<CAP, BIAS>(X::dot(qr, kf, half), gate, p.sc, slope2, (float)(i - j));
-        const float pr = __builtin_amdgcn_exp2f(s - st.x);
-        float ds = pr * (X::dot(gr, vf, half) - st.y);
+        const float s = dense_score<CAP, BIAS>(dense_dot<D, DT>(qr, dense_at(pe->k, sq, j, kvh)), gate, p.sc, slope2,
+                                               (float)(i - j));
+        const float w = __builtin_amdgcn_exp2f(s - lse2);
+        float ds = w * (dense_dot<D, DT>(gr, dense_at(pe->v, sq, j, kvh)) - di);
         if constexpr (CAP) ds *= 4.f * (gate - gate * gate);
-        if (bad_g) X::add_nonfinite(va, gr, pr, row_ok && i >= from, half);
-        if (bad_q) X::add_nonfinite(ka, qr, ds, row_ok && i >= from, half);
+        const int64_t at = (((int64_t)sg * pe->rows + row0 + j) * pe->Hkv + kvh) * D;
+        if (bad_g) {
+          if (pe->SG > 1) dense_patch<D, DT>(pe->part_v + at, gr, w, half);
+          else dense_patch<D, DT>(dense_at(pe->gv, sq, j, kvh), gr, w, half);
+        }
+        if (bad_q) {
+          if (pe->SG > 1) dense_patch<D, DT>(pe->part_k + at, qr, ds, half);
+          else dense_patch<D, DT>(dense_at(pe->gk, sq, j, kvh), qr, ds * pe->scale, half);
+        }
       }
     }
   }
-
-  if (p.SG > 1) {  // sums of these heads, joined by dense_join_kernel
-    if (!row_ok) return;
-    const int64_t at = (((int64_t)sg * p.rows + (int64_t)sq.b * p.T + sq.t0 + j) * p.Hkv + kvh) * D + 4 * half;
-#pragma unroll
-    for (int dt = 0; dt < X::DTILES; ++dt)
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const int d0 = dt * 32 + 8 * g;
-        *(f32x4_t*)(p.part_k + at + d0) = (f32x4_t){ka[dt][4 * g], ka[dt][4 * g + 1], ka[dt][4 * g + 2], ka[dt][4 * g + 3]};
-        *(f32x4_t*)(p.part_v + at + d0) = (f32x4_t){va[dt][4 * g], va[dt][4 * g + 1], va[dt][4 * g + 2], va[dt][4 * g + 3]};
-      }
-    return;
-  }
-  __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
-  dense_barrier();                     // every wave is done with the tiles
-  const int64_t kat = row_ok ? (int64_t)j * p.gk.s[1] : -1, vat = row_ok ? (int64_t)j * p.gv.s[1] : -1;
-  uint8_t* kst = ((wave & 2) ? q1_lds : q0_lds) + (wave & 1) * (32 * X::ROWB);
-  uint8_t* vst = ((wave & 2) ? g1_lds : g0_lds) + (wave & 1) * (32 * X::ROWB);
-  X::store(kst, ka, p.scale, dense_at(p.gk, sq, 0, kvh), kat, lane);
-  X::store(vst, va, 1.f, dense_at(p.gv, sq, 0, kvh), vat, lane);
 }
 
 // Joins the SG partial sums of every key's gradients: D / 4 lanes a row.
@@ -929,7 +999,8 @@ extern "C" int tasft_dense_bwd(const void* q, const void* k, const void* v, cons
   p.glse = grad_lse;
   if (grad_lse) p.sgl[0] = glse_strides[0], p.sgl[2] = glse_strides[1], p.sgl[1] = glse_strides[2];
   p.SG = dense_head_splits(num_seqs, num_kv_heads, p.G, p.L);
-  p.stats = (float2*)workspace;
+  p.lse2 = (float*)workspace;
+  p.di = p.lse2 + p.rows * p.Hq;
   const size_t stats = ((size_t)p.rows * p.Hq * 8 + 15) / 16 * 16;
   if (p.SG > 1) {
     p.part_k = (float*)((uint8_t*)workspace + stats);
@@ -939,7 +1010,8 @@ extern "C" int tasft_dense_bwd(const void* q, const void* k, const void* v, cons
   const hipStream_t st = (hipStream_t)stream;
   dense_dispatch(head_dim, dtype, softcap > 0.f, alibi_slopes != nullptr, [&](auto d, auto dt, auto c, auto b) {
     hipLaunchKernelGGL((dense_dq_kernel<d.value, dt.value, c.value, b.value>), grid_q, dim3(256), 0, st, p);
-    hipLaunchKernelGGL((dense_dkv_kernel<d.value, dt.value, c.value, b.value>), grid_k, dim3(256), 0, st, p);
+    hipLaunchKernelGGL((dense_dkv_kernel<d.value, dt.value, c.value, b.value>), grid_k,
+                       dim3(256), 0, st, p);
     if (p.SG > 1) {
       const int64_t lanes = p.rows * p.Hkv * (d.value / 4);
       hipLaunchKernelGGL((dense_join_kernel<d.value, dt.value>), dim3((unsigned)((lanes + 255) / 256)), dim3(256), 0, st, p);
