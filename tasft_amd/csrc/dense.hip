@@ -33,6 +33,8 @@ namespace tasft {
 
 constexpr int kDenseRows = 128;  // rows that a workgroup owns
 constexpr int kDenseTile = 64;   // rows of a tile that it walks over
+constexpr int kDenseStep = 32;   // the same of the kernel of dk and dv
+constexpr int kDenseRun = 4;     // groups that an XCD takes at a time, see dense_place
 constexpr float kDenseMove = 8.f;  // a new maximum moves the exp2 reference only if this far above it
 constexpr float kDenseLn2 = 0.69314718055994531f;
 
@@ -92,6 +94,27 @@ __device__ __forceinline__ uint16_t* dense_at(R& r, const DenseSeq& s, int i, in
   return r.p + s.b * r.s[0] + (int64_t)(s.t0 + i) * r.s[1] + h * r.s[2];
 }
 
+// A workgroup's group and tile. A group's workgroups walk over the same tensors and share an XCD's L2
+// (workgroup i runs on XCD i % 8). Groups are as narrow as that allows (a query head, or the heads that a
+// workgroup of dk and dv takes), so that every XCD gets some of every sequence, turned by one in each eight: else
+// an XCD would get all first or all last heads. An XCD takes kDenseRun of its groups at a time, tile by tile: the
+// longest rows of all of them first (in another order for each tile: workgroups go round an XCD's shader engines,
+// and one would get the same group every time; ten documents, 28 / 4 heads: the kernel of dk and dv 2030 us
+// without that, 1470 with; one group at a time 1500, and one sequence of 8192 5% slower).
+struct DensePlace {
+  int group, tile;
+};
+__device__ __forceinline__ DensePlace dense_place(int64_t groups, int tiles) {
+  const int64_t idx = blockIdx.x;
+  const bool xcds = (groups & 7) == 0;
+  const int64_t j = xcds ? idx >> 3 : idx, each = xcds ? groups >> 3 : groups;  // of an XCD
+  const int64_t run = j / (kDenseRun * tiles), r = j - run * (kDenseRun * tiles);
+  const int here = (int)min((int64_t)kDenseRun, each - run * kDenseRun);
+  const int tile = (int)(r / here);
+  const int64_t g = run * kDenseRun + (r + tile) % here;
+  return {(int)(xcds ? 8 * g + ((idx + g) & 7) : g), tile};
+}
+
 // The kernel's argument read again: what only the end of a kernel uses is not kept in scalar registers over
 // its main loop (they spilled).
 typedef const __attribute__((address_space(4))) DenseParams* DenseParamsPtr;
@@ -142,15 +165,15 @@ __device__ __forceinline__ uint32_t dense_finite2(uint32_t w) {
 
 typedef uint16_t dense_u16x2_t __attribute__((ext_vector_type(2)));
 
-// What one of four waves does with the tiles of 64 rows in LDS.
-template <int D, int DT>
+// What one of four waves does with tiles of ROWS rows in LDS.
+template <int D, int DT, int ROWS>
 struct DenseTiles {
   static constexpr int KSTEPS = D / 16;
   static constexpr int DTILES = D / 32;
   static constexpr int ROWB = D * 2;
-  static constexpr int TILE = kDenseTile * ROWB;
+  static constexpr int TILE = ROWS * ROWB;
   static constexpr int RPU = 1024 / ROWB;            // rows of a 1 KB DMA unit
-  static constexpr int UPW = kDenseTile / 4 / RPU;  // units of a wave's share of the copying
+  static constexpr int UPW = ROWS / 4 / RPU;  // units of a wave's share of the copying
   static constexpr int CPR = ROWB / 16;
 
   // What a lane brings of a tile: its part of row `row` (of the first of the wave's units), in chunk `chunk`.
@@ -166,13 +189,13 @@ struct DenseTiles {
   // Rows `first` .. of a head's tensor into a tile; rows from `len` on arrive as zeros.
   static __device__ __forceinline__ void dma(uint8_t* tile, const uint16_t* base, int64_t stride, Share at, int first,
                                              int len, int wave) {
-    const int rows = min(len - first, kDenseTile);
+    const int rows = min(len - first, ROWS);
     const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
         (void*)(base + (int64_t)first * stride), (short)0, rows > 0 ? (rows - 1) * (int)stride * 2 + ROWB : 0, 0x00020000);
     asm volatile("" : "+v"(at.chunk));  // formed again for every tile: the units' offsets are not kept
 #pragma unroll
     for (int u = 0; u < UPW; ++u) {  // RPU rows on the swizzle changes by an exclusive or
-      const int off = at.row + u * RPU * (int)stride * 2 + ((at.chunk ^ (D == 128 ? u : 2 * u)) << 4);
+      const int off = at.row + u * RPU * (int)stride * 2 + ((at.chunk ^ ((D == 128 ? u : 2 * u) & 3)) << 4);
       __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (TASFT_LDS void*)(tile + (wave * UPW + u) * 1024), 16, off, 0, 0, 0);
     }
   }
@@ -203,6 +226,18 @@ struct DenseTiles {
 #pragma unroll
       for (int k = 0; k < N; ++k) s = mfma16<DT>(a[k], b[part * N + k], s);
       if (PARTS > 1) __builtin_amdgcn_sched_barrier(0);
+    }
+    return s;
+  }
+  // Rows r0 .. r0 + 31 as the A operand, times rows c0 .. c0 + 31 of another tile as the B operand.
+  static __device__ __forceinline__ f32x16_t rows_times_rows(const uint8_t* tile, int r0, const uint8_t* other, int c0,
+                                                             Place at) {
+    f32x16_t s = (f32x16_t){};
+#pragma unroll
+    for (int k = 0; k < KSTEPS; ++k) {
+      const u32x4_t a = *(const u32x4_t*)(tile + (at.rows ^ k << 5) + r0 * ROWB);
+      const u32x4_t b = *(const u32x4_t*)(other + (at.rows ^ k << 5) + c0 * ROWB);
+      s = mfma16<DT>(a, b, s);
     }
     return s;
   }
@@ -379,7 +414,7 @@ __device__ __forceinline__ float dense_score(float s, float& gate, const ScorePa
 // ------------------------------------------------------------------------------------ forward
 template <int D, int DT, bool CAP, bool BIAS>
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) dense_fwd_kernel(const DenseParams p) {
-  using X = DenseTiles<D, DT>;
+  using X = DenseTiles<D, DT, kDenseTile>;
   constexpr bool UNITS = CAP || BIAS;  // scores are in units of log2 before their maximum
   __shared__ __attribute__((aligned(1024))) uint8_t k0_lds[X::TILE];
   __shared__ __attribute__((aligned(1024))) uint8_t v0_lds[X::TILE];
@@ -391,12 +426,9 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 31, half = lane >> 5;
   const typename X::Place place(lane);
-  int64_t group;
-  int member;
-  xcd_group_map(blockIdx.x, (int64_t)p.N * p.Hkv, p.tiles * p.G, &group, &member);
-  const int n = (int)(group / p.Hkv), kvh = (int)(group % p.Hkv);
-  const int h = kvh * p.G + member % p.G;
-  const int tile = p.tiles - 1 - member / p.G;  // the longest rows first
+  const DensePlace at = dense_place((int64_t)p.N * p.Hq, p.tiles);
+  const int n = at.group / p.Hq, h = at.group % p.Hq, kvh = h / p.G;
+  const int tile = p.tiles - 1 - at.tile;  // the longest rows first
   const DenseSeq sq = dense_seq(p, n);
   dense_rest(p, sq, n, tile, tid, [&](int b, int t) {
     dense_clear<D>(p.o, b, t, h, tid);
@@ -518,7 +550,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
 // ------------------------------------------------------------------------- backward: queries
 template <int D, int DT, bool CAP, bool BIAS>
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) dense_dq_kernel(const DenseParams p) {
-  using X = DenseTiles<D, DT>;
+  using X = DenseTiles<D, DT, kDenseTile>;
   __shared__ __attribute__((aligned(1024))) uint8_t k0_lds[X::TILE];
   __shared__ __attribute__((aligned(1024))) uint8_t v0_lds[X::TILE];
   __shared__ __attribute__((aligned(1024))) uint8_t k1_lds[X::TILE];
@@ -529,12 +561,9 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 31, half = lane >> 5;
   const typename X::Place place(lane);
-  int64_t group;
-  int member;
-  xcd_group_map(blockIdx.x, (int64_t)p.N * p.Hkv, p.tiles * p.G, &group, &member);
-  const int n = (int)(group / p.Hkv), kvh = (int)(group % p.Hkv);
-  const int h = kvh * p.G + member % p.G;
-  const int tile = p.tiles - 1 - member / p.G;
+  const DensePlace at = dense_place((int64_t)p.N * p.Hq, p.tiles);
+  const int n = at.group / p.Hq, h = at.group % p.Hq, kvh = h / p.G;
+  const int tile = p.tiles - 1 - at.tile;
   const DenseSeq sq = dense_seq(p, n);
   dense_rest(p, sq, n, tile, tid, [&](int b, int t) { dense_clear<D>(p.gq, b, t, h, tid); });
   const int r0 = tile * kDenseRows;
@@ -563,9 +592,9 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
   float D_i = X::dot(dense_at(p.o, sq, i, h), gf, half);
   if (p.glse) D_i -= p.glse[sq.b * p.sgl[0] + (sq.t0 + i) * p.sgl[1] + h * p.sgl[2]];
   if (row_ok && half == 0) {
-    const int64_t at = h * p.rows + (int64_t)sq.b * p.T + sq.t0 + i;
-    p.lse2[at] = lse2;
-    p.di[at] = D_i;
+    const int64_t row = h * p.rows + (int64_t)sq.b * p.T + sq.t0 + i;
+    p.lse2[row] = lse2;
+    p.di[row] = D_i;
   }
   const float slope2 = BIAS ? p.sc.slopes[h] * kLog2e : 0.f;
 
@@ -628,23 +657,23 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
 // ---------------------------------------------------------------------------- backward: keys
 template <int D, int DT, bool CAP, bool BIAS>
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) dense_dkv_kernel(const DenseParams p) {
-  using X = DenseTiles<D, DT>;
+  using X = DenseTiles<D, DT, kDenseStep>;
+  using V = DenseTiles<D, DT, kDenseRows>;
   __shared__ __attribute__((aligned(1024))) uint8_t q0_lds[X::TILE];
   __shared__ __attribute__((aligned(1024))) uint8_t g0_lds[X::TILE];
   __shared__ __attribute__((aligned(1024))) uint8_t q1_lds[X::TILE];
   __shared__ __attribute__((aligned(1024))) uint8_t g1_lds[X::TILE];
-  __shared__ __attribute__((aligned(1024))) float st0_lds[2][kDenseTile], st1_lds[2][kDenseTile];  // lse, D
+  __shared__ __attribute__((aligned(1024))) uint8_t v_lds[V::TILE];
+  __shared__ __attribute__((aligned(1024))) float st0_lds[2][kWave], st1_lds[2][kWave];  // lse, D
   __shared__ int found;
   const int tid = threadIdx.x, lane = tid & 63;
   if (tid == 0) found = 0;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 31, half = lane >> 5;
   const typename X::Place place(lane);
-  int64_t group;
-  int member;
-  xcd_group_map(blockIdx.x, (int64_t)p.N * p.Hkv, p.tiles * p.SG, &group, &member);
-  const int n = (int)(group / p.Hkv), kvh = (int)(group % p.Hkv);
-  const int sg = member % p.SG, tile = member / p.SG;  // causal: the first keys are seen by the most rows
+  // A group: the workgroups that walk over the same queries. Causal: the first keys are seen by the most rows.
+  const DensePlace at = dense_place((int64_t)p.N * p.Hkv * p.SG, p.tiles);
+  const int sg = at.group % p.SG, kvh = at.group / p.SG % p.Hkv, n = at.group / p.SG / p.Hkv, tile = at.tile;
   const DenseSeq sq = dense_seq(p, n);
   if (sg == 0)
     dense_rest(p, sq, n, tile, tid, [&](int b, int t) {
@@ -660,86 +689,77 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
   // by one before any_from.
   auto seen_from = [&](int key) { return p.causal && key >= sq.pre ? key : 0; };
   const int from = seen_from(j), all_from = seen_from(j_last), any_from = j_first <= j_last ? seen_from(j_first) : 0x7fffffff;
-  const int t_first = seen_from(r0) / kDenseTile, t_end = (sq.len - 1) / kDenseTile + 1;
-  const int g_first = kvh * p.G + sg * (p.G / p.SG), heads = p.G / p.SG;
+  const int t_first = seen_from(r0) / kDenseStep, t_last = (sq.len - 1) / kDenseStep;
+  const int g_first = kvh * p.G + sg * p.G / p.SG, heads = kvh * p.G + (sg + 1) * p.G / p.SG - g_first;
 
   const typename X::Share qoff(p.q.s[1], wave, lane), goff(p.go.s[1], wave, lane);
   const int64_t row0 = (int64_t)sq.b * p.T + sq.t0;
-  auto bring = [&](uint8_t* qt, uint8_t* gt, float (*st)[kDenseTile], int h, int t) TASFT_INLINE {
-    X::dma(qt, dense_at(p.q, sq, 0, h), p.q.s[1], qoff, t * kDenseTile, sq.len, wave);
-    X::dma(gt, dense_at(p.go, sq, 0, h), p.go.s[1], goff, t * kDenseTile, sq.len, wave);
-    if (wave < 2) {  // a row a lane; past the sequence's end zeros
-      const int rows = min(sq.len - t * kDenseTile, kDenseTile);
-      const float* from = (wave == 0 ? p.lse2 : p.di) + h * p.rows + row0 + t * kDenseTile;
+  auto bring = [&](uint8_t* qt, uint8_t* gt, float (*st)[kWave], int h, int t) TASFT_INLINE {
+    X::dma(qt, dense_at(p.q, sq, 0, h), p.q.s[1], qoff, t * kDenseStep, sq.len, wave);
+    X::dma(gt, dense_at(p.go, sq, 0, h), p.go.s[1], goff, t * kDenseStep, sq.len, wave);
+    if (wave < 2) {  // a row a lane (half of them are used); past the sequence's end zeros
+      const int rows = min(sq.len - t * kDenseStep, kWave);
+      const float* from = (wave == 0 ? p.lse2 : p.di) + h * p.rows + row0 + t * kDenseStep;
       const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)from, (short)0, rows * 4, 0x00020000);
       __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (TASFT_LDS void*)st[wave], 4, lane * 4, 0, 0, 0);
     }
   };
-  bring(q0_lds, g0_lds, st0_lds, g_first, t_first);
+  bring(q0_lds, g0_lds, st0_lds, g_first, t_last);
 
-  u32x4_t kf[X::KSTEPS], vf[X::KSTEPS];
+  // K as the B operand in registers; V, for which there is no room beside the sums, in LDS.
+  V::dma(v_lds, dense_at(p.v, sq, 0, kvh), p.v.s[1], typename V::Share(p.v.s[1], wave, lane), r0, sq.len, wave);
+  u32x4_t kf[X::KSTEPS];
   X::load_row(kf, dense_at(p.k, sq, j, kvh), half);
-  X::load_row(vf, dense_at(p.v, sq, j, kvh), half);
   f32x16_t ka[X::DTILES], va[X::DTILES];
 #pragma unroll
   for (int dt = 0; dt < X::DTILES; ++dt) ka[dt] = va[dt] = (f32x16_t){};
-  auto step = [&](const uint8_t* qa, const uint8_t* ga, const float (*st)[kDenseTile], uint8_t* qb, uint8_t* gb,
-                  float (*stb)[kDenseTile], int h, int t, int hn, int tn) TASFT_INLINE {
+  auto step = [&](const uint8_t* qa, const uint8_t* ga, const float (*st)[kWave], uint8_t* qb, uint8_t* gb,
+                  float (*stb)[kWave], int h, int t, int hn, int tn) TASFT_INLINE {
     __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0)
     dense_barrier();
     if (hn >= 0) bring(qb, gb, stb, hn, tn);
     const float slope2 = BIAS ? p.sc.slopes[h] * kLog2e : 0.f;
+    const int i0 = t * kDenseStep;
+    if (i0 + 31 < any_from) return;
+    const bool mixed = i0 < all_from;
+    const float* lse2 = st[0] + 4 * half;
+    const float* di = st[1] + 4 * half;
+    const int from0 = from - i0 - 4 * half;
+    f32x16_t s = X::rows_times(qa, 0, kf, place), w;
+    u32x4_t b[2];
+    dense_weights<CAP, BIAS>(s, p.sc, slope2, (float)(i0 + 4 * half - j), [&](int rr, float x, float g) {
+      w[rr] = __builtin_amdgcn_exp2f(x - lse2[8 * (rr >> 2) + (rr & 3)]);
+      return w[rr] * g;
+    });
+    if (mixed) {
+      asm volatile("");  // a branch, no selections in other tiles
 #pragma unroll
-    for (int t2 = 0; t2 < 2; ++t2) {
-      const int i0 = t * kDenseTile + 32 * t2;
-      if (i0 + 31 < any_from || i0 >= sq.len) continue;
-      const bool mixed = i0 < all_from;
-      const float* lse2 = st[0] + 32 * t2 + 4 * half;
-      const float* di = st[1] + 32 * t2 + 4 * half;
-      const int from0 = from - i0 - 4 * half;
-      // S, then dv, then dP, then dk: two of the four products' operands at a time. The registers hold no
-      // more beside dk, dv and the wave's K and V.
-      f32x16_t s = X::template rows_times<D == 128 ? 2 : 1>(qa, 32 * t2, kf, place);
-      u32x4_t b[2];
-      {
-        f32x16_t w;
-        dense_weights<CAP, BIAS>(s, p.sc, slope2, (float)(i0 + 4 * half - j), [&](int rr, float x, float g) {
-          w[rr] = __builtin_amdgcn_exp2f(x - lse2[8 * (rr >> 2) + (rr & 3)]);
-          return w[rr] * g;
-        });
-        if (mixed) {
-          asm volatile("");  // a branch, no selections in other tiles
-#pragma unroll
-          for (int rr = 0; rr < 16; ++rr) w[rr] = 8 * (rr >> 2) + (rr & 3) < from0 ? 0.f : w[rr];
-        }
-        X::pack(b, w);
-      }
-      __builtin_amdgcn_sched_barrier(0);
-      X::template columns_times<D == 128 ? 2 : 1>(ga, 32 * t2, b, mixed, va, place, &found);
-      __builtin_amdgcn_sched_barrier(0);
-      const f32x16_t dp = X::template rows_times<D == 128 ? 2 : 1>(ga, 32 * t2, vf, place);
-#pragma unroll
-      for (int rr = 0; rr < 16; ++rr) s[rr] *= dp[rr] - di[8 * (rr >> 2) + (rr & 3)];
-      if (mixed) {
-        asm volatile("");
-#pragma unroll
-        for (int rr = 0; rr < 16; ++rr) s[rr] = 8 * (rr >> 2) + (rr & 3) < from0 ? 0.f : s[rr];
-      }
-      X::pack(b, s);
-      __builtin_amdgcn_sched_barrier(0);
-      X::template columns_times<D == 128 ? 2 : 1>(qa, 32 * t2, b, mixed, ka, place, &found);
-      __builtin_amdgcn_sched_barrier(0);
+      for (int rr = 0; rr < 16; ++rr) w[rr] = 8 * (rr >> 2) + (rr & 3) < from0 ? 0.f : w[rr];
     }
+    X::pack(b, w);
+    X::template columns_times<D == 128 ? 2 : 1>(ga, 0, b, mixed, va, place, &found);
+    const f32x16_t dp = X::rows_times_rows(ga, 0, v_lds, wave * 32, place);
+#pragma unroll
+    for (int rr = 0; rr < 16; ++rr) s[rr] *= dp[rr] - di[8 * (rr >> 2) + (rr & 3)];
+    if (mixed) {
+      asm volatile("");
+#pragma unroll
+      for (int rr = 0; rr < 16; ++rr) s[rr] = 8 * (rr >> 2) + (rr & 3) < from0 ? 0.f : s[rr];
+    }
+    X::pack(b, s);
+    X::template columns_times<D == 128 ? 2 : 1>(qa, 0, b, mixed, ka, place, &found);
   };
-  int h = g_first, t = t_first;
-  const int steps = heads * (t_end - t_first);
+  // From the last rows, which every key's workgroup walks over, to the first: the workgroups of a group read the
+  // same tiles at the same time.
+  int h = g_first, t = t_last;
+  const int steps = heads * (t_last - t_first + 1);
   for (int done = 0; done < steps; done += 2) {
-    int hn = h, tn = t + 1;
-    if (tn == t_end) tn = t_first, ++hn;
+    int hn = h, tn = t - 1;
+    if (tn < t_first) tn = t_last, ++hn;
     step(q0_lds, g0_lds, st0_lds, q1_lds, g1_lds, st1_lds, h, t, done + 1 < steps ? hn : -1, tn);
     if (done + 1 >= steps) break;
-    h = hn, t = tn + 1;
-    if (t == t_end) t = t_first, ++h;
+    h = hn, t = tn - 1;
+    if (t < t_first) t = t_last, ++h;
     step(q1_lds, g1_lds, st1_lds, q0_lds, g0_lds, st0_lds, hn, tn, done + 2 < steps ? h : -1, t);
   }
 
@@ -760,8 +780,8 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
         }
     }
   } else {
-    uint8_t* kst = ((wave & 2) ? q1_lds : q0_lds) + (wave & 1) * (32 * X::ROWB);
-    uint8_t* vst = ((wave & 2) ? g1_lds : g0_lds) + (wave & 1) * (32 * X::ROWB);
+    uint8_t* kst = v_lds + wave * (32 * X::ROWB);
+    uint8_t* vst = (wave & 2 ? wave & 1 ? g1_lds : q1_lds : wave & 1 ? g0_lds : q0_lds);
     X::store(kst, ka, pe->scale, dense_at(pe->gk, sq, 0, kvh), row_ok ? (int64_t)j * pe->gk.s[1] : -1, lane);
     X::store(vst, va, 1.f, dense_at(pe->gv, sq, 0, kvh), row_ok ? (int64_t)j * pe->gv.s[1] : -1, lane);
   }
@@ -856,13 +876,12 @@ static int dense_rows(DenseRows& r, const char* what, const char* name, const vo
   return kOk;
 }
 
-// Workgroups that share a KV head's query heads: a divisor of the group that gives four rounds of two
-// workgroups on every CU, so that causal rows of unequal length even out.
+// Workgroups that share a KV head's query heads: as many as give four rounds of two workgroups on every CU, so
+// that causal rows of unequal length even out.
 static int dense_head_splits(int64_t num_seqs, int64_t num_kv_heads, int64_t group, int64_t max_seqlen) {
   const int64_t wgs = num_seqs * num_kv_heads * ((max_seqlen + kDenseRows - 1) / kDenseRows);
-  int64_t sg = 1;
-  while (sg < group && (group % sg != 0 || wgs * sg < 2048)) ++sg;
-  return (int)sg;
+  const int64_t want = (2048 + wgs - 1) / wgs;
+  return (int)(want < group ? want : group);
 }
 
 extern "C" size_t tasft_dense_bwd_workspace_bytes(int64_t num_seqs, int64_t rows, int64_t num_q_heads,
