@@ -328,9 +328,11 @@ chunk_rows_kernel(const ChunkParams p) {
       // a lower bit.
       const uint64_t bits = nodes_seen(key0);
       const int before = nodes_before(key0);
+      int low = 4 * half;
+      asm volatile("" : "+v"(low));  // formed here: 32 masks kept over the loop spilled
 #pragma unroll
       for (int rr = 0; rr < 16; ++rr) {
-        const int b0 = 4 * half + 8 * (rr >> 2) + (rr & 3), b1 = b0 + 32;
+        const int b0 = low + 8 * (rr >> 2) + (rr & 3), b1 = b0 + 32;
         const int up0 = before + __popcll(bits & (((uint64_t)1 << b0) - 1));
         const int up1 = before + __popcll(bits & (((uint64_t)1 << b1) - 1));
         const float d0 = (float)(key0 + b0 < sq.p0 ? key0 + b0 : sq.p0 + up0) - pos;
@@ -522,7 +524,8 @@ chunk_rows_kernel(const ChunkParams p) {
       const int cached = sq.p0 - key0;  // keys of the tile before the tree
       const uint64_t below = cached >= 64 ? ~(uint64_t)0 : cached > 0 ? ((uint64_t)1 << cached) - 1 : 0;
       const uint64_t bits = (nodes_seen(key0) | below) >> (4 * half);
-      const uint32_t lo = (uint32_t)bits, hi = (uint32_t)(bits >> 32);
+      uint32_t lo = (uint32_t)bits, hi = (uint32_t)(bits >> 32);
+      asm volatile("" : "+v"(lo), "+v"(hi));  // the selections one by one: 32 conditions at once spilled
 #pragma unroll
       for (int rr = 0; rr < 16; ++rr) {
         const int off = 8 * (rr >> 2) + (rr & 3);
