@@ -71,7 +71,7 @@ struct ChunkParams {
   int QT, P;                     // row tiles per sequence and KV head (or head), key splits
   float scale_log2;
   int causal;
-  ScoreParams sc;            // SCORED: a cap (cap_out not 0) and slopes, or neither
+  ScoreParams sc;            // SCORED: a cap, slopes, both or neither
   const uint64_t* ancestors; // SCORED: [T][words] or null
   int words;
 };
@@ -171,8 +171,8 @@ constexpr int kMaskTile = 64;  // positions of a masked one: two waves
 // long as the share). A template: the general form's scalar registers spilled, at a fifth of the time.
 // MASK: kDense, kPositions (64 positions of a head), kRows (a mask, the dense form's rows).
 enum ChunkMask { kDense = 0, kPositions = 1, kRows = 2 };
-// SCORES: kPlain, kScored (capped or biased scores, by uniform branches: they are brought to units of log2
-// before their maximum), kTree (these, and the new tokens are the nodes of a tree).
+// SCORES: kPlain, kScored (capped or biased scores, by uniform branches), kTree (these, and the new tokens are the
+// nodes of a tree).
 enum ChunkScores { kPlain = 0, kScored = 1, kTree = 2 };
 template <int D, int DT, int MASK, int PIECES, int SCORES>
 __global__ void __launch_bounds__(MASK == kPositions ? 128 : 256)
@@ -269,10 +269,10 @@ chunk_rows_kernel(const ChunkParams p) {
 
   // A tree's row: its node's words of ancestors (bit a of word w: node 64 w + a), and where the node is.
   const uint64_t* words = nullptr;
-  float pos = 0.f, slope2 = 0.f;
+  float pos = 0.f, slope = 0.f;  // (the slope in units of the values that the scores are made of)
   if constexpr (SCORED) {
     if (p.sc.slopes) {
-      slope2 = p.sc.slopes[h] * kLog2e;
+      slope = p.sc.slopes[h] * p.sc.slope_mul;
       pos = (float)(sq.p0 + i);
     }
     if constexpr (TREE) {
@@ -303,25 +303,18 @@ chunk_rows_kernel(const ChunkParams p) {
     }
     return count;
   };
-  // Brings the scores of a tile to units of log2: capped, biased by the distance.
-  auto modify = [&](f32x16_t& s0, f32x16_t& s1, int key0, bool mixed) TASFT_INLINE {
-    if (p.sc.cap_out != 0.f) {
+  // The values that a tile's scores are made of (scores.h): capped, biased by the distance. Returns what the
+  // scores, in units of log2, are to be more than those.
+  auto modify = [&](f32x16_t& s0, f32x16_t& s1, int key0, bool mixed) TASFT_INLINE -> float {
+    if (p.sc.cap_in != 0.f) {
 #pragma unroll
       for (int rr = 0; rr < 16; ++rr) {
         const float g0 = cap_gate(s0[rr], p.sc), g1 = cap_gate(s1[rr], p.sc);
-        if (p.sc.cap_wide) {
-          s0[rr] = cap_score_wide(s0[rr], g0, p.sc);
-          s1[rr] = cap_score_wide(s1[rr], g1, p.sc);
-        } else {
-          s0[rr] = cap_score(s0[rr], g0, p.sc);
-          s1[rr] = cap_score(s1[rr], g1, p.sc);
-        }
+        s0[rr] = p.sc.cap_score ? cap_score(s0[rr], g0, p.sc) : g0;
+        s1[rr] = p.sc.cap_score ? cap_score(s1[rr], g1, p.sc) : g1;
       }
-    } else {
-      s0 *= p.scale_log2;
-      s1 *= p.scale_log2;
     }
-    if (!p.sc.slopes) return;
+    if (!p.sc.slopes) return p.sc.add;
     const float d = (float)(key0 + 4 * half) - pos;
     if (TREE && mixed) {
       // A node's position is behind the cache by the number of its ancestors: of this row's, those with
@@ -337,17 +330,29 @@ chunk_rows_kernel(const ChunkParams p) {
         const int up1 = before + __popcll(bits & (((uint64_t)1 << b1) - 1));
         const float d0 = (float)(key0 + b0 < sq.p0 ? key0 + b0 : sq.p0 + up0) - pos;
         const float d1 = (float)(key0 + b1 < sq.p0 ? key0 + b1 : sq.p0 + up1) - pos;
-        s0[rr] = fmaf(-slope2, fabsf(d0), s0[rr]);
-        s1[rr] = fmaf(-slope2, fabsf(d1), s1[rr]);
+        s0[rr] = fmaf(-slope, fabsf(d0), s0[rr]);
+        s1[rr] = fmaf(-slope, fabsf(d1), s1[rr]);
       }
-      return;
+      return p.sc.add;
+    }
+    if (p.causal && !mixed) {
+      // No key is behind its row: the bias rises with the key, and the tile's part of it joins the
+      // exponential's argument (one instruction a score; 2 below).
+#pragma unroll
+      for (int rr = 0; rr < 16; ++rr) {
+        const float off = (float)(8 * (rr >> 2) + (rr & 3));
+        s0[rr] = fmaf(slope, off, s0[rr]);
+        s1[rr] = fmaf(slope, off + 32.f, s1[rr]);
+      }
+      return fmaf(slope * d, p.sc.mul, p.sc.add);
     }
 #pragma unroll
     for (int rr = 0; rr < 16; ++rr) {
       const float off = (float)(8 * (rr >> 2) + (rr & 3));
-      s0[rr] = fmaf(-slope2, fabsf(d + off), s0[rr]);
-      s1[rr] = fmaf(-slope2, fabsf(d + (off + 32.f)), s1[rr]);
+      s0[rr] = fmaf(-slope, fabsf(d + off), s0[rr]);
+      s1[rr] = fmaf(-slope, fabsf(d + (off + 32.f)), s1[rr]);
     }
+    return p.sc.add;
   };
 
   // The tiles of the split in order; masked: those that any row's block mask selects, with this
@@ -519,7 +524,8 @@ chunk_rows_kernel(const ChunkParams p) {
     const int key0 = kt * kTile;
     const int lim0 = MASK != kDense && !(own & 1) ? -1 : lim - key0 - 4 * half;
     const int lim1 = MASK != kDense && !(own & 2) ? -1 : lim - key0 - 4 * half - 32;
-    if constexpr (SCORED) modify(s0, s1, key0, mixed);
+    float more = 0.f;
+    if constexpr (SCORED) more = modify(s0, s1, key0, mixed);
     if (TREE && mixed) {
       const int cached = sq.p0 - key0;  // keys of the tile before the tree
       const uint64_t below = cached >= 64 ? ~(uint64_t)0 : cached > 0 ? ((uint64_t)1 << cached) - 1 : 0;
@@ -547,8 +553,9 @@ chunk_rows_kernel(const ChunkParams p) {
       ma = fmaxf(fmaxf(ma, s0[rr]), s0[rr + 1]);
       mb = fmaxf(fmaxf(mb, s1[rr]), s1[rr + 1]);
     }
-    float mloc = pair_max32(fmaxf(fmaxf(ma, s0[15]), fmaxf(mb, s1[15])));
-    if constexpr (!SCORED) mloc *= p.scale_log2;
+    float mloc = fmaxf(fmaxf(ma, s0[15]), fmaxf(mb, s1[15]));
+    if constexpr (SCORED) mloc = pair_max32(fmaf(mloc, p.sc.mul, more));
+    else mloc = pair_max32(mloc) * p.scale_log2;
     const bool move = mloc > m_ref + kChunkMove;
     if (__ballot(move)) {
       const float alpha = move ? __builtin_amdgcn_exp2f(m_ref - mloc) : 1.f;
@@ -558,11 +565,12 @@ chunk_rows_kernel(const ChunkParams p) {
       m_ref = move ? mloc : m_ref;
     }
     const float m_use = (m_ref == -INFINITY) ? 0.f : m_ref;
+    const float less = SCORED ? m_use - more : 0.f;
     float lsum0 = 0.f, lsum1 = 0.f;
 #pragma unroll
     for (int rr = 0; rr < 16; ++rr) {
-      const float e0 = __builtin_amdgcn_exp2f(SCORED ? s0[rr] - m_use : fmaf(s0[rr], p.scale_log2, -m_use));
-      const float e1 = __builtin_amdgcn_exp2f(SCORED ? s1[rr] - m_use : fmaf(s1[rr], p.scale_log2, -m_use));
+      const float e0 = __builtin_amdgcn_exp2f(SCORED ? fmaf(s0[rr], p.sc.mul, -less) : fmaf(s0[rr], p.scale_log2, -m_use));
+      const float e1 = __builtin_amdgcn_exp2f(SCORED ? fmaf(s1[rr], p.sc.mul, -less) : fmaf(s1[rr], p.scale_log2, -m_use));
       s0[rr] = e0;
       s1[rr] = e1;
       lsum0 += e0;
@@ -744,14 +752,14 @@ chunk_rows_kernel(const ChunkParams p) {
       }
       float score = pair_sum32(dot);
       if constexpr (SCORED) {
-        const float gate = cap_gate(score, p.sc);
-        score = p.sc.cap_out == 0.f ? score * p.scale_log2
-                : p.sc.cap_wide     ? cap_score_wide(score, gate, p.sc)
-                                    : cap_score(score, gate, p.sc);
+        if (p.sc.cap_in != 0.f) {
+          const float gate = cap_gate(score, p.sc);
+          score = p.sc.cap_score ? cap_score(score, gate, p.sc) : gate;
+        }
         // (A node's position is behind the cache by the number of its ancestors.)
-        if (p.sc.slopes) score = fmaf(-slope2, fabsf((float)(node ? sq.p0 + nodes_before(key) : key) - pos), score);
+        if (p.sc.slopes) score = fmaf(-slope, fabsf((float)(node ? sq.p0 + nodes_before(key) : key) - pos), score);
       }
-      const float pk = __builtin_amdgcn_exp2f(SCORED ? score - m_use : fmaf(score, pe->scale_log2, -m_use));
+      const float pk = __builtin_amdgcn_exp2f(SCORED ? fmaf(score, p.sc.mul, p.sc.add - m_use) : fmaf(score, pe->scale_log2, -m_use));
 #pragma unroll
       for (int dt = 0; dt < DTILES; ++dt)
 #pragma unroll

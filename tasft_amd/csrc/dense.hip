@@ -50,7 +50,7 @@ struct DenseParams {
   int64_t sl[3];
   const float* glse;  // or null
   int64_t sgl[3];
-  float* lse2;        // [head][row]: lse log2(e)
+  float* less;        // [head][row]: what the exponentials' arguments are less than x mul
   float* di;          // and D
   float* part_k;      // [SG][row][Hkv][D], or null
   float* part_v;
@@ -377,45 +377,45 @@ __device__ __forceinline__ void dense_patch(T* out, const uint16_t* x, float w, 
   }
 }
 
-// For each of the products s of 32 rows f(register, score in units of log2, derivative of the cap), into s.
-// Distance of register rr: |d + off(rr)|.
+// For each of the products s of 32 rows f(register, x, g), into s: x rises with the score (scores.h), g is a
+// quarter of the cap's derivative, 1 - tanh^2 = 4 (r - r^2) with r = -gate. Distance of register rr:
+// |d + off(rr)|; slope in units of x.
 template <bool CAP, bool BIAS, class F>
-__device__ __forceinline__ void dense_weights(f32x16_t& s, const ScoreParams& sc, float slope2, float d, F&& f) {
+__device__ __forceinline__ void dense_weights(f32x16_t& s, const ScoreParams& sc, float slope, float d, F&& f) {
   auto each = [&](auto score) TASFT_INLINE {
 #pragma unroll
     for (int rr = 0; rr < 16; ++rr) {
-      float g = 1.f, x;
+      float g = 1.f, x = s[rr];
       if constexpr (CAP) {
-        const float r = cap_gate(s[rr], sc);
-        x = score(s[rr], r, sc);
-        g = 4.f * (r - r * r);
-      } else {
-        x = s[rr] * sc.scale_log2;
+        const float gate = cap_gate(s[rr], sc);
+        x = score(s[rr], gate);
+        g = fmaf(-gate, gate, -gate);
       }
-      if constexpr (BIAS) x = fmaf(-slope2, fabsf(d + (float)(8 * (rr >> 2) + (rr & 3))), x);
+      if constexpr (BIAS) x = fmaf(-slope, fabsf(d + (float)(8 * (rr >> 2) + (rr & 3))), x);
       s[rr] = f(rr, x, g);
     }
   };
-  if (CAP && sc.cap_wide) each([](float a, float r, const ScoreParams& q) { return cap_score_wide(a, r, q); });
-  else each([](float a, float r, const ScoreParams& q) { return cap_score(a, r, q); });
+  if (CAP && (BIAS || sc.cap_score)) each([&](float a, float gate) { return cap_score(a, gate, sc); });
+  else each([](float, float gate) { return gate; });
 }
 
 // One score as above.
 template <bool CAP, bool BIAS>
-__device__ __forceinline__ float dense_score(float s, float& gate, const ScoreParams& sc, float slope2, float d) {
-  float x = s * sc.scale_log2;
+__device__ __forceinline__ float dense_score(float s, float& g, const ScoreParams& sc, float slope, float d) {
+  float x = s;
+  g = 1.f;
   if constexpr (CAP) {
-    gate = cap_gate(s, sc);
-    x = sc.cap_wide ? cap_score_wide(s, gate, sc) : cap_score(s, gate, sc);
+    const float gate = cap_gate(s, sc);
+    x = sc.cap_score ? cap_score(s, gate, sc) : gate;
+    g = fmaf(-gate, gate, -gate);
   }
-  return BIAS ? fmaf(-slope2, fabsf(d), x) : x;
+  return BIAS ? fmaf(-slope, fabsf(d), x) : x;
 }
 
 // ------------------------------------------------------------------------------------ forward
 template <int D, int DT, bool CAP, bool BIAS>
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) dense_fwd_kernel(const DenseParams p) {
   using X = DenseTiles<D, DT, kDenseTile>;
-  constexpr bool UNITS = CAP || BIAS;  // scores are in units of log2 before their maximum
   __shared__ __attribute__((aligned(1024))) uint8_t k0_lds[X::TILE];
   __shared__ __attribute__((aligned(1024))) uint8_t v0_lds[X::TILE];
   __shared__ __attribute__((aligned(1024))) uint8_t k1_lds[X::TILE];
@@ -446,7 +446,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
 
   u32x4_t qf[X::KSTEPS];
   X::load_row(qf, dense_at(p.q, sq, i, h), half);
-  const float slope2 = BIAS ? p.sc.slopes[h] * kLog2e : 0.f;
+  const float slope = BIAS ? p.sc.slopes[h] * p.sc.slope_mul : 0.f;
   const uint16_t* kbase = dense_at(p.k, sq, 0, kvh);
   const uint16_t* vbase = dense_at(p.v, sq, 0, kvh);
   const typename X::Share koff(p.k.s[1], wave, lane), voff(p.v.s[1], wave, lane);
@@ -468,11 +468,11 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
     if (key0 > any_see) return;
     const bool mixed = key0 + kDenseTile - 1 > all_see;
     f32x16_t s0 = X::rows_times(ka, 0, qf, place), s1 = X::rows_times(ka, 32, qf, place);
-    if constexpr (UNITS) {
+    if constexpr (CAP || BIAS) {
       const float d = (float)(key0 + 4 * half - i);
       auto same = [](int, float x, float) { return x; };
-      dense_weights<CAP, BIAS>(s0, p.sc, slope2, d, same);
-      dense_weights<CAP, BIAS>(s1, p.sc, slope2, d + 32.f, same);
+      dense_weights<CAP, BIAS>(s0, p.sc, slope, d, same);
+      dense_weights<CAP, BIAS>(s1, p.sc, slope, d + 32.f, same);
     }
     if (mixed) {
       asm volatile("");  // a branch, no selections in other tiles
@@ -490,7 +490,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
       ma = fmaxf(fmaxf(ma, s0[rr]), s0[rr + 1]);
       mb = fmaxf(fmaxf(mb, s1[rr]), s1[rr + 1]);
     }
-    const float mloc = pair_max32(fmaxf(fmaxf(ma, s0[15]), fmaxf(mb, s1[15]))) * (UNITS ? 1.f : p.sc.scale_log2);
+    const float mloc = fmaf(pair_max32(fmaxf(fmaxf(ma, s0[15]), fmaxf(mb, s1[15]))), p.sc.mul, CAP ? p.sc.add : 0.f);
     const bool move = mloc > m_ref + kDenseMove;
     if (__ballot(move)) {
       const float alpha = move ? __builtin_amdgcn_exp2f(m_ref - mloc) : 1.f;
@@ -499,12 +499,12 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
       for (int dt = 0; dt < X::DTILES; ++dt) oacc[dt] *= alpha;
       m_ref = move ? mloc : m_ref;
     }
-    const float m_use = m_ref == -INFINITY ? 0.f : m_ref;
+    const float less = (m_ref == -INFINITY ? 0.f : m_ref) - (CAP ? p.sc.add : 0.f);
     float sum0 = 0.f, sum1 = 0.f;
 #pragma unroll
     for (int rr = 0; rr < 16; ++rr) {
-      s0[rr] = __builtin_amdgcn_exp2f(UNITS ? s0[rr] - m_use : fmaf(s0[rr], p.sc.scale_log2, -m_use));
-      s1[rr] = __builtin_amdgcn_exp2f(UNITS ? s1[rr] - m_use : fmaf(s1[rr], p.sc.scale_log2, -m_use));
+      s0[rr] = __builtin_amdgcn_exp2f(fmaf(s0[rr], p.sc.mul, -less));
+      s1[rr] = __builtin_amdgcn_exp2f(fmaf(s1[rr], p.sc.mul, -less));
       sum0 += s0[rr];
       sum1 += s1[rr];
     }
@@ -534,15 +534,15 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
 
   if (found) {
     __threadfence();
-    const float lse2 = m_ref + __builtin_amdgcn_logf(l_tot);
+    const float less = m_ref + __builtin_amdgcn_logf(l_tot) - pe->sc.add;
 #pragma nounroll
     for (int key = (all_see + 1) / kDenseTile * kDenseTile; key <= any_see; ++key) {
       const uint16_t* vr = vbase + (int64_t)key * pe->v.s[1];
       if (!X::has_nonfinite(vr, lane) || !row_ok || key > lim) continue;
       float gate;
       const float s = dense_score<CAP, BIAS>(dense_dot<D, DT>(dense_at(pe->q, sq, i, h), kbase + (int64_t)key * pe->k.s[1]),
-                                             gate, p.sc, slope2, (float)(key - i));
-      dense_patch<D, DT>(dense_at(pe->o, sq, i, h), vr, __builtin_amdgcn_exp2f(s - lse2), half);
+                                             gate, p.sc, slope, (float)(key - i));
+      dense_patch<D, DT>(dense_at(pe->o, sq, i, h), vr, __builtin_amdgcn_exp2f(fmaf(s, pe->sc.mul, -less)), half);
     }
   }
 }
@@ -588,15 +588,17 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
   X::load_row(qf, dense_at(p.q, sq, i, h), half);
   X::load_row(gf, dense_at(p.go, sq, i, h), half);
   const int64_t li = sq.b * p.sl[0] + (sq.t0 + i) * p.sl[1] + h * p.sl[2];
-  const float lse2 = p.lse[li] * kLog2e;
+  // What the exponential's argument is less than x mul: with a cap the weights come four times as large, for its
+  // derivative.
+  const float less = fmaf(p.lse[li], kLog2e, CAP ? -2.f - p.sc.add : 0.f);
   float D_i = X::dot(dense_at(p.o, sq, i, h), gf, half);
   if (p.glse) D_i -= p.glse[sq.b * p.sgl[0] + (sq.t0 + i) * p.sgl[1] + h * p.sgl[2]];
   if (row_ok && half == 0) {
     const int64_t row = h * p.rows + (int64_t)sq.b * p.T + sq.t0 + i;
-    p.lse2[row] = lse2;
+    p.less[row] = less;
     p.di[row] = D_i;
   }
-  const float slope2 = BIAS ? p.sc.slopes[h] * kLog2e : 0.f;
+  const float slope = BIAS ? p.sc.slopes[h] * p.sc.slope_mul : 0.f;
 
   f32x16_t acc[X::DTILES];
 #pragma unroll
@@ -611,8 +613,9 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
       if (key0 > any_see) continue;
       const bool mixed = key0 + 31 > all_see;
       f32x16_t s = X::rows_times(ka, 32 * t2, qf, place), dp = X::rows_times(va, 32 * t2, gf, place);
-      dense_weights<CAP, BIAS>(s, p.sc, slope2, (float)(key0 + 4 * half - i), [&](int rr, float x, float g) {
-        return __builtin_amdgcn_exp2f(x - lse2) * g * (dp[rr] - D_i);
+      dense_weights<CAP, BIAS>(s, p.sc, slope, (float)(key0 + 4 * half - i), [&](int rr, float x, float g) {
+        const float w = __builtin_amdgcn_exp2f(fmaf(x, p.sc.mul, -less)) * (dp[rr] - D_i);
+        return CAP ? w * g : w;
       });
       if (mixed) {
         asm volatile("");  // a branch, no selections in other tiles
@@ -644,11 +647,11 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
       const uint16_t* kr = kbase + (int64_t)key * pe->k.s[1];
       if (!X::has_nonfinite(kr, lane) || !row_ok || key > lim) continue;
       float gate;
-      const float s = dense_score<CAP, BIAS>(dense_dot<D, DT>(dense_at(pe->q, sq, i, h), kr), gate, p.sc, slope2,
+      const float s = dense_score<CAP, BIAS>(dense_dot<D, DT>(dense_at(pe->q, sq, i, h), kr), gate, p.sc, slope,
                                              (float)(key - i));
-      float ds = __builtin_amdgcn_exp2f(s - lse2) *
+      float ds = __builtin_amdgcn_exp2f(fmaf(s, pe->sc.mul, -less)) *
                  (dense_dot<D, DT>(dense_at(pe->go, sq, i, h), vbase + (int64_t)key * pe->v.s[1]) - D_i);
-      if constexpr (CAP) ds *= 4.f * (gate - gate * gate);
+      ds *= gate;
       dense_patch<D, DT>(dense_at(pe->gq, sq, i, h), kr, ds * pe->scale, half);
     }
   }
@@ -699,7 +702,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
     X::dma(gt, dense_at(p.go, sq, 0, h), p.go.s[1], goff, t * kDenseStep, sq.len, wave);
     if (wave < 2) {  // a row a lane (half of them are used); past the sequence's end zeros
       const int rows = min(sq.len - t * kDenseStep, kWave);
-      const float* from = (wave == 0 ? p.lse2 : p.di) + h * p.rows + row0 + t * kDenseStep;
+      const float* from = (wave == 0 ? p.less : p.di) + h * p.rows + row0 + t * kDenseStep;
       const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)from, (short)0, rows * 4, 0x00020000);
       __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (TASFT_LDS void*)st[wave], 4, lane * 4, 0, 0, 0);
     }
@@ -718,18 +721,18 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
     __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0)
     dense_barrier();
     if (hn >= 0) bring(qb, gb, stb, hn, tn);
-    const float slope2 = BIAS ? p.sc.slopes[h] * kLog2e : 0.f;
+    const float slope = BIAS ? p.sc.slopes[h] * p.sc.slope_mul : 0.f;
     const int i0 = t * kDenseStep;
     if (i0 + 31 < any_from) return;
     const bool mixed = i0 < all_from;
-    const float* lse2 = st[0] + 4 * half;
+    const float* less = st[0] + 4 * half;
     const float* di = st[1] + 4 * half;
     const int from0 = from - i0 - 4 * half;
     f32x16_t s = X::rows_times(qa, 0, kf, place), w;
     u32x4_t b[2];
-    dense_weights<CAP, BIAS>(s, p.sc, slope2, (float)(i0 + 4 * half - j), [&](int rr, float x, float g) {
-      w[rr] = __builtin_amdgcn_exp2f(x - lse2[8 * (rr >> 2) + (rr & 3)]);
-      return w[rr] * g;
+    dense_weights<CAP, BIAS>(s, p.sc, slope, (float)(i0 + 4 * half - j), [&](int rr, float x, float g) {
+      w[rr] = __builtin_amdgcn_exp2f(fmaf(x, p.sc.mul, -less[8 * (rr >> 2) + (rr & 3)]));
+      return CAP ? w[rr] * g : w[rr];
     });
     if (mixed) {
       asm volatile("");  // a branch, no selections in other tiles
@@ -783,7 +786,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
     uint8_t* kst = v_lds + wave * (32 * X::ROWB);
     uint8_t* vst = (wave & 2 ? wave & 1 ? g1_lds : q1_lds : wave & 1 ? g0_lds : q0_lds);
     X::store(kst, ka, pe->scale, dense_at(pe->gk, sq, 0, kvh), row_ok ? (int64_t)j * pe->gk.s[1] : -1, lane);
-    X::store(vst, va, 1.f, dense_at(pe->gv, sq, 0, kvh), row_ok ? (int64_t)j * pe->gv.s[1] : -1, lane);
+    X::store(vst, va, CAP ? 0.25f : 1.f, dense_at(pe->gv, sq, 0, kvh), row_ok ? (int64_t)j * pe->gv.s[1] : -1, lane);
   }
 
   if (found) {
@@ -792,25 +795,25 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
     const int end = min((all_from + 31) / 32 * 32, sq.len);
 #pragma nounroll
     for (int gh = g_first; gh < g_first + heads; ++gh) {
-      const float slope2 = BIAS ? pe->sc.slopes[gh] * kLog2e : 0.f;
+      const float slope = BIAS ? pe->sc.slopes[gh] * pe->sc.slope_mul : 0.f;
 #pragma nounroll
       for (int i = any_from / 32 * 32; i < end; ++i) {
         const uint16_t* qr = dense_at(pe->q, sq, i, gh);
         const uint16_t* gr = dense_at(pe->go, sq, i, gh);
         const bool bad_q = X::has_nonfinite(qr, lane), bad_g = X::has_nonfinite(gr, lane);
         if (!bad_q && !bad_g) continue;
-        const float lse2 = pe->lse2[gh * pe->rows + row0 + i], di = pe->di[gh * pe->rows + row0 + i];
+        const float less = pe->less[gh * pe->rows + row0 + i], di = pe->di[gh * pe->rows + row0 + i];
         if (!row_ok || i < from) continue;
         float gate;
-        const float s = dense_score<CAP, BIAS>(dense_dot<D, DT>(qr, dense_at(pe->k, sq, j, kvh)), gate, p.sc, slope2,
+        const float s = dense_score<CAP, BIAS>(dense_dot<D, DT>(qr, dense_at(pe->k, sq, j, kvh)), gate, p.sc, slope,
                                                (float)(i - j));
-        const float w = __builtin_amdgcn_exp2f(s - lse2);
+        const float w = __builtin_amdgcn_exp2f(fmaf(s, pe->sc.mul, -less));
         float ds = w * (dense_dot<D, DT>(gr, dense_at(pe->v, sq, j, kvh)) - di);
-        if constexpr (CAP) ds *= 4.f * (gate - gate * gate);
+        ds *= gate;
         const int64_t at = (((int64_t)sg * pe->rows + row0 + j) * pe->Hkv + kvh) * D;
         if (bad_g) {
           if (pe->SG > 1) dense_patch<D, DT>(pe->part_v + at, gr, w, half);
-          else dense_patch<D, DT>(dense_at(pe->gv, sq, j, kvh), gr, w, half);
+          else dense_patch<D, DT>(dense_at(pe->gv, sq, j, kvh), gr, CAP ? 0.25f * w : w, half);
         }
         if (bad_q) {
           if (pe->SG > 1) dense_patch<D, DT>(pe->part_k + at, qr, ds, half);
@@ -852,6 +855,7 @@ __global__ void __launch_bounds__(256) dense_join_kernel(const DenseParams p) {
     v += *(const f32x4_t*)(p.part_v + at + s * step);
   }
   k *= p.scale;
+  if (p.sc.cap_in != 0.f) v *= 0.25f;  // (four times the weights, see dense_dq_kernel)
   *(u32x2_t*)(p.gk.p + b * p.gk.s[0] + (int64_t)t * p.gk.s[1] + kvh * p.gk.s[2] + c * 4) =
       (u32x2_t){pack16x2<DT>(k[0], k[1]), pack16x2<DT>(k[2], k[3])};
   *(u32x2_t*)(p.gv.p + b * p.gv.s[0] + (int64_t)t * p.gv.s[1] + kvh * p.gv.s[2] + c * 4) =
@@ -1018,8 +1022,8 @@ extern "C" int tasft_dense_bwd(const void* q, const void* k, const void* v, cons
   p.glse = grad_lse;
   if (grad_lse) p.sgl[0] = glse_strides[0], p.sgl[2] = glse_strides[1], p.sgl[1] = glse_strides[2];
   p.SG = dense_head_splits(num_seqs, num_kv_heads, p.G, p.L);
-  p.lse2 = (float*)workspace;
-  p.di = p.lse2 + p.rows * p.Hq;
+  p.less = (float*)workspace;
+  p.di = p.less + p.rows * p.Hq;
   const size_t stats = ((size_t)p.rows * p.Hq * 8 + 15) / 16 * 16;
   if (p.SG > 1) {
     p.part_k = (float*)((uint8_t*)workspace + stats);
