@@ -638,8 +638,10 @@ int tasft_evict_paged(void* k_pages, void* v_pages, const int32_t* block_table, 
  * softcap tanh(s / softcap) if softcap > 0, then s - alibi_slopes[h] |i - j| (NULL: none):
  * out_i = softmax_j(s) v_j, lse_i = log sum_j exp(s) (NULL: not wanted). Rows without a token of a
  * sequence: 0 and -inf. head_dim 64 or 128; strides (b, h, s, d) of q, k, v, out and (b, h, s) of lse.
+ * out_rest (NULL: not wanted): a byte for each element of out, [rows][Hq][head_dim] (rows: tokens if packed, else
+ * num_seqs * tokens), what its rounding left over, for the backward.
  */
-int tasft_dense_fwd(const void* q, const void* k, const void* v, void* out, float* lse,
+int tasft_dense_fwd(const void* q, const void* k, const void* v, void* out, float* lse, void* out_rest,
                     const int32_t* cu_seqlens, const int32_t* seq_lens, const int32_t* prefix_lens,
                     const float* alibi_slopes, int64_t num_seqs, int64_t tokens, int64_t num_q_heads,
                     int64_t num_kv_heads, int64_t max_seqlen, int64_t head_dim, const int64_t* q_strides,
@@ -651,12 +653,12 @@ size_t tasft_dense_bwd_workspace_bytes(int64_t num_seqs, int64_t rows, int64_t n
                                        int64_t num_kv_heads, int64_t max_seqlen, int64_t head_dim);
 
 /*
- * Its backward: grad_q, grad_k (summed over the query heads of a KV head) and grad_v from out and lse of the
- * forward, grad_out and grad_lse (NULL: none). Every sum has a fixed order. Rows without a token of a
+ * Its backward: grad_q, grad_k (summed over the query heads of a KV head) and grad_v from out, lse and
+ * out_rest of the forward (NULL: out as it was rounded), grad_out and grad_lse (NULL: none). Every sum has a fixed order. Rows without a token of a
  * sequence get 0. Gradients must not overlap anything else.
  */
 int tasft_dense_bwd(const void* q, const void* k, const void* v, const void* out, const float* lse,
-                    const void* grad_out, const float* grad_lse, void* grad_q, void* grad_k, void* grad_v,
+                    const void* out_rest, const void* grad_out, const float* grad_lse, void* grad_q, void* grad_k, void* grad_v,
                     void* workspace, size_t workspace_bytes, const int32_t* cu_seqlens, const int32_t* seq_lens,
                     const int32_t* prefix_lens, const float* alibi_slopes, int64_t num_seqs, int64_t tokens,
                     int64_t num_q_heads, int64_t num_kv_heads, int64_t max_seqlen, int64_t head_dim,

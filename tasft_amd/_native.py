@@ -186,13 +186,13 @@ _SIGNATURES: dict[str, tuple[object, list[object]]] = {
     ),
     "tasft_dense_fwd": (
         _I,
-        [_P, _P, _P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I64P, _I64P, _I64P,
+        [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I64P, _I64P, _I64P,
          _I64P, _I64P, _F, _F, _I, _I, _P],
     ),
     "tasft_dense_bwd_workspace_bytes": (_SZ, [_I64, _I64, _I64, _I64, _I64, _I64]),
     "tasft_dense_bwd": (
         _I,
-        [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _SZ, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64,
+        [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _SZ, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64,
          _I64, _I64P, _I64P, _I64P, _I64P, _I64P, _I64P, _I64P, _I64P, _I64P, _I64P, _F, _F, _I, _I, _P],
     ),
     "tasft_draft_tree": (_I, [_P, _P, _P, _P, _P, _I64, _I64, _I64, _P]),

@@ -50,6 +50,7 @@ struct DenseParams {
   int64_t sl[3];
   const float* glse;  // or null
   int64_t sgl[3];
+  int8_t* rest;       // [row][Hq][D]: what the rounding of out left over (dense_rest_of), or null
   float* less;        // [head][row]: what the exponentials' arguments are less than x mul
   float* di;          // and D
   float* part_k;      // [SG][row][Hkv][D], or null
@@ -143,6 +144,28 @@ __device__ __forceinline__ void dense_rest(const DenseParams& p, const DenseSeq&
 template <int D>
 __device__ __forceinline__ void dense_clear(const DenseRows& r, int b, int t, int h, int tid) {
   if (tid < D / 8) *(u32x4_t*)(r.p + b * r.s[0] + (int64_t)t * r.s[1] + h * r.s[2] + tid * 8) = (u32x4_t){0u, 0u, 0u, 0u};
+}
+
+// What a rounding to 16 bits leaves over, in 256ths of the rounded value's last place (at most half of one).
+// D_i = do_i . o_i goes into every dS of a row with one sign: with o as it was rounded, rows that see few keys
+// had half again the error of all the other roundings together. A byte an element is kept for it.
+template <int DT>
+__device__ __forceinline__ int dense_place_exponent(uint32_t bits16) {  // of the last place, less 127
+  if constexpr (DT == kF16) return max((int)(bits16 >> 10 & 31), 1) - 25;
+  else return (int)(bits16 >> 7 & 255) - 134;
+}
+template <int DT>
+__device__ __forceinline__ int dense_rest_of(float x, uint32_t bits16) {
+  const int e = dense_place_exponent<DT>(bits16);
+  // (Values whose last place is under 2^-119, or that are no numbers, leave nothing over.)
+  const float q = e < -119 || e > 120 ? 0.f : (x - bits16_to_f32<DT>(bits16)) * __uint_as_float((uint32_t)(135 - e) << 23);
+  return (int)fminf(fmaxf(__builtin_rintf(q), -127.f), 127.f);
+}
+template <int DT>
+__device__ __forceinline__ float dense_with_rest(uint32_t bits16, int q) {
+  const int e = dense_place_exponent<DT>(bits16);
+  const float x = bits16_to_f32<DT>(bits16);
+  return e < -119 || e > 120 ? x : fmaf((float)q, __uint_as_float((uint32_t)(119 + e) << 23), x);
 }
 
 // Position of 16-byte chunk cc of row r in LDS: of 16 consecutive rows the same chunk, and of 4
@@ -344,6 +367,21 @@ struct DenseTiles {
     }
     return pair_sum32(sum);
   }
+  // The same with what a rounding left over of the row in memory added to it.
+  static __device__ __forceinline__ float dot(const uint16_t* row, const int8_t* rest, const u32x4_t (&f)[KSTEPS], int half) {
+    float sum = 0.f;
+#pragma unroll
+    for (int ks = 0; ks < KSTEPS; ++ks) {
+      const u32x4_t x = *(const u32x4_t*)(row + half * 8 + ks * 16);
+      const u32x2_t q = *(const u32x2_t*)(rest + half * 8 + ks * 16);
+      float y[8];
+      unpack16x8<DT>(f[ks], y);
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        sum = fmaf(dense_with_rest<DT>(x[j >> 1] >> (16 * (j & 1)) & 0xffffu, (int8_t)(q[j >> 2] >> (8 * (j & 3)))), y[j], sum);
+    }
+    return pair_sum32(sum);
+  }
   static __device__ __forceinline__ bool has_nonfinite(const uint16_t* row, int lane) {
     const uint32_t w = *(const uint32_t*)(row + (lane * 2) % D);
     return __ballot(dense_finite2<DT>(w) != w) != 0;
@@ -530,7 +568,23 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
   __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
   dense_barrier();                     // every wave is done with the tiles
   uint8_t* ost = ((wave & 2) ? v0_lds : k0_lds) + (wave & 1) * (32 * X::ROWB);
-  X::store(ost, oacc, 1.f / (l_tot > 0.f ? l_tot : 1.f), dense_at(pe->o, sq, 0, h), row_ok ? (int64_t)i * pe->o.s[1] : -1, lane);
+  const float inv = 1.f / (l_tot > 0.f ? l_tot : 1.f);
+  X::store(ost, oacc, inv, dense_at(pe->o, sq, 0, h), row_ok ? (int64_t)i * pe->o.s[1] : -1, lane);
+  if (pe->rest && row_ok) {
+    int8_t* to = pe->rest + (((int64_t)sq.b * pe->T + sq.t0 + i) * pe->Hq + h) * D + 4 * half;
+#pragma unroll
+    for (int dt = 0; dt < X::DTILES; ++dt)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        uint32_t q = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float x = oacc[dt][4 * g + e] * inv;
+          q |= ((uint32_t)dense_rest_of<DT>(x, f32_to16<DT>(x)) & 255u) << (8 * e);
+        }
+        *(uint32_t*)(to + dt * 32 + 8 * g) = q;
+      }
+  }
 
   if (found) {
     __threadfence();
@@ -591,7 +645,8 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
   // What the exponential's argument is less than x mul: with a cap the weights come four times as large, for its
   // derivative.
   const float less = fmaf(p.lse[li], kLog2e, CAP ? -2.f - p.sc.add : 0.f);
-  float D_i = X::dot(dense_at(p.o, sq, i, h), gf, half);
+  float D_i = p.rest ? X::dot(dense_at(p.o, sq, i, h), p.rest + (((int64_t)sq.b * p.T + sq.t0 + i) * p.Hq + h) * D, gf, half)
+                     : X::dot(dense_at(p.o, sq, i, h), gf, half);
   if (p.glse) D_i -= p.glse[sq.b * p.sgl[0] + (sq.t0 + i) * p.sgl[1] + h * p.sgl[2]];
   if (row_ok && half == 0) {
     const int64_t row = h * p.rows + (int64_t)sq.b * p.T + sq.t0 + i;
@@ -958,7 +1013,7 @@ static void dense_dispatch(int64_t head_dim, int dtype, bool cap, bool bias, F&&
   else with_dtype(std::integral_constant<int, 64>{});
 }
 
-extern "C" int tasft_dense_fwd(const void* q, const void* k, const void* v, void* out, float* lse,
+extern "C" int tasft_dense_fwd(const void* q, const void* k, const void* v, void* out, float* lse, void* out_rest,
                                const int32_t* cu_seqlens, const int32_t* seq_lens, const int32_t* prefix_lens,
                                const float* alibi_slopes, int64_t num_seqs, int64_t tokens, int64_t num_q_heads,
                                int64_t num_kv_heads, int64_t max_seqlen, int64_t head_dim, const int64_t* q_strides,
@@ -976,6 +1031,8 @@ extern "C" int tasft_dense_fwd(const void* q, const void* k, const void* v, void
   if (const int rc = dense_rows(p.o, what, "out", out, o_strides)) return rc;
   if (lse && (!lse_strides || !strides_nonneg(lse_strides, 3)))
     return set_error(kErrInvalidArgument, "dense attention: strides of lse must be non-negative");
+  if ((uintptr_t)out_rest & 7) return set_error(kErrInvalidArgument, "dense attention: out_rest must be 8-byte aligned");
+  p.rest = (int8_t*)out_rest;
   p.lse = lse;
   if (lse) p.sl[0] = lse_strides[0], p.sl[2] = lse_strides[1], p.sl[1] = lse_strides[2];
   const dim3 grid((unsigned)((int64_t)p.N * p.Hq * p.tiles));
@@ -986,7 +1043,7 @@ extern "C" int tasft_dense_fwd(const void* q, const void* k, const void* v, void
 }
 
 extern "C" int tasft_dense_bwd(const void* q, const void* k, const void* v, const void* out, const float* lse,
-                               const void* grad_out, const float* grad_lse, void* grad_q, void* grad_k, void* grad_v,
+                               const void* out_rest, const void* grad_out, const float* grad_lse, void* grad_q, void* grad_k, void* grad_v,
                                void* workspace, size_t workspace_bytes, const int32_t* cu_seqlens,
                                const int32_t* seq_lens, const int32_t* prefix_lens, const float* alibi_slopes,
                                int64_t num_seqs, int64_t tokens, int64_t num_q_heads, int64_t num_kv_heads,
@@ -1017,6 +1074,9 @@ extern "C" int tasft_dense_bwd(const void* q, const void* k, const void* v, cons
     return set_error(kErrWorkspace, "dense attention backward: workspace too small");
   if ((uintptr_t)workspace & 15)
     return set_error(kErrInvalidArgument, "dense attention backward: workspace must be 16-byte aligned");
+  if ((uintptr_t)out_rest & 7)
+    return set_error(kErrInvalidArgument, "dense attention backward: out_rest must be 8-byte aligned");
+  p.rest = (int8_t*)out_rest;
   p.lse = (float*)lse;
   p.sl[0] = lse_strides[0], p.sl[2] = lse_strides[1], p.sl[1] = lse_strides[2];
   p.glse = grad_lse;

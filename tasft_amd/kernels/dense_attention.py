@@ -70,7 +70,7 @@ class _Call:
     """What a call's kernels take beside the tensors that they differentiate."""
 
     __slots__ = ("causal", "cu", "dtype", "lens", "longest", "num_seqs", "prefix", "scale", "slopes", "softcap",
-                 "tokens")
+                 "strides", "tokens")
 
 
 def _sizes(q: torch.Tensor, k: torch.Tensor, c: _Call):
@@ -78,31 +78,34 @@ def _sizes(q: torch.Tensor, k: torch.Tensor, c: _Call):
     return c.num_seqs, c.tokens, q.shape[1], k.shape[1], c.longest, q.shape[-1]
 
 
-def _forward(q, k, v, c: _Call, want_lse: bool):
+def _forward(q, k, v, c: _Call, want_lse: bool, want_rest: bool):
+    """out, its log-sums and what its rounding left over, a byte an element (for the backward), or None."""
     out = _new_like(q)
+    dev = q.device
     lse = None
     if want_lse:
         # A head's sums lie together: that is how the kernels read them.
-        lse = (torch.empty(q.shape[:3], dtype=torch.float32, device=q.device) if q.ndim == 4
-               else torch.empty((q.shape[1], q.shape[0]), dtype=torch.float32, device=q.device).t())
+        lse = (torch.empty(q.shape[:3], dtype=torch.float32, device=dev) if q.ndim == 4
+               else torch.empty((q.shape[1], q.shape[0]), dtype=torch.float32, device=dev).t())
+    rest = torch.empty((q.numel(),), dtype=torch.int8, device=dev) if want_rest else None
     if q.numel() == 0:
-        return out, lse
+        return out, lse, rest
+    c.strides = (_strides4(q), _strides4(k), _strides4(v), _strides4(out), None if lse is None else _strides3(lse))
     lib = _native.load_library()
-    with _native.on_device(q.device):
+    with _native.on_device(dev):
         status = lib.tasft_dense_fwd(
-            q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _native.ptr(lse), _native.ptr(c.cu),
-            _native.ptr(c.lens), _native.ptr(c.prefix), _native.ptr(c.slopes), *_sizes(q, k, c), _strides4(q),
-            _strides4(k), _strides4(v), _strides4(out), None if lse is None else _strides3(lse), c.scale, c.softcap,
-            c.causal, c.dtype, _native.stream_handle(q.device))
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _native.ptr(lse), _native.ptr(rest),
+            _native.ptr(c.cu), _native.ptr(c.lens), _native.ptr(c.prefix), _native.ptr(c.slopes), *_sizes(q, k, c),
+            *c.strides, c.scale, c.softcap, c.causal, c.dtype, _native.stream_handle(dev))
     _native.check(status, "tasft_dense_fwd", {"q": list(q.shape), "k": list(k.shape)})
-    return out, lse
+    return out, lse, rest
 
 
 class _Dense(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, c: _Call):
-        out, lse = _forward(q, k, v, c, True)
-        ctx.save_for_backward(q, k, v, out, lse, c.cu, c.lens, c.prefix, c.slopes)
+        out, lse, rest = _forward(q, k, v, c, True, True)
+        ctx.save_for_backward(q, k, v, out, lse, rest, c.cu, c.lens, c.prefix, c.slopes)
         ctx.call = c
         ctx.set_materialize_grads(False)
         return out, lse
@@ -112,24 +115,24 @@ class _Dense(torch.autograd.Function):
     def backward(ctx, go, glse):
         if go is None and glse is None:
             return None, None, None, None
-        q, k, v, out, lse, cu, lens, prefix, slopes = ctx.saved_tensors
+        q, k, v, out, lse, rest, cu, lens, prefix, slopes = ctx.saved_tensors
         c = ctx.call
         gq, gk, gv = _new_like(q), _new_like(k), _new_like(v)
         if q.numel() == 0:
             return gq, gk, gv, None
         go = torch.zeros_like(out) if go is None else _ready(go)
         lib = _native.load_library()
+        sizes = _sizes(q, k, c)
         rows = c.tokens if cu is not None else c.num_seqs * c.tokens
-        size = lib.tasft_dense_bwd_workspace_bytes(c.num_seqs, rows, q.shape[1], k.shape[1], c.longest, q.shape[-1])
-        workspace = torch.empty(size, dtype=torch.uint8, device=q.device)
+        ws_bytes = lib.tasft_dense_bwd_workspace_bytes(sizes[0], rows, *sizes[2:])
+        workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device)
         with _native.on_device(q.device):
             status = lib.tasft_dense_bwd(
-                q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), go.data_ptr(),
-                _native.ptr(glse), gq.data_ptr(), gk.data_ptr(), gv.data_ptr(), workspace.data_ptr(), size,
-                _native.ptr(cu), _native.ptr(lens), _native.ptr(prefix), _native.ptr(slopes), *_sizes(q, k, c),
-                _strides4(q), _strides4(k), _strides4(v), _strides4(out), _strides3(lse), _strides4(go),
-                None if glse is None else _strides3(glse), _strides4(gq), _strides4(gk), _strides4(gv), c.scale,
-                c.softcap, c.causal, c.dtype, _native.stream_handle(q.device))
+                q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), rest.data_ptr(),
+                go.data_ptr(), _native.ptr(glse), gq.data_ptr(), gk.data_ptr(), gv.data_ptr(), workspace.data_ptr(),
+                ws_bytes, _native.ptr(cu), _native.ptr(lens), _native.ptr(prefix), _native.ptr(slopes), *sizes,
+                *c.strides, _strides4(go), None if glse is None else _strides3(glse), _strides4(gq), _strides4(gk),
+                _strides4(gv), c.scale, c.softcap, c.causal, c.dtype, _native.stream_handle(q.device))
         _native.check(status, "tasft_dense_bwd", {"q": list(q.shape), "k": list(k.shape)})
         return gq, gk, gv, None
 
@@ -192,7 +195,8 @@ def dense_attention(
         ``[B, Hq, S, D]`` / ``[T, Hq, D]`` in q's layout; rows of padding and of tokens behind the last
         document are 0, and so are their gradients. With ``return_lse`` also ``[B, Hq, S]`` / ``[T, Hq]``
         fp32 (differentiable too), -inf for those rows. Equal calls give equal bits, gradients
-        included. A second derivative is refused. As for every operator of a graph of gradients: to
+        included. What is kept for the backward: q, k, v, the output with a byte more an element, and the
+        log-sums. A second derivative is refused. As for every operator of a graph of gradients: to
         capture a backward pass into a HIP graph, drop eager results of the same leaves first (torch
         ends the process otherwise).
     """
@@ -260,7 +264,7 @@ def dense_attention(
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         out, lse = _Dense.apply(q, k, v, c)
     else:
-        out, lse = _forward(q, k, v, c, return_lse)
+        out, lse, _ = _forward(q, k, v, c, return_lse, False)
     return (out, lse) if return_lse else out
 
 

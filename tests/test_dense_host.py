@@ -77,8 +77,8 @@ def test_c_entries_refuse_before_any_launch():
     st = _native.kept_strides((64 * 10 * 4, 640, 64, 1))
     sl = _native.kept_strides((40, 10, 1))
 
-    def fwd(q=fake, sizes=(2, 10, 4, 2, 10, 64), qs=st, scale=0.1, cap=0.0, dtype=0, cu=None, lens=None, lse_strides=sl):
-        return lib.tasft_dense_fwd(q, fake, fake, fake, fake, cu, lens, None, None, *sizes, qs, st, st, st, lse_strides,
+    def fwd(q=fake, sizes=(2, 10, 4, 2, 10, 64), qs=st, scale=0.1, cap=0.0, dtype=0, cu=None, lens=None, lse_strides=sl, rest=None):
+        return lib.tasft_dense_fwd(q, fake, fake, fake, fake, rest, cu, lens, None, None, *sizes, qs, st, st, st, lse_strides,
                                    scale, cap, 1, dtype, None)
 
     def refused(rc, code, text):
@@ -105,8 +105,8 @@ def test_c_entries_refuse_before_any_launch():
     assert lib.tasft_dense_bwd_workspace_bytes(2, 20, 4, 3, 10, 64) == 0
     assert lib.tasft_dense_bwd_workspace_bytes(1024, 20, 4, 2, 10, 64) == 20 * 4 * 8
 
-    def bwd(ws=fake, size=size, glse=None):
-        return lib.tasft_dense_bwd(fake, fake, fake, fake, fake, fake, glse, fake, fake, fake, ws, size, None, None,
+    def bwd(ws=fake, size=size, glse=None, rest=None):
+        return lib.tasft_dense_bwd(fake, fake, fake, fake, fake, rest, fake, glse, fake, fake, fake, ws, size, None, None,
                                    None, None, 2, 10, 4, 2, 10, 64, st, st, st, st, sl, st, None, st, st, st, 0.1,
                                    0.0, 1, 0, None)
 
@@ -114,6 +114,8 @@ def test_c_entries_refuse_before_any_launch():
     refused(bwd(ws=None), -4, b"workspace")
     refused(bwd(ws=ctypes.c_void_p(8)), -1, b"aligned")
     refused(bwd(glse=fake), -1, b"null")
+    refused(bwd(rest=ctypes.c_void_p(4)), -1, b"out_rest")
+    refused(fwd(rest=ctypes.c_void_p(4)), -1, b"out_rest")
 
 
 @pytest.mark.parametrize("cap", [0.0, 5.0])
