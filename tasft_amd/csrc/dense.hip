@@ -927,7 +927,8 @@ static int dense_rows(DenseRows& r, const char* what, const char* name, const vo
   if (s[3] != 1) return set_error(kErrInvalidArgument, "%s: head dims of %s must be contiguous", what, name);
   if ((s[0] & 7) || (s[1] & 7) || (s[2] & 7) || ((uintptr_t)ptr & 15))
     return set_error(kErrInvalidArgument, "%s: strides of %s must be multiples of 8 on a 16-byte aligned base", what, name);
-  if (s[2] >= (int64_t)1 << 24) return set_error(kErrUnsupported, "%s: token stride of %s too large", what, name);
+  // (128 rows are addressed with 32-bit byte offsets.)
+  if (s[2] >= (int64_t)1 << 23) return set_error(kErrUnsupported, "%s: token stride of %s too large", what, name);
   r.p = (uint16_t*)ptr;
   r.s[0] = s[0];
   r.s[1] = s[2];

@@ -78,63 +78,75 @@ def _sizes(q: torch.Tensor, k: torch.Tensor, c: _Call):
     return c.num_seqs, c.tokens, q.shape[1], k.shape[1], c.longest, q.shape[-1]
 
 
-def _forward(q, k, v, c: _Call, want_lse: bool, want_rest: bool):
-    """out, its log-sums and what its rounding left over, a byte an element (for the backward), or None."""
+def _forward(q, k, v, c: _Call, want_lse: bool, want_kept: bool):
+    """out, its log-sums (or None), and what the backward needs beside them (or None): what out's rounding left
+    over, a byte an element, and behind it the log-sums if they are not wanted."""
     out = _new_like(q)
     dev = q.device
-    lse = None
+    lse, kept, lse_ptr, rest_ptr = None, None, None, None
+    rows = q.numel() // q.shape[-1]
     if want_lse:
         # A head's sums lie together: that is how the kernels read them.
         lse = (torch.empty(q.shape[:3], dtype=torch.float32, device=dev) if q.ndim == 4
                else torch.empty((q.shape[1], q.shape[0]), dtype=torch.float32, device=dev).t())
-    rest = torch.empty((q.numel(),), dtype=torch.int8, device=dev) if want_rest else None
+        lse_ptr = lse.data_ptr()
+    if want_kept:
+        kept = torch.empty((q.numel() + (0 if want_lse else 4 * rows),), dtype=torch.int8, device=dev)
+        rest_ptr = kept.data_ptr()
+        if not want_lse:
+            lse_ptr = rest_ptr + q.numel()
     if q.numel() == 0:
-        return out, lse, rest
-    c.strides = (_strides4(q), _strides4(k), _strides4(v), _strides4(out), None if lse is None else _strides3(lse))
+        return out, lse, kept
+    # (b, h, s) strides of the log-sums, [B, H, S] or the transpose of [H, T].
+    heads, tokens = q.shape[1], c.tokens
+    c.strides = (_strides4(q), _strides4(k), _strides4(v), _strides4(out),
+                 _native.kept_strides((heads * tokens if q.ndim == 4 else 0, tokens, 1)))
     lib = _native.load_library()
     with _native.on_device(dev):
         status = lib.tasft_dense_fwd(
-            q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _native.ptr(lse), _native.ptr(rest),
-            _native.ptr(c.cu), _native.ptr(c.lens), _native.ptr(c.prefix), _native.ptr(c.slopes), *_sizes(q, k, c),
-            *c.strides, c.scale, c.softcap, c.causal, c.dtype, _native.stream_handle(dev))
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse_ptr, rest_ptr, _native.ptr(c.cu),
+            _native.ptr(c.lens), _native.ptr(c.prefix), _native.ptr(c.slopes), *_sizes(q, k, c), *c.strides, c.scale,
+            c.softcap, c.causal, c.dtype, _native.stream_handle(dev))
     _native.check(status, "tasft_dense_fwd", {"q": list(q.shape), "k": list(k.shape)})
-    return out, lse, rest
+    return out, lse, kept
 
 
 class _Dense(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, c: _Call):
-        out, lse, rest = _forward(q, k, v, c, True, True)
-        ctx.save_for_backward(q, k, v, out, lse, rest, c.cu, c.lens, c.prefix, c.slopes)
+    def forward(ctx, q, k, v, c: _Call, return_lse: bool):
+        out, lse, kept = _forward(q, k, v, c, return_lse, True)
+        ctx.save_for_backward(q, k, v, out, lse, kept, c.cu, c.lens, c.prefix, c.slopes)
         ctx.call = c
         ctx.set_materialize_grads(False)
-        return out, lse
+        return (out, lse) if return_lse else out
 
     @staticmethod
     @first_order_only
-    def backward(ctx, go, glse):
+    def backward(ctx, go, glse=None):
         if go is None and glse is None:
-            return None, None, None, None
-        q, k, v, out, lse, rest, cu, lens, prefix, slopes = ctx.saved_tensors
+            return None, None, None, None, None
+        q, k, v, out, lse, kept, cu, lens, prefix, slopes = ctx.saved_tensors
         c = ctx.call
         gq, gk, gv = _new_like(q), _new_like(k), _new_like(v)
         if q.numel() == 0:
-            return gq, gk, gv, None
+            return gq, gk, gv, None, None
         go = torch.zeros_like(out) if go is None else _ready(go)
+        rest_ptr = kept.data_ptr()
         lib = _native.load_library()
         sizes = _sizes(q, k, c)
         rows = c.tokens if cu is not None else c.num_seqs * c.tokens
         ws_bytes = lib.tasft_dense_bwd_workspace_bytes(sizes[0], rows, *sizes[2:])
-        workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device)
+        workspace = torch.empty((ws_bytes,), dtype=torch.uint8, device=q.device)
         with _native.on_device(q.device):
             status = lib.tasft_dense_bwd(
-                q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), rest.data_ptr(),
-                go.data_ptr(), _native.ptr(glse), gq.data_ptr(), gk.data_ptr(), gv.data_ptr(), workspace.data_ptr(),
-                ws_bytes, _native.ptr(cu), _native.ptr(lens), _native.ptr(prefix), _native.ptr(slopes), *sizes,
-                *c.strides, _strides4(go), None if glse is None else _strides3(glse), _strides4(gq), _strides4(gk),
-                _strides4(gv), c.scale, c.softcap, c.causal, c.dtype, _native.stream_handle(q.device))
+                q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
+                rest_ptr + q.numel() if lse is None else lse.data_ptr(), rest_ptr, go.data_ptr(), _native.ptr(glse),
+                gq.data_ptr(), gk.data_ptr(), gv.data_ptr(), workspace.data_ptr(), ws_bytes, _native.ptr(cu),
+                _native.ptr(lens), _native.ptr(prefix), _native.ptr(slopes), *sizes, *c.strides, _strides4(go),
+                None if glse is None else _strides3(glse), _strides4(gq), _strides4(gk), _strides4(gv), c.scale,
+                c.softcap, c.causal, c.dtype, _native.stream_handle(q.device))
         _native.check(status, "tasft_dense_bwd", {"q": list(q.shape), "k": list(k.shape)})
-        return gq, gk, gv, None
+        return gq, gk, gv, None, None
 
 
 def _lengths(t: torch.Tensor, n: int, most: int, what: str, device: torch.device) -> torch.Tensor:
@@ -196,7 +208,9 @@ def dense_attention(
         document are 0, and so are their gradients. With ``return_lse`` also ``[B, Hq, S]`` / ``[T, Hq]``
         fp32 (differentiable too), -inf for those rows. Equal calls give equal bits, gradients
         included. What is kept for the backward: q, k, v, the output with a byte more an element, and the
-        log-sums. A second derivative is refused. As for every operator of a graph of gradients: to
+        log-sums. In fp16 the weights' gradients are rounded to fp16 for their products: scale the loss,
+        as for every fp16 gradient, so that they stay above 2^-14 where they matter.
+        An infinity of v whose weight rounds to 0 gives NaN in the rows that see it. A second derivative is refused. As for every operator of a graph of gradients: to
         capture a backward pass into a HIP graph, drop eager results of the same leaves first (torch
         ends the process otherwise).
     """
@@ -262,9 +276,8 @@ def dense_attention(
     c.slopes = check_slopes(alibi_slopes, qs[1], dev)
     q, k, v = _ready(q), _ready(k), _ready(v)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
-        out, lse = _Dense.apply(q, k, v, c)
-    else:
-        out, lse, _ = _forward(q, k, v, c, return_lse, False)
+        return _Dense.apply(q, k, v, c, return_lse)
+    out, lse, _ = _forward(q, k, v, c, return_lse, False)
     return (out, lse) if return_lse else out
 
 

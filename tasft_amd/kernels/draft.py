@@ -77,6 +77,13 @@ def _check_tree(parents: torch.Tensor, cu_seqlens: torch.Tensor, max_nodes: int 
     return max_nodes
 
 
+def _parents_on(parents: torch.Tensor, device: torch.device) -> torch.Tensor:
+    """``parents`` as the kernels read them; what 32 bits do not hold is no node."""
+    if parents.dtype == torch.int64 and not parents.is_cpu:
+        parents = parents.clamp(-1, 0x7fffffff)
+    return int32_on(parents, device)
+
+
 def draft_tree(parents: torch.Tensor, cu_seqlens: torch.Tensor, kv_lens: torch.Tensor, *,
                max_nodes: int | None = None) -> DraftTree:
     """Ancestors and positions of the nodes of drafted trees, in one launch for all layers of a step.
@@ -106,7 +113,7 @@ def draft_tree(parents: torch.Tensor, cu_seqlens: torch.Tensor, kv_lens: torch.T
     positions = torch.empty((T,), dtype=torch.int32, device=dev)
     if T == 0:
         return DraftTree(ancestors, positions)
-    parents, cu, lens = int32_on(parents, dev), int32_on(cu_seqlens, dev), int32_on(kv_lens, dev)
+    parents, cu, lens = _parents_on(parents, dev), int32_on(cu_seqlens, dev), int32_on(kv_lens, dev)
     with _native.on_device(dev):
         status = _native.load_library().tasft_draft_tree(
             parents.data_ptr(), cu.data_ptr(), lens.data_ptr(), ancestors.data_ptr(), positions.data_ptr(), n, T, most,
@@ -150,7 +157,7 @@ def accept_draft(parents: torch.Tensor, tokens: torch.Tensor, targets: torch.Ten
     if T == 0:
         following = following.fill_(-1) if first_targets is None else first_targets.clone()
         return AcceptedDraft(path.fill_(-1), counts.zero_(), following)
-    parents, cu = int32_on(parents, dev), int32_on(cu_seqlens, dev)
+    parents, cu = _parents_on(parents, dev), int32_on(cu_seqlens, dev)
     tokens, targets = tokens.contiguous(), targets.contiguous()
     with _native.on_device(dev):
         status = _native.load_library().tasft_draft_accept(

@@ -97,7 +97,7 @@ def test_c_entries_refuse_before_any_launch():
     refused(fwd(qs=_native.kept_strides((2560, 640, 64, 2))), -1, b"contiguous")
     refused(fwd(qs=_native.kept_strides((2560, 640, 68, 1))), -1, b"multiples of 8")
     refused(fwd(qs=_native.kept_strides((2560, -640, 64, 1))), -1, b"non-negative")
-    refused(fwd(qs=_native.kept_strides((2560, 640, 1 << 24, 1))), -2, b"token stride")
+    refused(fwd(qs=_native.kept_strides((2560, 640, 1 << 23, 1))), -2, b"token stride")
     refused(fwd(q=ctypes.c_void_p(18)), -1, b"16-byte")
     refused(fwd(lse_strides=None), -1, b"lse")
     size = lib.tasft_dense_bwd_workspace_bytes(2, 20, 4, 2, 10, 64)

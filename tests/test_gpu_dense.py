@@ -417,6 +417,25 @@ def test_offsets_past_32_bits():
     assert all(torch.equal(a, b) for a, b in zip(run(*close), run(*far)))
 
 
+@pytest.mark.parametrize("d", [64, 128])
+def test_tokens_far_apart(d):
+    """Tokens as far apart as the kernels take them (16 MB, less a little): the same bits as close ones."""
+    dev = require_gpu()
+    s, stride = 130, (1 << 23) - 8
+    g = torch.Generator(device=dev).manual_seed(0)
+    close = [torch.randn((1, 1, s, d), generator=g, device=dev).to(BF) for _ in range(4)]
+    room = torch.empty(s * stride, dtype=BF, device=dev)  # the four side by side
+    far = [room.as_strided((1, 1, s, d), (0, 0, stride, 1), i * d).copy_(x) for i, x in enumerate(close)]
+
+    def run(q, k, v, go):
+        q, k, v = (x.detach().requires_grad_(True) for x in (q, k, v))
+        out = dense_attention(q, k, v)
+        return [x.contiguous() for x in (out.detach(), *torch.autograd.grad(out, (q, k, v), go))]
+
+    print(f"dense far tokens {d}", flush=True)
+    assert all(torch.equal(a, b) for a, b in zip(run(*close), run(*far)))
+
+
 def test_a_training_step_with_rotary():
     """Projections, rotation, capped attention and their gradients together, against the same step in
     64 bits."""

@@ -63,6 +63,10 @@ def test_plans_of_odd_parents_and_cut_trees():
     print("plan odd", flush=True)
     tree = draft_tree(parents.to(dev), cu.to(dev), torch.tensor([10], device=dev), max_nodes=64)
     assert torch.equal(tree.ancestors.cpu(), ref.bits(rows, 1))
+    wide = parents.long()
+    wide[7], wide[8] = 1 << 32, -(1 << 32) + 2  # of which 32 bits would be earlier nodes
+    assert torch.equal(draft_tree(wide.to(dev), cu.to(dev), torch.tensor([10], device=dev), max_nodes=64).ancestors,
+                       tree.ancestors)
     tree = draft_tree(parents.to(dev), cu.to(dev), torch.tensor([30], device=dev), max_nodes=6)
     assert torch.equal(tree.ancestors[:6].cpu(), ref.bits(rows, 1)[:6]) and not tree.ancestors[6:].any()
     assert tree.positions[:6].tolist() == [20 + len(r) - 1 for r in rows[:6]]
