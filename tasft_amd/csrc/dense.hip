@@ -50,7 +50,7 @@ struct DenseParams {
   int64_t sl[3];
   const float* glse;  // or null
   int64_t sgl[3];
-  int8_t* rest;       // [row][Hq][D]: what the rounding of out left over (dense_rest_of), or null
+  int8_t* rest;       // [row][Hq][D]: what out's rounding left over (dense_rest_of), or null
   float* less;        // [head][row]: what the exponentials' arguments are less than x mul
   float* di;          // and D
   float* part_k;      // [SG][row][Hkv][D], or null
@@ -95,13 +95,13 @@ __device__ __forceinline__ uint16_t* dense_at(R& r, const DenseSeq& s, int i, in
   return r.p + s.b * r.s[0] + (int64_t)(s.t0 + i) * r.s[1] + h * r.s[2];
 }
 
-// A workgroup's group and tile. A group's workgroups walk over the same tensors and share an XCD's L2
-// (workgroup i runs on XCD i % 8). Groups are as narrow as that allows (a query head, or the heads that a
-// workgroup of dk and dv takes), so that every XCD gets some of every sequence, turned by one in each eight: else
-// an XCD would get all first or all last heads. An XCD takes kDenseRun of its groups at a time, tile by tile: the
-// longest rows of all of them first (in another order for each tile: workgroups go round an XCD's shader engines,
-// and one would get the same group every time; ten documents, 28 / 4 heads: the kernel of dk and dv 2030 us
-// without that, 1470 with; one group at a time 1500, and one sequence of 8192 5% slower).
+// The group and tile of a workgroup of dk and dv. A group's workgroups walk over the same queries and share an
+// XCD's L2 (workgroup i runs on XCD i % 8). Groups are as narrow as that allows (the heads that a workgroup
+// takes), so that every XCD gets some of every sequence, turned by one in each eight: else an XCD would get all
+// first or all last heads. An XCD takes kDenseRun of its groups at a time, tile by tile: the longest columns of all
+// of them first (in another order for each tile: workgroups go round an XCD's shader engines, and one would get
+// the same group every time; ten documents, 28 / 4 heads: 2030 us without that, 1470 with; one group at a time
+// 1500, and one sequence of 8192 5% slower).
 struct DensePlace {
   int group, tile;
 };
@@ -146,26 +146,22 @@ __device__ __forceinline__ void dense_clear(const DenseRows& r, int b, int t, in
   if (tid < D / 8) *(u32x4_t*)(r.p + b * r.s[0] + (int64_t)t * r.s[1] + h * r.s[2] + tid * 8) = (u32x4_t){0u, 0u, 0u, 0u};
 }
 
-// What a rounding to 16 bits leaves over, in 256ths of the rounded value's last place (at most half of one).
-// D_i = do_i . o_i goes into every dS of a row with one sign: with o as it was rounded, rows that see few keys
-// had half again the error of all the other roundings together. A byte an element is kept for it.
+// What a rounding to 16 bits leaves over, as the difference of the two values' fp32 words in a byte: in 256ths of
+// the rounded value's last place. D_i = do_i . o_i goes into every dS of a row with one sign: with o as it was
+// rounded, rows that see few keys had half again the error of all the other roundings together.
 template <int DT>
-__device__ __forceinline__ int dense_place_exponent(uint32_t bits16) {  // of the last place, less 127
-  if constexpr (DT == kF16) return max((int)(bits16 >> 10 & 31), 1) - 25;
-  else return (int)(bits16 >> 7 & 255) - 134;
-}
+constexpr int dense_rest_bits() { return DT == kF16 ? 5 : 8; }  // of a word, below the byte
 template <int DT>
-__device__ __forceinline__ int dense_rest_of(float x, uint32_t bits16) {
-  const int e = dense_place_exponent<DT>(bits16);
-  // (Values whose last place is under 2^-119, or that are no numbers, leave nothing over.)
-  const float q = e < -119 || e > 120 ? 0.f : (x - bits16_to_f32<DT>(bits16)) * __uint_as_float((uint32_t)(135 - e) << 23);
-  return (int)fminf(fmaxf(__builtin_rintf(q), -127.f), 127.f);
+__device__ __forceinline__ uint32_t dense_rest_of(float x, uint32_t bits16) {
+  constexpr int S = dense_rest_bits<DT>();
+  const int left = (int)(__float_as_uint(x) - __float_as_uint(bits16_to_f32<DT>(bits16)));
+  const int q = (left + (1 << (S - 1))) >> S;
+  return (uint32_t)max(min(q, 127), -128) & 255u;
 }
+// (Infinities and NaN stay what they are: the one leaves nothing over, the other has room for a byte.)
 template <int DT>
 __device__ __forceinline__ float dense_with_rest(uint32_t bits16, int q) {
-  const int e = dense_place_exponent<DT>(bits16);
-  const float x = bits16_to_f32<DT>(bits16);
-  return e < -119 || e > 120 ? x : fmaf((float)q, __uint_as_float((uint32_t)(119 + e) << 23), x);
+  return __uint_as_float(__float_as_uint(bits16_to_f32<DT>(bits16)) + (uint32_t)(q * (1 << dense_rest_bits<DT>())));
 }
 
 // Position of 16-byte chunk cc of row r in LDS: of 16 consecutive rows the same chunk, and of 4
@@ -464,9 +460,12 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 31, half = lane >> 5;
   const typename X::Place place(lane);
-  const DensePlace at = dense_place((int64_t)p.N * p.Hq, p.tiles);
-  const int n = at.group / p.Hq, h = at.group % p.Hq, kvh = h / p.G;
-  const int tile = p.tiles - 1 - at.tile;  // the longest rows first
+  // The query heads of a KV head share an XCD's L2.
+  int64_t group;
+  int member;
+  xcd_group_map(blockIdx.x, (int64_t)p.N * p.Hkv, p.tiles * p.G, &group, &member);
+  const int n = (int)(group / p.Hkv), kvh = (int)(group % p.Hkv), h = kvh * p.G + member % p.G;
+  const int tile = p.tiles - 1 - member / p.G;  // the longest rows first
   const DenseSeq sq = dense_seq(p, n);
   dense_rest(p, sq, n, tile, tid, [&](int b, int t) {
     dense_clear<D>(p.o, b, t, h, tid);
@@ -580,7 +579,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const float x = oacc[dt][4 * g + e] * inv;
-          q |= ((uint32_t)dense_rest_of<DT>(x, f32_to16<DT>(x)) & 255u) << (8 * e);
+          q |= dense_rest_of<DT>(x, f32_to16<DT>(x)) << (8 * e);
         }
         *(uint32_t*)(to + dt * 32 + 8 * g) = q;
       }
@@ -615,9 +614,12 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 31, half = lane >> 5;
   const typename X::Place place(lane);
-  const DensePlace at = dense_place((int64_t)p.N * p.Hq, p.tiles);
-  const int n = at.group / p.Hq, h = at.group % p.Hq, kvh = h / p.G;
-  const int tile = p.tiles - 1 - at.tile;
+  // The query heads of a KV head share an XCD's L2.
+  int64_t group;
+  int member;
+  xcd_group_map(blockIdx.x, (int64_t)p.N * p.Hkv, p.tiles * p.G, &group, &member);
+  const int n = (int)(group / p.Hkv), kvh = (int)(group % p.Hkv), h = kvh * p.G + member % p.G;
+  const int tile = p.tiles - 1 - member / p.G;
   const DenseSeq sq = dense_seq(p, n);
   dense_rest(p, sq, n, tile, tid, [&](int b, int t) { dense_clear<D>(p.gq, b, t, h, tid); });
   const int r0 = tile * kDenseRows;
@@ -729,7 +731,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 31, half = lane >> 5;
   const typename X::Place place(lane);
-  // A group: the workgroups that walk over the same queries. Causal: the first keys are seen by the most rows.
+  // Causal: the first keys are seen by the most rows.
   const DensePlace at = dense_place((int64_t)p.N * p.Hkv * p.SG, p.tiles);
   const int sg = at.group % p.SG, kvh = at.group / p.SG % p.Hkv, n = at.group / p.SG / p.Hkv, tile = at.tile;
   const DenseSeq sq = dense_seq(p, n);
