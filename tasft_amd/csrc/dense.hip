@@ -158,10 +158,11 @@ __device__ __forceinline__ uint32_t dense_rest_of(float x, uint32_t bits16) {
   const int q = (left + (1 << (S - 1))) >> S;
   return (uint32_t)max(min(q, 127), -128) & 255u;
 }
-// (Infinities and NaN stay what they are: the one leaves nothing over, the other has room for a byte.)
+// (Infinities and NaN stay what they are, also where they came to a result after its rest.)
 template <int DT>
 __device__ __forceinline__ float dense_with_rest(uint32_t bits16, int q) {
-  return __uint_as_float(__float_as_uint(bits16_to_f32<DT>(bits16)) + (uint32_t)(q * (1 << dense_rest_bits<DT>())));
+  const uint32_t word = __float_as_uint(bits16_to_f32<DT>(bits16));
+  return __uint_as_float((word & 0x7f800000u) == 0x7f800000u ? word : word + (uint32_t)(q * (1 << dense_rest_bits<DT>())));
 }
 
 // Position of 16-byte chunk cc of row r in LDS: of 16 consecutive rows the same chunk, and of 4
