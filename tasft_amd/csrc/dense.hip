@@ -33,7 +33,8 @@ namespace tasft {
 
 constexpr int kDenseRows = 128;  // rows that a workgroup owns
 constexpr int kDenseTile = 64;   // rows of a tile that it walks over
-constexpr int kDenseStep = 32;   // the same of the kernel of dk and dv
+template <int D>
+constexpr int dense_step() { return D == 128 ? 32 : 64; }  // the same of the kernel of dk and dv
 constexpr int kDenseRun = 4;     // groups that an XCD takes at a time, see dense_place
 constexpr float kDenseMove = 8.f;  // a new maximum moves the exp2 reference only if this far above it
 constexpr float kDenseLn2 = 0.69314718055994531f;
@@ -718,13 +719,15 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
 // ---------------------------------------------------------------------------- backward: keys
 template <int D, int DT, bool CAP, bool BIAS>
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) dense_dkv_kernel(const DenseParams p) {
-  using X = DenseTiles<D, DT, kDenseStep>;
+  constexpr int STEP = dense_step<D>();
+  constexpr bool V_LDS = D == 128;
+  using X = DenseTiles<D, DT, STEP>;
   using V = DenseTiles<D, DT, kDenseRows>;
   __shared__ __attribute__((aligned(1024))) uint8_t q0_lds[X::TILE];
   __shared__ __attribute__((aligned(1024))) uint8_t g0_lds[X::TILE];
   __shared__ __attribute__((aligned(1024))) uint8_t q1_lds[X::TILE];
   __shared__ __attribute__((aligned(1024))) uint8_t g1_lds[X::TILE];
-  __shared__ __attribute__((aligned(1024))) uint8_t v_lds[V::TILE];
+  __shared__ __attribute__((aligned(1024))) uint8_t v_lds[V_LDS ? V::TILE : 16];
   __shared__ __attribute__((aligned(1024))) float st0_lds[2][kWave], st1_lds[2][kWave];  // lse, D
   __shared__ int found;
   const int tid = threadIdx.x, lane = tid & 63;
@@ -750,27 +753,30 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
   // by one before any_from.
   auto seen_from = [&](int key) { return p.causal && key >= sq.pre ? key : 0; };
   const int from = seen_from(j), all_from = seen_from(j_last), any_from = j_first <= j_last ? seen_from(j_first) : 0x7fffffff;
-  const int t_first = seen_from(r0) / kDenseStep, t_last = (sq.len - 1) / kDenseStep;
+  const int t_first = seen_from(r0) / STEP, t_last = (sq.len - 1) / STEP;
   const int g_first = kvh * p.G + sg * p.G / p.SG, heads = kvh * p.G + (sg + 1) * p.G / p.SG - g_first;
 
   const typename X::Share qoff(p.q.s[1], wave, lane), goff(p.go.s[1], wave, lane);
   const int64_t row0 = (int64_t)sq.b * p.T + sq.t0;
   auto bring = [&](uint8_t* qt, uint8_t* gt, float (*st)[kWave], int h, int t) TASFT_INLINE {
-    X::dma(qt, dense_at(p.q, sq, 0, h), p.q.s[1], qoff, t * kDenseStep, sq.len, wave);
-    X::dma(gt, dense_at(p.go, sq, 0, h), p.go.s[1], goff, t * kDenseStep, sq.len, wave);
-    if (wave < 2) {  // a row a lane (half of them are used); past the sequence's end zeros
-      const int rows = min(sq.len - t * kDenseStep, kWave);
-      const float* from = (wave == 0 ? p.less : p.di) + h * p.rows + row0 + t * kDenseStep;
+    X::dma(qt, dense_at(p.q, sq, 0, h), p.q.s[1], qoff, t * STEP, sq.len, wave);
+    X::dma(gt, dense_at(p.go, sq, 0, h), p.go.s[1], goff, t * STEP, sq.len, wave);
+    if (wave < 2) {  // a row a lane (at D = 128 half of them are used); past the sequence's end zeros
+      const int rows = min(sq.len - t * STEP, kWave);
+      const float* from = (wave == 0 ? p.less : p.di) + h * p.rows + row0 + t * STEP;
       const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)from, (short)0, rows * 4, 0x00020000);
       __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (TASFT_LDS void*)st[wave], 4, lane * 4, 0, 0, 0);
     }
   };
   bring(q0_lds, g0_lds, st0_lds, g_first, t_last);
 
-  // K as the B operand in registers; V, for which there is no room beside the sums, in LDS.
-  V::dma(v_lds, dense_at(p.v, sq, 0, kvh), p.v.s[1], typename V::Share(p.v.s[1], wave, lane), r0, sq.len, wave);
-  u32x4_t kf[X::KSTEPS];
+  // K as the B operand in registers; V too, or at D = 128, where there is no room for it beside the sums, in LDS.
+  u32x4_t kf[X::KSTEPS], vf[X::KSTEPS];
   X::load_row(kf, dense_at(p.k, sq, j, kvh), half);
+  if constexpr (V_LDS)
+    V::dma(v_lds, dense_at(p.v, sq, 0, kvh), p.v.s[1], typename V::Share(p.v.s[1], wave, lane), r0, sq.len, wave);
+  else
+    X::load_row(vf, dense_at(p.v, sq, j, kvh), half);
   f32x16_t ka[X::DTILES], va[X::DTILES];
 #pragma unroll
   for (int dt = 0; dt < X::DTILES; ++dt) ka[dt] = va[dt] = (f32x16_t){};
@@ -780,35 +786,40 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
     dense_barrier();
     if (hn >= 0) bring(qb, gb, stb, hn, tn);
     const float slope = BIAS ? p.sc.slopes[h] * p.sc.slope_mul : 0.f;
-    const int i0 = t * kDenseStep;
-    if (i0 + 31 < any_from) return;
-    const bool mixed = i0 < all_from;
-    const float* less = st[0] + 4 * half;
-    const float* di = st[1] + 4 * half;
-    const int from0 = from - i0 - 4 * half;
-    f32x16_t s = X::rows_times(qa, 0, kf, place), w;
-    u32x4_t b[2];
-    dense_weights<CAP, BIAS>(s, p.sc, slope, (float)(i0 + 4 * half - j), [&](int rr, float x, float g) {
-      w[rr] = __builtin_amdgcn_exp2f(fmaf(x, p.sc.mul, -less[8 * (rr >> 2) + (rr & 3)]));
-      return CAP ? w[rr] * g : w[rr];
-    });
-    if (mixed) {
-      asm volatile("");  // a branch, no selections in other tiles
 #pragma unroll
-      for (int rr = 0; rr < 16; ++rr) w[rr] = 8 * (rr >> 2) + (rr & 3) < from0 ? 0.f : w[rr];
+    for (int t2 = 0; t2 < STEP / 32; ++t2) {
+      const int i0 = t * STEP + 32 * t2;
+      if (i0 + 31 < any_from || (STEP > 32 && i0 >= sq.len)) continue;
+      const bool mixed = i0 < all_from;
+      const float* less = st[0] + 32 * t2 + 4 * half;
+      const float* di = st[1] + 32 * t2 + 4 * half;
+      const int from0 = from - i0 - 4 * half;
+      f32x16_t s = X::rows_times(qa, 32 * t2, kf, place), w;
+      u32x4_t b[2];
+      dense_weights<CAP, BIAS>(s, p.sc, slope, (float)(i0 + 4 * half - j), [&](int rr, float x, float g) {
+        w[rr] = __builtin_amdgcn_exp2f(fmaf(x, p.sc.mul, -less[8 * (rr >> 2) + (rr & 3)]));
+        return CAP ? w[rr] * g : w[rr];
+      });
+      if (mixed) {
+        asm volatile("");  // a branch, no selections in other tiles
+#pragma unroll
+        for (int rr = 0; rr < 16; ++rr) w[rr] = 8 * (rr >> 2) + (rr & 3) < from0 ? 0.f : w[rr];
+      }
+      X::pack(b, w);
+      X::template columns_times<D == 128 ? 2 : 1>(ga, 32 * t2, b, mixed, va, place, &found);
+      f32x16_t dp;
+      if constexpr (V_LDS) dp = X::rows_times_rows(ga, 32 * t2, v_lds, wave * 32, place);
+      else dp = X::rows_times(ga, 32 * t2, vf, place);
+#pragma unroll
+      for (int rr = 0; rr < 16; ++rr) s[rr] *= dp[rr] - di[8 * (rr >> 2) + (rr & 3)];
+      if (mixed) {
+        asm volatile("");
+#pragma unroll
+        for (int rr = 0; rr < 16; ++rr) s[rr] = 8 * (rr >> 2) + (rr & 3) < from0 ? 0.f : s[rr];
+      }
+      X::pack(b, s);
+      X::template columns_times<D == 128 ? 2 : 1>(qa, 32 * t2, b, mixed, ka, place, &found);
     }
-    X::pack(b, w);
-    X::template columns_times<D == 128 ? 2 : 1>(ga, 0, b, mixed, va, place, &found);
-    const f32x16_t dp = X::rows_times_rows(ga, 0, v_lds, wave * 32, place);
-#pragma unroll
-    for (int rr = 0; rr < 16; ++rr) s[rr] *= dp[rr] - di[8 * (rr >> 2) + (rr & 3)];
-    if (mixed) {
-      asm volatile("");
-#pragma unroll
-      for (int rr = 0; rr < 16; ++rr) s[rr] = 8 * (rr >> 2) + (rr & 3) < from0 ? 0.f : s[rr];
-    }
-    X::pack(b, s);
-    X::template columns_times<D == 128 ? 2 : 1>(qa, 0, b, mixed, ka, place, &found);
   };
   // From the last rows, which every key's workgroup walks over, to the first: the workgroups of a group read the
   // same tiles at the same time.
@@ -841,8 +852,8 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
         }
     }
   } else {
-    uint8_t* kst = v_lds + wave * (32 * X::ROWB);
     uint8_t* vst = (wave & 2 ? wave & 1 ? g1_lds : q1_lds : wave & 1 ? g0_lds : q0_lds);
+    uint8_t* kst = V_LDS ? v_lds + wave * (32 * X::ROWB) : vst + 32 * X::ROWB;
     X::store(kst, ka, pe->scale, dense_at(pe->gk, sq, 0, kvh), row_ok ? (int64_t)j * pe->gk.s[1] : -1, lane);
     X::store(vst, va, CAP ? 0.25f : 1.f, dense_at(pe->gv, sq, 0, kvh), row_ok ? (int64_t)j * pe->gv.s[1] : -1, lane);
   }
