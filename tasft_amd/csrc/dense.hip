@@ -950,12 +950,16 @@ static int dense_rows(DenseRows& r, const char* what, const char* name, const vo
   return kOk;
 }
 
-// Workgroups that share a KV head's query heads: as many as give four rounds of two workgroups on every CU, so
-// that causal rows of unequal length even out.
-static int dense_head_splits(int64_t num_seqs, int64_t num_kv_heads, int64_t group, int64_t max_seqlen) {
-  const int64_t wgs = num_seqs * num_kv_heads * ((max_seqlen + kDenseRows - 1) / kDenseRows);
-  const int64_t want = (2048 + wgs - 1) / wgs;
-  return (int)(want < group ? want : group);
+// Workgroups that share a KV head's query heads, so that there are two rounds of the 512 that the GPU holds, and
+// causal columns of unequal length even out: 4 x 2048 tokens of 32 / 8 heads backward and forward 819 us with one,
+// 760 with two, 817 with four, 899 with three (two heads, one, one); 16 x 1024 (1024 workgroups already) 873 with
+// one, 929 with two; ten ragged documents, 28 / 4 heads, 3930 and 3130. Their partial sums cost as much whatever
+// the sequences' length, so that long ones take four rounds (2 x 4096 1272 us with two, 1292 with four; 8192 2826
+// and 2780). Shares that would be of one and two heads become single heads.
+static int dense_head_splits(int64_t rows, int64_t num_kv_heads, int64_t group, int64_t max_seqlen) {
+  const int64_t wgs = (rows + kDenseRows - 1) / kDenseRows * num_kv_heads;
+  const int64_t want = ((max_seqlen >= 6144 ? 2048 : 1024) + wgs - 1) / wgs;
+  return (int)(2 * want > group && want > 1 ? group : want);
 }
 
 extern "C" size_t tasft_dense_bwd_workspace_bytes(int64_t num_seqs, int64_t rows, int64_t num_q_heads,
@@ -963,7 +967,7 @@ extern "C" size_t tasft_dense_bwd_workspace_bytes(int64_t num_seqs, int64_t rows
   if (num_seqs <= 0 || rows <= 0 || num_q_heads <= 0 || num_kv_heads <= 0 || max_seqlen <= 0 || head_dim <= 0 ||
       num_q_heads % num_kv_heads != 0)
     return 0;
-  const int sg = dense_head_splits(num_seqs, num_kv_heads, num_q_heads / num_kv_heads, max_seqlen);
+  const int sg = dense_head_splits(rows, num_kv_heads, num_q_heads / num_kv_heads, max_seqlen);
   const size_t stats = ((size_t)rows * num_q_heads * 8 + 15) / 16 * 16;
   return stats + (sg > 1 ? (size_t)sg * rows * num_kv_heads * head_dim * 8 : 0);
 }
@@ -1096,7 +1100,7 @@ extern "C" int tasft_dense_bwd(const void* q, const void* k, const void* v, cons
   p.sl[0] = lse_strides[0], p.sl[2] = lse_strides[1], p.sl[1] = lse_strides[2];
   p.glse = grad_lse;
   if (grad_lse) p.sgl[0] = glse_strides[0], p.sgl[2] = glse_strides[1], p.sgl[1] = glse_strides[2];
-  p.SG = dense_head_splits(num_seqs, num_kv_heads, p.G, p.L);
+  p.SG = dense_head_splits(p.rows, num_kv_heads, p.G, p.L);
   p.less = (float*)workspace;
   p.di = p.less + p.rows * p.Hq;
   const size_t stats = ((size_t)p.rows * p.Hq * 8 + 15) / 16 * 16;

@@ -103,7 +103,7 @@ def test_c_entries_refuse_before_any_launch():
     size = lib.tasft_dense_bwd_workspace_bytes(2, 20, 4, 2, 10, 64)
     assert size == 20 * 4 * 8 + 2 * 20 * 2 * 64 * 8  # statistics, two partial sums of dk and dv
     assert lib.tasft_dense_bwd_workspace_bytes(2, 20, 4, 3, 10, 64) == 0
-    assert lib.tasft_dense_bwd_workspace_bytes(1024, 20, 4, 2, 10, 64) == 20 * 4 * 8
+    assert lib.tasft_dense_bwd_workspace_bytes(1024, 70000, 4, 2, 100, 64) == 70000 * 4 * 8  # no partial sums
 
     def bwd(ws=fake, size=size, glse=None, rest=None):
         return lib.tasft_dense_bwd(fake, fake, fake, fake, fake, rest, fake, glse, fake, fake, fake, ws, size, None, None,
