@@ -791,20 +791,25 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
       const int i0 = t * STEP + 32 * t2;
       if (i0 + 31 < any_from || (STEP > 32 && i0 >= sq.len)) continue;
       const bool mixed = i0 < all_from;
+      // Rows behind the sequence's end came as zeros, and make weights of the bias alone (or NaN of an infinite key).
+      const bool cut = mixed || i0 + 31 >= sq.len;
       const float* less = st[0] + 32 * t2 + 4 * half;
       const float* di = st[1] + 32 * t2 + 4 * half;
-      const int from0 = from - i0 - 4 * half;
+      // Elements of rows that do not see the key become 0.
+      auto keep = [&](f32x16_t& x) TASFT_INLINE {
+        int first = from - i0 - 4 * half;
+        const uint32_t rows = sq.len - from;
+        asm volatile("" : "+v"(first));  // formed here, and a branch: no selections in other tiles
+#pragma unroll
+        for (int rr = 0; rr < 16; ++rr) x[rr] = (uint32_t)(8 * (rr >> 2) + (rr & 3) - first) < rows ? x[rr] : 0.f;
+      };
       f32x16_t s = X::rows_times(qa, 32 * t2, kf, place), w;
       u32x4_t b[2];
       dense_weights<CAP, BIAS>(s, p.sc, slope, (float)(i0 + 4 * half - j), [&](int rr, float x, float g) {
         w[rr] = __builtin_amdgcn_exp2f(fmaf(x, p.sc.mul, -less[8 * (rr >> 2) + (rr & 3)]));
         return CAP ? w[rr] * g : w[rr];
       });
-      if (mixed) {
-        asm volatile("");  // a branch, no selections in other tiles
-#pragma unroll
-        for (int rr = 0; rr < 16; ++rr) w[rr] = 8 * (rr >> 2) + (rr & 3) < from0 ? 0.f : w[rr];
-      }
+      if (cut) keep(w);
       X::pack(b, w);
       X::template columns_times<D == 128 ? 2 : 1>(ga, 32 * t2, b, mixed, va, place, &found);
       f32x16_t dp;
@@ -812,11 +817,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
       else dp = X::rows_times(ga, 32 * t2, vf, place);
 #pragma unroll
       for (int rr = 0; rr < 16; ++rr) s[rr] *= dp[rr] - di[8 * (rr >> 2) + (rr & 3)];
-      if (mixed) {
-        asm volatile("");
-#pragma unroll
-        for (int rr = 0; rr < 16; ++rr) s[rr] = 8 * (rr >> 2) + (rr & 3) < from0 ? 0.f : s[rr];
-      }
+      if (cut) keep(s);
       X::pack(b, s);
       X::template columns_times<D == 128 ? 2 : 1>(qa, 32 * t2, b, mixed, ka, place, &found);
     }

@@ -69,7 +69,7 @@ def reference(q, k, v, go, glse, *, causal, scale, cap, slopes, prefix, dtype):
         qh, kh, vh, out, lse = (x.detach() for x in (qh, kh, vh, out, lse))
         # Bounds.
         s = scores(qh, kh, scale, cap, slope)
-        far = slope * (torch.arange(n)[:, None] - torch.arange(n)[None]).abs()
+        far = abs(slope) * (torch.arange(n)[:, None] - torch.arange(n)[None]).abs()
         raw = qh.abs() @ kh.abs().t() * scale
         err = ((d + 3) * raw + 4 * (1 + raw + far)) * 2.0 ** -24
         if cap:

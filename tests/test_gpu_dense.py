@@ -270,6 +270,43 @@ def test_what_a_row_does_not_see_does_not_reach_it(cap, prefix, dtype):
     assert bool(torch.isnan(gk[see[at]]).all()) and bool(torch.isnan(gv[see[at]]).all())
 
 
+@pytest.mark.parametrize(("d", "dtype", "cap"), [(64, HF, 0), (128, BF, 0), (128, HF, 25.0), (64, BF, 25.0)])
+def test_slopes_that_favour_distance(d, dtype, cap):
+    """Negative slopes, whose bias alone is far above every score, at lengths that end inside a tile."""
+    dev = require_gpu()
+    lens, hq, hkv = [37, 211, 1], 4, 2
+    slopes = torch.tensor([-1.0, -0.25, 0.5, -0.0625])
+    rows = ref.inputs(lens, hq, hkv, d, dtype, seed=d)
+    want = [ref.reference(*r, causal=True, scale=1 / math.sqrt(d), cap=cap, slopes=slopes, prefix=0, dtype=dtype)
+            for r in rows]
+    q, k, v, go, gl = (ref.packed(r[i] for r in rows).to(dev) for i in range(5))
+    for x in (q, k, v):
+        x.requires_grad_(True)
+    offs = torch.tensor([0] + lens).cumsum(0).to(torch.int32)
+    print(f"dense negative slopes {d} {dtype} {cap}", flush=True)
+    out, lse = dense_attention(q, k, v, cu_seqlens=offs, return_lse=True, softcap=cap or None,
+                               alibi_slopes=slopes.to(dev))
+    grads = torch.autograd.grad((out, lse), (q, k, v), (go, gl))
+    check_all(out, lse, grads, want, lens, lambda x, n: x[offs[n]:offs[n + 1]])
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("causal", [True, False])
+def test_a_key_of_no_weight(d, causal):
+    """A key of -inf where every query is positive: its scores are -inf, its weight and gradients 0."""
+    dev = require_gpu()
+    n, at = 71, 40
+    q, k, v, go, _ = ref.inputs([n], 2, 1, d, BF, seed=6)[0]
+    q[..., 3] = q[..., 3].abs() + 1.0
+    k[at, 0, 3] = -math.inf
+    q, k, v = (x.to(dev).requires_grad_(True) for x in (q, k, v))
+    print(f"dense key of no weight {d} {causal}", flush=True)
+    out = dense_attention(q, k, v, cu_seqlens=torch.tensor([0, n]), causal=causal)
+    _, gk, gv = torch.autograd.grad(out, (q, k, v), go.to(dev))
+    assert bool(torch.isfinite(out).all()) and bool(torch.isfinite(gk).all()) and bool(torch.isfinite(gv).all())
+    assert not gk[at].any() and not gv[at].any() and bool(gv[at - 1].any())
+
+
 def test_max_seqlen_cuts():
     """Tokens behind a document's first max_seqlen are not there: their rows and gradients are 0."""
     dev = require_gpu()
