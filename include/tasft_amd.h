@@ -654,13 +654,13 @@ size_t tasft_dense_bwd_workspace_bytes(int64_t num_seqs, int64_t rows, int64_t n
 
 /*
  * Its backward: grad_q, grad_k (summed over the query heads of a KV head) and grad_v from out, lse and
- * out_rest of the forward (NULL: out as it was rounded), grad_out and grad_lse (NULL: none). Every sum has a fixed order. Rows without a token of a
- * sequence get 0. Gradients must not overlap anything else.
+ * out_rest of the forward (NULL: out as it was rounded), grad_out and grad_lse (NULL: none). Every sum has a
+ * fixed order. Rows without a token of a sequence get 0. Gradients must not overlap anything else.
  */
 int tasft_dense_bwd(const void* q, const void* k, const void* v, const void* out, const float* lse,
-                    const void* out_rest, const void* grad_out, const float* grad_lse, void* grad_q, void* grad_k, void* grad_v,
-                    void* workspace, size_t workspace_bytes, const int32_t* cu_seqlens, const int32_t* seq_lens,
-                    const int32_t* prefix_lens, const float* alibi_slopes, int64_t num_seqs, int64_t tokens,
+                    const void* out_rest, const void* grad_out, const float* grad_lse, void* grad_q, void* grad_k,
+                    void* grad_v, void* workspace, size_t workspace_bytes, const int32_t* cu_seqlens,
+                    const int32_t* seq_lens, const int32_t* prefix_lens, const float* alibi_slopes, int64_t num_seqs, int64_t tokens,
                     int64_t num_q_heads, int64_t num_kv_heads, int64_t max_seqlen, int64_t head_dim,
                     const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides,
                     const int64_t* o_strides, const int64_t* lse_strides, const int64_t* go_strides,
@@ -684,7 +684,7 @@ int tasft_dense_bwd(const void* q, const void* k, const void* v, const void* out
  * tasft_draft_commit_paged: the keys and values of node path[n][j] go from slot start + path[n][j] to
  * start + j, start = kv_lens[n] - (nodes of n), j < counts[n], in the pools and table of
  * tasft_chunk_paged_fwd (16-bit, strides (page, token, head, d)); slot_positions ([N][Hkv][slots], NULL: none)
- * alike; kv_lens_out[n] = start + counts[n]. max_nodes: the width of path. An index below its place or no
+ * alike; kv_lens_out[n] = start + counts[n]. max_nodes: the width of path. An index not past its place, or no
  * node's, a slot outside the table and a page outside the pool are not moved.
  */
 int tasft_draft_tree(const int32_t* parents, const int32_t* cu_seqlens, const int32_t* kv_lens,

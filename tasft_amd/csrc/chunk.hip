@@ -1443,8 +1443,8 @@ extern "C" int tasft_chunk_scored_fwd(
     int64_t num_splits, const int64_t* q_strides, const int64_t* kp_strides, const int64_t* vp_strides,
     const int64_t* o_strides, const int64_t* mask_strides, int64_t block_table_stride, float scale, float softcap,
     int causal, int dtype, void* stream) {
-  if (!(scale > 0.f) || !(softcap >= 0.f))
-    return set_error(kErrInvalidArgument, "chunk attention: scale must be positive and softcap not negative");
+  if (!score_range(scale, softcap))
+    return set_error(kErrInvalidArgument, "chunk attention: scale must be positive, softcap not negative, and neither out of range");
   if (ancestors && (ancestor_words <= 0 || ancestor_words > 1 << 20 || ((uintptr_t)ancestors & 7)))
     return set_error(kErrInvalidArgument, "chunk attention: ancestors must be 8-byte aligned rows of 1 to 2^20 words");
   ChunkParams p = {};
@@ -1456,7 +1456,6 @@ extern "C" int tasft_chunk_scored_fwd(
                    mask_rows, page_size, num_pages, max_pages, num_splits, q_strides, kp_strides, vp_strides, o_strides,
                    mask_strides, block_table_stride, scale, causal, dtype, stream, p, true);
 }
-
 
 template <int D, int DT>
 static void launch_weights(const WeightParams& w, hipStream_t stream) {

@@ -985,8 +985,8 @@ static int dense_params(DenseParams& p, const char* what, const int32_t* cu, con
     return set_error(kErrInvalidArgument, "%s: num_q_heads must be a multiple of num_kv_heads", what);
   if (head_dim != 64 && head_dim != 128)
     return set_error(kErrUnsupported, "%s: head_dim must be 64 or 128, got %lld", what, (long long)head_dim);
-  if (!(scale > 0.f) || !(softcap >= 0.f))
-    return set_error(kErrInvalidArgument, "%s: scale must be positive and softcap not negative", what);
+  if (!score_range(scale, softcap))
+    return set_error(kErrInvalidArgument, "%s: scale must be positive, softcap not negative, and neither out of range", what);
   if (cu && seq_lens) return set_error(kErrInvalidArgument, "%s: cu_seqlens or seq_lens, not both", what);
   const int64_t lim = 0x7fffffff - 255;
   if (num_seqs > lim || tokens > lim || num_q_heads > 65535 || (!cu && num_seqs * tokens > ((int64_t)1 << 40)))
@@ -1063,9 +1063,10 @@ extern "C" int tasft_dense_fwd(const void* q, const void* k, const void* v, void
 }
 
 extern "C" int tasft_dense_bwd(const void* q, const void* k, const void* v, const void* out, const float* lse,
-                               const void* out_rest, const void* grad_out, const float* grad_lse, void* grad_q, void* grad_k, void* grad_v,
-                               void* workspace, size_t workspace_bytes, const int32_t* cu_seqlens,
-                               const int32_t* seq_lens, const int32_t* prefix_lens, const float* alibi_slopes,
+                               const void* out_rest, const void* grad_out, const float* grad_lse, void* grad_q,
+                               void* grad_k, void* grad_v, void* workspace, size_t workspace_bytes,
+                               const int32_t* cu_seqlens, const int32_t* seq_lens, const int32_t* prefix_lens,
+                               const float* alibi_slopes,
                                int64_t num_seqs, int64_t tokens, int64_t num_q_heads, int64_t num_kv_heads,
                                int64_t max_seqlen, int64_t head_dim, const int64_t* q_strides, const int64_t* k_strides,
                                const int64_t* v_strides, const int64_t* o_strides, const int64_t* lse_strides,

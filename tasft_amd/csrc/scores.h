@@ -61,4 +61,11 @@ inline ScoreParams score_params(float scale, float softcap, const float* slopes)
   return s;
 }
 
+// Whether fp32 holds a scale, its cap and what is made of them.
+inline bool score_range(float scale, float softcap) {
+  const double most = 3e38, s = scale, c = softcap;
+  if (!(scale > 0.f) || !(softcap >= 0.f) || !(s * 1.5 < most) || !(1.0 / s < most)) return false;
+  return softcap == 0.f || (c * 3.0 < most && s / c * 3.0 < most);
+}
+
 }  // namespace tasft

@@ -640,8 +640,8 @@ class BlockSparseFlashAttention:
         ancestors: torch.Tensor | None = None,
     ) -> torch.Tensor | tuple[torch.Tensor, torch.Tensor]:
         """Attention of a chunk of new tokens of each sequence over its paged cache: a piece of a
-        long prompt, drafted tokens (a chain or a tree) to be checked, or one token each. The cache already holds the
-        new tokens (``append_paged``). The reference has no such call (its vLLM backend attends
+        long prompt, drafted tokens (a chain or a tree) to be checked, or one token each. The cache already
+        holds the new tokens (``append_paged``). The reference has no such call (its vLLM backend attends
         within the tokens of a call, ``tasft/inference/vllm_patch.py:172-176``).
 
         Args:

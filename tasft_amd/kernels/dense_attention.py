@@ -25,8 +25,8 @@ def check_softcap(softcap: float | None) -> float:
     if softcap is None:
         return 0.0
     softcap = float(softcap)
-    if not 0.0 < softcap < math.inf:
-        raise ValueError(f"softcap must be positive and finite, got {softcap}")
+    if not 1e-30 <= softcap <= 1e30:
+        raise ValueError(f"softcap must be positive and finite (1e-30 to 1e30), got {softcap}")
     return softcap
 
 
@@ -210,9 +210,10 @@ def dense_attention(
         included. What is kept for the backward: q, k, v, the output with a byte more an element, and the
         log-sums. In fp16 the weights' gradients are rounded to fp16 for their products: scale the loss,
         as for every fp16 gradient, so that they stay above 2^-14 where they matter.
-        An infinity of v whose weight rounds to 0 gives NaN in the rows that see it. A second derivative is refused. As for every operator of a graph of gradients: to
-        capture a backward pass into a HIP graph, drop eager results of the same leaves first (torch
-        ends the process otherwise).
+        A row all of whose scores are -inf is 0, with log-sum -inf (its gradients are NaN); an infinity of v
+        whose weight rounds to 0 gives NaN in the rows that see it. A second derivative is refused. As for
+        every operator of a graph of gradients: to capture a backward pass into a HIP graph, drop eager
+        results of the same leaves first (torch ends the process otherwise).
     """
     qs, dev = tuple(q.shape), q.device
     packed = cu_seqlens is not None
@@ -234,8 +235,8 @@ def dense_attention(
                           context={"head_dim": qs[-1], "supported": sorted(_VALID_HEAD_DIMS)})
     c.softcap = check_softcap(softcap)
     c.scale = 1.0 / math.sqrt(qs[-1]) if scale is None else float(scale)
-    if not 0.0 < c.scale < math.inf:
-        raise ValueError(f"scale must be positive and finite, got {scale}")
+    if not 1e-30 <= c.scale <= 1e30:
+        raise ValueError(f"scale must be positive and finite (1e-30 to 1e30), got {scale}")
     if prefix_lens is not None and not causal:
         raise ValueError("prefix_lens needs causal=True: without it every key is seen")
     if packed:

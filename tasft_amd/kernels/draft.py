@@ -187,7 +187,7 @@ def commit_draft_paged(
         block_table: ``[N, max_pages]``; kv_lens: ``[N]``, all nodes included, cu_seqlens: ``[N + 1]``, as in the
             step's other calls.
         path: ``[N, W]`` rising node indices, counts: ``[N]`` how many of them (``accept_draft``). An index that
-            does not rise, or is no node, is not moved.
+            is not past its own place in the path, or is no node, is not moved.
         slot_positions: ``[N, Hkv, max_pages * page_size]`` int32 contiguous, if kept: moved alike.
 
     Returns:

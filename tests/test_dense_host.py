@@ -46,6 +46,10 @@ def test_shapes_and_types(change, match):
     ({"softcap": -1.0}, ValueError, "softcap"),
     ({"softcap": math.inf}, ValueError, "softcap"),
     ({"softcap": math.nan}, ValueError, "softcap"),
+    ({"softcap": 1e-50}, ValueError, "softcap"),  # 0 in 32 bits
+    ({"softcap": 1e39}, ValueError, "softcap"),
+    ({"scale": 1e-50}, ValueError, "scale"),
+    ({"scale": 1e39}, ValueError, "scale"),
     ({"scale": 0.0}, ValueError, "scale"),
     ({"scale": math.nan}, ValueError, "scale"),
     ({"causal": False, "prefix_lens": torch.tensor([1, 1])}, ValueError, "prefix_lens"),
@@ -93,6 +97,10 @@ def test_c_entries_refuse_before_any_launch():
     refused(fwd(scale=0.0), -1, b"scale")
     refused(fwd(cap=-1.0), -1, b"softcap")
     refused(fwd(cap=float("nan")), -1, b"softcap")
+    refused(fwd(cap=float("inf")), -1, b"softcap")
+    refused(fwd(scale=float("inf")), -1, b"scale")
+    refused(fwd(scale=1e30, cap=1e-30), -1, b"out of range")  # their quotient
+    refused(fwd(scale=1e-39), -1, b"out of range")
     refused(fwd(cu=fake, lens=fake), -1, b"not both")
     refused(fwd(qs=_native.kept_strides((2560, 640, 64, 2))), -1, b"contiguous")
     refused(fwd(qs=_native.kept_strides((2560, 640, 68, 1))), -1, b"multiples of 8")
