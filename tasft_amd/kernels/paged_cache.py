@@ -272,7 +272,7 @@ def accumulate_key_weights(
     Args:
         q, k_pages, block_table, kv_lens, cu_seqlens, block_mask, max_seqlen, causal: as given to
             ``forward_chunk_paged`` (``block_size``: that of the attention object).
-        lse: ``[T, Hq]`` fp32, its second result.
+        lse: ``[T, Hq]`` fp32, its second result (of plain scores: a cap, slopes and a tree are not known here).
         scores: ``[N, Hkv, max_pages * page_size]`` fp32, or None for zeros; not changed.
 
     Returns:
