@@ -34,6 +34,14 @@
 // three workgroups a CU instead of four: 481 instead of 402 us); the same heads of every sequence on
 // one XCD (no gain, 376 instead of 362 us where a group's keys were then read twice); a higher wave
 // priority during the products (2% slower dense, 2% faster masked).
+//
+// Scored forms: a cap, a bias by distance or both (scores.h), chosen by uniform branches, and trees of new tokens,
+// whose rows see the cache and the nodes that their ancestor words name (cached tiles are as in a chain; only the
+// tiles with nodes look at the words). Beside the plain form: one token of 64 requests of up to 8192 keys, capped,
+// 317 us and 303 (HBM, 5.0 TB/s); 1024 tokens over 16384, 28 / 4 heads, biased, 295 and 255 (one instruction a
+// score more); trees of 64 nodes of 16 requests of up to 8192, 143 and 139.
+// Measured and not kept: the bias as what the products start from (16 instructions a tile less, 5 registers
+// spilled: 304 us instead of 302, and capped single tokens 339 instead of 312).
 #include <type_traits>
 
 #include "scores.h"
