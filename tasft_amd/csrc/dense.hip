@@ -28,7 +28,9 @@
 // 60 us (4.9 TB/s). Ten documents of up to 3500 tokens, 28 / 4 heads: 747, 984, 1482 and 43 us. 4 x 77 tokens: 11,
 // 12, 13 and 4 us, a chain of loads, products and stores.
 // Measured and not kept: the scores of the next tile beside the exponentials of this one (spilled: forward 2000 to
-// 3000 us instead of 700 to 800; with 512 registers and one wave a SIMD 1290 to 1420), two blocks of rows a wave
+// 3000 us instead of 700 to 800; with 512 registers and one wave a SIMD 1290 to 1420), the products of half a tile
+// instruction by instruction beside the exponentials of the other half (no spills; forward 815 us instead of 800 and
+// 775 instead of 757, steadily at work, where the clock falls with the power drawn), two blocks of rows a wave
 // with 512 registers (copies between register files and spills), a higher wave priority during the products (1%).
 #include <type_traits>
 
