@@ -98,6 +98,27 @@ def test_accept(index, first, dtype):
     assert got.next_tokens.dtype == dtype and got.next_tokens.tolist() == want[2]
 
 
+@pytest.mark.parametrize("stop", [1, 63, 64, 1000, 4096])
+def test_accept_chains(stop):
+    """The deepest trees there are: chains that agree up to a node, beside one that agrees to its end."""
+    dev = require_gpu()
+    sizes = [4096, 300, 1]
+    parents = [i - 1 for n in sizes for i in range(n)]
+    tokens = torch.ones(sum(sizes), dtype=torch.int64)
+    targets = tokens.clone()
+    if 0 < stop < 4096:
+        tokens[stop] = 7
+    cu = offsets(sizes)
+    want = ref.accept(parents, tokens.tolist(), targets.tolist(), cu.tolist(), None, 4096)
+    assert want[1] == [stop, 300, 1]
+    p = torch.tensor(parents, dtype=torch.int32, device=dev)
+    print(f"accept chain {stop}", flush=True)
+    got = accept_draft(p, tokens.to(dev), targets.to(dev), cu.to(dev), max_nodes=4096)
+    assert got.path.tolist() == want[0] and got.counts.tolist() == want[1] and got.next_tokens.tolist() == want[2]
+    tree = draft_tree(p, cu.to(dev), torch.tensor(sizes, device=dev), max_nodes=4096)
+    assert torch.equal(tree.ancestors.cpu(), ref.bits(ref.chains(parents, cu.tolist()), 64))
+
+
 def _pools(kv, sizes, hkv, d, page, dtype, seed, spare=2):
     _, k, v, table, lens, cu = paged_ref.make(sizes, kv, hkv, hkv, d, page, dtype, seed=seed, spare_pages=spare)
     return k.nan_to_num(3.0), v.nan_to_num(4.0, posinf=5.0), table, lens, cu
