@@ -15,8 +15,9 @@
 // the accumulator of S^T (or S) is the B operand of the product that follows, and the tiles that the
 // workgroup walks over lie in LDS, brought by DMA a tile ahead, read in rows and (transposed) in
 // columns. A workgroup owns 128 rows, four waves 32 each; tiles have 64 rows. P and dS are rounded to
-// the input type for their products (as the MFMA takes them): results are off by up to half a step of
-// their weighted magnitudes more than with P and dS in 32 bits. Maxima, sums and accumulators are fp32.
+// the input type for their products (as the MFMA takes them; dS of few rows in two parts, kDenseFew): results are
+// off by up to half a step of their weighted magnitudes more than with P and dS in 32 bits. Maxima, sums and
+// accumulators are fp32.
 //
 // Tokens that a row does not see do not reach it: where only some rows of a tile see a key, infinities
 // and NaN of what the zero weights would multiply are left out of the product and added to the rows
@@ -26,7 +27,7 @@
 // registers allow) overlap them in part. 8192 tokens, 32 / 8 heads of 128, bf16, capped: forward 672 us (0.82
 // PFLOP/s, MFMA busy 37%), dq 869 us (three products, 0.95, 44%), dk and dv 1169 us (four, 0.94, 43%), their join
 // 60 us (4.9 TB/s). Ten documents of up to 3500 tokens, 28 / 4 heads: 747, 984, 1482 and 43 us. 4 x 77 tokens: 11,
-// 12, 13 and 4 us, a chain of loads, products and stores.
+// 13, 15 and 4 us, a chain of loads, products and stores.
 // Measured and not kept: the scores of the next tile beside the exponentials of this one (spilled: forward 2000 to
 // 3000 us instead of 700 to 800; with 512 registers and one wave a SIMD 1290 to 1420), the products of half a tile
 // instruction by instruction beside the exponentials of the other half (no spills; forward 815 us instead of 800 and
@@ -47,6 +48,13 @@ constexpr int kDenseTile = 64;   // rows of a tile that it walks over
 template <int D>
 constexpr int dense_step() { return D == 128 ? 32 : 64; }  // the same of the kernel of dk and dv
 constexpr int kDenseRun = 4;     // groups that an XCD takes at a time, see dense_place
+// dS in two parts, what its rounding left over in a product of its own, where few roundings make a result: for
+// sequences of at most kDenseFew tokens (dq and dk of 2 to 11 tokens were off by 1.5 to 1.64 times what rounding the
+// result alone is, elsewhere by 1.47), and where a call has at most kDenseFewRows rows of all heads, which the host
+// bounds, to kDenseFewLen (4 x 77 tokens of 8 / 2 heads: dq 11.8 and 13.0 us, dk and dv 13.1 and 14.8, the call
+// 149 us with either; 64 x 256 tokens of 32 / 8, which do without, would take 517 us instead of 466).
+constexpr int kDenseFew = 32, kDenseFewLen = 512;
+constexpr int64_t kDenseFewRows = 32768;
 constexpr float kDenseMove = 8.f;  // a new maximum moves the exp2 reference only if this far above it
 constexpr float kDenseLn2 = 0.69314718055994531f;
 
@@ -77,6 +85,7 @@ struct DenseParams {
   int tiles;                // workgroups along a sequence
   int SG;                   // workgroups that share a KV head's query heads
   int causal;
+  int few;                  // sequences of at most so many tokens take dS in two parts
 };
 
 struct DenseSeq {
@@ -335,6 +344,17 @@ struct DenseTiles {
     for (int pp = 0; pp < 2; ++pp)
       b[pp] = (u32x4_t){pack16x2<DT>(s[8 * pp], s[8 * pp + 1]), pack16x2<DT>(s[8 * pp + 2], s[8 * pp + 3]),
                         pack16x2<DT>(s[8 * pp + 4], s[8 * pp + 5]), pack16x2<DT>(s[8 * pp + 6], s[8 * pp + 7])};
+  }
+  // What packing left over, packed (nothing of infinities).
+  static __device__ __forceinline__ void pack_rest(u32x4_t (&b)[2], const f32x16_t& s, const u32x4_t (&had)[2]) {
+#pragma unroll
+    for (int pp = 0; pp < 2; ++pp)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t w = had[pp][j];
+        b[pp][j] = dense_finite2<DT>(pack16x2<DT>(s[8 * pp + 2 * j] - bits16_to_f32<DT>(w & 0xffffu),
+                                                  s[8 * pp + 2 * j + 1] - bits16_to_f32<DT>(w >> 16)));
+      }
   }
   // A wave's 32 rows of the transposed accumulators times f, to `out` (row `col` at element `at`, < 0:
   // not there), whole rows through 32 rows of LDS of its own.
@@ -695,6 +715,11 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
       }
       u32x4_t sb[2];
       X::pack(sb, s);
+      if (sq.len <= p.few) {
+        u32x4_t lo[2];
+        X::pack_rest(lo, s, sb);
+        X::columns_times(ka, 32 * t2, lo, mixed, acc, place, &found);
+      }
       X::columns_times(ka, 32 * t2, sb, mixed, acc, place, &found);
     }
   };
@@ -830,6 +855,11 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
       for (int rr = 0; rr < 16; ++rr) s[rr] *= dp[rr] - di[8 * (rr >> 2) + (rr & 3)];
       if (cut) keep(s);
       X::pack(b, s);
+      if (sq.len <= p.few) {
+        u32x4_t lo[2];
+        X::pack_rest(lo, s, b);
+        X::template columns_times<D == 128 ? 2 : 1>(qa, 32 * t2, lo, mixed, ka, place, &found);
+      }
       X::template columns_times<D == 128 ? 2 : 1>(qa, 32 * t2, b, mixed, ka, place, &found);
     }
   };
@@ -1017,6 +1047,7 @@ static int dense_params(DenseParams& p, const char* what, const int32_t* cu, con
   p.tiles = (p.L + kDenseRows - 1) / kDenseRows;
   p.SG = 1;
   p.causal = causal;
+  p.few = p.rows * p.Hq <= kDenseFewRows ? kDenseFewLen : kDenseFew;
   // Launches of fewer than 2^32 threads.
   const int64_t most = 0xffffffffll / 256;
   if (num_seqs * num_q_heads > most || num_seqs * num_q_heads * p.tiles > most ||

@@ -307,6 +307,26 @@ def test_a_key_of_no_weight(d, causal):
     assert not gk[at].any() and not gv[at].any() and bool(gv[at - 1].any())
 
 
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("lens", [[2, 3, 2, 3], [5, 8, 11, 4], [60, 90], [400]])
+def test_few_rows_lose_little_to_the_rounding_of_ds(lens, dtype):
+    """The errors of dq and dk together against those of rounding the exact result alone: a second rounding of
+    the same relative size, of dS, would make it the square root of 2 in the mean, and by chance more."""
+    dev = require_gpu()
+    hq, hkv, d = 8, 2, 128
+    rows = ref.inputs(lens, hq, hkv, d, dtype, seed=sum(lens))
+    want = want_of((lens, hq, hkv, d, dtype, True, 0, False, None), rows, use_glse=False)
+    q, k, v, go = (ref.packed(r[i] for r in rows).to(dev) for i in range(4))
+    for x in (q, k, v):
+        x.requires_grad_(True)
+    print(f"dense few rows {lens} {dtype}", flush=True)
+    out = dense_attention(q, k, v, cu_seqlens=torch.tensor([0] + lens).cumsum(0))
+    for name, got in zip(("gq", "gk"), torch.autograd.grad(out, (q, k), go)):
+        exact = torch.cat([w[name] for w in want])
+        least = (exact.to(dtype).double() - exact).norm()
+        assert float((got.cpu().double() - exact).norm() / least) < math.sqrt(2), name
+
+
 def test_max_seqlen_cuts():
     """Tokens behind a document's first max_seqlen are not there: their rows and gradients are 0."""
     dev = require_gpu()
