@@ -50,11 +50,12 @@ constexpr int dense_step() { return D == 128 ? 32 : 64; }  // the same of the ke
 constexpr int kDenseRun = 4;     // groups that an XCD takes at a time, see dense_place
 // dS in two parts, what its rounding left over in a product of its own, where few roundings make a result: for
 // sequences of at most kDenseFew tokens (dq and dk of 2 to 11 tokens were off by 1.5 to 1.64 times what rounding the
-// result alone is, elsewhere by 1.47), and where a call has at most kDenseFewRows rows of all heads, which the host
-// bounds, to kDenseFewLen (4 x 77 tokens of 8 / 2 heads: dq 11.8 and 13.0 us, dk and dv 13.1 and 14.8, the call
-// 149 us with either; 64 x 256 tokens of 32 / 8, which do without, would take 517 us instead of 466).
-constexpr int kDenseFew = 32, kDenseFewLen = 512;
-constexpr int64_t kDenseFewRows = 32768;
+// result alone is, elsewhere by 1.47), and as long as a call's rows of all heads and their keys make at most
+// kDenseFewScores: that costs 10 us or so where the host bounds the call (4 x 77 tokens of 8 / 2 heads: dq 11.8 and
+// 13.0 us, dk and dv 13.1 and 14.8, 2 x 512 of 32 / 8 24.6 and 31.1, 33 and 41, the calls 150 us with either; 64 x
+// 256, which do without, would take 517 us instead of 466).
+constexpr int kDenseFew = 32;
+constexpr int64_t kDenseFewScores = 1 << 24;
 constexpr float kDenseMove = 8.f;  // a new maximum moves the exp2 reference only if this far above it
 constexpr float kDenseLn2 = 0.69314718055994531f;
 
@@ -1047,7 +1048,8 @@ static int dense_params(DenseParams& p, const char* what, const int32_t* cu, con
   p.tiles = (p.L + kDenseRows - 1) / kDenseRows;
   p.SG = 1;
   p.causal = causal;
-  p.few = p.rows * p.Hq <= kDenseFewRows ? kDenseFewLen : kDenseFew;
+  const int64_t few = kDenseFewScores / (p.rows * p.Hq);
+  p.few = (int)(few < kDenseFew ? kDenseFew : few);
   // Launches of fewer than 2^32 threads.
   const int64_t most = 0xffffffffll / 256;
   if (num_seqs * num_q_heads > most || num_seqs * num_q_heads * p.tiles > most ||
