@@ -205,6 +205,18 @@ __device__ __forceinline__ uint32_t dense_finite2(uint32_t w) {
   return w;
 }
 
+// a + both of a pair of 16-bit values, in fp32.
+template <int DT>
+__device__ __forceinline__ float dense_add2(uint32_t w, float a) {
+  if constexpr (DT == kF16) {
+    typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+    return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, w), __builtin_bit_cast(f16x2, 0x3c003c00u), a, false);
+  } else {
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, w), __builtin_bit_cast(bf16x2, 0x3f803f80u), a, false);
+  }
+}
+
 typedef uint16_t dense_u16x2_t __attribute__((ext_vector_type(2)));
 
 // What one of four waves does with tiles of ROWS rows in LDS.
@@ -338,6 +350,14 @@ struct DenseTiles {
         }
       if (PARTS > 1) __builtin_amdgcn_sched_barrier(0);
     }
+  }
+  // a + the sum of packed values.
+  static __device__ __forceinline__ float sum(const u32x4_t (&b)[2], float a) {
+#pragma unroll
+    for (int pp = 0; pp < 2; ++pp)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) a = dense_add2<DT>(b[pp][j], a);
+    return a;
   }
   // The registers of a 32 x 32 product as the B operand of columns_times.
   static __device__ __forceinline__ void pack(u32x4_t (&b)[2], const f32x16_t& s) {
@@ -529,7 +549,9 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
   f32x16_t oacc[X::DTILES];
 #pragma unroll
   for (int dt = 0; dt < X::DTILES; ++dt) oacc[dt] = (f32x16_t){};
-  float m_ref = -INFINITY, l_run = 0.f;
+  // The weights' sum, for the log-sum, and their sum as they were rounded, for the output: its error is then of
+  // what is added up less its mean, none where one key has all the weight (and D's, with the output, too).
+  float m_ref = -INFINITY, l_run = 0.f, l_out = 0.f;
 
   auto step = [&](const uint8_t* ka, const uint8_t* va, uint8_t* kb, uint8_t* vb, int t) TASFT_INLINE {
     __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0)
@@ -566,6 +588,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
     if (__ballot(move)) {
       const float alpha = move ? __builtin_amdgcn_exp2f(m_ref - mloc) : 1.f;
       l_run *= alpha;
+      l_out *= alpha;
 #pragma unroll
       for (int dt = 0; dt < X::DTILES; ++dt) oacc[dt] *= alpha;
       m_ref = move ? mloc : m_ref;
@@ -584,6 +607,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
     for (int t2 = 0; t2 < 2; ++t2) {
       u32x4_t pb[2];
       X::pack(pb, t2 ? s1 : s0);
+      l_out = X::sum(pb, l_out);
       X::columns_times(va, 32 * t2, pb, mixed, oacc, place, &found);
     }
   };
@@ -601,7 +625,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
   __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
   dense_barrier();                     // every wave is done with the tiles
   uint8_t* ost = ((wave & 2) ? v0_lds : k0_lds) + (wave & 1) * (32 * X::ROWB);
-  const float inv = 1.f / (l_tot > 0.f ? l_tot : 1.f);
+  const float l_div = pair_sum32(l_out), inv = 1.f / (l_div > 0.f ? l_div : 1.f);
   X::store(ost, oacc, inv, dense_at(pe->o, sq, 0, h), row_ok ? (int64_t)i * pe->o.s[1] : -1, lane);
   if (pe->rest && row_ok) {
     int8_t* to = pe->rest + (((int64_t)sq.b * pe->T + sq.t0 + i) * pe->Hq + h) * D + 4 * half;

@@ -308,6 +308,28 @@ def test_a_key_of_no_weight(d, causal):
 
 
 @pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("less", [14.5, 16.0, 17.5])
+def test_many_small_weights(less, dtype):
+    """One key far above 4000 others, whose weights (2^-less of its own) fp16 holds with few bits."""
+    dev = require_gpu()
+    n, d = 4001, 64
+    q = torch.zeros((n, 1, d), dtype=dtype)
+    q[..., 0] = 8.0
+    k = torch.zeros((n, 1, d), dtype=dtype)
+    k[0, 0, 0] = less * math.log(2.0)
+    v = torch.ones((n, 1, d), dtype=dtype)
+    v[0] = 0.0
+    print(f"dense small weights {less} {dtype}", flush=True)
+    out = dense_attention(*(x.to(dev) for x in (q, k, v)), cu_seqlens=torch.tensor([0, n]), causal=False)
+    small = math.exp(-float(k[0, 0, 0]))
+    want = 4000 * small / (1 + 4000 * small)
+    # P's rounding (fp16 below 2^-14: 2^-25 of a weight of 1), in the sum and in the divisor, and out's own.
+    u = ref.half_step(dtype)
+    bound = 3 * u * want + (2 * 4000 * 2.0 ** -25 if dtype == HF else 0.0) + 2.0 ** -12 * want
+    assert float((out.cpu().double() - want).abs().max()) <= bound
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
 @pytest.mark.parametrize("lens", [[2, 3, 2, 3], [5, 8, 11, 4], [60, 90], [400]])
 def test_few_rows_lose_little_to_the_rounding_of_ds(lens, dtype):
     """The errors of dq and dk together against those of rounding the exact result alone: a second rounding of
