@@ -24,9 +24,9 @@
 // that see them after the last tile.
 //
 // Bound by the products and the vector work of a wave following each other: two waves a SIMD (all that the
-// registers allow) overlap them in part. 8192 tokens, 32 / 8 heads of 128, bf16, capped: forward 672 us (0.82
-// PFLOP/s, MFMA busy 37%), dq 869 us (three products, 0.95, 44%), dk and dv 1169 us (four, 0.94, 43%), their join
-// 60 us (4.9 TB/s). Ten documents of up to 3500 tokens, 28 / 4 heads: 747, 984, 1482 and 43 us. 4 x 77 tokens: 11,
+// registers allow) overlap them in part. 8192 tokens, 32 / 8 heads of 128, bf16, capped: forward 689 us (0.80
+// PFLOP/s, MFMA busy 37%), dq 840 us (three products, 0.98, 47%), dk and dv 1160 us (four, 0.95, 43%), their join
+// 60 us (4.9 TB/s). Ten documents of up to 3500 tokens, 28 / 4 heads: 770, 985, 1430 and 44 us. 4 x 77 tokens: 11,
 // 13, 15 and 4 us, a chain of loads, products and stores.
 // Measured and not kept: the scores of the next tile beside the exponentials of this one (spilled: forward 2000 to
 // 3000 us instead of 700 to 800; with 512 registers and one wave a SIMD 1290 to 1420), the products of half a tile
@@ -550,7 +550,8 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
 #pragma unroll
   for (int dt = 0; dt < X::DTILES; ++dt) oacc[dt] = (f32x16_t){};
   // The weights' sum, for the log-sum, and their sum as they were rounded, for the output: its error is then of
-  // what is added up less its mean, none where one key has all the weight (and D's, with the output, too).
+  // what is added up less its mean, none where one key has all the weight (and D's, with the output, too: out was off
+  // by up to 1.24 times its own rounding without it and is by 1.17, dq by 1.50 and 1.47; 782 us became 801).
   float m_ref = -INFINITY, l_run = 0.f, l_out = 0.f;
 
   auto step = [&](const uint8_t* ka, const uint8_t* va, uint8_t* kb, uint8_t* vb, int t) TASFT_INLINE {

@@ -5,8 +5,8 @@
 //
 // All three are bound by latency: a few kilobytes, read by a chain of dependent loads. Parents are
 // brought to LDS once, so that a step up a tree costs an LDS read and not a trip to L2. 64 trees of 64 nodes, 8
-// deep: 3.1 us for the plan, 4.0 to accept; 4 of 500, 20 deep: 3.0 and 5.2. Kept nodes of 64 requests, 8 heads of
-// 128, moved: 8.4 us from an idle card; of one request 2.8.
+// deep: 3.0 us for the plan, 4.6 to accept; 4 of 500, 20 deep: 3.1 and 5.3. Kept nodes of 64 requests, 8 heads of
+// 128, moved: 8.2 us from an idle card; of one request 2.5.
 #include "common.h"
 
 #include "../../include/tasft_amd.h"
