@@ -639,7 +639,8 @@ int tasft_evict_paged(void* k_pages, void* v_pages, const int32_t* block_table, 
  * out_i = softmax_j(s) v_j, lse_i = log sum_j exp(s) (NULL: not wanted). Rows without a token of a
  * sequence: 0 and -inf. head_dim 64 or 128; strides (b, h, s, d) of q, k, v, out and (b, h, s) of lse.
  * out_rest (NULL: not wanted): a byte for each element of out, [rows][Hq][head_dim] (rows: tokens if packed, else
- * num_seqs * tokens), what its rounding left over, for the backward.
+ * num_seqs * tokens), what its rounding left over, for the backward. Scales and caps that fp32 does not hold,
+ * or not their quotient with all of its bits, are refused.
  */
 int tasft_dense_fwd(const void* q, const void* k, const void* v, void* out, float* lse, void* out_rest,
                     const int32_t* cu_seqlens, const int32_t* seq_lens, const int32_t* prefix_lens,

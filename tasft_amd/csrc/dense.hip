@@ -962,7 +962,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
 }
 
 // Joins the SG partial sums of every key's gradients: D / 4 lanes a row.
-template <int D, int DT>
+template <int D, int DT, bool CAP>
 __global__ void __launch_bounds__(256) dense_join_kernel(const DenseParams p) {
   constexpr int LPR = D / 4;
   const int64_t row = ((int64_t)blockIdx.x * 256 + threadIdx.x) / LPR;
@@ -992,7 +992,7 @@ __global__ void __launch_bounds__(256) dense_join_kernel(const DenseParams p) {
     v += *(const f32x4_t*)(p.part_v + at + s * step);
   }
   k *= p.scale;
-  if (p.sc.cap_in != 0.f) v *= 0.25f;  // (four times the weights, see dense_dq_kernel)
+  if (CAP) v *= 0.25f;  // (four times the weights, see dense_dq_kernel)
   *(u32x2_t*)(p.gk.p + b * p.gk.s[0] + (int64_t)t * p.gk.s[1] + kvh * p.gk.s[2] + c * 4) =
       (u32x2_t){pack16x2<DT>(k[0], k[1]), pack16x2<DT>(k[2], k[3])};
   *(u32x2_t*)(p.gv.p + b * p.gv.s[0] + (int64_t)t * p.gv.s[1] + kvh * p.gv.s[2] + c * 4) =
@@ -1187,7 +1187,7 @@ extern "C" int tasft_dense_bwd(const void* q, const void* k, const void* v, cons
                        dim3(256), 0, st, p);
     if (p.SG > 1) {
       const int64_t lanes = p.rows * p.Hkv * (d.value / 4);
-      hipLaunchKernelGGL((dense_join_kernel<d.value, dt.value>), dim3((unsigned)((lanes + 255) / 256)), dim3(256), 0, st, p);
+      hipLaunchKernelGGL((dense_join_kernel<d.value, dt.value, c.value>), dim3((unsigned)((lanes + 255) / 256)), dim3(256), 0, st, p);
     }
   });
   return check_launch(what);

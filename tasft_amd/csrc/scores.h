@@ -61,11 +61,12 @@ inline ScoreParams score_params(float scale, float softcap, const float* slopes)
   return s;
 }
 
-// Whether fp32 holds a scale, its cap and what is made of them.
+// Whether fp32 holds a scale, its cap and what is made of them (scale / cap too with all of its bits: rounded to 0
+// it would make every score 0, and no cap of one).
 inline bool score_range(float scale, float softcap) {
-  const double most = 3e38, s = scale, c = softcap;
+  const double most = 3e38, least = 1.2e-38, s = scale, c = softcap;
   if (!(scale > 0.f) || !(softcap >= 0.f) || !(s * 1.5 < most) || !(1.0 / s < most)) return false;
-  return softcap == 0.f || (c * 3.0 < most && s / c * 3.0 < most);
+  return softcap == 0.f || (c * 3.0 < most && s / c * 3.0 < most && s / c > least);
 }
 
 }  // namespace tasft

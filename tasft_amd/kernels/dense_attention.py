@@ -188,7 +188,7 @@ def dense_attention(
         k, v: ``[B, Hkv, S, D]`` / ``[T, Hkv, D]``, ``Hq % Hkv == 0`` (query head h reads KV head
             ``h // (Hq // Hkv)``).
         causal: token i sees keys ``j <= i`` of its sequence; False: all of them.
-        softcap: positive cap of the scores' magnitude.
+        softcap: positive cap of the scores' magnitude (and ``scale / softcap`` between 1e-37 and 1e37).
         alibi_slopes: ``[Hq]`` (fp32 on the device is read as it is).
         prefix_lens: ``[B]`` / ``[N]`` integers: with ``causal`` the first ``prefix_lens[n]`` tokens of a
             sequence are seen by all of its tokens.
