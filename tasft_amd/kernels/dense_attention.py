@@ -69,13 +69,18 @@ def _strides3(t: torch.Tensor):
 class _Call:
     """What a call's kernels take beside the tensors that they differentiate."""
 
-    __slots__ = ("causal", "cu", "dtype", "lens", "longest", "num_seqs", "prefix", "scale", "slopes", "softcap",
-                 "strides", "tokens")
+    __slots__ = ("causal", "cu", "dtype", "layout", "lens", "longest", "num_seqs", "prefix", "scale", "slopes",
+                 "softcap", "strides", "tokens")
 
 
 def _sizes(q: torch.Tensor, k: torch.Tensor, c: _Call):
     """num_seqs, tokens, q heads, KV heads, max_seqlen, head_dim of the C interface."""
     return c.num_seqs, c.tokens, q.shape[1], k.shape[1], c.longest, q.shape[-1]
+
+
+def _layout(q, k, v, out, lse):
+    """The strides that a call's saved tensors have."""
+    return q.stride(), k.stride(), v.stride(), out.stride(), None if lse is None else lse.stride()
 
 
 def _forward(q, k, v, c: _Call, want_lse: bool, want_kept: bool):
@@ -101,6 +106,8 @@ def _forward(q, k, v, c: _Call, want_lse: bool, want_kept: bool):
     heads, tokens = q.shape[1], c.tokens
     c.strides = (_strides4(q), _strides4(k), _strides4(v), _strides4(out),
                  _native.kept_strides((heads * tokens if q.ndim == 4 else 0, tokens, 1)))
+    if want_kept:
+        c.layout = _layout(q, k, v, out, lse)
     lib = _native.load_library()
     with _native.on_device(dev):
         status = lib.tasft_dense_fwd(
@@ -127,8 +134,16 @@ class _Dense(torch.autograd.Function):
             return None, None, None, None, None
         q, k, v, out, lse, kept, cu, lens, prefix, slopes = ctx.saved_tensors
         c = ctx.call
+        strides = c.strides if q.numel() else None
+        # Hooks on saved tensors (copies to host memory among them) give back values, not strides.
+        if strides and (_layout(q, k, v, out, lse) != c.layout or
+                        (q.data_ptr() | k.data_ptr() | v.data_ptr() | out.data_ptr()) & 15 or kept.data_ptr() & 7):
+            q, k, v, out, kept = _ready(q), _ready(k), _ready(v), _ready(out), kept.clone()
+            cu, lens, prefix, slopes = (None if t is None else t.contiguous() for t in (cu, lens, prefix, slopes))
+            strides = (_strides4(q), _strides4(k), _strides4(v), _strides4(out),
+                       strides[4] if lse is None else _strides3(lse))
         gq, gk, gv = _new_like(q), _new_like(k), _new_like(v)
-        if q.numel() == 0:
+        if not strides:
             return gq, gk, gv, None, None
         go = torch.zeros_like(out) if go is None else _ready(go)
         rest_ptr = kept.data_ptr()
@@ -142,7 +157,7 @@ class _Dense(torch.autograd.Function):
                 q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
                 rest_ptr + q.numel() if lse is None else lse.data_ptr(), rest_ptr, go.data_ptr(), _native.ptr(glse),
                 gq.data_ptr(), gk.data_ptr(), gv.data_ptr(), workspace.data_ptr(), ws_bytes, _native.ptr(cu),
-                _native.ptr(lens), _native.ptr(prefix), _native.ptr(slopes), *sizes, *c.strides, _strides4(go),
+                _native.ptr(lens), _native.ptr(prefix), _native.ptr(slopes), *sizes, *strides, _strides4(go),
                 None if glse is None else _strides3(glse), _strides4(gq), _strides4(gk), _strides4(gv), c.scale,
                 c.softcap, c.causal, c.dtype, _native.stream_handle(q.device))
         _native.check(status, "tasft_dense_bwd", {"q": list(q.shape), "k": list(k.shape)})

@@ -2,10 +2,15 @@
 from __future__ import annotations
 
 import ctypes
+import sys
 
 import pytest
+import torch
 
+import tasft_amd.kernels  # noqa: F401
 from tasft_amd import _native
+
+module = sys.modules["tasft_amd.kernels.dense_attention"]
 
 FAKE = ctypes.c_void_p(16)  # never dereferenced
 
@@ -22,3 +27,80 @@ def test_quotients_that_fp32_does_not_hold(scale, cap):
         FAKE, FAKE, FAKE, FAKE, None, None, FAKE, FAKE, FAKE, None, None, 0, None, 0, 2, 200, 4, 2, 100, 64, 64, 3, 8, 4,
         3, 1, st, st, st, st, st, 3, scale, cap, 1, 0, None)
     assert rc == -1 and b"out of range" in lib.tasft_last_error()
+
+
+class Recorder:
+    """Stands for the library: notes the addresses and strides that a backward call is given."""
+
+    def __init__(self):
+        self.seen = None
+
+    def tasft_dense_fwd(self, *args):
+        return 0
+
+    def tasft_dense_bwd_workspace_bytes(self, *args):
+        return 64
+
+    def tasft_dense_bwd(self, *args):
+        self.seen = args
+        return 0
+
+
+def fused(b, s, heads, d):
+    """Heads of a projection as views of it, [B, H, S, D]."""
+    wide = torch.zeros((b, s, sum(heads), d), dtype=torch.bfloat16)
+    return [x.transpose(1, 2) for x in wide.split(heads, 2)]
+
+
+@pytest.mark.parametrize("packed", [False, True])
+@pytest.mark.parametrize("return_lse", [False, True])
+@pytest.mark.parametrize("odd", [False, True])
+def test_backward_reads_saved_tensors_as_they_come_back(monkeypatch, packed, return_lse, odd):
+    """Hooks on saved tensors give back values, not strides (torch's own copies to host memory do not keep those
+    of a slice): each address goes to the kernels with the strides of the tensor that lies there."""
+    lib = Recorder()
+    monkeypatch.setattr(_native, "load_library", lambda: lib)
+    monkeypatch.setattr(_native, "stream_handle", lambda device: 0)
+    q, k, v = fused(2, 10, (4, 2, 2), 64)
+    if packed:
+        q, k, v = (x[0].transpose(0, 1) for x in (q, k, v))
+    q, k, v = (x.detach().requires_grad_(True) for x in (q, k, v))
+    assert not q.is_contiguous() and not k.is_contiguous()
+    c = module._Call()
+    c.causal, c.dtype, c.scale, c.softcap, c.longest = 1, 0, 0.125, 0.0, 10
+    c.num_seqs, c.tokens = (1 if packed else 2), 10
+    c.cu = torch.tensor([0, 10], dtype=torch.int32) if packed else None
+    c.lens = c.prefix = c.slopes = None
+    back = {}
+
+    def unpack(t):
+        # Dense, as from a buffer of many tensors, at a place that the kernels read or (odd) do not.
+        room = torch.empty(t.numel() * t.element_size() + 64, dtype=torch.uint8)
+        shift = (2 if t.dtype == torch.bfloat16 else 4) if odd else 0
+        off = -room.data_ptr() % 16 + shift
+        t = room[off:off + t.numel() * t.element_size()].view(t.dtype).view(t.shape).copy_(t)
+        back[t.data_ptr()] = t
+        return t
+
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t.detach().contiguous().clone(), unpack):
+        got = module._Dense.apply(q, k, v, c, return_lse)
+    out = got[0] if return_lse else got
+    copies = []
+    ready = module._ready
+    monkeypatch.setattr(module, "_ready", lambda t: copies.append(ready(t)) or copies[-1])
+    torch.autograd.grad(out.float().sum(), (q, k, v))
+    args = lib.seen
+    for t in copies:
+        back[t.data_ptr()] = t
+    sizes_at = next(i for i, a in enumerate(args) if not isinstance(a, (int, type(None))))  # the first strides
+    strides = args[sizes_at:sizes_at + 6]
+    for at, (name, like) in enumerate((("q", q), ("k", k), ("v", v), ("out", q))):
+        t = back[args[at]]
+        assert tuple(t.shape) == tuple(like.shape) and args[at] % 16 == 0, name
+        assert list(strides[at]) == list(module._strides4(t)), name
+    if return_lse:
+        t = back[args[4]]
+        assert list(strides[4]) == list(module._strides3(t))
+    else:
+        assert list(strides[4]) == [0 if packed else 40, 10, 1]
+    assert args[5] % 8 == 0  # what out's rounding left over
