@@ -11,6 +11,7 @@ from __future__ import annotations
 import math
 
 import torch
+from torch.autograd import forward_ad
 
 from tasft_amd import _native
 from tasft_amd._autograd import first_order_only
@@ -226,9 +227,9 @@ def dense_attention(
         log-sums. In fp16 the weights' gradients are rounded to fp16 for their products: scale the loss,
         as for every fp16 gradient, so that they stay above 2^-14 where they matter.
         A row all of whose scores are -inf is 0, with log-sum -inf (its gradients are NaN); an infinity of v
-        whose weight rounds to 0 gives NaN in the rows that see it. A second derivative is refused. As for
-        every operator of a graph of gradients: to capture a backward pass into a HIP graph, drop eager
-        results of the same leaves first (torch ends the process otherwise).
+        whose weight rounds to 0 gives NaN in the rows that see it. A second derivative and forward mode are
+        refused. As for every operator of a graph of gradients: to capture a backward pass into a HIP graph,
+        drop eager results of the same leaves first (torch ends the process otherwise).
     """
     qs, dev = tuple(q.shape), q.device
     packed = cu_seqlens is not None
@@ -283,6 +284,11 @@ def dense_attention(
             raise ValueError("max_seqlen goes with cu_seqlens")
         c.num_seqs, c.tokens, c.longest = qs[0], qs[2], max(qs[2], 1)
     c.causal = 1 if causal else 0
+    # (A dual tensor does not require grad.)
+    if forward_ad._current_level >= 0 and any(
+            t is not None and forward_ad.unpack_dual(t).tangent is not None for t in (q, k, v, alibi_slopes)):
+        raise KernelError("q, k, v and alibi_slopes must not carry tangents: dense attention has no forward-mode "
+                          "derivative", context={})
     if not q.is_cuda or k.device != dev or v.device != dev:
         raise KernelError("Tensors must be on one CUDA device",
                           context={"q": str(dev), "k": str(k.device), "v": str(v.device)})

@@ -6,9 +6,11 @@ import sys
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
-import tasft_amd.kernels  # noqa: F401
 from tasft_amd import _native
+from tasft_amd.exceptions import KernelError
+from tasft_amd.kernels import dense_attention
 
 module = sys.modules["tasft_amd.kernels.dense_attention"]
 
@@ -104,3 +106,19 @@ def test_backward_reads_saved_tensors_as_they_come_back(monkeypatch, packed, ret
     else:
         assert list(strides[4]) == [0 if packed else 40, 10, 1]
     assert args[5] % 8 == 0  # what out's rounding left over
+
+
+@pytest.mark.parametrize("which", range(4))
+@pytest.mark.parametrize("grad", [False, True])
+def test_tangents_are_refused(which, grad):
+    """A tangent would be lost: a dual tensor does not require grad."""
+    args = [torch.zeros((2, h, 10, 64), dtype=torch.bfloat16) for h in (4, 2, 2)] + [torch.ones(4)]
+    with torch.set_grad_enabled(grad), forward_ad.dual_level():
+        with pytest.raises(KernelError, match="one CUDA device"):  # what a level alone leaves as it is
+            dense_attention(*args[:3], alibi_slopes=args[3])
+        args[which] = forward_ad.make_dual(args[which], torch.ones_like(args[which]))
+        with pytest.raises(KernelError, match="forward-mode"):
+            dense_attention(*args[:3], alibi_slopes=args[3])
+    args = [torch.zeros((2, h, 10, 64), dtype=torch.bfloat16) for h in (4, 2, 2)]
+    with pytest.raises(KernelError, match="forward-mode"):
+        torch.func.jvp(lambda q: dense_attention(q, *args[1:]), (args[0],), (args[0],))
