@@ -77,11 +77,11 @@ def _check_tree(parents: torch.Tensor, cu_seqlens: torch.Tensor, max_nodes: int 
     return max_nodes
 
 
-def _parents_on(parents: torch.Tensor, device: torch.device) -> torch.Tensor:
-    """``parents`` as the kernels read them; what 32 bits do not hold is no node."""
-    if parents.dtype == torch.int64 and not parents.is_cpu:
-        parents = parents.clamp(-1, 0x7fffffff)
-    return int32_on(parents, device)
+def _nodes_on(nodes: torch.Tensor, device: torch.device) -> torch.Tensor:
+    """Indices of nodes (or how many there are) as the kernels read them; what 32 bits do not hold stays no node."""
+    if nodes.dtype == torch.int64:
+        nodes = nodes.clamp(-1, 0x7fffffff)
+    return int32_on(nodes, device)
 
 
 def draft_tree(parents: torch.Tensor, cu_seqlens: torch.Tensor, kv_lens: torch.Tensor, *,
@@ -113,7 +113,7 @@ def draft_tree(parents: torch.Tensor, cu_seqlens: torch.Tensor, kv_lens: torch.T
     positions = torch.empty((T,), dtype=torch.int32, device=dev)
     if T == 0:
         return DraftTree(ancestors, positions)
-    parents, cu, lens = _parents_on(parents, dev), int32_on(cu_seqlens, dev), int32_on(kv_lens, dev)
+    parents, cu, lens = _nodes_on(parents, dev), int32_on(cu_seqlens, dev), int32_on(kv_lens, dev)
     with _native.on_device(dev):
         status = _native.load_library().tasft_draft_tree(
             parents.data_ptr(), cu.data_ptr(), lens.data_ptr(), ancestors.data_ptr(), positions.data_ptr(), n, T, most,
@@ -157,7 +157,7 @@ def accept_draft(parents: torch.Tensor, tokens: torch.Tensor, targets: torch.Ten
     if T == 0:
         following = following.fill_(-1) if first_targets is None else first_targets.clone()
         return AcceptedDraft(path.fill_(-1), counts.zero_(), following)
-    parents, cu = _parents_on(parents, dev), int32_on(cu_seqlens, dev)
+    parents, cu = _nodes_on(parents, dev), int32_on(cu_seqlens, dev)
     tokens, targets = tokens.contiguous(), targets.contiguous()
     with _native.on_device(dev):
         status = _native.load_library().tasft_draft_accept(
@@ -225,7 +225,7 @@ def commit_draft_paged(
         raise KernelError("Tensors must be on one CUDA device",
                           context={"k_pages": str(dev), "v_pages": str(v_pages.device)})
     table, lens, cu = int32_on(block_table, dev), int32_on(kv_lens, dev), int32_on(cu_seqlens, dev)
-    path, counts = int32_on(path, dev), int32_on(counts, dev)
+    path, counts = _nodes_on(path, dev), _nodes_on(counts, dev)
     out = torch.empty((n,), dtype=torch.int32, device=dev)
     with _native.on_device(dev):
         status = _native.load_library().tasft_draft_commit_paged(
