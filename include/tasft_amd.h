@@ -649,7 +649,8 @@ int tasft_dense_fwd(const void* q, const void* k, const void* v, void* out, floa
                     const int64_t* k_strides, const int64_t* v_strides, const int64_t* o_strides,
                     const int64_t* lse_strides, float scale, float softcap, int causal, int dtype, void* stream);
 
-/* Bytes of workspace tasft_dense_bwd needs; rows: tokens if packed, else num_seqs * tokens. */
+/* Bytes of workspace tasft_dense_bwd needs; rows: tokens if packed, else num_seqs * tokens; max_seqlen as it is
+ * given to tasft_dense_bwd (without cu_seqlens it limits nothing; how the heads are shared out goes by it). */
 size_t tasft_dense_bwd_workspace_bytes(int64_t num_seqs, int64_t rows, int64_t num_q_heads,
                                        int64_t num_kv_heads, int64_t max_seqlen, int64_t head_dim);
 

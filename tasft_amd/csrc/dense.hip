@@ -1159,8 +1159,8 @@ extern "C" int tasft_dense_bwd(const void* q, const void* k, const void* v, cons
     return set_error(kErrInvalidArgument, "dense attention backward: null pointer argument");
   if (!strides_nonneg(lse_strides, 3) || (grad_lse && !strides_nonneg(glse_strides, 3)))
     return set_error(kErrInvalidArgument, "dense attention backward: strides must be non-negative");
-  if (!workspace || workspace_bytes < tasft_dense_bwd_workspace_bytes(num_seqs, p.rows, num_q_heads, num_kv_heads, p.L,
-                                                                      head_dim))
+  if (!workspace || workspace_bytes < tasft_dense_bwd_workspace_bytes(num_seqs, p.rows, num_q_heads, num_kv_heads,
+                                                                      max_seqlen, head_dim))
     return set_error(kErrWorkspace, "dense attention backward: workspace too small");
   if ((uintptr_t)workspace & 15)
     return set_error(kErrInvalidArgument, "dense attention backward: workspace must be 16-byte aligned");
@@ -1171,7 +1171,7 @@ extern "C" int tasft_dense_bwd(const void* q, const void* k, const void* v, cons
   p.sl[0] = lse_strides[0], p.sl[2] = lse_strides[1], p.sl[1] = lse_strides[2];
   p.glse = grad_lse;
   if (grad_lse) p.sgl[0] = glse_strides[0], p.sgl[2] = glse_strides[1], p.sgl[1] = glse_strides[2];
-  p.SG = dense_head_splits(p.rows, num_kv_heads, p.G, p.L);
+  p.SG = dense_head_splits(p.rows, num_kv_heads, p.G, max_seqlen);  // as given: as the workspace's size was asked for
   p.less = (float*)workspace;
   p.di = p.less + p.rows * p.Hq;
   const size_t stats = ((size_t)p.rows * p.Hq * 8 + 15) / 16 * 16;

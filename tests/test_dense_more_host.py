@@ -122,3 +122,23 @@ def test_tangents_are_refused(which, grad):
     args = [torch.zeros((2, h, 10, 64), dtype=torch.bfloat16) for h in (4, 2, 2)]
     with pytest.raises(KernelError, match="forward-mode"):
         torch.func.jvp(lambda q: dense_attention(q, *args[1:]), (args[0],), (args[0],))
+
+
+@pytest.mark.parametrize("packed", [False, True])
+@pytest.mark.parametrize("most", [5000, 6144, 8192, 100000])
+def test_backward_workspace_is_what_its_size_was_asked_for(packed, most):
+    """Whatever max_seqlen is given: the size function and the backward go by the same number."""
+    lib = _native.load_library()
+    tokens, hq, hkv, d = 8192, 32, 8, 64
+    size = lib.tasft_dense_bwd_workspace_bytes(1, tokens, hq, hkv, most, d)
+    st = _native.kept_strides((hq * tokens * d, tokens * d, d, 1))
+    sl = _native.kept_strides((hq * tokens, tokens, 1))
+    unaligned = ctypes.c_void_p(8)
+
+    def call(given):
+        return lib.tasft_dense_bwd(FAKE, FAKE, FAKE, FAKE, FAKE, None, FAKE, None, FAKE, FAKE, FAKE, unaligned, given,
+                                   FAKE if packed else None, None, None, None, 1, tokens, hq, hkv, most, d, st, st, st, st,
+                                   sl, st, None, st, st, st, 0.1, 0.0, 1, 0, None)
+
+    assert call(size) == -1 and b"aligned" in lib.tasft_last_error()  # enough: what is refused next is its address
+    assert call(size - 1) == -4 and b"workspace" in lib.tasft_last_error()
