@@ -8,6 +8,7 @@ the same scores in ``BlockSparseFlashAttention.forward_chunk_paged``.
 """
 from __future__ import annotations
 
+import functools
 import math
 
 import torch
@@ -55,33 +56,26 @@ def _new_like(t: torch.Tensor) -> torch.Tensor:
     return out if _native.kernel_layout(out) else torch.empty(t.shape, dtype=t.dtype, device=t.device)
 
 
-def _strides4(t: torch.Tensor):
-    """(b, h, s, d) strides of ``[B, H, S, D]``, or of packed ``[T, H, D]`` as one batch entry."""
-    st = t.stride()
+def _strides4(st: tuple[int, ...]):
+    """(b, h, s, d) strides of ``[B, H, S, D]``, or of packed ``[T, H, D]`` as one batch entry, from a tensor's."""
     return _native.kept_strides(st if len(st) == 4 else (0, st[1], st[0], st[2]))
 
 
-def _strides3(t: torch.Tensor):
-    """(b, h, s) strides of ``[B, H, S]``, or of ``[T, H]``."""
-    st = t.stride()
+def _strides3(st: tuple[int, ...]):
+    """(b, h, s) strides of ``[B, H, S]``, or of ``[T, H]``, from a tensor's."""
     return _native.kept_strides(st if len(st) == 3 else (0, st[1], st[0]))
 
 
 class _Call:
     """What a call's kernels take beside the tensors that they differentiate."""
 
-    __slots__ = ("causal", "cu", "dtype", "layout", "lens", "longest", "num_seqs", "prefix", "scale", "slopes",
+    __slots__ = ("causal", "cu", "dtype", "layout", "lens", "longest", "num_seqs", "prefix", "scale", "sizes", "slopes",
                  "softcap", "strides", "tokens")
 
 
-def _sizes(q: torch.Tensor, k: torch.Tensor, c: _Call):
-    """num_seqs, tokens, q heads, KV heads, max_seqlen, head_dim of the C interface."""
-    return c.num_seqs, c.tokens, q.shape[1], k.shape[1], c.longest, q.shape[-1]
-
-
-def _layout(q, k, v, out, lse):
-    """The strides that a call's saved tensors have."""
-    return q.stride(), k.stride(), v.stride(), out.stride(), None if lse is None else lse.stride()
+@functools.lru_cache(maxsize=1024)
+def _workspace_bytes(num_seqs: int, rows: int, *sizes: int) -> int:
+    return _native.load_library().tasft_dense_bwd_workspace_bytes(num_seqs, rows, *sizes)
 
 
 def _forward(q, k, v, c: _Call, want_lse: bool, want_kept: bool):
@@ -105,15 +99,15 @@ def _forward(q, k, v, c: _Call, want_lse: bool, want_kept: bool):
         return out, lse, kept
     # (b, h, s) strides of the log-sums, [B, H, S] or the transpose of [H, T].
     heads, tokens = q.shape[1], c.tokens
-    c.strides = (_strides4(q), _strides4(k), _strides4(v), _strides4(out),
-                 _native.kept_strides((heads * tokens if q.ndim == 4 else 0, tokens, 1)))
-    if want_kept:
-        c.layout = _layout(q, k, v, out, lse)
+    # num_seqs, tokens, q heads, KV heads, max_seqlen, head_dim of the C interface.
+    c.sizes = c.num_seqs, tokens, heads, k.shape[1], c.longest, q.shape[-1]
+    c.layout = q.stride(), k.stride(), v.stride(), out.stride()
+    c.strides = (*map(_strides4, c.layout), _native.kept_strides((heads * tokens if q.ndim == 4 else 0, tokens, 1)))
     lib = _native.load_library()
     with _native.on_device(dev):
         status = lib.tasft_dense_fwd(
             q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse_ptr, rest_ptr, _native.ptr(c.cu),
-            _native.ptr(c.lens), _native.ptr(c.prefix), _native.ptr(c.slopes), *_sizes(q, k, c), *c.strides, c.scale,
+            _native.ptr(c.lens), _native.ptr(c.prefix), _native.ptr(c.slopes), *c.sizes, *c.strides, c.scale,
             c.softcap, c.causal, c.dtype, _native.stream_handle(dev))
     _native.check(status, "tasft_dense_fwd", {"q": list(q.shape), "k": list(k.shape)})
     return out, lse, kept
@@ -135,32 +129,33 @@ class _Dense(torch.autograd.Function):
             return None, None, None, None, None
         q, k, v, out, lse, kept, cu, lens, prefix, slopes = ctx.saved_tensors
         c = ctx.call
-        strides = c.strides if q.numel() else None
+        gq, gk, gv = _new_like(q), _new_like(k), _new_like(v)
+        if q.numel() == 0:
+            return gq, gk, gv, None, None
         # Hooks on saved tensors (copies to host memory among them) give back values, not strides.
-        if strides and (_layout(q, k, v, out, lse) != c.layout or
-                        (q.data_ptr() | k.data_ptr() | v.data_ptr() | out.data_ptr()) & 15 or kept.data_ptr() & 7):
+        strides, layout = c.strides, (q.stride(), k.stride(), v.stride(), out.stride())
+        at = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr()
+        if layout != c.layout or (at[0] | at[1] | at[2] | at[3]) & 15 or kept.data_ptr() & 7:
             q, k, v, out, kept = _ready(q), _ready(k), _ready(v), _ready(out), kept.clone()
             cu, lens, prefix, slopes = (None if t is None else t.contiguous() for t in (cu, lens, prefix, slopes))
-            strides = (_strides4(q), _strides4(k), _strides4(v), _strides4(out),
-                       strides[4] if lse is None else _strides3(lse))
-        gq, gk, gv = _new_like(q), _new_like(k), _new_like(v)
-        if not strides:
-            return gq, gk, gv, None, None
+            strides = (*(_strides4(t.stride()) for t in (q, k, v, out)), strides[4])
+            at = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr()
+        if lse is not None:
+            strides = (*strides[:4], _strides3(lse.stride()))
         go = torch.zeros_like(out) if go is None else _ready(go)
         rest_ptr = kept.data_ptr()
         lib = _native.load_library()
-        sizes = _sizes(q, k, c)
         rows = c.tokens if cu is not None else c.num_seqs * c.tokens
-        ws_bytes = lib.tasft_dense_bwd_workspace_bytes(sizes[0], rows, *sizes[2:])
+        ws_bytes = _workspace_bytes(c.num_seqs, rows, *c.sizes[2:])
         workspace = torch.empty((ws_bytes,), dtype=torch.uint8, device=q.device)
         with _native.on_device(q.device):
             status = lib.tasft_dense_bwd(
-                q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
-                rest_ptr + q.numel() if lse is None else lse.data_ptr(), rest_ptr, go.data_ptr(), _native.ptr(glse),
-                gq.data_ptr(), gk.data_ptr(), gv.data_ptr(), workspace.data_ptr(), ws_bytes, _native.ptr(cu),
-                _native.ptr(lens), _native.ptr(prefix), _native.ptr(slopes), *sizes, *strides, _strides4(go),
-                None if glse is None else _strides3(glse), _strides4(gq), _strides4(gk), _strides4(gv), c.scale,
-                c.softcap, c.causal, c.dtype, _native.stream_handle(q.device))
+                *at, rest_ptr + q.numel() if lse is None else lse.data_ptr(), rest_ptr, go.data_ptr(),
+                _native.ptr(glse), gq.data_ptr(), gk.data_ptr(), gv.data_ptr(), workspace.data_ptr(), ws_bytes,
+                _native.ptr(cu), _native.ptr(lens), _native.ptr(prefix), _native.ptr(slopes), *c.sizes, *strides,
+                _strides4(go.stride()), None if glse is None else _strides3(glse.stride()), _strides4(gq.stride()),
+                _strides4(gk.stride()), _strides4(gv.stride()), c.scale, c.softcap, c.causal, c.dtype,
+                _native.stream_handle(q.device))
         _native.check(status, "tasft_dense_bwd", {"q": list(q.shape), "k": list(k.shape)})
         return gq, gk, gv, None, None
 
