@@ -39,7 +39,10 @@
 // whose rows see the cache and the nodes that their ancestor words name (cached tiles are as in a chain; only the
 // tiles with nodes look at the words). Beside the plain form: one token of 64 requests of up to 8192 keys, capped,
 // 317 us and 303 (HBM, 5.0 TB/s); 1024 tokens over 16384, 28 / 4 heads, biased, 295 and 255 (one instruction a
-// score more); trees of 64 nodes of 16 requests of up to 8192, 143 and 139.
+// score more); trees of 64 nodes of 16 requests of up to 8192, 143 and 139 (the former 138 on a rested card, 170 after
+// twenty launches in a row).
+// The tree kernels keep 65 to 75 scalar registers in vector ones, the scored masked ones 8 to 40 (plain: at most 13),
+// and with pages of 8 tokens at heads of 128 the tree kernels a vector register in scratch memory.
 // Measured and not kept: the bias as what the products start from (16 instructions a tile less, 5 registers
 // spilled: 304 us instead of 302, and capped single tokens 339 instead of 312).
 #include <type_traits>

@@ -24,10 +24,14 @@
 // that see them after the last tile.
 //
 // Bound by the products and the vector work of a wave following each other: two waves a SIMD (all that the
-// registers allow) overlap them in part. 8192 tokens, 32 / 8 heads of 128, bf16, capped: forward 689 us (0.80
-// PFLOP/s, MFMA busy 37%), dq 840 us (three products, 0.98, 47%), dk and dv 1160 us (four, 0.95, 43%), their join
-// 60 us (4.9 TB/s). Ten documents of up to 3500 tokens, 28 / 4 heads: 770, 985, 1430 and 44 us. 4 x 77 tokens: 11,
-// 13, 15 and 4 us, a chain of loads, products and stores.
+// registers allow) overlap them in part. 8192 tokens, 32 / 8 heads of 128, bf16, capped: forward 693 us (0.79
+// PFLOP/s, MFMA busy 37% of the cycles, the vector unit 66%: a capped score takes two exponentials and a
+// reciprocal), dq 852 us (three products, 0.97, 47 and 63%), dk and dv 1177 us (four, 0.93, 43 and 51%), their join
+// 59 us (5.0 TB/s). Ten documents of up to 3500 tokens, 28 / 4 heads: 765 (41 and 43%), 974 (48 and 35%), 1468 (42
+// and 31%) and 42 us. 4 x 77 tokens: 11, 13, 15 and 4 us, a chain of loads, products and stores. (Medians of 23
+// launches in a row; the clock moves them: the forward's first three took 843 us, its last ten 668.)
+// At heads of 128 the kernel of dk and dv keeps 11 registers in scratch memory with a cap and a bias, one with a cap
+// alone; no other kernel does.
 // Measured and not kept: the scores of the next tile beside the exponentials of this one (spilled: forward 2000 to
 // 3000 us instead of 700 to 800; with 512 registers and one wave a SIMD 1290 to 1420), the products of half a tile
 // instruction by instruction beside the exponentials of the other half (no spills; forward 815 us instead of 800 and
@@ -1022,8 +1026,10 @@ static int dense_rows(DenseRows& r, const char* what, const char* name, const vo
 // causal columns of unequal length even out: 4 x 2048 tokens of 32 / 8 heads backward and forward 819 us with one,
 // 760 with two, 817 with four, 899 with three (two heads, one, one); 16 x 1024 (1024 workgroups already) 873 with
 // one, 929 with two; ten ragged documents, 28 / 4 heads, 3930 and 3130. Their partial sums cost as much whatever
-// the sequences' length, so that long ones take four rounds (2 x 4096 1272 us with two, 1292 with four; 8192 2826
-// and 2780). Shares that would be of one and two heads become single heads.
+// the sequences' length, so that long ones take four rounds. In turn on one card, two rounds and four: ten documents
+// 3150 us and 3620, 4 x 2048 capped and biased 957 and 1019, 2 x 4096 1256 and 1286, 8192 2357 and 2335 (capped 2757
+// and 2723), 2 x 8192 4705 and 4641: little to gain beyond 6144, but to lose before it. Shares that would be of one
+// and two heads become single heads.
 static int dense_head_splits(int64_t rows, int64_t num_kv_heads, int64_t group, int64_t max_seqlen) {
   const int64_t wgs = (rows + kDenseRows - 1) / kDenseRows * num_kv_heads;
   const int64_t want = ((max_seqlen >= 6144 ? 2048 : 1024) + wgs - 1) / wgs;

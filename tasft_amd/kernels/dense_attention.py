@@ -3,8 +3,8 @@ documents and prefixes.
 
 The reference trains its gates beside attention that it computes densely, storing the
 ``[B, H, S, S]`` scores (``tasft/modules/tasft_attention.py:426-466``); ``gate_target_from_qk`` takes
-the gate's target from Q and K without them, and ``dense_attention`` the attention itself. Serving has
-the same scores in ``BlockSparseFlashAttention.forward_chunk_paged``.
+the gate's target from Q and K without them (of scores without a cap or slopes), and ``dense_attention``
+the attention itself. Serving has the same scores in ``BlockSparseFlashAttention.forward_chunk_paged``.
 """
 from __future__ import annotations
 
@@ -217,10 +217,12 @@ def dense_attention(
     Returns:
         ``[B, Hq, S, D]`` / ``[T, Hq, D]`` in q's layout; rows of padding and of tokens behind the last
         document are 0, and so are their gradients. With ``return_lse`` also ``[B, Hq, S]`` / ``[T, Hq]``
-        fp32 (differentiable too), -inf for those rows. Equal calls give equal bits, gradients
-        included. What is kept for the backward: q, k, v, the output with a byte more an element, and the
-        log-sums. In fp16 the weights' gradients are rounded to fp16 for their products: scale the loss,
-        as for every fp16 gradient, so that they stay above 2^-14 where they matter.
+        fp32 (differentiable too), -inf for those rows. Equal calls give equal bits, gradients included; in
+        another batch a sequence's gradients may differ in their last bits (how dS is rounded and heads are
+        shared out goes by the tokens of the whole call). What is kept for the backward: q, k, v, the output
+        with a byte more an element, and the log-sums. In fp16 the weights' gradients are rounded to fp16
+        for their products: scale the loss, as for every fp16 gradient, so that they stay above 2^-14 where
+        they matter.
         A row all of whose scores are -inf is 0, with log-sum -inf (its gradients are NaN); an infinity of v
         whose weight rounds to 0 gives NaN in the rows that see it. A second derivative and forward mode are
         refused. As for every operator of a graph of gradients: to capture a backward pass into a HIP graph,

@@ -8,9 +8,10 @@ A step of a server that drafts trees (the root is the last token that it produce
     out = attn.forward_chunk_paged(q, k_pages, v_pages, table, kv_lens, cu, max_seqlen=most,
                                    ancestors=tree.ancestors)
     kept = accept_draft(parents, tokens, targets, cu, max_nodes=most)
-    kv_lens = commit_draft_paged(k_pages, v_pages, table, kv_lens, cu, kept.path, kept.counts)
+    new_lens = commit_draft_paged(k_pages, v_pages, table, kv_lens, cu, kept.path, kept.counts)
 
-with the appending, the attention and the commit in every layer. The reference drafts nothing (its vLLM
+with the appending, the attention and the commit in every layer (from the same ``kv_lens``: the new lengths are the
+same for all of them). The reference drafts nothing (its vLLM
 backend hands decoding back to vLLM, ``tasft/inference/vllm_patch.py:189-196``).
 """
 from __future__ import annotations

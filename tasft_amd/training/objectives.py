@@ -124,6 +124,11 @@ def gate_target_from_qk(
             ``"row"`` over the key blocks of each query block, ``"none"`` raw block maxima.
         temperature: divide pooled maxima by this before the softmax.
         clamp: if set, clamp finite maxima to ``[-clamp, clamp]`` first.
+
+    The scores are those of a layer without a cap: ``dense_attention``'s ``softcap`` and ``alibi_slopes`` have no
+    counterpart here. A cap rises with the score, so a capped layer's target is made of the raw maxima ``m``
+    (``normalize="none"``), ``torch.where(m == -inf, m, softcap * tanh(m / softcap))``, and their softmax; a bias
+    by distance (without a cap) goes in as an ``attention_mask``.
     """
     _check_target_inputs(q, k, normalize, temperature)
     status = _new_status(q.device) if attention_mask is not None else None
@@ -279,7 +284,8 @@ def gate_loss_from_qk(
     is a constant of the loss, as the reference's detached scores are; the KL and its
     gradient with respect to ``gate_soft_scores`` come from one HIP kernel, so
     ``loss.backward()`` reaches the gate (and, through ``AttnGate``'s HIP backward, its
-    parameters). NaN or Inf in ``gate_soft_scores`` raises ``NaNDetectedError``.
+    parameters). NaN or Inf in ``gate_soft_scores`` raises ``NaNDetectedError``. The target is that of scores
+    without a cap (``gate_target_from_qk``).
     """
     if gate_soft_scores.ndim != 4:
         raise KernelError("gate_soft_scores must be [B, H, NB, NB]",

@@ -95,14 +95,12 @@ LARGE = [
 ]
 
 
-@pytest.mark.parametrize("batched", [False, True])
-@pytest.mark.parametrize("index", range(len(LARGE)))
+@pytest.mark.parametrize(("index", "batched"), [(i, b) for i, c in enumerate(LARGE) for b in (False, True)
+                                                if not (b and c[10])])  # (max_seqlen goes with documents)
 def test_large_calls(index, batched):
     """dS in one part, and heads shared out unevenly or not at all, as calls of many tokens take them: two kinds of
     sequences, mixed, each copy bit for bit, and a copy of each within the bounds of the 64-bit form."""
     lens, copies, hq, hkv, d, dtype, causal, cap, alibi, prefix, most, shares = LARGE[index]
-    if batched and most:
-        pytest.skip("max_seqlen goes with documents")
     dev = require_gpu()
     longest = max(lens) + (5 if batched else 0)
     total = 2 * copies * longest if batched else copies * sum(lens)
